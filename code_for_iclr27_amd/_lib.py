@@ -94,6 +94,16 @@ SIGNATURES = {
     "lr_packed_attention_scratch_bytes": [],
     "lr_packed_attention_noalloc": [_P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I64,
                                     _I64, _I64, _I, _I64, _F, _P, _P],
+    "lr_paged_page_bytes": [_I64, _I64],
+    "lr_paged_append": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P, _P, _P,
+                        _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P],
+    "lr_paged_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64],
+    "lr_paged_attention": [_P, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I,
+                           _I64, _P, _F, _P, _P, _SZ, _P],
+    "lr_paged_read": [_P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I, _I64, _P, _P, _P, _P, _P],
+    "lr_paged_compact_workspace_bytes": [_I64],
+    "lr_paged_compact": [_P, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _SZ,
+                         _P],
     "lr_head_logits": [_P, _I64, _P, _P, _I64, _I64, _I, _P, _P],
     "lr_margin_stats_workspace_bytes": [_I64, _I64],
     "lr_margin_stats": [_P, _I64, _I64, _P, _P, _P, _P, _P, _SZ, _P],
@@ -108,6 +118,9 @@ _RESTYPES = {"lr_last_error": ctypes.c_char_p, "lr_score_workspace_bytes": ctype
              "lr_packed_attention_workspace_bytes": ctypes.c_size_t,
              "lr_packed_attention_scratch_bytes": ctypes.c_size_t,
              "lr_packed_attention_pending_workspace_bytes": ctypes.c_size_t,
+             "lr_paged_page_bytes": ctypes.c_int64,
+             "lr_paged_attention_workspace_bytes": ctypes.c_size_t,
+             "lr_paged_compact_workspace_bytes": ctypes.c_size_t,
              "lr_row_sum_workspace_bytes": ctypes.c_size_t,
              "lr_margin_stats_workspace_bytes": ctypes.c_size_t,
              "lr_pre_gradient_layers_workspace_bytes": ctypes.c_size_t}

@@ -244,6 +244,13 @@ struct Library {
   decltype(&lr_packed_attention_workspace_bytes) attention_workspace_bytes = nullptr;
   decltype(&lr_packed_attention_pending) packed_attention_pending = nullptr;
   decltype(&lr_packed_attention_pending_workspace_bytes) pending_workspace_bytes = nullptr;
+  decltype(&lr_paged_append) paged_append = nullptr;
+  decltype(&lr_paged_attention) paged_attention = nullptr;
+  decltype(&lr_paged_attention_workspace_bytes) paged_attention_workspace_bytes = nullptr;
+  decltype(&lr_paged_read) paged_read = nullptr;
+  decltype(&lr_paged_compact) paged_compact = nullptr;
+  decltype(&lr_paged_compact_workspace_bytes) paged_compact_workspace_bytes = nullptr;
+  decltype(&lr_paged_page_bytes) paged_page_bytes = nullptr;
   decltype(&lr_last_error) last_error = nullptr;
   decltype(&lr_staging_alloc) staging_alloc = nullptr;
   decltype(&lr_staging_free) staging_free = nullptr;
@@ -312,6 +319,19 @@ void bind_attention(int64_t packed_attention, int64_t workspace_bytes, int64_t p
   bind_one(library.attention_workspace_bytes, workspace_bytes);
   bind_one(library.packed_attention_pending, pending);
   bind_one(library.pending_workspace_bytes, pending_workspace_bytes);
+}
+
+void bind_paged(int64_t append, int64_t attention, int64_t attention_workspace_bytes, int64_t read,
+                int64_t compact, int64_t compact_workspace_bytes, int64_t page_bytes,
+                int64_t last_error) {
+  bind_one(library.paged_append, append);
+  bind_one(library.paged_attention, attention);
+  bind_one(library.paged_attention_workspace_bytes, attention_workspace_bytes);
+  bind_one(library.paged_read, read);
+  bind_one(library.paged_compact, compact);
+  bind_one(library.paged_compact_workspace_bytes, compact_workspace_bytes);
+  bind_one(library.paged_page_bytes, page_bytes);
+  bind_one(library.last_error, last_error);
 }
 
 void check_call(int status) {
@@ -1371,6 +1391,214 @@ torch::Tensor attention_launch(const torch::Tensor& queries, const torch::Tensor
 }
 
 // ---------------------------------------------------------------------------------------
+// The paged 4-bit KV cache's operators (paged.py): checks, output and workspace allocation and
+// launch on torch's current stream.
+
+void* current_stream(const torch::Device& device);
+
+struct PagedOperands {
+  const torch::Tensor &pages, &table, &lengths;
+  int64_t dim, page_size;
+};
+
+void check_paged_layer(const PagedOperands& p) {
+  require(library.paged_append != nullptr, "library entry points are not bound");
+  const int64_t bytes = library.paged_page_bytes(p.page_size, p.dim);
+  require(bytes > 0, "Head dimension must be 64, 128 or 256 and page size 16, 32, 64, 128 or 256");
+  for (const torch::Tensor* t : {&p.pages, &p.table, &p.lengths}) {
+    require(t->is_cuda() && t->is_contiguous(), "Expected contiguous CUDA tensor");
+    require(t->device() == p.pages.device(), "CUDA devices differ");
+  }
+  require(p.pages.scalar_type() == torch::kUInt8 && p.pages.dim() == 2 && p.pages.size(1) == bytes,
+          "Pages must be uint8 [pages, page_bytes(page_size, dim)]");
+  require(p.lengths.scalar_type() == torch::kInt32 && p.lengths.dim() == 1 && p.lengths.numel() > 0,
+          "Lengths must be int32 [segments]");
+  require(p.table.scalar_type() == torch::kInt32 && p.table.dim() == 2 &&
+              p.table.size(0) == p.lengths.numel(),
+          "Page table must be int32 [segments, max_pages]");
+}
+
+const int32_t* paged_counts(const py::object& counts_in, int64_t batch, const torch::Device& device,
+                            torch::Tensor& keep) {
+  if (counts_in.is_none()) return nullptr;
+  keep = counts_in.cast<torch::Tensor>();
+  require(keep.is_cuda() && keep.device() == device && keep.is_contiguous() &&
+              keep.scalar_type() == torch::kInt32 && keep.dim() == 1 && keep.numel() == batch,
+          "Counts must be a contiguous CUDA int32 [batch]");
+  return keep.data_ptr<int32_t>();
+}
+
+int paged_type(torch::ScalarType type) {
+  require(type == torch::kBFloat16 || type == torch::kHalf || type == torch::kFloat32,
+          "Paged rows are bf16, f16 or f32");
+  return type == torch::kBFloat16 ? LR_DTYPE_BF16 : type == torch::kHalf ? LR_DTYPE_F16 : LR_DTYPE_F32;
+}
+
+// Element strides of the batch, head and row dimensions; a dimension of one has any.
+void row_strides(const torch::Tensor& t, int64_t (&strides)[3]) {
+  for (int i = 0; i < 3; ++i) strides[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+
+const void* address_or_null(const torch::Tensor& t) { return t.numel() ? t.data_ptr() : nullptr; }
+
+py::object paged_append_launch(const torch::Tensor& pages, const torch::Tensor& table,
+                               const torch::Tensor& lengths, int64_t kv_heads, int64_t dim,
+                               int64_t page_size, const torch::Tensor& keys,
+                               const torch::Tensor& values, const torch::Tensor& positions,
+                               const py::object& cos_in, const py::object& sin_in,
+                               const py::object& queries_in, const py::object& counts_in) {
+  check_paged_layer({pages, table, lengths, dim, page_size});
+  require(keys.dim() == 4 && keys.sizes() == values.sizes(),
+          "New keys and values must be [batch, kv_heads, length, dim]");
+  const int64_t batch = keys.size(0), added = keys.size(2);
+  require(kv_heads > 0 && batch > 0 && keys.size(1) == kv_heads && keys.size(3) == dim &&
+              batch * kv_heads == lengths.numel(),
+          "New keys and values must be [batch, kv_heads, length, dim]");
+  const auto type = keys.scalar_type();
+  const int dtype = paged_type(type);
+  torch::Tensor queries, cosine, sine, counts;
+  if (!queries_in.is_none()) queries = queries_in.cast<torch::Tensor>();
+  const torch::Tensor* const operands[] = {&keys, &values, &queries};
+  for (const torch::Tensor* t : operands) {
+    if (!t->defined()) continue;
+    require(t->is_cuda() && t->device() == pages.device(), "CUDA devices differ");
+    require(t->scalar_type() == type, "query and key must have the same dtype");
+    require(t->dim() == 4 && t->size(0) == batch && t->size(2) == added && t->size(3) == dim,
+            "New queries must be [batch, query_heads, length, dim]");
+    require(t->stride(3) == 1 || added == 0, "Input tensor must have contiguous last dimension");
+  }
+  require(!queries.defined() || (queries.size(1) > 0 && queries.size(1) % kv_heads == 0),
+          "Number of heads in key/value must divide number of heads in query");
+  require(positions.is_cuda() && positions.device() == pages.device() &&
+              positions.is_contiguous() && positions.scalar_type() == torch::kInt64 &&
+              positions.sizes() == torch::IntArrayRef({batch, added}),
+          "Positions must be a contiguous CUDA int64 [batch, length]");
+  require(cos_in.is_none() == sin_in.is_none(), "Rotation tables go together");
+  if (!cos_in.is_none()) {
+    cosine = cos_in.cast<torch::Tensor>();
+    sine = sin_in.cast<torch::Tensor>();
+    for (const torch::Tensor* t : {&cosine, &sine})
+      require(t->is_cuda() && t->device() == pages.device() && t->is_contiguous() &&
+                  t->scalar_type() == torch::kFloat32 && t->dim() == 2 &&
+                  t->sizes() == cosine.sizes() && t->size(0) > 0 && t->size(1) > 0,
+              "Rotation tables must be contiguous CUDA float32 [positions, half]");
+  }
+  const int32_t* count = paged_counts(counts_in, batch, pages.device(), counts);
+  const c10::DeviceGuard guard(pages.device());
+  torch::Tensor out;
+  int64_t query_strides[3] = {}, key_strides[3], value_strides[3];
+  row_strides(keys, key_strides);
+  row_strides(values, value_strides);
+  if (queries.defined()) {
+    out = torch::empty(queries.sizes(), queries.options().memory_format(c10::MemoryFormat::Contiguous));
+    row_strides(queries, query_strides);
+  }
+  if (added > 0)
+    check_call(library.paged_append(
+        keys.data_ptr(), key_strides, values.data_ptr(), value_strides,
+        queries.defined() ? queries.data_ptr() : nullptr, query_strides,
+        out.defined() ? out.data_ptr() : nullptr, batch, kv_heads,
+        queries.defined() ? queries.size(1) : 0, added, dim, dtype, positions.data_ptr<int64_t>(),
+        cosine.defined() ? cosine.data_ptr<float>() : nullptr,
+        sine.defined() ? sine.data_ptr<float>() : nullptr, cosine.defined() ? cosine.size(0) : 0,
+        cosine.defined() ? cosine.size(1) : 0, count, const_cast<void*>(address_or_null(pages)),
+        pages.size(0), page_size, table.numel() ? table.data_ptr<int32_t>() : nullptr,
+        table.size(1), lengths.data_ptr<int32_t>(), current_stream(pages.device())));
+  return out.defined() ? py::cast(out) : py::none();
+}
+
+torch::Tensor paged_attention_launch(const torch::Tensor& pages, const torch::Tensor& table,
+                                     const torch::Tensor& lengths, int64_t kv_heads, int64_t dim,
+                                     int64_t page_size, const torch::Tensor& queries,
+                                     int64_t max_keys, const py::object& counts_in, double scale) {
+  check_paged_layer({pages, table, lengths, dim, page_size});
+  require(queries.dim() == 4 && kv_heads > 0 && queries.size(3) == dim &&
+              queries.size(0) * kv_heads == lengths.numel(),
+          "Queries must be [batch, query_heads, length, dim]");
+  const int64_t batch = queries.size(0), heads = queries.size(1), length = queries.size(2);
+  require(heads > 0 && heads % kv_heads == 0,
+          "Number of heads in key/value must divide number of heads in query");
+  const auto type = queries.scalar_type();
+  require(type == torch::kHalf || type == torch::kBFloat16,
+          "FlashAttention only supports fp16 and bf16 data type");
+  require(queries.is_cuda() && queries.device() == pages.device(), "CUDA devices differ");
+  require(queries.stride(3) == 1 || length == 0, "Input tensor must have contiguous last dimension");
+  require(max_keys >= 0, "Invalid max_seqlen_k");
+  torch::Tensor counts;
+  const int32_t* count = paged_counts(counts_in, batch, pages.device(), counts);
+  const c10::DeviceGuard guard(pages.device());
+  torch::Tensor out = torch::empty({batch, length, heads * dim},
+                                   queries.options().memory_format(c10::MemoryFormat::Contiguous));
+  if (length == 0) return out;
+  max_keys = std::min(max_keys, table.size(1) * page_size);
+  const size_t size = library.paged_attention_workspace_bytes(
+      batch * kv_heads, heads / kv_heads, length, pages.size(0) ? max_keys : 0, dim);
+  torch::Tensor workspace;
+  if (size)
+    workspace = torch::empty({static_cast<int64_t>(size)}, queries.options().dtype(torch::kUInt8));
+  int64_t strides[3];
+  row_strides(queries, strides);
+  check_call(library.paged_attention(
+      queries.data_ptr(), strides, address_or_null(pages), pages.size(0), page_size,
+      table.numel() ? table.data_ptr<int32_t>() : nullptr, table.size(1),
+      lengths.data_ptr<int32_t>(), batch, kv_heads, heads / kv_heads, length, dim,
+      type == torch::kBFloat16 ? LR_DTYPE_BF16 : LR_DTYPE_F16, max_keys, count,
+      static_cast<float>(scale), out.data_ptr(), size ? workspace.data_ptr() : nullptr, size,
+      current_stream(pages.device())));
+  return out;
+}
+
+std::vector<torch::Tensor> paged_read_launch(const torch::Tensor& pages, const torch::Tensor& table,
+                                             const torch::Tensor& lengths, int64_t dim,
+                                             int64_t page_size, int64_t total,
+                                             const py::object& type_in) {
+  check_paged_layer({pages, table, lengths, dim, page_size});
+  require(total >= 0 && total <= INT32_MAX, "Invalid packed rows");
+  const auto type = torch::python::detail::py_object_to_dtype(type_in);
+  const int dtype = paged_type(type);
+  const c10::DeviceGuard guard(pages.device());
+  const auto options = pages.options().dtype(type);
+  torch::Tensor keys = torch::empty({total, dim}, options), values = torch::empty({total, dim}, options);
+  torch::Tensor positions = torch::empty({total, 1}, pages.options().dtype(torch::kFloat32));
+  torch::Tensor cumulative = torch::empty({lengths.numel() + 1}, lengths.options());
+  check_call(library.paged_read(
+      address_or_null(pages), pages.size(0), page_size,
+      table.numel() ? table.data_ptr<int32_t>() : nullptr, table.size(1),
+      lengths.data_ptr<int32_t>(), lengths.numel(), dim, dtype, total,
+      total ? keys.data_ptr() : nullptr, total ? values.data_ptr() : nullptr,
+      total ? positions.data_ptr<float>() : nullptr, cumulative.data_ptr<int32_t>(),
+      current_stream(pages.device())));
+  return {keys, values, positions, cumulative};
+}
+
+torch::Tensor paged_compact_launch(const torch::Tensor& pages, const torch::Tensor& table,
+                                   const torch::Tensor& lengths, int64_t dim, int64_t page_size,
+                                   const torch::Tensor& removed, const torch::Tensor& target) {
+  check_paged_layer({pages, table, lengths, dim, page_size});
+  for (const torch::Tensor* t : {&removed, &target}) {
+    require(t->is_cuda() && t->is_contiguous(), "Expected contiguous CUDA tensor");
+    require(t->device() == pages.device(), "CUDA devices differ");
+  }
+  require(removed.dim() == 1 && removed.scalar_type() == torch::kInt64, "Removed indices must be int64");
+  require(target.scalar_type() == torch::kInt32 && target.dim() == 2 &&
+              target.size(0) == lengths.numel(),
+          "Page table must be int32 [segments, max_pages]");
+  const c10::DeviceGuard guard(pages.device());
+  torch::Tensor new_lengths = torch::empty_like(lengths);
+  const size_t size = library.paged_compact_workspace_bytes(lengths.numel());
+  torch::Tensor workspace =
+      torch::empty({static_cast<int64_t>(size)}, pages.options().dtype(torch::kUInt8));
+  check_call(library.paged_compact(
+      const_cast<void*>(address_or_null(pages)), pages.size(0), page_size,
+      table.numel() ? table.data_ptr<int32_t>() : nullptr, table.size(1),
+      lengths.data_ptr<int32_t>(), lengths.numel(), dim,
+      removed.numel() ? removed.data_ptr<int64_t>() : nullptr, removed.numel(),
+      target.numel() ? target.data_ptr<int32_t>() : nullptr, target.size(1),
+      new_lengths.data_ptr<int32_t>(), workspace.data_ptr(), size, current_stream(pages.device())));
+  return new_lengths;
+}
+
+// ---------------------------------------------------------------------------------------
 // The per-layer drop-ins _C.append and _C.compact with their checks, output allocation and
 // launch in C++ (a decode step makes one append per layer; from Python each call cost ~20 us of
 // host time in tensor checks, five allocations and the ctypes call). Same checks, order and
@@ -1736,6 +1964,12 @@ PYBIND11_MODULE(_plan, module) {
              "Bind lr_packed_attention and its workspace size (addresses from the ctypes handle)");
   module.def("packed_attention", &attention_launch,
              "packed_attention: checks, output and workspace allocation and launch from C++");
+  module.def("bind_paged", &bind_paged, "Bind the paged cache's entry points");
+  module.def("paged_append", &paged_append_launch, "paged.append: checks, output and launch");
+  module.def("paged_attention", &paged_attention_launch,
+             "paged.attention: checks, output and workspace allocation and launch");
+  module.def("paged_read", &paged_read_launch, "paged.read: checks, outputs and launch");
+  module.def("paged_compact", &paged_compact_launch, "paged.compact: checks, output and launch");
   module.def("reinsert_prepare", &reinsert_prepare,
              "Check a reinsertion and build its pinned table + metadata block");
   module.def("reinsert_table", &reinsert_table,

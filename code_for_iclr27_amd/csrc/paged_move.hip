@@ -1,0 +1,586 @@
+// Rows into, out of and within the paged 4-bit KV cache (paged.hpp states its layout).
+//
+// append: new K and V rows behind each segment's rows, K (and the step's queries) rotated to their
+// positions on the way. D / 8 threads a row, eight channels each: the rotation pairs channels i and
+// i + half, so a thread loads its channels and their partners; the products are rounded one by one
+// (no fused multiply-add), in f32. Four threads share a block: its largest magnitude goes round
+// them in the vector ALU, the scale is the largest power of two X with 4 X <= amax, doubled where
+// amax >= 7 X (so that no element loses more to saturation than to rounding), and the conversion
+// instruction rounds to the nearest code, ties to even, and saturates.
+//
+// read: the rows as 16- or 32-bit rows packed by segment, the layout of the other operators. A
+// first launch sums the lengths (the packed layout's cumulative lengths, an output).
+//
+// compact: the rows that stay, in order, into other pages. A first launch finds each segment's part
+// of the removed rows and its new length.
+
+#include <algorithm>
+
+#include "paged.hpp"
+
+namespace lr {
+
+int check_paged(const void* pages, int64_t page_count, int64_t page_size, int64_t dim,
+                const int32_t* table, int64_t max_pages, const int32_t* lengths,
+                int64_t segments) {
+  LR_REQUIRE(dim == 64 || dim == 128 || dim == 256, "Head dimension must be 64, 128 or 256");
+  LR_REQUIRE(paged_bytes(page_size, dim) > 0, "Page size must be 16, 32, 64, 128 or 256");
+  LR_REQUIRE(segments > 0 && segments <= INT32_MAX && page_count >= 0 && max_pages >= 0 &&
+                 page_count <= INT32_MAX,
+             "Invalid page table");
+  LR_REQUIRE(max_pages <= INT32_MAX / 2 / page_size, "A segment holds fewer than 2^30 rows");
+  LR_REQUIRE(lengths && (table || max_pages == 0) && (pages || page_count == 0),
+             "Invalid page table");
+  LR_REQUIRE(reinterpret_cast<uintptr_t>(pages) % 16 == 0, "Pages must be 16-byte aligned");
+  return LR_OK;
+}
+
+namespace {
+
+constexpr int kThreads = 256;
+
+typedef float move_f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned move_u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned move_u32x2 __attribute__((ext_vector_type(2)));
+
+template <typename T>
+struct Eight;  // eight elements in memory
+template <>
+struct Eight<float> {
+  move_f32x4 lo, hi;
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    lo = move_f32x4{v[0], v[1], v[2], v[3]};
+    hi = move_f32x4{v[4], v[5], v[6], v[7]};
+  }
+};
+template <typename T>
+struct Eight {
+  typedef T vec __attribute__((ext_vector_type(8)));
+  vec x;
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(x[e]);
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = static_cast<T>(v[e]);  // round to nearest even
+  }
+};
+
+// Rows [batch, heads, added, D] with the strides (elements) of the first three dimensions.
+struct Rows {
+  const void* base;
+  int64_t batch, head, row;
+};
+
+struct AppendArgs {
+  Rows keys, values, queries;
+  void* out_queries;          // [batch, query_heads, added, D], contiguous
+  const int64_t* positions;   // [batch, added]
+  const float* cos;           // [table_rows, half], or half = 0
+  const float* sin;
+  int64_t table_rows;
+  int half;
+  unsigned kv_heads, query_heads, added;
+  unsigned kv_rows, query_rows;  // batch * heads * added
+  unsigned kv_blocks;            // workgroups of the keys, and of the values
+  const int32_t* counts;         // [batch] rows of `added` that are there, or NULL
+  ScaleRange range;
+  PagedCache cache;
+};
+
+template <int BIT>
+__device__ __forceinline__ float quad_max(float x) {
+  return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                      0, __builtin_bit_cast(int, x), BIT == 0 ? 0xB1 : 0x4E, 0xF, 0xF, false)));
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs a) {
+  constexpr int kRowThreads = D / 8, kRowsPerBlock = kThreads / kRowThreads;
+  // blocks: the keys', the values', the queries'
+  const int what = blockIdx.x < a.kv_blocks ? 0 : blockIdx.x < 2 * a.kv_blocks ? 1 : 2;
+  const unsigned block = blockIdx.x - what * a.kv_blocks;
+  const unsigned row = block * kRowsPerBlock + threadIdx.x / kRowThreads;
+  const int c = threadIdx.x % kRowThreads;
+  // whole quads are in or out: the exchanges below stay within a row
+  if (row >= (what == 2 ? a.query_rows : a.kv_rows)) return;
+  const unsigned heads = what == 2 ? a.query_heads : a.kv_heads;
+  const unsigned segment = row / a.added, i = row - segment * a.added;
+  const unsigned b = segment / heads, h = segment - b * heads;
+  if (what != 2 && a.counts != nullptr && static_cast<int64_t>(i) >= a.counts[b]) return;
+
+  const Rows& rows = what == 0 ? a.keys : what == 1 ? a.values : a.queries;
+  const T* source = static_cast<const T*>(rows.base) + b * rows.batch + h * rows.head + i * rows.row;
+  float x[8];
+  const Eight<T> mine = *reinterpret_cast<const Eight<T>*>(source + 8 * c);
+  mine.get(x);
+  const int64_t position = a.positions[static_cast<int64_t>(b) * a.added + i];
+  if (what != 1 && 8 * c < 2 * a.half) {
+    const bool first = 8 * c < a.half;
+    float y[8], cosine[8], sine[8];
+    const Eight<T> partner =
+        *reinterpret_cast<const Eight<T>*>(source + (first ? 8 * c + a.half : 8 * c - a.half));
+    partner.get(y);
+    const bool known = position >= 0 && position < a.table_rows;
+    const int64_t at = (known ? position : 0) * a.half + (first ? 8 * c : 8 * c - a.half);
+    reinterpret_cast<const Eight<float>*>(a.cos + at)->get(cosine);
+    reinterpret_cast<const Eight<float>*>(a.sin + at)->get(sine);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float p = x[e] * cosine[e], q = y[e] * sine[e];
+      x[e] = known ? (first ? p - q : p + q) : __builtin_nanf("");
+    }
+  }
+  if (what == 2) {
+    Eight<T> result;
+    result.set(x);
+    *reinterpret_cast<Eight<T>*>(static_cast<T*>(a.out_queries) + static_cast<int64_t>(row) * D +
+                                 8 * c) = result;
+    return;
+  }
+
+  float top = 0.0f, sum = 0.0f;  // sum: NaN if an element is not finite
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    top = fmaxf(top, __builtin_fabsf(x[e]));
+    sum = __builtin_fmaf(x[e], 0.0f, sum);
+  }
+  top = sum == sum ? top : __builtin_huge_valf();
+  top = quad_max<1>(quad_max<0>(top));
+  const bool finite = top < __builtin_huge_valf();
+  int exponent = static_cast<int>((__builtin_bit_cast(unsigned, top) + 0x200000u) >> 23) - 129;
+  exponent = exponent < a.range.low ? a.range.low : exponent > a.range.high ? a.range.high : exponent;
+  const unsigned byte = finite ? static_cast<unsigned>(exponent + 127) : kScaleNaN;
+  const float scale = scale_of(finite ? byte : 127u);
+  unsigned codes = 0;
+  if (finite) {
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], scale, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], scale, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], scale, 2);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], scale, 3);
+  }
+
+  const PagedCache& cache = a.cache;
+  const int n = cache.lengths[segment];
+  const int64_t at = static_cast<int64_t>(n) + i;
+  if (n < 0 || at >= static_cast<int64_t>(cache.max_pages) << cache.shift) return;
+  const int to = static_cast<int>(at);
+  const int64_t id = cache.table[static_cast<int64_t>(segment) * cache.max_pages + (to >> cache.shift)];
+  if (id < 0 || id >= cache.page_count) return;
+  const int slot = to & ((1 << cache.shift) - 1);
+  uint8_t* page = cache.pages + id * (Page<D>::bytes(1) << cache.shift);
+  *reinterpret_cast<unsigned*>(page + Page<D>::codes(cache.shift, what, slot) + 4 * c) = codes;
+  if (c % 4 == 0) page[Page<D>::scales(cache.shift, what, slot) + c / 4] = static_cast<uint8_t>(byte);
+  if (what == 0 && c == 0)
+    *reinterpret_cast<float*>(page + Page<D>::position(cache.shift, slot)) =
+        static_cast<float>(position);
+}
+
+// ---------------------------------------------------------------------------------------
+// The packed layout's first rows, cumulative[s] = rows of the segments before s; one workgroup.
+// With `starts` also each segment's part of `removed` (sorted packed rows, starts[s] = how many lie
+// before the segment) and the length that it leaves.
+struct SumArgs {
+  PagedCache cache;
+  int64_t segments;
+  int32_t* cumulative;        // [segments + 1], or NULL
+  const int64_t* removed;
+  int64_t removed_count;
+  int64_t* starts;            // [segments + 1], or NULL
+  int64_t* first_rows;        // [segments] with starts
+  int32_t* new_lengths;       // [segments] with starts
+};
+
+__device__ __forceinline__ int64_t lower_bound(const int64_t* sorted, int64_t count, int64_t value) {
+  int64_t low = 0, high = count;
+  while (low < high) {
+    const int64_t mid = (low + high) / 2;
+    if (sorted[mid] < value) low = mid + 1;
+    else high = mid;
+  }
+  return low;
+}
+
+constexpr int kSumThreads = 1024;
+
+// A packed row number as the i32 of the packed layout (rows past 2^31 - 1 are not read).
+__device__ __forceinline__ int32_t packed_row(int64_t row) {
+  return static_cast<int32_t>(row < INT32_MAX ? row : INT32_MAX);
+}
+
+__global__ __launch_bounds__(kSumThreads) void paged_sum_kernel(SumArgs a) {
+  __shared__ int64_t wave_total[kSumThreads / 64];
+  __shared__ int64_t before;  // rows of the segments of earlier rounds
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x == 0) before = 0;
+  __syncthreads();
+  for (int64_t s0 = 0; s0 < a.segments; s0 += kSumThreads) {
+    const int64_t s = s0 + threadIdx.x;
+    const int64_t n = s < a.segments ? a.cache.rows(s) : 0;
+    int64_t sum = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t other = __shfl_up(sum, d);
+      if (lane >= d) sum += other;
+    }
+    if (lane == 63) wave_total[wave] = sum;
+    __syncthreads();
+    int64_t first = before + sum - n, total = before;
+    for (int w = 0; w < kSumThreads / 64; ++w) {
+      if (w < wave) first += wave_total[w];
+      total += wave_total[w];
+    }
+    if (s < a.segments) {
+      if (a.cumulative != nullptr) a.cumulative[s] = packed_row(first);
+      if (a.starts != nullptr) {
+        const int64_t low = lower_bound(a.removed, a.removed_count, first);
+        const int64_t high = lower_bound(a.removed, a.removed_count, first + n);
+        const int64_t gone = high - low < n ? high - low : n;
+        a.starts[s] = low;
+        a.first_rows[s] = first;
+        a.new_lengths[s] = static_cast<int32_t>(n - gone);
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) before = total;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0 && a.cumulative != nullptr)
+    a.cumulative[a.segments] = packed_row(before);
+}
+
+// ---------------------------------------------------------------------------------------
+struct ReadArgs {
+  PagedCache cache;
+  int64_t segments, total;
+  const int32_t* cumulative;
+  void* keys;
+  void* values;
+  float* positions;
+};
+
+// The segment that packed row `row` belongs to: the largest s with cumulative[s] <= row (and so
+// one that is not empty, if row < cumulative[segments]).
+__device__ __forceinline__ int64_t segment_of(const int32_t* cumulative, int64_t segments, int64_t row) {
+  int64_t low = 0, high = segments;
+  while (high - low > 1) {
+    const int64_t mid = (low + high) / 2;
+    if (cumulative[mid] <= row) low = mid;
+    else high = mid;
+  }
+  return low;
+}
+
+template <typename T>
+__device__ __forceinline__ Eight<T> eight_values(unsigned codes, float scale) {
+  if constexpr (std::is_same<T, float>::value) {
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 0);
+    const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 1);
+    const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 2);
+    const auto d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 3);
+    return {move_f32x4{a[0], a[1], b[0], b[1]}, move_f32x4{c[0], c[1], d[0], d[1]}};
+  } else {
+    return {__builtin_bit_cast(typename Eight<T>::vec, expand8<T>(codes, scale))};
+  }
+}
+
+// D / 8 threads a row, eight channels of its K and V each.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void paged_read_kernel(ReadArgs a) {
+  constexpr int kRowThreads = D / 8, kRowsPerBlock = kThreads / kRowThreads;
+  const int c = threadIdx.x % kRowThreads;
+  const int64_t stop = min(a.total, static_cast<int64_t>(a.cumulative[a.segments]));
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + threadIdx.x / kRowThreads;
+  if (row >= stop) return;
+  const PagedCache& cache = a.cache;
+  const int64_t segment = segment_of(a.cumulative, a.segments, row);
+  const int at = static_cast<int>(row - a.cumulative[segment]);
+  const int64_t id = cache.table[segment * cache.max_pages + (at >> cache.shift)];
+  if (id < 0 || id >= cache.page_count) return;
+  const int slot = at & ((1 << cache.shift) - 1);
+  const uint8_t* page = cache.pages + id * (Page<D>::bytes(1) << cache.shift);
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const unsigned codes =
+        *reinterpret_cast<const unsigned*>(page + Page<D>::codes(cache.shift, which, slot) + 4 * c);
+    const unsigned byte = page[Page<D>::scales(cache.shift, which, slot) + c / 4];
+    T* out = static_cast<T*>(which == 0 ? a.keys : a.values) + row * D + 8 * c;
+    *reinterpret_cast<Eight<T>*>(out) = eight_values<T>(codes, scale_of(byte));
+  }
+  if (c == 0)
+    a.positions[row] = *reinterpret_cast<const float*>(page + Page<D>::position(cache.shift, slot));
+}
+
+// ---------------------------------------------------------------------------------------
+struct CompactArgs {
+  PagedCache cache;
+  int64_t segments;
+  int chunks;                   // row chunks of a segment (each 64 rows)
+  const int32_t* target;        // [segments, target_pages]
+  int target_pages;
+  const int64_t* removed;
+  int64_t removed_count;
+  const int64_t* starts;
+  const int64_t* first_rows;
+  const int32_t* new_lengths;
+};
+
+// A wave moves 64 rows of a segment: lane r finds where row r comes from (row + how many removed
+// rows lie at or before it), then all lanes copy 16 bytes each of the rows' codes.
+template <int D>
+__global__ __launch_bounds__(kThreads) void paged_compact_kernel(CompactArgs a) {
+  constexpr int kChunks = D / 32;  // 16-byte pieces of a row's codes
+  using Scales = std::conditional_t<D == 64, uint16_t, std::conditional_t<D == 128, uint32_t, uint64_t>>;
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
+  const int64_t segment = unit / a.chunks;
+  if (segment >= a.segments) return;
+  const int row0 = static_cast<int>(unit - segment * a.chunks) * 64;
+  const PagedCache& cache = a.cache;
+  const int rows = min(a.new_lengths[segment], a.target_pages << cache.shift);
+  if (row0 >= rows) return;
+  const int row = row0 + lane;
+  const int mask = (1 << cache.shift) - 1;
+  int64_t from = -1, to = -1;  // byte offsets of the rows' pages; slots apart
+  int from_slot = 0, to_slot = 0;
+  if (row < rows) {
+    const int64_t first = a.first_rows[segment], low = a.starts[segment];
+    const int64_t length = cache.rows(segment);
+    int64_t j = 0, high = min(length - a.new_lengths[segment], a.removed_count - low);
+    while (j < high) {  // removed rows whose index less their rank is at most `row`
+      const int64_t mid = (j + high) / 2;
+      if (a.removed[low + mid] - first - mid <= row) j = mid + 1;
+      else high = mid;
+    }
+    const int source = static_cast<int>(row + j);
+    if (source < length) {
+      const int64_t id = cache.table[segment * cache.max_pages + (source >> cache.shift)];
+      const int64_t target = a.target[segment * a.target_pages + (row >> cache.shift)];
+      if (id >= 0 && id < cache.page_count && target >= 0 && target < cache.page_count) {
+        from = id * (Page<D>::bytes(1) << cache.shift);
+        to = target * (Page<D>::bytes(1) << cache.shift);
+        from_slot = source & mask;
+        to_slot = row & mask;
+      }
+    }
+  }
+  if (from >= 0) {
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+      *reinterpret_cast<Scales*>(cache.pages + to + Page<D>::scales(cache.shift, which, to_slot)) =
+          *reinterpret_cast<const Scales*>(cache.pages + from +
+                                           Page<D>::scales(cache.shift, which, from_slot));
+    *reinterpret_cast<float*>(cache.pages + to + Page<D>::position(cache.shift, to_slot)) =
+        *reinterpret_cast<const float*>(cache.pages + from + Page<D>::position(cache.shift, from_slot));
+  }
+  move_u32x4 data[2][kChunks];
+  int64_t target[kChunks];
+#pragma unroll
+  for (int u = 0; u < kChunks; ++u) {
+    const int piece = u * 64 + lane, r = piece / kChunks, c = piece % kChunks;
+    const int64_t page = __shfl(from, r);
+    const int slot = __shfl(from_slot, r);
+    target[u] = __shfl(to, r);
+    const int target_slot = __shfl(to_slot, r);
+    if (page < 0) target[u] = -1;
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+      if (page >= 0)
+        data[which][u] = *reinterpret_cast<const move_u32x4*>(
+            cache.pages + page + Page<D>::codes(cache.shift, which, slot) + 16 * c);
+    if (page >= 0) target[u] += Page<D>::codes(cache.shift, 0, target_slot) + 16 * c;
+  }
+#pragma unroll
+  for (int u = 0; u < kChunks; ++u)
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+      if (target[u] >= 0)
+        *reinterpret_cast<move_u32x4*>(cache.pages + target[u] +
+                                       Page<D>::codes(cache.shift, which, 0)) = data[which][u];
+}
+
+template <typename F>
+int dispatch_type(int dtype, F&& f) {
+  switch (dtype) {
+    case LR_DTYPE_BF16: return f.template operator()<__bf16>();
+    case LR_DTYPE_F16: return f.template operator()<_Float16>();
+    default: return f.template operator()<float>();
+  }
+}
+
+bool paged_type(int dtype) {
+  return dtype == LR_DTYPE_BF16 || dtype == LR_DTYPE_F16 || dtype == LR_DTYPE_F32;
+}
+
+}  // namespace
+}  // namespace lr
+
+using namespace lr;
+
+extern "C" int64_t lr_paged_page_bytes(int64_t page_size, int64_t dim) {
+  return paged_bytes(page_size, dim);
+}
+
+extern "C" int lr_paged_append(const void* keys, const int64_t* key_strides, const void* values,
+                               const int64_t* value_strides, const void* queries,
+                               const int64_t* query_strides, void* out_queries, int64_t batch,
+                               int64_t kv_heads, int64_t query_heads, int64_t added, int64_t dim,
+                               int dtype, const int64_t* positions, const float* cos,
+                               const float* sin, int64_t table_rows, int64_t half,
+                               const int32_t* counts, void* pages, int64_t page_count,
+                               int64_t page_size, const int32_t* table, int64_t max_pages,
+                               const int32_t* lengths, void* stream) {
+  clear_error();
+  LR_REQUIRE(paged_type(dtype), "Appended rows must be bf16, f16 or f32");
+  LR_REQUIRE(batch > 0 && kv_heads > 0 && added >= 0 && query_heads >= 0 &&
+                 (query_heads > 0) == (queries != nullptr),
+             "Invalid appended shape");
+  LR_REQUIRE(batch <= INT32_MAX / kv_heads, "Invalid appended shape");
+  if (int status = check_paged(pages, page_count, page_size, dim, table, max_pages, lengths,
+                               batch * kv_heads))
+    return status;
+  if (added == 0) return LR_OK;
+  LR_REQUIRE(keys && values && positions && key_strides && value_strides &&
+                 (queries == nullptr) == (out_queries == nullptr) &&
+                 (queries == nullptr || query_strides != nullptr),
+             "Invalid appended KV");
+  LR_REQUIRE(half >= 0 && half % 8 == 0 && 2 * half <= dim && table_rows >= 0 &&
+                 (half == 0 || (cos && sin && table_rows > 0)),
+             "Rotated channels must be a multiple of 16, at most the head dimension, with tables");
+  LR_REQUIRE(added <= INT32_MAX / (batch * kv_heads) &&
+                 (query_heads == 0 || added <= INT32_MAX / batch / query_heads),
+             "Appended grid too large");
+  uintptr_t alignment = reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values) |
+                        reinterpret_cast<uintptr_t>(queries) |
+                        reinterpret_cast<uintptr_t>(out_queries) | reinterpret_cast<uintptr_t>(cos) |
+                        reinterpret_cast<uintptr_t>(sin);
+  const int64_t elem = dtype == LR_DTYPE_F32 ? 4 : 2;
+  for (int i = 0; i < 3; ++i) {
+    alignment |= static_cast<uintptr_t>((key_strides[i] | value_strides[i]) * elem);
+    if (queries != nullptr) alignment |= static_cast<uintptr_t>(query_strides[i] * elem);
+  }
+  LR_REQUIRE(alignment % 16 == 0, "Appended operands must be 16-byte aligned");
+
+  AppendArgs args{};
+  auto rows = [](const void* base, const int64_t* strides) {
+    return base ? Rows{base, strides[0], strides[1], strides[2]} : Rows{};
+  };
+  args.keys = rows(keys, key_strides);
+  args.values = rows(values, value_strides);
+  args.queries = rows(queries, query_strides);
+  args.out_queries = out_queries;
+  args.positions = positions;
+  args.cos = cos;
+  args.sin = sin;
+  args.table_rows = table_rows;
+  args.half = static_cast<int>(half);
+  args.kv_heads = static_cast<unsigned>(kv_heads);
+  args.query_heads = static_cast<unsigned>(query_heads);
+  args.added = static_cast<unsigned>(added);
+  args.kv_rows = static_cast<unsigned>(batch * kv_heads * added);
+  args.query_rows = static_cast<unsigned>(batch * query_heads * added);
+  args.counts = counts;
+  args.range = dtype == LR_DTYPE_F16 ? kHalfRange : kWideRange;
+  args.cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
+  const int64_t per_block = kThreads / (dim / 8);
+  const int64_t kv_blocks = ceil_div(args.kv_rows, per_block);
+  const int64_t blocks = 2 * kv_blocks + ceil_div(args.query_rows, per_block);
+  LR_REQUIRE(blocks < (int64_t{1} << 31), "Appended grid too large");
+  args.kv_blocks = static_cast<unsigned>(kv_blocks);
+  return dispatch_type(dtype, [&]<typename T>() {
+    return dispatch_dim(dim, [&]<int D>() {
+      hipLaunchKernelGGL((paged_append_kernel<T, D>), dim3(static_cast<unsigned>(blocks)),
+                         dim3(kThreads), 0, as_stream(stream), args);
+      return check_launch("paged_append");
+    });
+  });
+}
+
+extern "C" int lr_paged_read(const void* pages, int64_t page_count, int64_t page_size,
+                             const int32_t* table, int64_t max_pages, const int32_t* lengths,
+                             int64_t segments, int64_t dim, int dtype, int64_t total, void* keys,
+                             void* values, float* positions, int32_t* cumulative, void* stream) {
+  clear_error();
+  LR_REQUIRE(paged_type(dtype), "Rows are read as bf16, f16 or f32");
+  if (int status = check_paged(pages, page_count, page_size, dim, table, max_pages, lengths, segments))
+    return status;
+  LR_REQUIRE(total >= 0 && total <= INT32_MAX && cumulative &&
+                 (total == 0 || (keys && values && positions)),
+             "Invalid packed buffers");
+  LR_REQUIRE(((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) % 16) == 0,
+             "Packed buffers must be 16-byte aligned");
+  SumArgs sums{};
+  sums.cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
+  sums.segments = segments;
+  sums.cumulative = cumulative;
+  hipLaunchKernelGGL(paged_sum_kernel, dim3(1), dim3(kSumThreads), 0, as_stream(stream), sums);
+  if (int status = check_launch("paged_read lengths")) return status;
+  if (total == 0) return LR_OK;
+  const ReadArgs args{sums.cache, segments, total, cumulative, keys, values, positions};
+  const int64_t blocks = ceil_div(total, kThreads / (dim / 8));
+  return dispatch_type(dtype, [&]<typename T>() {
+    return dispatch_dim(dim, [&]<int D>() {
+      hipLaunchKernelGGL((paged_read_kernel<T, D>), dim3(static_cast<unsigned>(blocks)),
+                         dim3(kThreads), 0, as_stream(stream), args);
+      return check_launch("paged_read");
+    });
+  });
+}
+
+extern "C" size_t lr_paged_compact_workspace_bytes(int64_t segments) {
+  return segments > 0 ? static_cast<size_t>(2 * segments) * sizeof(int64_t) : 0;
+}
+
+extern "C" int lr_paged_compact(void* pages, int64_t page_count, int64_t page_size,
+                                const int32_t* table, int64_t max_pages, const int32_t* lengths,
+                                int64_t segments, int64_t dim, const int64_t* removed,
+                                int64_t removed_count, const int32_t* target, int64_t target_pages,
+                                int32_t* new_lengths, void* workspace, size_t workspace_size,
+                                void* stream) {
+  clear_error();
+  if (int status = check_paged(pages, page_count, page_size, dim, table, max_pages, lengths, segments))
+    return status;
+  LR_REQUIRE(removed_count >= 0 && (removed_count == 0 || removed) && new_lengths &&
+                 target_pages >= 0 && target_pages <= INT32_MAX / 2 / page_size &&
+                 (target || target_pages == 0),
+             "Invalid compaction");
+  LR_REQUIRE(workspace && workspace_size >= lr_paged_compact_workspace_bytes(segments) &&
+                 reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+             "Compaction workspace too small");
+  SumArgs sums{};
+  sums.cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
+  sums.segments = segments;
+  sums.removed = removed;
+  sums.removed_count = removed_count;
+  sums.starts = static_cast<int64_t*>(workspace);
+  sums.first_rows = sums.starts + segments;
+  sums.new_lengths = new_lengths;
+  hipLaunchKernelGGL(paged_sum_kernel, dim3(1), dim3(kSumThreads), 0, as_stream(stream), sums);
+  if (int status = check_launch("paged_compact lengths")) return status;
+  CompactArgs args{};
+  args.cache = sums.cache;
+  args.segments = segments;
+  // rows that a segment can keep: what both tables hold
+  const int64_t rows = std::min(max_pages, target_pages) * page_size;
+  if (rows == 0) return LR_OK;
+  args.chunks = static_cast<int>(ceil_div(rows, 64));
+  args.target = target;
+  args.target_pages = static_cast<int>(target_pages);
+  args.removed = removed;
+  args.removed_count = removed_count;
+  args.starts = sums.starts;
+  args.first_rows = sums.first_rows;
+  args.new_lengths = new_lengths;
+  const int64_t blocks = ceil_div(segments * args.chunks, kThreads / 64);
+  LR_REQUIRE(blocks < (int64_t{1} << 31), "Compaction grid too large");
+  return dispatch_dim(dim, [&]<int D>() {
+    hipLaunchKernelGGL((paged_compact_kernel<D>), dim3(static_cast<unsigned>(blocks)),
+                       dim3(kThreads), 0, as_stream(stream), args);
+    return check_launch("paged_compact");
+  });
+}

@@ -528,6 +528,85 @@ int lr_packed_attention_noalloc(const void* queries, int64_t q_batch_stride,
                                 int64_t max_keys, float scale, void* out, void* stream);
 
 /* ---------------------------------------------------------------------------------------
+ * A paged KV cache held in 4 bits. No counterpart in the reference, whose cache is packed 16-bit
+ * rows: these are the append (cache.py:33-52), the attention (attention.py:15-35), the row
+ * compaction (cache.py:157-161) and the way back to packed rows for a cache of a quarter of the
+ * size, appended to in place.
+ *
+ * Layout. Segment s = request b * kv_heads + KV head h. Its row i lies in page
+ * table[s * max_pages + i / page_size], slot i % page_size; it has lengths[s] rows (clamped to
+ * [0, max_pages * page_size]). A page is lr_paged_page_bytes(page_size, dim) bytes: the keys'
+ * codes [page_size, dim / 2], the values' codes, the keys' scales [page_size, dim / 32], the
+ * values' scales, the rows' positions (f32). Channels 32 k .. 32 k + 31 of a row form a block of
+ * OCP MX FP4: E2M1 codes (the even channel in the low nibble) times 2^(scale - 127); scale 255:
+ * the block is NaN. A block's scale is the largest power of two X with 4 X <= amax, doubled where
+ * amax >= 7 X, and codes round to the nearest value, ties to the even code. Blocks with a
+ * non-finite element are stored as NaN. X stays within [2^-125, 2^125], or [2^-23, 2^13] for rows
+ * appended as f16, so that every value is exact in that type (larger magnitudes saturate, smaller
+ * round to 0). page_size in {16, 32, 64, 128, 256}, dim in {64, 128, 256}. Page ids outside
+ * [0, page_count) do not exist: their rows are not written, not read (lr_paged_read leaves the
+ * output rows unwritten) and not attended to. Pages may be shared by segments that only read
+ * them. All arrays are device arrays but the strides (three element strides, of the batch, head
+ * and row dimensions, in host memory).
+ * ------------------------------------------------------------------------------------- */
+
+/* Bytes of a page (host only); 0 for a page size or head dimension outside the lists above. */
+int64_t lr_paged_page_bytes(int64_t page_size, int64_t dim);
+
+/* Stores rows i < counts[b] (i < added without counts) of keys/values [batch, kv_heads, added, dim]
+ * as rows lengths[s] + i of their segments; lengths stay as they are (the caller adds the counts
+ * once the step is done). With tables, the first 2 * half channels of a key are rotated first, in
+ * pairs (c, c + half), by the angles whose cosines and sines are rows positions[b * added + i] of
+ * cos/sin f32 [table_rows, half] (half a multiple of 8), in f32; a position outside the tables
+ * gives NaN. half = 0: no rotation. queries [batch, query_heads, added, dim] (or NULL) are rotated
+ * as well, all rows, into out_queries (contiguous, rounded once). positions i64 [batch, added] are
+ * kept with the rows, as f32. dtype: LR_DTYPE_BF16, _F16 or _F32; operands 16-byte aligned, the
+ * last dimension contiguous. Rows past the table's end are not stored. One launch. */
+int lr_paged_append(const void* keys, const int64_t* key_strides, const void* values,
+                    const int64_t* value_strides, const void* queries,
+                    const int64_t* query_strides, void* out_queries, int64_t batch,
+                    int64_t kv_heads, int64_t query_heads, int64_t added, int64_t dim, int dtype,
+                    const int64_t* positions, const float* cos, const float* sin,
+                    int64_t table_rows, int64_t half, const int32_t* counts, void* pages,
+                    int64_t page_count, int64_t page_size, const int32_t* table, int64_t max_pages,
+                    const int32_t* lengths, void* stream);
+
+/* Attention of a step's queries [batch, kv_heads * groups, length, dim] (bf16 or f16) over each
+ * segment's lengths[s] rows and the rows appended behind them in this step: query i < counts[b]
+ * (i < length without counts) sees rows j <= lengths[s] + i; other queries, and those that see no
+ * row, give zeros. out [batch, length, kv_heads * groups, dim], contiguous. max_keys bounds
+ * lengths[s] + length (rows at or past it are not visited). scale is positive. Products, softmax
+ * and sums are f32 (the probabilities enter as exact sums of bf16 pieces). workspace: as for
+ * lr_packed_attention; 0 bytes and one launch when the keys are not split. */
+size_t lr_paged_attention_workspace_bytes(int64_t segments, int64_t groups, int64_t length,
+                                          int64_t max_keys, int64_t dim);
+int lr_paged_attention(const void* queries, const int64_t* query_strides, const void* pages,
+                       int64_t page_count, int64_t page_size, const int32_t* table,
+                       int64_t max_pages, const int32_t* lengths, int64_t batch, int64_t kv_heads,
+                       int64_t groups, int64_t length, int64_t dim, int dtype, int64_t max_keys,
+                       const int32_t* counts, float scale, void* out, void* workspace,
+                       size_t workspace_size, void* stream);
+
+/* The rows the cache stands for, packed by segment: keys/values [total, dim] (bf16, f16 or f32),
+ * positions f32 [total], cumulative i32 [segments + 1] (the packed layout's cu_seqlens_k). Rows
+ * at or past `total` are dropped; output rows past the last segment's are left as they are. */
+int lr_paged_read(const void* pages, int64_t page_count, int64_t page_size, const int32_t* table,
+                  int64_t max_pages, const int32_t* lengths, int64_t segments, int64_t dim,
+                  int dtype, int64_t total, void* keys, void* values, float* positions,
+                  int32_t* cumulative, void* stream);
+
+/* Moves the rows that stay, in order, to the pages of `target` [segments, target_pages], which
+ * share none with `table`; removed: i64, sorted, unique row numbers in the packed order of
+ * lr_paged_read. new_lengths [segments]: the rows that stay. Rows past the target table's end are
+ * dropped, and table, lengths and the source pages stay as they are. */
+size_t lr_paged_compact_workspace_bytes(int64_t segments);
+int lr_paged_compact(void* pages, int64_t page_count, int64_t page_size, const int32_t* table,
+                     int64_t max_pages, const int32_t* lengths, int64_t segments, int64_t dim,
+                     const int64_t* removed, int64_t removed_count, const int32_t* target,
+                     int64_t target_pages, int32_t* new_lengths, void* workspace,
+                     size_t workspace_size, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Audit vector-Jacobian helpers (the margin objective and its gradients)
  * ------------------------------------------------------------------------------------- */
 
