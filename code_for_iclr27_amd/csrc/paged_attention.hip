@@ -109,7 +109,8 @@ __device__ __forceinline__ int value_swizzle(int row) {
   return quarter << 2 ^ ((group & 1) << 1 | group >> 1);
 }
 
-// Codes and scales of a unit: two blocks of 16 rows, a lane's words of one row each.
+// Codes and scales of a unit: two blocks of 16 rows, a lane's words of one row each. Words 4 h ..
+// 4 h + 3 (d256: h = 0, 1; else all) belong to one block of channels.
 template <int D>
 struct UnitCodes {
   static constexpr int kWords = D / 32, kBytes = D == 256 ? 2 : 1;
@@ -136,22 +137,31 @@ __device__ __forceinline__ int word_chunk(int j, int w) {
   return D == 64 ? 2 * j + w : 16 * (w >> 2) + 4 * j + (w & 3);
 }
 
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <typename T, int D, int NT>
-__global__ __launch_bounds__(kAttnThreads, D == 256 || NT == 4 ? 2 : 3) void paged_attention_kernel(
-    PagedAttnArgs a) {
+__global__ __launch_bounds__(kAttnThreads) __attribute__((amdgpu_waves_per_eu(
+    D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : D * NT <= 256 ? 2 : 1))) void paged_attention_kernel(PagedAttnArgs a) {
   using Vec = AttnVec<T>;
   using X8 = typename Vec::x8;
   using Codes = UnitCodes<D>;
   constexpr int KW = D / 32, DT = D / 16;
   constexpr int kRows = 16 * NT;
-  __shared__ __align__(1024) uint16_t v_lds[kAttnWaves][kUnit * D];
+  constexpr int DH = D == 256 ? 128 : D;  // channels of V in LDS at a time
+  constexpr int kHalves = D / DH, kHalfWords = DH / 32;
+  __shared__ __align__(1024) uint16_t v_lds[kAttnWaves][kUnit * DH];
   __shared__ float wave_ml[kAttnWaves][16][2];
 
   const int lane = threadIdx.x & 63, m = lane & 15, j = lane >> 4;
   const int wave = static_cast<int>(wave_index());
   const unsigned unit = blockIdx.x / a.splits, split = blockIdx.x - unit * a.splits;
   const unsigned seg = unit / a.tiles, tile = unit - seg * a.tiles;
-  const unsigned rows = static_cast<unsigned>(a.length) * static_cast<unsigned>(a.groups);
+  const unsigned groups = static_cast<unsigned>(a.groups);
+  const unsigned rows = static_cast<unsigned>(a.length) * groups;
   const unsigned row0 = tile * kRows;
   const int rows_here = static_cast<int>(min(rows - row0, static_cast<unsigned>(kRows)));
   const TileKeys keys = tile_keys(a, seg, row0, row0 + rows_here - 1);
@@ -176,16 +186,15 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 || NT == 4 ? 2 : 3) void pag
   for (int t = 0; t < NT; ++t) {
     const bool valid = 16 * t + m < rows_here;
     const unsigned row = row0 + (valid ? 16 * t + m : 0);
-    const unsigned i = row / static_cast<unsigned>(a.groups), g = row - i * a.groups;
+    const unsigned i = row / groups, g = row - i * groups;
     const unsigned b = seg / static_cast<unsigned>(a.kv_heads), h = seg - b * a.kv_heads;
     limit[t] = valid && static_cast<int>(i) < keys.count
                    ? min(keys.cached + static_cast<int>(i), keys.key_end - 1) : -1;
     const T* p = static_cast<const T*>(a.queries) + b * a.q_batch +
-                 static_cast<int64_t>(h * a.groups + g) * a.q_head + i * a.q_query;
+                 static_cast<int64_t>(h * groups + g) * a.q_head + i * a.q_query;
 #pragma unroll
     for (int w = 0; w < KW; ++w) q[t][w] = __builtin_bit_cast(X8, load16(p + 8 * word_chunk<D>(j, w)));
   }
-  const unsigned groups = static_cast<unsigned>(a.groups);
   const int all_see = static_cast<int>((row0 + rows_here - 1) / groups) < keys.count
                           ? min(keys.cached + static_cast<int>(row0 / groups), keys.key_end - 1)
                           : -1;
@@ -201,189 +210,205 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 || NT == 4 ? 2 : 3) void pag
     const int id = table[min(key, keys.key_end - 1) >> cache.shift];
     return id >= 0 && id < cache.page_count ? id : -1;
   };
+  // A page and a slot are the wave's, so addresses are scalar but for the lane's place in 16 rows.
+  const unsigned lane_codes = m * Page<D>::kCodes + (D == 64 ? 8 : 16) * j;
+  const unsigned lane_scale = m * Page<D>::kScales + (D == 64 ? j >> 1 : j);
   auto load = [&](Codes& u, int key0, int id0, int id1) {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
       const int id = blk == 0 ? id0 : id1;
-      const int slot = ((key0 + 16 * blk) & mask) + m;
-      const uint8_t* page = cache.pages + (id < 0 ? 0 : id) * page_bytes;
-      const int at = D == 64 ? 8 * j : 16 * j;
-      load_codes<D>(u.k[blk], page + Page<D>::codes(cache.shift, 0, slot) + at);
-      load_codes<D>(u.v[blk], page + Page<D>::codes(cache.shift, 1, slot) + at);
-      const int block = D == 64 ? j >> 1 : j;
+      const int slot = (key0 + 16 * blk) & mask;
+      const uint8_t* page = reinterpret_cast<const uint8_t*>(
+          uniform_address(cache.pages + (id < 0 ? 0 : id) * page_bytes));
+      load_codes<D>(u.k[blk], page + Page<D>::codes(cache.shift, 0, slot) + lane_codes);
+      load_codes<D>(u.v[blk], page + Page<D>::codes(cache.shift, 1, slot) + lane_codes);
 #pragma unroll
       for (int i = 0; i < Codes::kBytes; ++i) {
-        u.ks[blk][i] = page[Page<D>::scales(cache.shift, 0, slot) + block + 4 * i];
-        u.vs[blk][i] = page[Page<D>::scales(cache.shift, 1, slot) + block + 4 * i];
+        u.ks[blk][i] = page[Page<D>::scales(cache.shift, 0, slot) + 4 * i + lane_scale];
+        u.vs[blk][i] = page[Page<D>::scales(cache.shift, 1, slot) + 4 * i + lane_scale];
       }
     }
   };
 
   float reference[NT], sum[NT];  // in exponents of two; a row's reference is the same in its four lanes
   attn_f32x4 out[NT][DT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    reference[t] = kNegInf, sum[t] = 0.0f;
-#pragma unroll
-    for (int ct = 0; ct < DT; ++ct) out[t][ct] = attn_f32x4{0.f, 0.f, 0.f, 0.f};
-  }
   char* const my_values = reinterpret_cast<char*>(&v_lds[wave][0]);
   uint32_t read_at;  // of the lane's transposed reads: row 4 j + m / 4, columns 4 (m % 4) .. + 3
   {
     const int row = 4 * j + (m >> 2), chunk = (m & 3) >> 1;
-    read_at = lds_address(my_values) + row * (2 * D) + 16 * (chunk ^ value_swizzle<D>(row)) + 8 * (m & 1);
+    read_at = lds_address(my_values) + row * (2 * DH) + 16 * (chunk ^ value_swizzle<DH>(row)) +
+              8 * (m & 1);
   }
+  auto write_values = [&](const Codes& u, int half) {
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      char* row = my_values + (16 * blk + m) * (2 * DH);
+#pragma unroll
+      for (int w = 0; w < kHalfWords; ++w)
+        *reinterpret_cast<attn_u32x4*>(row + 16 * (word_chunk<DH>(j, w) ^ value_swizzle<DH>(m))) =
+            expand8<__bf16>(u.v[blk][kHalfWords * half + w],
+                            scale_of(u.vs[blk][Codes::kBytes == 2 ? half : 0]));
+    }
+  };
 
-  auto compute = [&](Codes& u, int key0, int id0, int id1) {
-    // rows that are not there: no score, zeros for V
-    if (key0 + kUnit > keys.key_end || id0 < 0 || id1 < 0) {
+  // The wave's units of the chunk. SAFE: blocks of V that read as NaN are kept out of the product
+  // and added to the rows that see their key.
+  auto pass = [&]<bool SAFE>() {
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
-        const bool there = key0 + 16 * blk + m < keys.key_end && (blk == 0 ? id0 : id1) >= 0;
+    for (int t = 0; t < NT; ++t) {
+      reference[t] = kNegInf, sum[t] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < KW; ++w) u.v[blk][w] = there ? u.v[blk][w] : 0u;
-#pragma unroll
-        for (int i = 0; i < Codes::kBytes; ++i) u.vs[blk][i] = there ? u.vs[blk][i] : 127u;
-      }
+      for (int ct = 0; ct < DT; ++ct) out[t][ct] = attn_f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // blocks of V that read as NaN
-    uint64_t poison[2][Codes::kBytes];
-    bool poisoned = false;
+    int key = begin + kUnit * wave;
+    if (key >= end) return;
+    Codes u;
+    int id0 = page_id(key), id1 = page_id(key + 16);
+    load(u, key, id0, id1);
+    while (true) {
+      const bool more = key + kStep < end;
+      const int next0 = page_id(key + kStep), next1 = page_id(key + kStep + 16);
+      if (key + kUnit > keys.key_end || id0 < 0 || id1 < 0) {  // rows that are not there: zeros for V
 #pragma unroll
-    for (int blk = 0; blk < 2; ++blk)
+        for (int blk = 0; blk < 2; ++blk) {
+          const bool there = key + 16 * blk + m < keys.key_end && (blk == 0 ? id0 : id1) >= 0;
 #pragma unroll
-      for (int i = 0; i < Codes::kBytes; ++i) {
-        poison[blk][i] = __ballot(u.vs[blk][i] == kScaleNaN);
-        poisoned = poisoned || poison[blk][i] != 0;
+          for (int w = 0; w < KW; ++w) u.v[blk][w] = there ? u.v[blk][w] : 0u;
+#pragma unroll
+          for (int i = 0; i < Codes::kBytes; ++i) u.vs[blk][i] = there ? u.vs[blk][i] : 127u;
+        }
       }
-    if (poisoned) {
+      if constexpr (SAFE) {
+#pragma unroll 1
+        for (int left = 0; left < kUnit; ++left) {
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
+          for (int i = 0; i < Codes::kBytes; ++i)
 #pragma unroll
-        for (int i = 0; i < Codes::kBytes; ++i)
-          if (u.vs[blk][i] == kScaleNaN) {
-            u.vs[blk][i] = 127u;
+            for (int b = 0; b < 4; ++b) {  // the lane that holds block b + 4 i of row `left`
+              const int from = (D == 64 ? 2 * b : b) * 16 + (left & 15);
+              if (D == 64 && b >= 2) continue;
+              const unsigned byte = __shfl(left < 16 ? u.vs[0][i] : u.vs[1][i], from);
+              if (byte != kScaleNaN) continue;
 #pragma unroll
-            for (int w = 0; w < KW / Codes::kBytes; ++w) u.v[blk][i * (KW / Codes::kBytes) + w] = 0u;
-          }
+              for (int t = 0; t < NT; ++t)
+                if (key + left <= limit[t])
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-        for (int i = 0; i < Codes::kBytes; ++i)
-          for (uint64_t left = poison[blk][i]; left != 0; left &= left - 1) {
-            const int bit = __builtin_ctzll(left), key = key0 + 16 * blk + (bit & 15);
-            const int block = (D == 64 ? bit >> 5 : bit >> 4) + 4 * i;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              const float add = key <= limit[t] ? __builtin_nanf("") : 0.0f;
-#pragma unroll
-              for (int ct = 0; ct < DT; ++ct)
-                if (ct / 2 == block)
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) out[t][ct][r] += add;
+                  for (int r = 0; r < 4; ++r) {
+                    out[t][2 * (b + 4 * i)][r] = __builtin_nanf("");
+                    out[t][2 * (b + 4 * i) + 1][r] = __builtin_nanf("");
+                  }
             }
-          }
-    }
-    // V rows to LDS (the last unit's reads are done: a wave's LDS accesses stay in order)
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
-      char* row = my_values + (16 * blk + m) * (2 * D);
-#pragma unroll
-      for (int w = 0; w < KW; ++w)
-        *reinterpret_cast<attn_u32x4*>(row + 16 * (word_chunk<D>(j, w) ^ value_swizzle<D>(m))) =
-            expand8<__bf16>(u.v[blk][w], scale_of(u.vs[blk][w / 4]));
-    }
-    // S^T
-    attn_f32x4 s[NT][2];
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) s[t][blk] = attn_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        const X8 k = __builtin_bit_cast(X8, expand8<T>(u.k[blk][w], scale_of(u.ks[blk][w / 4])));
-#pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][blk] = Vec::mfma(k, q[t][w], s[t][blk]);
-      }
-    }
-    if (key0 + kUnit - 1 > all_see || id0 < 0 || id1 < 0) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
+        }
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (key0 + 16 * blk + 4 * j + r > limit[t] || (blk == 0 ? id0 : id1) < 0)
-              s[t][blk][r] = kNegInf;
-    }
-    attn_u32x4 piece[NT][3];
+          for (int i = 0; i < Codes::kBytes; ++i)
+            if (u.vs[blk][i] == kScaleNaN) {
+              u.vs[blk][i] = 127u;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float top = kNegInf;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) top = fmaxf(fmaxf(top, s[t][0][r]), s[t][1][r]);
-      LanePair pair = lane_pair<16>(top);
-      pair = lane_pair<32>(fmaxf(pair.first, pair.second));
-      top = fmaxf(pair.first, pair.second) * a.to_log2;
-      if (__any(top > reference[t] + kPagedSlack)) {
-        const float raised = fmaxf(reference[t], top);
-        const float factor =
-            reference[t] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(reference[t] - raised);
-        sum[t] *= factor;
-#pragma unroll
-        for (int ct = 0; ct < DT; ++ct)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) out[t][ct][r] *= factor;
-        reference[t] = raised;
+              for (int w = 0; w < KW / Codes::kBytes; ++w) u.v[blk][i * 4 + w] = 0u;
+            }
       }
-      const float base = reference[t] == kNegInf ? 0.0f : reference[t];
-      float p[8];
+      // V rows to LDS (the last unit's reads are done: a wave's LDS accesses stay in order)
+      write_values(u, 0);
+      // S^T
+      attn_f32x4 s[NT][2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], a.to_log2, -base));
-        sum[t] += p[e];
+      for (int blk = 0; blk < 2; ++blk) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][blk] = attn_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          const X8 k = __builtin_bit_cast(
+              X8, expand8<T>(u.k[blk][w], scale_of(u.ks[blk][Codes::kBytes == 2 ? w / 4 : 0])));
+#pragma unroll
+          for (int t = 0; t < NT; ++t) s[t][blk] = Vec::mfma(k, q[t][w], s[t][blk]);
+        }
       }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) split_bf16(p[2 * w], p[2 * w + 1], piece[t], w);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    // O^T += V^T P^T
-#pragma unroll
-    for (int ct = 0; ct < DT; ++ct) {
-      const uint32_t at = read_at ^ (32 * ct);
-      auto read = [&](uint32_t p) {
-        return __builtin_bit_cast(paged_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) paged_s16x4*)(uintptr_t)p));
-      };
-      const paged_u32x2 lo = read(at), hi = read(at + 16 * (2 * D));
-      const attn_bf16x8 v = __builtin_bit_cast(attn_bf16x8, attn_u32x4{lo[0], lo[1], hi[0], hi[1]});
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
+      Codes here;  // d256: the second half's codes of V outlive the next unit's loads
+      if constexpr (kHalves == 2) here = u;
+      if (more) load(u, key + kStep, next0, next1);
+      if (key + kUnit - 1 > all_see || id0 < 0 || id1 < 0) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-          out[t][ct] = AttnVec<__bf16>::mfma(v, __builtin_bit_cast(attn_bf16x8, piece[t][i]), out[t][ct]);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  };
-
-  // The wave's units, the next one's codes loaded while one is worked on.
-  int key = begin + kUnit * wave;
-  if (key < end) {
-    Codes now, next;
-    int id0 = page_id(key), id1 = page_id(key + 16);
-    load(now, key, id0, id1);
-    for (; key < end; key += kStep) {
-      const int next0 = page_id(key + kStep), next1 = page_id(key + kStep + 16);
-      load(next, key + kStep, next0, next1);
-      compute(now, key, id0, id1);
-      now = next;
+#pragma unroll
+          for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (key + 16 * blk + 4 * j + r > limit[t] || (blk == 0 ? id0 : id1) < 0)
+                s[t][blk][r] = kNegInf;
+      }
+      attn_u32x4 piece[NT][3];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float top = kNegInf;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(fmaxf(top, s[t][0][r]), s[t][1][r]);
+        LanePair pair = lane_pair<16>(top);
+        pair = lane_pair<32>(fmaxf(pair.first, pair.second));
+        top = fmaxf(pair.first, pair.second) * a.to_log2;
+        if (__any(top > reference[t] + kPagedSlack)) {
+          const float raised = fmaxf(reference[t], top);
+          const float factor =
+              reference[t] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(reference[t] - raised);
+          sum[t] *= factor;
+#pragma unroll
+          for (int ct = 0; ct < DT; ++ct)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) out[t][ct][r] *= factor;
+          reference[t] = raised;
+        }
+        const float base = reference[t] == kNegInf ? 0.0f : reference[t];
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], a.to_log2, -base));
+          sum[t] += p[e];
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) split_bf16(p[2 * w], p[2 * w + 1], piece[t], w);
+      }
+      // O^T += V^T P^T
+#pragma unroll
+      for (int half = 0; half < kHalves; ++half) {
+        if (half > 0) {
+          wave_fence();
+          if constexpr (kHalves == 2) write_values(here, 1);
+        }
+        wave_fence();
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c) {
+          const uint32_t at = read_at ^ (32 * c);
+          auto read = [&](uint32_t p) {
+            return __builtin_bit_cast(paged_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) paged_s16x4*)(uintptr_t)p));
+          };
+          const paged_u32x2 lo = read(at), hi = read(at + 16 * (2 * DH));
+          const attn_bf16x8 v = __builtin_bit_cast(attn_bf16x8, attn_u32x4{lo[0], lo[1], hi[0], hi[1]});
+          const int ct = DH / 16 * half + c;
+#pragma unroll
+          for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              out[t][ct] = AttnVec<__bf16>::mfma(v, __builtin_bit_cast(attn_bf16x8, piece[t][i]), out[t][ct]);
+        }
+      }
+      wave_fence();
+      if (!more) break;
+      key += kStep;
       id0 = next0, id1 = next1;
     }
-  }
+  };
+  pass.template operator()<false>();
+  // 0 * NaN is NaN: a wave with a sum that is not finite takes its keys again.
+  float poison = 0.0f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int ct = 0; ct < DT; ++ct)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) poison = __builtin_fmaf(out[t][ct][r], 0.0f, poison);
+  if (__any(poison != poison)) pass.template operator()<true>();
 
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -391,24 +416,25 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 || NT == 4 ? 2 : 3) void pag
     pair = lane_pair<32>(pair.first + pair.second);
     sum[t] = pair.first + pair.second;
   }
-  // Wave states to LDS, a tile of 16 rows at a time: 16-byte chunk c of row r in slot c ^ r.
-  constexpr int kItems = 16 * (D / 8);
+  // Wave states to LDS, 16 rows and DH channels at a time: 16-byte chunk c of row r in slot c ^ r.
+  constexpr int kItems = 16 * (DH / 8);
   const int64_t slot = (static_cast<int64_t>(unit) * a.splits + split) * a.tile_rows;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
+  for (int step = 0; step < NT * kHalves; ++step) {
+    const int t = step / kHalves, half = step % kHalves;
     if (16 * t >= rows_here) break;
     __syncthreads();
-    float* const mine = reinterpret_cast<float*>(my_values) + m * D;
+    float* const mine = reinterpret_cast<float*>(my_values) + m * DH;
 #pragma unroll
-    for (int ct = 0; ct < DT; ++ct)
-      *reinterpret_cast<attn_f32x4*>(mine + 4 * ((4 * ct + j) ^ m)) = out[t][ct];
-    if (j == 0) {
+    for (int c = 0; c < DH / 16; ++c)
+      *reinterpret_cast<attn_f32x4*>(mine + 4 * ((4 * c + j) ^ m)) = out[t][DH / 16 * half + c];
+    if (j == 0 && half == 0) {
       wave_ml[wave][m][0] = reference[t];
       wave_ml[wave][m][1] = sum[t];
     }
     __syncthreads();
     for (int item = threadIdx.x; item < kItems; item += kAttnThreads) {
-      const int r = item / (D / 8), c = item - r * (D / 8);
+      const int r = item / (DH / 8), c = item - r * (DH / 8);
       if (16 * t + r >= rows_here) break;
       float top = kNegInf, total = 0.0f, o[8] = {};
 #pragma unroll
@@ -419,7 +445,7 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 || NT == 4 ? 2 : 3) void pag
         const float weight =
             wave_ml[w][r][0] == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(wave_ml[w][r][0] - top);
         total = __builtin_fmaf(weight, wave_ml[w][r][1], total);
-        const float* wo = reinterpret_cast<const float*>(&v_lds[w][0]) + r * D;
+        const float* wo = reinterpret_cast<const float*>(&v_lds[w][0]) + r * DH;
         const attn_f32x4 lo = *reinterpret_cast<const attn_f32x4*>(wo + 4 * ((2 * c) ^ r));
         const attn_f32x4 hi = *reinterpret_cast<const attn_f32x4*>(wo + 4 * ((2 * c + 1) ^ r));
 #pragma unroll
@@ -428,17 +454,18 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 || NT == 4 ? 2 : 3) void pag
           o[4 + e] = __builtin_fmaf(weight, hi[e], o[4 + e]);
         }
       }
+      const int channel = DH * half + 8 * c;
       if (keys.needed == 1) {
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] *= inv;
-        *reinterpret_cast<attn_u32x4*>(paged_output<T, D>(a, seg, row0 + 16 * t + r) + 8 * c) =
+        *reinterpret_cast<attn_u32x4*>(paged_output<T, D>(a, seg, row0 + 16 * t + r) + channel) =
             pack8<T>(o);
       } else {
-        float* po = a.part_o + (slot + 16 * t + r) * D + 8 * c;
+        float* po = a.part_o + (slot + 16 * t + r) * D + channel;
         *reinterpret_cast<attn_f32x4*>(po) = attn_f32x4{o[0], o[1], o[2], o[3]};
         *reinterpret_cast<attn_f32x4*>(po + 4) = attn_f32x4{o[4], o[5], o[6], o[7]};
-        if (c == 0) {
+        if (channel == 0) {
           a.part_ml[(slot + 16 * t + r) * 2] = top;
           a.part_ml[(slot + 16 * t + r) * 2 + 1] = total;
         }
