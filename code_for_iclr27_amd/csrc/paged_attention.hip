@@ -3,25 +3,38 @@
 // i + 1 of those appended behind them (counts[b], or `length`, rows): keys j <= lengths[s] + i.
 // Queries at or past counts[b] output zeros, as does a query that sees no key.
 //
-// Work split: row = i * G + g numbers a segment's query rows; a workgroup of four waves owns a tile
-// of 16 * NT rows and a chunk of keys, each wave every fourth unit of 32 keys. Codes go from memory
-// to registers (16 bytes a lane: a block of one row), the conversion instruction makes them 16-bit
+// Work split: row = i * G + g numbers a segment's query rows; a workgroup of four (eight) waves owns a
+// tile of 16 rows and a chunk of keys, each wave every fourth (eighth) unit of 32 keys. Calls of many
+// rows take tiles of 32 (paged_tile_kernel); plan_paged has the rules. Codes go from memory to
+// registers (16 bytes a lane: a block of one row), the conversion instruction makes them 16-bit
 // values, and both products run on v_mfma_f32_16x16x32:
 //   S^T = K Q^T   A: 16 keys, a lane's eight channels of one key. The contraction's channel order is
 //                 free, so a lane's block stays where it was loaded. A lane gets one query's scores
 //                 of 4 + 4 keys.
 //   O^T += V^T P^T  B: the probabilities where S^T left them (the key order is free as well); A: the
 //                 same keys of one channel, read transposed from the wave's V rows in LDS.
-// The values are exact in the 16-bit type, and P (f32) enters as a sum of three bf16 pieces, 3 x 8
-// bits by truncation, whose products with V are exact: scores, probabilities, sums and outputs are
-// f32 throughout and only the output is rounded.
+// The values are exact in the 16-bit type. P enters as the sum of two bf16 pieces, whose products
+// with V are exact: 8 bits by truncation and 8 of the rest by rounding, within 2^-17 of P and without
+// a bias, against an output step of 2^-8 or 2^-11 (a third piece, all of P's bits, cost a third more
+// products: 1000 queries onto 4,000 rows 158 us against 136). Scores, exponentials, their sum and the
+// products' sums are f32 throughout.
 //
-// The exponentials' reference moves when a row's maximum has outgrown it by 2^kSlack (the tile
-// kernel of attention_tile.hip does the same). The waves' states meet in LDS; tiles whose keys span
-// several chunks leave partial states, which a second launch merges.
+// The exponentials' reference moves when a row's maximum has outgrown it by 2^kPagedSlack (as in
+// attention_tile.hip). The waves' states meet in LDS; tiles whose keys span several chunks leave
+// partial states, which a second launch merges.
 //
-// A masked key contributes nothing: its score becomes -inf, and a block of V that reads as NaN is
-// kept out of the product and added to the rows that see its key (0 * NaN is NaN).
+// A masked key contributes nothing: its score becomes -inf, its P 0. As 0 * NaN is NaN, a wave that
+// ends with a non-finite sum takes its keys again, with the blocks of V that read as NaN kept out of
+// the product and added to the rows that see their key.
+//
+// What bounds it. Decode of a long cache: memory (eight requests of 36k rows, 8 heads, G4, d128: 312 MB
+// of codes in 62 us, 5.0 TB/s; a large copy reaches 5.2). Short ones: the two launches (8 segments of
+// 2,250 rows: 8 us, 2,250 rows of eight requests 11 us). Prefill: the vector instructions, 233 a unit
+// of 32 keys and 32 rows beside 24 MFMAs (a quarter each for the values, the exponentials and the
+// pieces), 71% of a SIMD's issue slots: 1000 queries onto 4,000 rows 128 us, where the packed kernel
+// on the same rows in 16 bits takes 171. Tried and no faster: units in flight two ahead, the
+// exponentials laid between the MFMAs of the last unit's product by hand, a raised wave priority for
+// the products, tiles of 64 rows.
 
 #include <algorithm>
 #include <cmath>
@@ -36,9 +49,11 @@ namespace {
 typedef short paged_s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned paged_u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kUnit = 32;                  // keys of a wave's step
-constexpr int kStep = kUnit * kAttnWaves;  // and of the workgroup's
+constexpr int kUnit = 32;       // keys of a wave's step
+constexpr int kSmallRows = 16;  // rows of a tile: decode and a few query rows
+constexpr int kTileRows = 32;   // many query rows
 constexpr float kPagedSlack = 4.0f;
+constexpr int kPieces = 2;      // of a probability
 
 struct PagedAttnArgs {
   const void* queries;  // element strides below; the last dimension is contiguous
@@ -47,7 +62,7 @@ struct PagedAttnArgs {
   const int32_t* counts;  // [batch] or NULL
   int kv_heads, groups, length;
   int max_keys;           // no key at or past it is visited
-  unsigned tiles, splits;
+  unsigned segments, tiles, splits;
   int tile_rows;          // rows of a tile's partial states
   int chunk;              // keys of a split, a multiple of kStep
   float to_log2;          // scale * log2(e)
@@ -86,17 +101,15 @@ __device__ __forceinline__ T* paged_output(const PagedAttnArgs& a, unsigned seg,
           h * groups + g) * D;
 }
 
-// Two f32 values as sums of three bf16 pieces each, word `w` of the piece vectors: the top halves
-// of x, of x minus that, and of what is left (the differences are exact, the last has 8 bits).
-__device__ __forceinline__ void split_bf16(float x, float y, attn_u32x4 (&piece)[3], int w) {
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    const unsigned a = __builtin_bit_cast(unsigned, x), b = __builtin_bit_cast(unsigned, y);
-    piece[i][w] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-    if (i == 2) break;
-    x -= __builtin_bit_cast(float, a & 0xffff0000u);
-    y -= __builtin_bit_cast(float, b & 0xffff0000u);
-  }
+// Two f32 values as sums of two bf16 pieces each, word `w` of the piece vectors: the top halves of x,
+// and the rest (an exact difference) rounded to nearest.
+__device__ __forceinline__ void split_bf16(float x, float y, attn_u32x4 (&piece)[kPieces], int w) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const unsigned a = __builtin_bit_cast(unsigned, x), b = __builtin_bit_cast(unsigned, y);
+  piece[0][w] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  const bf16x2 rest = {static_cast<__bf16>(x - __builtin_bit_cast(float, a & 0xffff0000u)),
+                       static_cast<__bf16>(y - __builtin_bit_cast(float, b & 0xffff0000u))};
+  piece[1][w] = __builtin_bit_cast(unsigned, rest);
 }
 
 // V rows in LDS: 16-byte chunk c of row r in slot c ^ x(r). Eight lanes that write one chunk of
@@ -109,6 +122,102 @@ __device__ __forceinline__ int value_swizzle(int row) {
   return quarter << 2 ^ ((group & 1) << 1 | group >> 1);
 }
 
+typedef const __attribute__((address_space(4))) int32_t* PageIds;  // read by scalar loads
+__device__ __forceinline__ PageIds page_table(const PagedCache& cache, unsigned seg) {
+  return (PageIds)(cache.table + static_cast<int64_t>(seg) * cache.max_pages);
+}
+
+// A block's segment, tile and split. Consecutive blocks take consecutive segments, so with 8 segments
+// (or a divisor or multiple of it) each XCD's L2 serves its own segments' rows (1000 queries onto
+// 4,000 rows: 125 us against 135 with consecutive tiles); within a segment the tiles with the most
+// visible keys come first, so that the launch's tail is short.
+struct Place {
+  unsigned seg, tile, split, unit;
+};
+__device__ __forceinline__ Place block_place(const PagedAttnArgs& a) {
+  Place p;
+  const unsigned rest = blockIdx.x / a.segments;
+  p.seg = blockIdx.x - rest * a.segments;
+  const unsigned back = rest / a.splits;
+  p.split = rest - back * a.splits;
+  p.tile = a.tiles - 1 - back;
+  p.unit = p.seg * a.tiles + p.tile;
+  return p;
+}
+
+__device__ __forceinline__ int rows_of_tile(const PagedAttnArgs& a, unsigned row0, int most) {
+  const unsigned rows = static_cast<unsigned>(a.length) * static_cast<unsigned>(a.groups);
+  return static_cast<int>(min(rows - row0, static_cast<unsigned>(most)));
+}
+
+// A query row: its query and its place (elements) in the queries.
+struct TileRow {
+  int query;
+  int64_t offset;
+};
+__device__ __forceinline__ TileRow tile_row(const PagedAttnArgs& a, unsigned seg, unsigned row) {
+  const unsigned groups = static_cast<unsigned>(a.groups), heads = static_cast<unsigned>(a.kv_heads);
+  const unsigned i = row / groups, g = row - i * groups, b = seg / heads, h = seg - b * heads;
+  return {static_cast<int>(i), b * a.q_batch + static_cast<int64_t>(h * groups + g) * a.q_head + i * a.q_query};
+}
+// The last key that a query sees (-1: none), and the last one that every row of a tile sees.
+__device__ __forceinline__ int last_key(const TileKeys& keys, int query) {
+  return query < keys.count ? min(keys.cached + query, keys.key_end - 1) : -1;
+}
+__device__ __forceinline__ int all_rows_see(const PagedAttnArgs& a, const TileKeys& keys, unsigned row0, int rows) {
+  const unsigned groups = static_cast<unsigned>(a.groups);
+  const int last = static_cast<int>((row0 + rows - 1) / groups);
+  return last < keys.count ? min(keys.cached + static_cast<int>(row0 / groups), keys.key_end - 1) : -1;
+}
+
+// Zeros for rows that see no key.
+template <typename T, int D>
+__device__ __forceinline__ void zero_rows(const PagedAttnArgs& a, unsigned seg, unsigned row0, int rows) {
+  for (int item = threadIdx.x; item < rows * (D / 8); item += blockDim.x) {
+    const int r = item / (D / 8), c = item - r * (D / 8);
+    *reinterpret_cast<attn_u32x4*>(paged_output<T, D>(a, seg, row0 + r) + 8 * c) =
+        attn_u32x4{0u, 0u, 0u, 0u};
+  }
+}
+
+// Eight channels of a row from the waves' states: the output, or (`whole` false) the chunk's partial
+// state at `slot`.
+template <typename T, int D, int WAVES, typename ML, typename State>
+__device__ __forceinline__ void finish_item(const PagedAttnArgs& a, unsigned seg, unsigned row,
+                                            int channel, int64_t slot, bool whole, ML ml, State state) {
+  float top = kNegInf, total = 0.0f, o[8] = {};
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, ml(w, 0));
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const float reference = ml(w, 0), sum = ml(w, 1);
+    attn_f32x4 lo, hi;
+    state(w, lo, hi);
+    if (reference == kNegInf && sum == 0.0f) continue;  // saw no key
+    const float weight = reference == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(reference - top);
+    total = __builtin_fmaf(weight, sum, total);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] = __builtin_fmaf(weight, lo[e], o[e]);
+      o[4 + e] = __builtin_fmaf(weight, hi[e], o[4 + e]);
+    }
+  }
+  if (whole) {
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= inv;
+    *reinterpret_cast<attn_u32x4*>(paged_output<T, D>(a, seg, row) + channel) = pack8<T>(o);
+    return;
+  }
+  float* po = a.part_o + slot * D + channel;
+  *reinterpret_cast<attn_f32x4*>(po) = attn_f32x4{o[0], o[1], o[2], o[3]};
+  *reinterpret_cast<attn_f32x4*>(po + 4) = attn_f32x4{o[4], o[5], o[6], o[7]};
+  if (channel == 0) {
+    a.part_ml[slot * 2] = top;
+    a.part_ml[slot * 2 + 1] = total;
+  }
+}
+
 // Codes and scales of a unit: two blocks of 16 rows, a lane's words of one row each. Words 4 h ..
 // 4 h + 3 (d256: h = 0, 1; else all) belong to one block of channels.
 template <int D>
@@ -117,15 +226,19 @@ struct UnitCodes {
   unsigned k[2][kWords], v[2][kWords], ks[2][kBytes], vs[2][kBytes];
 };
 
+// Memory addressed as a wave-uniform base and a lane's offset. (In the global address space: a generic
+// load also counts as an LDS access, and every wait for LDS would be one for memory.)
+typedef const __attribute__((address_space(1))) uint8_t* PagedBytes;
+
 template <int D>
-__device__ __forceinline__ void load_codes(unsigned (&words)[D / 32], const uint8_t* p) {
+__device__ __forceinline__ void load_codes(unsigned (&words)[D / 32], PagedBytes p) {
   if constexpr (D == 64) {
-    const paged_u32x2 x = *reinterpret_cast<const paged_u32x2*>(p);
+    const paged_u32x2 x = *(const __attribute__((address_space(1))) paged_u32x2*)p;
     words[0] = x[0], words[1] = x[1];
   } else {
 #pragma unroll
     for (int half = 0; half < D / 128; ++half) {
-      const attn_u32x4 x = load16(p + 64 * half);
+      const attn_u32x4 x = *(const __attribute__((address_space(1))) attn_u32x4*)(p + 64 * half);
 #pragma unroll
       for (int e = 0; e < 4; ++e) words[4 * half + e] = x[e];
     }
@@ -137,79 +250,76 @@ __device__ __forceinline__ int word_chunk(int j, int w) {
   return D == 64 ? 2 * j + w : 16 * (w >> 2) + 4 * j + (w & 3);
 }
 
+// Four rows' elements of one column from LDS: lanes 4 k .. 4 k + 3 of each 16 address row k (8 bytes
+// each), lane i receives column i of the 16.
+__device__ __forceinline__ paged_u32x2 read_transposed(uint32_t p) {
+  return __builtin_bit_cast(paged_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) paged_s16x4*)(uintptr_t)p));
+}
+
 __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <typename T, int D, int NT>
-__global__ __launch_bounds__(kAttnThreads) __attribute__((amdgpu_waves_per_eu(
-    D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : D * NT <= 256 ? 2 : 1))) void paged_attention_kernel(PagedAttnArgs a) {
+// Tiles of 16 rows: decode, and a few query rows.
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(
+    WAVES == 8 || D == 256 ? 2 : D == 64 ? 4 : 3)))
+void paged_attention_kernel(PagedAttnArgs a) {
+  constexpr int kStep = kUnit * WAVES;  // keys of the workgroup's step
   using Vec = AttnVec<T>;
   using X8 = typename Vec::x8;
   using Codes = UnitCodes<D>;
   constexpr int KW = D / 32, DT = D / 16;
-  constexpr int kRows = 16 * NT;
   constexpr int DH = D == 256 ? 128 : D;  // channels of V in LDS at a time
   constexpr int kHalves = D / DH, kHalfWords = DH / 32;
-  __shared__ __align__(1024) uint16_t v_lds[kAttnWaves][kUnit * DH];
-  __shared__ float wave_ml[kAttnWaves][16][2];
+  __shared__ __align__(1024) uint16_t v_lds[WAVES][kUnit * DH];
+  __shared__ float wave_ml[WAVES][kSmallRows][2];
+  __shared__ __align__(16) attn_u32x4 q_lds[KW][64];
 
   const int lane = threadIdx.x & 63, m = lane & 15, j = lane >> 4;
   const int wave = static_cast<int>(wave_index());
-  const unsigned unit = blockIdx.x / a.splits, split = blockIdx.x - unit * a.splits;
-  const unsigned seg = unit / a.tiles, tile = unit - seg * a.tiles;
-  const unsigned groups = static_cast<unsigned>(a.groups);
-  const unsigned rows = static_cast<unsigned>(a.length) * groups;
-  const unsigned row0 = tile * kRows;
-  const int rows_here = static_cast<int>(min(rows - row0, static_cast<unsigned>(kRows)));
+  const Place place = block_place(a);
+  const unsigned seg = place.seg, row0 = place.tile * kSmallRows;
+  const int rows_here = rows_of_tile(a, row0, kSmallRows);
+  // The pages of the wave's first unit, looked up beside the segment's length (an entry past the
+  // segment's last page is not used): the two memory round trips overlap.
+  const PagedCache& cache = a.cache;
+  const PageIds table = page_table(cache, seg);
+  auto in_pool = [&](int id) { return id >= 0 && id < cache.page_count ? id : -1; };
+  int first0 = -1, first1 = -1;
+  if (a.max_keys > 0) {
+    const int key = static_cast<int>(place.split) * a.chunk + kUnit * wave;
+    first0 = table[min(key >> cache.shift, cache.max_pages - 1)];
+    first1 = table[min((key + 16) >> cache.shift, cache.max_pages - 1)];
+  }
   const TileKeys keys = tile_keys(a, seg, row0, row0 + rows_here - 1);
-  if (keys.needed == 0) {  // no visible key for any row of this tile: zeros
-    if (split != 0) return;
-    for (int item = threadIdx.x; item < rows_here * (D / 8); item += kAttnThreads) {
-      const int r = item / (D / 8), c = item - r * (D / 8);
-      *reinterpret_cast<attn_u32x4*>(paged_output<T, D>(a, seg, row0 + r) + 8 * c) =
-          attn_u32x4{0u, 0u, 0u, 0u};
-    }
+  if (keys.needed == 0) {  // no visible key for any row of this tile
+    if (place.split == 0) zero_rows<T, D>(a, seg, row0, rows_here);
     return;
   }
-  if (static_cast<int>(split) >= keys.needed) return;  // uniform across the workgroup
-  const int begin = static_cast<int>(split) * a.chunk;
+  if (static_cast<int>(place.split) >= keys.needed) return;  // uniform across the workgroup
+  const int begin = static_cast<int>(place.split) * a.chunk;
   const int end = min(begin + a.chunk, keys.key_end);
+  first0 = in_pool(first0);
+  first1 = in_pool(first1);
 
-  // Queries (B operand: row m of a tile, the channels of word w of lane group j) and the last key
-  // that a lane's rows see; `all_see`: the last one that every row of the workgroup sees.
-  X8 q[NT][KW];
-  int limit[NT];
+  // Queries (B operand: row m, the channels of word w of lane group j) in LDS for every wave, and the
+  // last key that the lane's row sees.
+  const TileRow row = tile_row(a, seg, row0 + (m < rows_here ? m : 0));
+  const int limit = m < rows_here ? last_key(keys, row.query) : -1;
+  const int all_see = all_rows_see(a, keys, row0, rows_here);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const bool valid = 16 * t + m < rows_here;
-    const unsigned row = row0 + (valid ? 16 * t + m : 0);
-    const unsigned i = row / groups, g = row - i * groups;
-    const unsigned b = seg / static_cast<unsigned>(a.kv_heads), h = seg - b * a.kv_heads;
-    limit[t] = valid && static_cast<int>(i) < keys.count
-                   ? min(keys.cached + static_cast<int>(i), keys.key_end - 1) : -1;
-    const T* p = static_cast<const T*>(a.queries) + b * a.q_batch +
-                 static_cast<int64_t>(h * groups + g) * a.q_head + i * a.q_query;
-#pragma unroll
-    for (int w = 0; w < KW; ++w) q[t][w] = __builtin_bit_cast(X8, load16(p + 8 * word_chunk<D>(j, w)));
-  }
-  const int all_see = static_cast<int>((row0 + rows_here - 1) / groups) < keys.count
-                          ? min(keys.cached + static_cast<int>(row0 / groups), keys.key_end - 1)
-                          : -1;
+  for (int w = 0; w < KW; ++w)
+    if (wave == w % WAVES)
+      q_lds[w][lane] = load16(static_cast<const T*>(a.queries) + row.offset + 8 * word_chunk<D>(j, w));
 
-  const PagedCache& cache = a.cache;
-  const __attribute__((address_space(4))) int32_t* table =
-      (const __attribute__((address_space(4))) int32_t*)(cache.table +
-                                                         static_cast<int64_t>(seg) * cache.max_pages);
   const int64_t page_bytes = Page<D>::bytes(1) << cache.shift;
   const int mask = (1 << cache.shift) - 1;
   // Page of 16 rows from `key` on (one page: page sizes are multiples of 16); -1: outside the pool.
-  auto page_id = [&](int key) {
-    const int id = table[min(key, keys.key_end - 1) >> cache.shift];
-    return id >= 0 && id < cache.page_count ? id : -1;
-  };
+  auto page_id = [&](int key) { return in_pool(table[min(key, keys.key_end - 1) >> cache.shift]); };
   // A page and a slot are the wave's, so addresses are scalar but for the lane's place in 16 rows.
   const unsigned lane_codes = m * Page<D>::kCodes + (D == 64 ? 8 : 16) * j;
   const unsigned lane_scale = m * Page<D>::kScales + (D == 64 ? j >> 1 : j);
@@ -218,8 +328,8 @@ __global__ __launch_bounds__(kAttnThreads) __attribute__((amdgpu_waves_per_eu(
     for (int blk = 0; blk < 2; ++blk) {
       const int id = blk == 0 ? id0 : id1;
       const int slot = (key0 + 16 * blk) & mask;
-      const uint8_t* page = reinterpret_cast<const uint8_t*>(
-          uniform_address(cache.pages + (id < 0 ? 0 : id) * page_bytes));
+      const PagedBytes page =
+          (PagedBytes)uniform_address(cache.pages + (id < 0 ? 0 : id) * page_bytes);
       load_codes<D>(u.k[blk], page + Page<D>::codes(cache.shift, 0, slot) + lane_codes);
       load_codes<D>(u.v[blk], page + Page<D>::codes(cache.shift, 1, slot) + lane_codes);
 #pragma unroll
@@ -230,44 +340,42 @@ __global__ __launch_bounds__(kAttnThreads) __attribute__((amdgpu_waves_per_eu(
     }
   };
 
-  float reference[NT], sum[NT];  // in exponents of two; a row's reference is the same in its four lanes
-  attn_f32x4 out[NT][DT];
+  float reference, sum;  // in exponents of two; a row's reference is the same in its four lanes
+  attn_f32x4 out[DT];
   char* const my_values = reinterpret_cast<char*>(&v_lds[wave][0]);
   uint32_t read_at;  // of the lane's transposed reads: row 4 j + m / 4, columns 4 (m % 4) .. + 3
   {
-    const int row = 4 * j + (m >> 2), chunk = (m & 3) >> 1;
-    read_at = lds_address(my_values) + row * (2 * DH) + 16 * (chunk ^ value_swizzle<DH>(row)) +
-              8 * (m & 1);
+    const int r = 4 * j + (m >> 2), chunk = (m & 3) >> 1;
+    read_at = lds_address(my_values) + r * (2 * DH) + 16 * (chunk ^ value_swizzle<DH>(r)) + 8 * (m & 1);
   }
   auto write_values = [&](const Codes& u, int half) {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      char* row = my_values + (16 * blk + m) * (2 * DH);
+      char* to = my_values + (16 * blk + m) * (2 * DH);
 #pragma unroll
       for (int w = 0; w < kHalfWords; ++w)
-        *reinterpret_cast<attn_u32x4*>(row + 16 * (word_chunk<DH>(j, w) ^ value_swizzle<DH>(m))) =
+        *reinterpret_cast<attn_u32x4*>(to + 16 * (word_chunk<DH>(j, w) ^ value_swizzle<DH>(m))) =
             expand8<__bf16>(u.v[blk][kHalfWords * half + w],
                             scale_of(u.vs[blk][Codes::kBytes == 2 ? half : 0]));
     }
   };
 
-  // The wave's units of the chunk. SAFE: blocks of V that read as NaN are kept out of the product
-  // and added to the rows that see their key.
+  // The wave's units of the chunk. SAFE: blocks of V that read as NaN are kept out of the product and
+  // added to the rows that see their key, and no exponential exceeds one.
   auto pass = [&]<bool SAFE>() {
+    reference = kNegInf, sum = 0.0f;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      reference[t] = kNegInf, sum[t] = 0.0f;
-#pragma unroll
-      for (int ct = 0; ct < DT; ++ct) out[t][ct] = attn_f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int ct = 0; ct < DT; ++ct) out[ct] = attn_f32x4{0.f, 0.f, 0.f, 0.f};
     int key = begin + kUnit * wave;
     if (key >= end) return;
     Codes u;
-    int id0 = page_id(key), id1 = page_id(key + 16);
+    int id0 = SAFE ? page_id(key) : first0, id1 = SAFE ? page_id(key + 16) : first1;
     load(u, key, id0, id1);
+    int next0 = page_id(key + kStep), next1 = page_id(key + kStep + 16);
     while (true) {
+      // the unit after the next: its pages' ids arrive while this one is worked on
+      const int later0 = page_id(key + 2 * kStep), later1 = page_id(key + 2 * kStep + 16);
       const bool more = key + kStep < end;
-      const int next0 = page_id(key + kStep), next1 = page_id(key + kStep + 16);
       if (key + kUnit > keys.key_end || id0 < 0 || id1 < 0) {  // rows that are not there: zeros for V
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
@@ -285,18 +393,13 @@ __global__ __launch_bounds__(kAttnThreads) __attribute__((amdgpu_waves_per_eu(
           for (int i = 0; i < Codes::kBytes; ++i)
 #pragma unroll
             for (int b = 0; b < 4; ++b) {  // the lane that holds block b + 4 i of row `left`
-              const int from = (D == 64 ? 2 * b : b) * 16 + (left & 15);
               if (D == 64 && b >= 2) continue;
+              const int from = (D == 64 ? 2 * b : b) * 16 + (left & 15);
               const unsigned byte = __shfl(left < 16 ? u.vs[0][i] : u.vs[1][i], from);
-              if (byte != kScaleNaN) continue;
+              if (byte == kScaleNaN && key + left <= limit)
 #pragma unroll
-              for (int t = 0; t < NT; ++t)
-                if (key + left <= limit[t])
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) {
-                    out[t][2 * (b + 4 * i)][r] = __builtin_nanf("");
-                    out[t][2 * (b + 4 * i) + 1][r] = __builtin_nanf("");
-                  }
+                for (int r = 0; r < 4; ++r)
+                  out[2 * (b + 4 * i)][r] = out[2 * (b + 4 * i) + 1][r] = __builtin_nanf("");
             }
         }
 #pragma unroll
@@ -312,228 +415,445 @@ __global__ __launch_bounds__(kAttnThreads) __attribute__((amdgpu_waves_per_eu(
       // V rows to LDS (the last unit's reads are done: a wave's LDS accesses stay in order)
       write_values(u, 0);
       // S^T
-      attn_f32x4 s[NT][2];
+      attn_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
+      for (int w = 0; w < KW; ++w) {
+        const X8 q = __builtin_bit_cast(X8, q_lds[w][lane]);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][blk] = attn_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < KW; ++w) {
-          const X8 k = __builtin_bit_cast(
-              X8, expand8<T>(u.k[blk][w], scale_of(u.ks[blk][Codes::kBytes == 2 ? w / 4 : 0])));
-#pragma unroll
-          for (int t = 0; t < NT; ++t) s[t][blk] = Vec::mfma(k, q[t][w], s[t][blk]);
-        }
+        for (int blk = 0; blk < 2; ++blk)
+          s[blk] = Vec::mfma(__builtin_bit_cast(X8, expand8<T>(u.k[blk][w], scale_of(
+                                 u.ks[blk][Codes::kBytes == 2 ? w / 4 : 0]))), q, s[blk]);
       }
       Codes here;  // d256: the second half's codes of V outlive the next unit's loads
       if constexpr (kHalves == 2) here = u;
       if (more) load(u, key + kStep, next0, next1);
       if (key + kUnit - 1 > all_see || id0 < 0 || id1 < 0) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-          for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (key + 16 * blk + 4 * j + r > limit[t] || (blk == 0 ? id0 : id1) < 0)
-                s[t][blk][r] = kNegInf;
+          for (int r = 0; r < 4; ++r)
+            if (key + 16 * blk + 4 * j + r > limit || (blk == 0 ? id0 : id1) < 0) s[blk][r] = kNegInf;
       }
-      attn_u32x4 piece[NT][3];
+      float top = kNegInf;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float top = kNegInf;
+      for (int r = 0; r < 4; ++r) top = fmaxf(fmaxf(top, s[0][r]), s[1][r]);
+      LanePair pair = lane_pair<16>(top);
+      pair = lane_pair<32>(fmaxf(pair.first, pair.second));
+      top = fmaxf(pair.first, pair.second) * a.to_log2;
+      if (__any(top > reference + (SAFE ? 0.0f : kPagedSlack))) {
+        const float raised = fmaxf(reference, top);
+        const float factor = reference == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(reference - raised);
+        sum *= factor;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) top = fmaxf(fmaxf(top, s[t][0][r]), s[t][1][r]);
-        LanePair pair = lane_pair<16>(top);
-        pair = lane_pair<32>(fmaxf(pair.first, pair.second));
-        top = fmaxf(pair.first, pair.second) * a.to_log2;
-        if (__any(top > reference[t] + kPagedSlack)) {
-          const float raised = fmaxf(reference[t], top);
-          const float factor =
-              reference[t] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(reference[t] - raised);
-          sum[t] *= factor;
+        for (int ct = 0; ct < DT; ++ct)
 #pragma unroll
-          for (int ct = 0; ct < DT; ++ct)
+          for (int r = 0; r < 4; ++r) out[ct][r] *= factor;
+        reference = raised;
+      }
+      const float base = reference == kNegInf ? 0.0f : reference;
+      attn_u32x4 piece[kPieces];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) out[t][ct][r] *= factor;
-          reference[t] = raised;
-        }
-        const float base = reference[t] == kNegInf ? 0.0f : reference[t];
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], a.to_log2, -base));
-          sum[t] += p[e];
-        }
-#pragma unroll
-        for (int w = 0; w < 4; ++w) split_bf16(p[2 * w], p[2 * w + 1], piece[t], w);
+      for (int n = 0; n < 4; ++n) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n / 2][2 * (n % 2)], a.to_log2, -base));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n / 2][2 * (n % 2) + 1], a.to_log2, -base));
+        sum += x;
+        sum += y;
+        split_bf16(x, y, piece, n);
       }
       // O^T += V^T P^T
 #pragma unroll
       for (int half = 0; half < kHalves; ++half) {
-        if (half > 0) {
-          wave_fence();
-          if constexpr (kHalves == 2) write_values(here, 1);
-        }
+        if constexpr (kHalves == 2)
+          if (half > 0) {
+            wave_fence();
+            write_values(here, 1);
+          }
         wave_fence();
 #pragma unroll
         for (int c = 0; c < DH / 16; ++c) {
           const uint32_t at = read_at ^ (32 * c);
-          auto read = [&](uint32_t p) {
-            return __builtin_bit_cast(paged_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) paged_s16x4*)(uintptr_t)p));
-          };
-          const paged_u32x2 lo = read(at), hi = read(at + 16 * (2 * DH));
+          const paged_u32x2 lo = read_transposed(at), hi = read_transposed(at + 16 * (2 * DH));
           const attn_bf16x8 v = __builtin_bit_cast(attn_bf16x8, attn_u32x4{lo[0], lo[1], hi[0], hi[1]});
-          const int ct = DH / 16 * half + c;
+          attn_f32x4& o = out[DH / 16 * half + c];
 #pragma unroll
-          for (int i = 0; i < 3; ++i)
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-              out[t][ct] = AttnVec<__bf16>::mfma(v, __builtin_bit_cast(attn_bf16x8, piece[t][i]), out[t][ct]);
+          for (int i = 0; i < kPieces; ++i)
+            o = AttnVec<__bf16>::mfma(v, __builtin_bit_cast(attn_bf16x8, piece[i]), o);
         }
       }
       wave_fence();
       if (!more) break;
       key += kStep;
       id0 = next0, id1 = next1;
+      next0 = later0, next1 = later1;
     }
   };
+  __syncthreads();
   pass.template operator()<false>();
-  // 0 * NaN is NaN: a wave with a sum that is not finite takes its keys again.
-  float poison = 0.0f;
+  float poison = 0.0f;  // 0 * NaN is NaN: a wave with a sum that is not finite takes its keys again
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int ct = 0; ct < DT; ++ct)
 #pragma unroll
-    for (int ct = 0; ct < DT; ++ct)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) poison = __builtin_fmaf(out[t][ct][r], 0.0f, poison);
+    for (int r = 0; r < 4; ++r) poison = __builtin_fmaf(out[ct][r], 0.0f, poison);
   if (__any(poison != poison)) pass.template operator()<true>();
-
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    LanePair pair = lane_pair<16>(sum[t]);
+  {
+    LanePair pair = lane_pair<16>(sum);
     pair = lane_pair<32>(pair.first + pair.second);
-    sum[t] = pair.first + pair.second;
+    sum = pair.first + pair.second;
   }
-  // Wave states to LDS, 16 rows and DH channels at a time: 16-byte chunk c of row r in slot c ^ r.
-  constexpr int kItems = 16 * (DH / 8);
-  const int64_t slot = (static_cast<int64_t>(unit) * a.splits + split) * a.tile_rows;
+
+  // Wave states to LDS, DH channels at a time: 16-byte chunk c of row r in slot c ^ r.
+  constexpr int kItems = kSmallRows * (DH / 8);
+  const int64_t slot = (static_cast<int64_t>(place.unit) * a.splits + place.split) * a.tile_rows;
 #pragma unroll
-  for (int step = 0; step < NT * kHalves; ++step) {
-    const int t = step / kHalves, half = step % kHalves;
-    if (16 * t >= rows_here) break;
+  for (int half = 0; half < kHalves; ++half) {
     __syncthreads();
     float* const mine = reinterpret_cast<float*>(my_values) + m * DH;
 #pragma unroll
     for (int c = 0; c < DH / 16; ++c)
-      *reinterpret_cast<attn_f32x4*>(mine + 4 * ((4 * c + j) ^ m)) = out[t][DH / 16 * half + c];
+      *reinterpret_cast<attn_f32x4*>(mine + 4 * ((4 * c + j) ^ m)) = out[DH / 16 * half + c];
     if (j == 0 && half == 0) {
-      wave_ml[wave][m][0] = reference[t];
-      wave_ml[wave][m][1] = sum[t];
+      wave_ml[wave][m][0] = reference;
+      wave_ml[wave][m][1] = sum;
+    }
+    __syncthreads();
+    for (int item = threadIdx.x; item < kItems; item += 64 * WAVES) {
+      const int r = item / (DH / 8), c = item - r * (DH / 8);
+      if (r >= rows_here) break;
+      auto state = [&](int w, attn_f32x4& lo, attn_f32x4& hi) {
+        const float* wo = reinterpret_cast<const float*>(&v_lds[w][0]) + r * DH;
+        lo = *reinterpret_cast<const attn_f32x4*>(wo + 4 * ((2 * c) ^ r));
+        hi = *reinterpret_cast<const attn_f32x4*>(wo + 4 * ((2 * c + 1) ^ r));
+      };
+      finish_item<T, D, WAVES>(a, seg, row0 + r, DH * half + 8 * c, slot + r, keys.needed == 1,
+                               [&](int w, int i) { return wave_ml[w][r][i]; }, state);
+    }
+  }
+}
+
+// ---- Tiles of 32 rows -------------------------------------------------------------------------
+// The same with v_mfma_f32_32x32x16 for calls of many rows: a lane holds one query's scores of 16
+// keys, half a row of codes, and an MFMA of twice the work takes no more of the wave's issue slots
+// (8 of a SIMD's clocks against 4 a vector instruction, which bound this kernel).
+
+typedef float paged_f32x16 __attribute__((ext_vector_type(16)));
+
+template <typename T>
+__device__ __forceinline__ paged_f32x16 mfma32(attn_u32x4 a, attn_u32x4 b, paged_f32x16 c) {
+  if constexpr (std::is_same<T, __bf16>::value)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(attn_bf16x8, a),
+                                                   __builtin_bit_cast(attn_bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(attn_f16x8, a),
+                                                  __builtin_bit_cast(attn_f16x8, b), c, 0, 0, 0);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kAttnThreads) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : D == 128 ? 3 : 2)))
+void paged_tile_kernel(PagedAttnArgs a) {
+  constexpr int KS = D / 16;      // words of a lane, MFMA steps over the head dimension
+  constexpr int DT = D / 32;      // blocks of a row, column tiles of the output
+  constexpr int kStep = kUnit * kAttnWaves;
+  __shared__ __align__(1024) uint16_t v_lds[kAttnWaves][kUnit * D];
+  __shared__ __align__(16) attn_u32x4 q_lds[KS][64];
+  // the waves' softmax states at the end, in the place of the queries
+  float(*const wave_ml)[kTileRows][2] = reinterpret_cast<float(*)[kTileRows][2]>(&q_lds[0][0]);
+  static_assert(sizeof(q_lds) >= sizeof(float) * kAttnWaves * kTileRows * 2, "room for the states");
+
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int wave = static_cast<int>(wave_index());
+  const Place place = block_place(a);
+  const unsigned seg = place.seg, row0 = place.tile * kTileRows;
+  const int rows_here = rows_of_tile(a, row0, kTileRows);
+  const TileKeys keys = tile_keys(a, seg, row0, row0 + rows_here - 1);
+  if (keys.needed == 0) {  // no visible key for any row of this tile
+    if (place.split == 0) zero_rows<T, D>(a, seg, row0, rows_here);
+    return;
+  }
+  if (static_cast<int>(place.split) >= keys.needed) return;  // uniform across the workgroup
+  const int begin = static_cast<int>(place.split) * a.chunk;
+  const int end = min(begin + a.chunk, keys.key_end);
+
+  // Queries (B operand of step ks: channels half * D / 2 + 8 ks of row `col`) in LDS for every wave,
+  // and the last key that the lane's row sees.
+  const TileRow row = tile_row(a, seg, row0 + (col < rows_here ? col : 0));
+  const int limit = col < rows_here ? last_key(keys, row.query) : -1;
+  const int all_see = all_rows_see(a, keys, row0, rows_here);
+#pragma unroll
+  for (int n = 0; n < KS / kAttnWaves; ++n) {
+    const int ks = n * kAttnWaves + wave;
+    q_lds[ks][lane] = load16(static_cast<const T*>(a.queries) + row.offset + half * (D / 2) + 8 * ks);
+  }
+
+  const PagedCache& cache = a.cache;
+  const PageIds table = page_table(cache, seg);
+  const int64_t page_bytes = Page<D>::bytes(1) << cache.shift;
+  const int mask = (1 << cache.shift) - 1;
+  auto page_id = [&](int key) {
+    const int id = table[min(key, keys.key_end - 1) >> cache.shift];
+    return id >= 0 && id < cache.page_count ? id : -1;
+  };
+  // Lane (key, half): half a row's codes, words ks of channels half * D / 2 + 8 ks, and its blocks'
+  // scales.
+  struct Codes {
+    unsigned w[KS], scales;
+  };
+  auto load = [&](Codes& u, int which, int key, int id0, int id1) {
+    const int id = col < 16 ? id0 : id1, slot = (key + col) & mask;
+    const PagedBytes page = (PagedBytes)(cache.pages + (id < 0 ? 0 : id) * page_bytes);
+    const PagedBytes codes = page + (Page<D>::codes(cache.shift, which, slot) + half * (D / 4));
+#pragma unroll
+    for (int n = 0; n < KS / 4; ++n) {
+      const attn_u32x4 x = *(const __attribute__((address_space(1))) attn_u32x4*)(codes + 16 * n);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u.w[4 * n + e] = x[e];
+    }
+    const PagedBytes scales = page + (Page<D>::scales(cache.shift, which, slot) + half * (DT / 2));
+    if constexpr (D == 64) u.scales = *scales;
+    else if constexpr (D == 128) u.scales = *(const __attribute__((address_space(1))) uint16_t*)scales;
+    else u.scales = *(const __attribute__((address_space(1))) unsigned*)scales;
+  };
+  auto scale = [&](const Codes& u, int ks) {
+    return scale_of(D == 64 ? u.scales : u.scales >> (8 * (ks / 4)) & 255u);
+  };
+
+  float reference = kNegInf, sum = 0.0f;  // in exponents of two; the same in both halves
+  paged_f32x16 out[DT];
+  char* const my_values = reinterpret_cast<char*>(&v_lds[wave][0]);
+  auto write_values = [&](const Codes& v) {
+    char* row = my_values + col * (2 * D);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      *reinterpret_cast<attn_u32x4*>(row + 16 * ((half * KS + ks) ^ value_swizzle<D>(col))) =
+          expand8<__bf16>(v.w[ks], scale(v, ks));
+  };
+  // Transposed reads: row 4 half + (lane % 16) / 4 of eight, columns 16 (lane / 16 % 2) +
+  // 4 (lane % 4) .. + 3 of 32.
+  uint32_t read_at;
+  {
+    const int row = 4 * half + ((lane & 15) >> 2), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    read_at = lds_address(my_values) + row * (2 * D) + 16 * (chunk ^ value_swizzle<D>(row)) +
+              8 * (lane & 1);
+  }
+  auto read_column = [&](int k, int dt) {  // A operand: keys 16 k .. 16 k + 15 of 32 channels
+    // (eight rows on, value_swizzle differs in one bit)
+    const uint32_t at = (read_at ^ (64 * dt)) + 16 * k * (2 * D);
+    const paged_u32x2 lo = read_transposed(at), hi = read_transposed((at ^ 16) + 8 * (2 * D));
+    return attn_u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+
+  auto pass = [&]<bool SAFE>() {
+    reference = kNegInf, sum = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) out[dt][r] = 0.0f;
+    int key = begin + kUnit * wave;
+    if (key >= end) return;
+    Codes k, v;
+    int id0 = page_id(key), id1 = page_id(key + 16);
+    load(k, 0, key, id0, id1);
+    load(v, 1, key, id0, id1);
+    int next0 = page_id(key + kStep), next1 = page_id(key + kStep + 16);
+    while (true) {
+      const int later0 = page_id(key + 2 * kStep), later1 = page_id(key + 2 * kStep + 16);
+      const bool more = key + kStep < end;
+      if (key + kUnit > keys.key_end || id0 < 0 || id1 < 0) {  // rows that are not there: zeros for V
+        const bool there = key + col < keys.key_end && (col < 16 ? id0 : id1) >= 0;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) v.w[ks] = there ? v.w[ks] : 0u;
+        v.scales = there ? v.scales : 0x7f7f7f7fu;
+      }
+      if constexpr (SAFE) {
+#pragma unroll 1
+        for (int left = 0; left < kUnit; ++left) {
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            const unsigned bytes = __shfl(v.scales, left + 32 * (dt / (DT / 2)));
+            if ((bytes >> (8 * (dt % (DT / 2))) & 255u) == kScaleNaN && key + left <= limit)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) out[dt][r] = __builtin_nanf("");
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < DT / 2; ++b)
+          if ((v.scales >> (8 * b) & 255u) == kScaleNaN) {
+            v.scales &= ~(0x80u << (8 * b));  // 127
+#pragma unroll
+            for (int w = 0; w < 4; ++w) v.w[4 * b + w] = 0u;
+          }
+      }
+      // V rows to LDS (the last unit's reads are done: a wave's LDS accesses stay in order)
+      write_values(v);
+      // S^T
+      paged_f32x16 s;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(expand8<T>(k.w[ks], scale(k, ks)), q_lds[ks][lane], s);
+      if (more) {
+        load(k, 0, key + kStep, next0, next1);
+        load(v, 1, key + kStep, next0, next1);
+      }
+      if (key + kUnit - 1 > all_see || id0 < 0 || id1 < 0) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (key + 8 * (r >> 2) + 4 * half + (r & 3) > limit || (r < 8 ? id0 : id1) < 0) s[r] = kNegInf;
+      }
+      float top = kNegInf;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) top = fmaxf(fmaxf(top, s[2 * r]), s[2 * r + 1]);
+      const LanePair pair = lane_pair<32>(top);
+      top = fmaxf(pair.first, pair.second) * a.to_log2;
+      if (__any(top > reference + (SAFE ? 0.0f : kPagedSlack))) {
+        const float raised = fmaxf(reference, top);
+        const float factor = reference == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(reference - raised);
+        sum *= factor;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) out[dt][r] *= factor;
+        reference = raised;
+      }
+      const float base = reference == kNegInf ? 0.0f : reference;
+      attn_u32x4 piece[2][kPieces];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * n], a.to_log2, -base));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * n + 1], a.to_log2, -base));
+        sum += x;
+        sum += y;
+        split_bf16(x, y, piece[n / 4], n % 4);
+      }
+      // O^T += V^T P^T
+      wave_fence();
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const attn_u32x4 x = read_column(kk, dt);
+#pragma unroll
+          for (int n = 0; n < kPieces; ++n) out[dt] = mfma32<__bf16>(x, piece[kk][n], out[dt]);
+        }
+      wave_fence();
+      if (!more) break;
+      key += kStep;
+      id0 = next0, id1 = next1;
+      next0 = later0, next1 = later1;
+    }
+  };
+  __syncthreads();
+  pass.template operator()<false>();
+  float poison = 0.0f;  // 0 * NaN is NaN: a wave with a sum that is not finite takes its keys again
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) poison = __builtin_fmaf(out[dt][r], 0.0f, poison);
+  if (__any(poison != poison)) pass.template operator()<true>();
+  {
+    const LanePair pair = lane_pair<32>(sum);
+    sum = pair.first + pair.second;
+  }
+
+  // Wave states to LDS, D / 2 channels at a time: 16-byte chunk c of row r in slot c ^ (r % 8).
+  // (Lane (row, half) holds channels 32 dt + 8 c + 4 half + [0, 4).)
+  constexpr int DQ = D / 2, kParts = D / DQ, kItems = kTileRows * (DQ / 8);
+  const int64_t slot = (static_cast<int64_t>(place.unit) * a.splits + place.split) * a.tile_rows;
+#pragma unroll
+  for (int part = 0; part < kParts; ++part) {
+    __syncthreads();
+    float* const mine = reinterpret_cast<float*>(my_values) + col * DQ;
+#pragma unroll
+    for (int d = 0; d < DQ / 32; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const paged_f32x16& o = out[DQ / 32 * part + d];
+        *reinterpret_cast<attn_f32x4*>(mine + 4 * ((8 * d + 2 * c + half) ^ (col & 7))) =
+            attn_f32x4{o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]};
+      }
+    if (half == 0 && part == 0) {
+      wave_ml[wave][col][0] = reference;
+      wave_ml[wave][col][1] = sum;
     }
     __syncthreads();
     for (int item = threadIdx.x; item < kItems; item += kAttnThreads) {
-      const int r = item / (DH / 8), c = item - r * (DH / 8);
-      if (16 * t + r >= rows_here) break;
-      float top = kNegInf, total = 0.0f, o[8] = {};
-#pragma unroll
-      for (int w = 0; w < kAttnWaves; ++w) top = fmaxf(top, wave_ml[w][r][0]);
-#pragma unroll
-      for (int w = 0; w < kAttnWaves; ++w) {
-        if (wave_ml[w][r][0] == kNegInf && wave_ml[w][r][1] == 0.0f) continue;  // saw no key
-        const float weight =
-            wave_ml[w][r][0] == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(wave_ml[w][r][0] - top);
-        total = __builtin_fmaf(weight, wave_ml[w][r][1], total);
-        const float* wo = reinterpret_cast<const float*>(&v_lds[w][0]) + r * DH;
-        const attn_f32x4 lo = *reinterpret_cast<const attn_f32x4*>(wo + 4 * ((2 * c) ^ r));
-        const attn_f32x4 hi = *reinterpret_cast<const attn_f32x4*>(wo + 4 * ((2 * c + 1) ^ r));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o[e] = __builtin_fmaf(weight, lo[e], o[e]);
-          o[4 + e] = __builtin_fmaf(weight, hi[e], o[4 + e]);
-        }
-      }
-      const int channel = DH * half + 8 * c;
-      if (keys.needed == 1) {
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] *= inv;
-        *reinterpret_cast<attn_u32x4*>(paged_output<T, D>(a, seg, row0 + 16 * t + r) + channel) =
-            pack8<T>(o);
-      } else {
-        float* po = a.part_o + (slot + 16 * t + r) * D + channel;
-        *reinterpret_cast<attn_f32x4*>(po) = attn_f32x4{o[0], o[1], o[2], o[3]};
-        *reinterpret_cast<attn_f32x4*>(po + 4) = attn_f32x4{o[4], o[5], o[6], o[7]};
-        if (channel == 0) {
-          a.part_ml[(slot + 16 * t + r) * 2] = top;
-          a.part_ml[(slot + 16 * t + r) * 2 + 1] = total;
-        }
-      }
+      const int r = item / (DQ / 8), c = item - r * (DQ / 8);
+      if (r >= rows_here) break;
+      auto state = [&](int w, attn_f32x4& lo, attn_f32x4& hi) {
+        const float* wo = reinterpret_cast<const float*>(&v_lds[w][0]) + r * DQ;
+        lo = *reinterpret_cast<const attn_f32x4*>(wo + 4 * ((2 * c) ^ (r & 7)));
+        hi = *reinterpret_cast<const attn_f32x4*>(wo + 4 * ((2 * c + 1) ^ (r & 7)));
+      };
+      finish_item<T, D, kAttnWaves>(a, seg, row0 + r, DQ * part + 8 * c, slot + r, keys.needed == 1,
+                                    [&](int w, int i) { return wave_ml[w][r][i]; }, state);
     }
   }
 }
 
 // Second launch of a split call: a thread folds one (row, 8 channels) slice of every fourth chunk of
-// a tile, a round of chunks' states loaded together; the four threads of a slice meet in LDS.
-constexpr int kMergeItems = 64, kMergeParts = kAttnThreads / kMergeItems, kMergeLoads = 4;
+// a tile, LOADS chunks' states loaded together; the four threads of a slice meet in LDS. The first
+// round is loaded before the segment's length is known (the workspace holds every chunk of the
+// grid; those past the needed ones are not used), so that the two memory round trips overlap.
+constexpr int kMergeItems = 64, kMergeParts = kAttnThreads / kMergeItems;
 
-template <typename T, int D>
+template <typename T, int D, int LOADS>
 __global__ __launch_bounds__(kAttnThreads) void paged_merge_kernel(PagedAttnArgs a, unsigned blocks) {
-  __shared__ __align__(16) float merge_o[kMergeParts][kMergeItems][8];
-  __shared__ float merge_ml[kMergeParts][kMergeItems][2];
+  __shared__ __align__(16) attn_f32x4 merge_o[2][kMergeParts][kMergeItems];
+  __shared__ float merge_ml[2][kMergeParts][kMergeItems];
   const unsigned unit = blockIdx.x / blocks;
   const unsigned seg = unit / a.tiles, tile = unit - seg * a.tiles;
   const unsigned rows = static_cast<unsigned>(a.length) * static_cast<unsigned>(a.groups);
   const unsigned row0 = tile * a.tile_rows;
   const int rows_here = static_cast<int>(min(rows - row0, static_cast<unsigned>(a.tile_rows)));
-  const int needed = tile_keys(a, seg, row0, row0 + rows_here - 1).needed;
-  if (needed <= 1) return;  // the first launch wrote this tile's output
   const int local = threadIdx.x % kMergeItems, part = threadIdx.x / kMergeItems;
   const int item = static_cast<int>(blockIdx.x - unit * blocks) * kMergeItems + local;
   const int r = item / (D / 8), c = item - r * (D / 8);
   const bool valid = r < rows_here;
-  float top = kNegInf, total = 0.0f, o[8] = {};
-  auto fold = [&](float m, float l, const attn_f32x4& x, const attn_f32x4& y) {
-    if (m == kNegInf && l == 0.0f) return;  // saw no key
-    const float higher = fmaxf(top, m);
-    const float ws = top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
-    const float wo = m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - higher);
-    total = __builtin_fmaf(wo, l, total * ws);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      o[e] = __builtin_fmaf(wo, x[e], o[e] * ws);
-      o[4 + e] = __builtin_fmaf(wo, y[e], o[4 + e] * ws);
-    }
-    top = higher;
-  };
   const int64_t first = static_cast<int64_t>(unit) * a.splits * a.tile_rows + (valid ? r : 0);
-  for (int k0 = part; k0 < needed; k0 += kMergeParts * kMergeLoads) {
-    float m[kMergeLoads], l[kMergeLoads];
-    attn_f32x4 x[kMergeLoads], y[kMergeLoads];
+  float m[LOADS], l[LOADS];
+  attn_f32x4 x[LOADS], y[LOADS];
+  auto load = [&](int k0) {
 #pragma unroll
-    for (int i = 0; i < kMergeLoads; ++i) {
+    for (int i = 0; i < LOADS; ++i) {
       const int k = k0 + i * kMergeParts;
-      const int64_t at = first + static_cast<int64_t>(k < needed ? k : k0) * a.tile_rows;
-      m[i] = k < needed ? a.part_ml[at * 2] : kNegInf;
-      l[i] = k < needed ? a.part_ml[at * 2 + 1] : 0.0f;
+      const int64_t at = first + static_cast<int64_t>(k < static_cast<int>(a.splits) ? k : 0) * a.tile_rows;
+      m[i] = a.part_ml[at * 2];
+      l[i] = a.part_ml[at * 2 + 1];
       x[i] = *reinterpret_cast<const attn_f32x4*>(a.part_o + at * D + 8 * c);
       y[i] = *reinterpret_cast<const attn_f32x4*>(a.part_o + at * D + 8 * c + 4);
     }
+  };
+  load(part);
+  const int needed = tile_keys(a, seg, row0, row0 + rows_here - 1).needed;
+  if (needed <= 1) return;  // the first launch wrote this tile's output
+  float top = kNegInf, total = 0.0f, o[8] = {};
+  auto fold = [&](float state_m, float state_l, const attn_f32x4& lo, const attn_f32x4& hi) {
+    if (state_m == kNegInf && state_l == 0.0f) return;  // saw no key
+    const float higher = fmaxf(top, state_m);
+    const float ws = top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
+    const float wo = state_m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(state_m - higher);
+    total = __builtin_fmaf(wo, state_l, total * ws);
 #pragma unroll
-    for (int i = 0; i < kMergeLoads; ++i) fold(m[i], l[i], x[i], y[i]);
+    for (int e = 0; e < 4; ++e) {
+      o[e] = __builtin_fmaf(wo, lo[e], o[e] * ws);
+      o[4 + e] = __builtin_fmaf(wo, hi[e], o[4 + e] * ws);
+    }
+    top = higher;
+  };
+  for (int k0 = part; k0 < needed; k0 += kMergeParts * LOADS) {
+    if (k0 != part) load(k0);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      if (k0 + i * kMergeParts < needed) fold(m[i], l[i], x[i], y[i]);
   }
-  merge_ml[part][local][0] = top;
-  merge_ml[part][local][1] = total;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) merge_o[part][local][e] = o[e];
+  merge_ml[0][part][local] = top;
+  merge_ml[1][part][local] = total;
+  merge_o[0][part][local] = attn_f32x4{o[0], o[1], o[2], o[3]};
+  merge_o[1][part][local] = attn_f32x4{o[4], o[5], o[6], o[7]};
   __syncthreads();
   if (part != 0 || !valid) return;
-  for (int p = 1; p < kMergeParts; ++p) {
-    const float* w = merge_o[p][local];
-    fold(merge_ml[p][local][0], merge_ml[p][local][1], attn_f32x4{w[0], w[1], w[2], w[3]},
-         attn_f32x4{w[4], w[5], w[6], w[7]});
-  }
+#pragma unroll
+  for (int p = 1; p < kMergeParts; ++p)
+    fold(merge_ml[0][p][local], merge_ml[1][p][local], merge_o[0][p][local], merge_o[1][p][local]);
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] *= inv;
@@ -541,23 +861,39 @@ __global__ __launch_bounds__(kAttnThreads) void paged_merge_kernel(PagedAttnArgs
 }
 
 struct PagedPlan {
-  int tiles_of_16;       // NT
-  int tile_rows;
+  bool tile_kernel;
+  int waves, tile_rows;  // of a workgroup, of a tile's partial states
   int64_t tiles, units, splits, chunk;
 };
 
-PagedPlan plan_paged(int64_t segments, int64_t groups, int64_t length, int64_t max_keys, int64_t dim) {
+// Which kernel runs and how many chunks the keys get. Both sides measured, us (8 segments, G4, d128
+// unless said). Tiles of 32 rows where they fill most of the chip: 1000 queries onto 4,000 rows 128
+// against 155 in tiles of 16, 64 queries 19 either way. Decode and short calls: chunks until there are
+// 512 workgroups (256 in tiles of 32 rows: 300 queries of d256, G6, 67 against 82 with 512), at most
+// 32 a tile, whose states a merge takes in one round of loads (8,000 rows: 9.4 against 11.6 with 63);
+// none where four units a wave reach (500 rows: 7.1 against 8.0), and in the place of two chunks one
+// workgroup of eight waves (256 segments of 2,000 rows: 16.0 against 18.8).
+PagedPlan plan_paged(int64_t segments, int64_t groups, int64_t length, int64_t max_keys) {
   PagedPlan p{};
   const int64_t rows = length * groups;
-  p.tiles_of_16 = rows <= 16 ? 1 : rows <= 32 || dim == 256 ? 2 : 4;
-  p.tile_rows = static_cast<int>(std::min<int64_t>(rows, 16 * p.tiles_of_16));
-  p.tiles = ceil_div(rows, 16 * p.tiles_of_16);
+  p.tile_kernel = rows > kSmallRows && segments * ceil_div(rows, int64_t{kTileRows}) >= 192;
+  const int64_t tile = p.tile_kernel ? kTileRows : kSmallRows;
+  p.waves = kAttnWaves;
+  p.tile_rows = static_cast<int>(std::min(rows, tile));
+  p.tiles = ceil_div(rows, tile);
   p.units = segments * p.tiles;
-  const int64_t steps = std::max<int64_t>(1, ceil_div(max_keys, kStep));
-  const int64_t wanted = std::min(steps, ceil_div(1024, p.units));
+  int64_t step = kUnit * kAttnWaves, steps = std::max<int64_t>(1, ceil_div(max_keys, step));
+  int64_t wanted = std::min({steps, int64_t{32}, ceil_div(p.tile_kernel ? 256 : 512, p.units)});
+  if (steps <= 4) wanted = 1;
+  if (wanted == 2 && !p.tile_kernel) {
+    p.waves = 2 * kAttnWaves;
+    step *= 2;
+    steps = ceil_div(max_keys, step);
+    wanted = 1;
+  }
   const int64_t per = ceil_div(steps, wanted);
   p.splits = ceil_div(steps, per);
-  p.chunk = per * kStep;
+  p.chunk = per * step;
   return p;
 }
 
@@ -566,26 +902,32 @@ size_t plan_bytes(const PagedPlan& p, int64_t dim) {
   return static_cast<size_t>(p.units * p.splits * p.tile_rows) * static_cast<size_t>(dim + 2) * 4;
 }
 
-template <typename T, int D, int NT>
-int launch_paged(const PagedAttnArgs& args, const PagedPlan& plan, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_attention_kernel<T, D, NT>),
-                     dim3(static_cast<unsigned>(plan.units * plan.splits)), dim3(kAttnThreads), 0,
-                     stream, args);
-  if (int status = check_launch("paged_attention")) return status;
+template <typename T, int D>
+int launch_merge(const PagedAttnArgs& args, const PagedPlan& plan, hipStream_t stream) {
   if (plan.splits == 1) return LR_OK;
   const unsigned blocks =
       static_cast<unsigned>(ceil_div(static_cast<int64_t>(plan.tile_rows) * (D / 8), kMergeItems));
-  hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3(static_cast<unsigned>(plan.units) * blocks),
-                     dim3(kAttnThreads), 0, stream, args, blocks);
+  auto merge = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.units) * blocks), dim3(kAttnThreads),
+                       0, stream, args, blocks);
+  };
+  if (plan.splits <= 2 * kMergeParts) merge(paged_merge_kernel<T, D, 2>);
+  else if (plan.splits <= 5 * kMergeParts) merge(paged_merge_kernel<T, D, 5>);
+  else merge(paged_merge_kernel<T, D, 8>);
   return check_launch("paged_attention merge");
 }
 
 template <typename T, int D>
-int launch_paged_rows(const PagedAttnArgs& args, const PagedPlan& plan, hipStream_t stream) {
-  if (plan.tiles_of_16 == 1) return launch_paged<T, D, 1>(args, plan, stream);
-  if (D == 256 || plan.tiles_of_16 == 2) return launch_paged<T, D, 2>(args, plan, stream);
-  if constexpr (D != 256) return launch_paged<T, D, 4>(args, plan, stream);
-  return LR_OK;
+int launch_paged(const PagedAttnArgs& args, const PagedPlan& plan, hipStream_t stream) {
+  auto attend = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.units * plan.splits)),
+                       dim3(static_cast<unsigned>(64 * plan.waves)), 0, stream, args);
+  };
+  if (plan.tile_kernel) attend(paged_tile_kernel<T, D>);
+  else if (plan.waves == kAttnWaves) attend(paged_attention_kernel<T, D, kAttnWaves>);
+  else attend(paged_attention_kernel<T, D, 2 * kAttnWaves>);
+  if (int status = check_launch("paged_attention")) return status;
+  return launch_merge<T, D>(args, plan, stream);
 }
 
 }  // namespace
@@ -597,7 +939,7 @@ extern "C" size_t lr_paged_attention_workspace_bytes(int64_t segments, int64_t g
                                                      int64_t length, int64_t max_keys,
                                                      int64_t dim) {
   if (segments <= 0 || groups <= 0 || length <= 0 || max_keys < 0 || dim <= 0) return 0;
-  return plan_bytes(plan_paged(segments, groups, length, max_keys, dim), dim);
+  return plan_bytes(plan_paged(segments, groups, length, max_keys), dim);
 }
 
 extern "C" int lr_paged_attention(const void* queries, const int64_t* query_strides,
@@ -626,7 +968,7 @@ extern "C" int lr_paged_attention(const void* queries, const int64_t* query_stri
   LR_REQUIRE(alignment % 16 == 0, "Attention operands must be 16-byte aligned");
   // keys there can be: what a table holds, of a pool that has pages
   max_keys = page_count == 0 ? 0 : std::min(max_keys, max_pages * page_size);
-  const PagedPlan plan = plan_paged(segments, groups, length, max_keys, dim);
+  const PagedPlan plan = plan_paged(segments, groups, length, max_keys);
   const size_t needed = plan_bytes(plan, dim);
   LR_REQUIRE(workspace_size >= needed && (needed == 0 || workspace != nullptr),
              "Attention workspace too small");
@@ -647,6 +989,7 @@ extern "C" int lr_paged_attention(const void* queries, const int64_t* query_stri
   args.groups = static_cast<int>(groups);
   args.length = static_cast<int>(length);
   args.max_keys = static_cast<int>(max_keys);
+  args.segments = static_cast<unsigned>(segments);
   args.tiles = static_cast<unsigned>(plan.tiles);
   args.splits = static_cast<unsigned>(plan.splits);
   args.tile_rows = plan.tile_rows;
@@ -658,7 +1001,7 @@ extern "C" int lr_paged_attention(const void* queries, const int64_t* query_stri
     args.part_o = args.part_ml + plan.units * plan.splits * plan.tile_rows * 2;
   }
   return dispatch_dim(dim, [&]<int D>() {
-    return dtype == LR_DTYPE_BF16 ? launch_paged_rows<__bf16, D>(args, plan, as_stream(stream))
-                                  : launch_paged_rows<_Float16, D>(args, plan, as_stream(stream));
+    return dtype == LR_DTYPE_BF16 ? launch_paged<__bf16, D>(args, plan, as_stream(stream))
+                                  : launch_paged<_Float16, D>(args, plan, as_stream(stream));
   });
 }

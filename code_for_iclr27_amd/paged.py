@@ -131,9 +131,8 @@ def _native():
     return _native_module
 
 
-def _forward_only(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"paged.{name}: the 4-bit cache has no backward pass (forward only)")
+def _forward_only(name):
+    raise RuntimeError(f"paged.{name}: the 4-bit cache has no backward pass (forward only)")
 
 
 def append(layer, keys, values, positions, rotary=None, queries=None, counts=None):
@@ -148,7 +147,9 @@ def append(layer, keys, values, positions, rotary=None, queries=None, counts=Non
     the tables gives NaN. ``counts`` int32 [batch] on the device: request b brings its first
     counts[b] rows only (a padded batch, or a request that has ended). Rows that the table has no
     page for are not stored."""
-    _forward_only("append", keys, values, queries)
+    if torch.is_grad_enabled() and (keys.requires_grad or values.requires_grad
+                                    or queries is not None and queries.requires_grad):
+        _forward_only("append")
     cos, sin = (None, None) if rotary is None else rotary
     return (_native_module or _native()).paged_append(
         layer.pages, layer.table, layer.lengths, layer.kv_heads, layer.dim, layer.page_size, keys,
@@ -164,7 +165,8 @@ def attention(layer, queries, max_length, counts=None, scale=None):
     ``max_length``: a bound on every segment's cached rows plus ``length`` (host int; rows past it
     are not visited). ``scale`` defaults to dim^-0.5. The rows must have been appended as bf16, or
     in the queries' dtype (f16 queries read larger values as infinities)."""
-    _forward_only("attention", queries)
+    if queries.requires_grad and torch.is_grad_enabled():
+        _forward_only("attention")
     return (_native_module or _native()).paged_attention(
         layer.pages, layer.table, layer.lengths, layer.kv_heads, layer.dim, layer.page_size,
         queries, int(max_length), counts, float(layer.dim ** -0.5 if scale is None else scale))
