@@ -258,23 +258,11 @@ __global__ __launch_bounds__(kSumThreads) void paged_sum_kernel(SumArgs a) {
 struct ReadArgs {
   PagedCache cache;
   int64_t segments, total;
-  const int32_t* cumulative;
+  int32_t* cumulative;  // [segments + 1]: written by the fused form, read by the other
   void* keys;
   void* values;
   float* positions;
 };
-
-// The segment that packed row `row` belongs to: the largest s with cumulative[s] <= row (and so
-// one that is not empty, if row < cumulative[segments]).
-__device__ __forceinline__ int64_t segment_of(const int32_t* cumulative, int64_t segments, int64_t row) {
-  int64_t low = 0, high = segments;
-  while (high - low > 1) {
-    const int64_t mid = (low + high) / 2;
-    if (cumulative[mid] <= row) low = mid;
-    else high = mid;
-  }
-  return low;
-}
 
 template <typename T>
 __device__ __forceinline__ Eight<T> eight_values(unsigned codes, float scale) {
@@ -289,31 +277,101 @@ __device__ __forceinline__ Eight<T> eight_values(unsigned codes, float scale) {
   }
 }
 
-// D / 8 threads a row, eight channels of its K and V each.
-template <typename T, int D>
+constexpr int kReadRows = 64;             // of a workgroup
+constexpr int kFusedSegments = kThreads;  // one length a thread
+
+// Cumulative lengths of up to kFusedSegments segments in LDS, by every workgroup for itself.
+__device__ __forceinline__ void sum_lengths(const PagedCache& cache, int segments, int32_t* cumulative) {
+  __shared__ int64_t wave_total[kThreads / 64];
+  const int thread = static_cast<int>(threadIdx.x), lane = thread & 63, wave = thread >> 6;
+  int64_t sum = thread < segments ? cache.rows(thread) : 0;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t other = __shfl_up(sum, d);
+    if (lane >= d) sum += other;
+  }
+  if (lane == 63) wave_total[wave] = sum;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) sum += wave_total[w];
+  if (thread == 0) cumulative[0] = 0;
+  if (thread < segments) cumulative[thread + 1] = packed_row(sum);
+  __syncthreads();
+}
+
+// The segment that packed row `row` < cumulative[segments] belongs to: the largest s with
+// cumulative[s] <= row.
+__device__ __forceinline__ int segment_of(const int32_t* cumulative, int segments, int row) {
+  int low = 0, high = segments;
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (cumulative[mid] <= row) low = mid;
+    else high = mid;
+  }
+  return low;
+}
+
+// A workgroup takes 64 packed rows: the first wave finds each one's page and slot, then D / 8 threads
+// a row expand eight channels each, four rows' loads in flight.
+template <typename T, int D, bool FUSED>
 __global__ __launch_bounds__(kThreads) void paged_read_kernel(ReadArgs a) {
-  constexpr int kRowThreads = D / 8, kRowsPerBlock = kThreads / kRowThreads;
-  const int c = threadIdx.x % kRowThreads;
-  const int64_t stop = min(a.total, static_cast<int64_t>(a.cumulative[a.segments]));
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + threadIdx.x / kRowThreads;
-  if (row >= stop) return;
+  constexpr int kRowThreads = D / 8, kRowsAtOnce = kThreads / kRowThreads;
+  constexpr int kRounds = kReadRows / kRowsAtOnce, kTogether = kRounds < 4 ? kRounds : 4;
+  __shared__ int32_t sums[FUSED ? kFusedSegments + 1 : 1];
+  __shared__ int64_t row_page[kReadRows];  // byte offset of the row's page, or -1
+  __shared__ int row_slot[kReadRows];
   const PagedCache& cache = a.cache;
-  const int64_t segment = segment_of(a.cumulative, a.segments, row);
-  const int at = static_cast<int>(row - a.cumulative[segment]);
-  const int64_t id = cache.table[segment * cache.max_pages + (at >> cache.shift)];
-  if (id < 0 || id >= cache.page_count) return;
-  const int slot = at & ((1 << cache.shift) - 1);
-  const uint8_t* page = cache.pages + id * (Page<D>::bytes(1) << cache.shift);
+  const int segments = static_cast<int>(a.segments);
+  const int32_t* cumulative = a.cumulative;
+  if constexpr (FUSED) {
+    sum_lengths(cache, segments, sums);
+    if (blockIdx.x == 0)
+      for (int s = threadIdx.x; s <= segments; s += kThreads) a.cumulative[s] = sums[s];
+    cumulative = sums;
+  }
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kReadRows;
+  if (threadIdx.x < kReadRows) {
+    const int64_t row = row0 + threadIdx.x;
+    int64_t page = -1;
+    int slot = 0;
+    if (row < a.total && row < cumulative[segments]) {
+      const int segment = segment_of(cumulative, segments, static_cast<int>(row));
+      const int at = static_cast<int>(row) - cumulative[segment];
+      const int64_t id = cache.table[static_cast<int64_t>(segment) * cache.max_pages + (at >> cache.shift)];
+      if (id >= 0 && id < cache.page_count) {
+        page = id * (Page<D>::bytes(1) << cache.shift);
+        slot = at & ((1 << cache.shift) - 1);
+        a.positions[row] = *reinterpret_cast<const float*>(cache.pages + page +
+                                                           Page<D>::position(cache.shift, slot));
+      }
+    }
+    row_page[threadIdx.x] = page;
+    row_slot[threadIdx.x] = slot;
+  }
+  __syncthreads();
+  const int c = threadIdx.x % kRowThreads, first = threadIdx.x / kRowThreads;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    const unsigned codes =
-        *reinterpret_cast<const unsigned*>(page + Page<D>::codes(cache.shift, which, slot) + 4 * c);
-    const unsigned byte = page[Page<D>::scales(cache.shift, which, slot) + c / 4];
-    T* out = static_cast<T*>(which == 0 ? a.keys : a.values) + row * D + 8 * c;
-    *reinterpret_cast<Eight<T>*>(out) = eight_values<T>(codes, scale_of(byte));
+    T* const out = static_cast<T*>(which == 0 ? a.keys : a.values) + row0 * D + 8 * c;
+#pragma unroll
+    for (int r0 = 0; r0 < kRounds; r0 += kTogether) {
+      unsigned codes[kTogether], byte[kTogether];
+      bool there[kTogether];
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) {
+        const int r = (r0 + i) * kRowsAtOnce + first, slot = row_slot[r];
+        there[i] = row_page[r] >= 0;
+        // (a row that is not there reads the pool's first one, and is not written)
+        const uint8_t* p = cache.pages + (there[i] ? row_page[r] : 0);
+        codes[i] = *reinterpret_cast<const unsigned*>(p + Page<D>::codes(cache.shift, which, slot) + 4 * c);
+        byte[i] = p[Page<D>::scales(cache.shift, which, slot) + c / 4];
+      }
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i)
+        if (there[i])
+          *reinterpret_cast<Eight<T>*>(out + static_cast<int64_t>((r0 + i) * kRowsAtOnce + first) * D) =
+              eight_values<T>(codes[i], scale_of(byte[i]));
+    }
   }
-  if (c == 0)
-    a.positions[row] = *reinterpret_cast<const float*>(page + Page<D>::position(cache.shift, slot));
 }
 
 // ---------------------------------------------------------------------------------------
@@ -514,19 +572,28 @@ extern "C" int lr_paged_read(const void* pages, int64_t page_count, int64_t page
              "Invalid packed buffers");
   LR_REQUIRE(((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) % 16) == 0,
              "Packed buffers must be 16-byte aligned");
+  // One launch where a workgroup can sum the lengths itself, beside its rows' lookups; calls without
+  // rows or pages have only the sums to write.
+  const bool fused = segments <= kFusedSegments && total > 0 && page_count > 0;
   SumArgs sums{};
   sums.cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
   sums.segments = segments;
   sums.cumulative = cumulative;
-  hipLaunchKernelGGL(paged_sum_kernel, dim3(1), dim3(kSumThreads), 0, as_stream(stream), sums);
-  if (int status = check_launch("paged_read lengths")) return status;
-  if (total == 0) return LR_OK;
+  if (!fused) {
+    hipLaunchKernelGGL(paged_sum_kernel, dim3(1), dim3(kSumThreads), 0, as_stream(stream), sums);
+    if (int status = check_launch("paged_read lengths")) return status;
+    if (total == 0 || page_count == 0) return LR_OK;
+  }
   const ReadArgs args{sums.cache, segments, total, cumulative, keys, values, positions};
-  const int64_t blocks = ceil_div(total, kThreads / (dim / 8));
+  const int64_t blocks = ceil_div(total, kReadRows);
   return dispatch_type(dtype, [&]<typename T>() {
     return dispatch_dim(dim, [&]<int D>() {
-      hipLaunchKernelGGL((paged_read_kernel<T, D>), dim3(static_cast<unsigned>(blocks)),
-                         dim3(kThreads), 0, as_stream(stream), args);
+      auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                           as_stream(stream), args);
+      };
+      if (fused) launch(paged_read_kernel<T, D, true>);
+      else launch(paged_read_kernel<T, D, false>);
       return check_launch("paged_read");
     });
   });
