@@ -1586,15 +1586,15 @@ torch::Tensor paged_compact_launch(const torch::Tensor& pages, const torch::Tens
   const c10::DeviceGuard guard(pages.device());
   torch::Tensor new_lengths = torch::empty_like(lengths);
   const size_t size = library.paged_compact_workspace_bytes(lengths.numel());
-  torch::Tensor workspace =
-      torch::empty({static_cast<int64_t>(size)}, pages.options().dtype(torch::kUInt8));
+  torch::Tensor workspace;
+  if (size) workspace = torch::empty({static_cast<int64_t>(size)}, pages.options());
   check_call(library.paged_compact(
       const_cast<void*>(address_or_null(pages)), pages.size(0), page_size,
       table.numel() ? table.data_ptr<int32_t>() : nullptr, table.size(1),
       lengths.data_ptr<int32_t>(), lengths.numel(), dim,
       removed.numel() ? removed.data_ptr<int64_t>() : nullptr, removed.numel(),
       target.numel() ? target.data_ptr<int32_t>() : nullptr, target.size(1),
-      new_lengths.data_ptr<int32_t>(), workspace.data_ptr(), size, current_stream(pages.device())));
+      new_lengths.data_ptr<int32_t>(), size ? workspace.data_ptr() : nullptr, size, current_stream(pages.device())));
   return new_lengths;
 }
 

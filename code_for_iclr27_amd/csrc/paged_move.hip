@@ -182,76 +182,57 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------
-// The packed layout's first rows, cumulative[s] = rows of the segments before s; one workgroup.
-// With `starts` also each segment's part of `removed` (sorted packed rows, starts[s] = how many lie
-// before the segment) and the length that it leaves.
-struct SumArgs {
-  PagedCache cache;
-  int64_t segments;
-  int32_t* cumulative;        // [segments + 1], or NULL
-  const int64_t* removed;
-  int64_t removed_count;
-  int64_t* starts;            // [segments + 1], or NULL
-  int64_t* first_rows;        // [segments] with starts
-  int32_t* new_lengths;       // [segments] with starts
-};
-
-__device__ __forceinline__ int64_t lower_bound(const int64_t* sorted, int64_t count, int64_t value) {
-  int64_t low = 0, high = count;
-  while (low < high) {
-    const int64_t mid = (low + high) / 2;
-    if (sorted[mid] < value) low = mid + 1;
-    else high = mid;
-  }
-  return low;
-}
-
+// Rows of the segments before each one, sums[s], and of all, sums[segments]: by one workgroup in a launch
+// of its own, or (up to kFusedSegments segments, a length a thread) by every workgroup for itself.
 constexpr int kSumThreads = 1024;
+constexpr int kFusedSegments = kThreads;
 
 // A packed row number as the i32 of the packed layout (rows past 2^31 - 1 are not read).
-__device__ __forceinline__ int32_t packed_row(int64_t row) {
-  return static_cast<int32_t>(row < INT32_MAX ? row : INT32_MAX);
+template <typename Sum>
+__device__ __forceinline__ Sum packed_row(int64_t row) {
+  if constexpr (sizeof(Sum) == 4) return static_cast<Sum>(row < INT32_MAX ? row : INT32_MAX);
+  else return row;
 }
 
-__global__ __launch_bounds__(kSumThreads) void paged_sum_kernel(SumArgs a) {
+// The sum of `n` over the workgroup's threads up to and with this one.
+template <int THREADS>
+__device__ __forceinline__ int64_t running_sum(int64_t n, int64_t (&wave_total)[THREADS / 64]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t sum = n;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t other = __shfl_up(sum, d);
+    if (lane >= d) sum += other;
+  }
+  if (lane == 63) wave_total[wave] = sum;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) sum += wave_total[w];
+  return sum;
+}
+
+template <typename Sum>
+__global__ __launch_bounds__(kSumThreads) void paged_sum_kernel(PagedCache cache, int64_t segments, Sum* sums) {
   __shared__ int64_t wave_total[kSumThreads / 64];
   __shared__ int64_t before;  // rows of the segments of earlier rounds
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (threadIdx.x == 0) before = 0;
-  __syncthreads();
-  for (int64_t s0 = 0; s0 < a.segments; s0 += kSumThreads) {
+  if (threadIdx.x == 0) before = 0, sums[0] = 0;
+  for (int64_t s0 = 0; s0 < segments; s0 += kSumThreads) {
     const int64_t s = s0 + threadIdx.x;
-    const int64_t n = s < a.segments ? a.cache.rows(s) : 0;
-    int64_t sum = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t other = __shfl_up(sum, d);
-      if (lane >= d) sum += other;
-    }
-    if (lane == 63) wave_total[wave] = sum;
+    const int64_t sum = running_sum<kSumThreads>(s < segments ? cache.rows(s) : 0, wave_total) + before;
+    if (s < segments) sums[s + 1] = packed_row<Sum>(sum);
     __syncthreads();
-    int64_t first = before + sum - n, total = before;
-    for (int w = 0; w < kSumThreads / 64; ++w) {
-      if (w < wave) first += wave_total[w];
-      total += wave_total[w];
-    }
-    if (s < a.segments) {
-      if (a.cumulative != nullptr) a.cumulative[s] = packed_row(first);
-      if (a.starts != nullptr) {
-        const int64_t low = lower_bound(a.removed, a.removed_count, first);
-        const int64_t high = lower_bound(a.removed, a.removed_count, first + n);
-        const int64_t gone = high - low < n ? high - low : n;
-        a.starts[s] = low;
-        a.first_rows[s] = first;
-        a.new_lengths[s] = static_cast<int32_t>(n - gone);
-      }
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) before = total;
+    if (threadIdx.x == kSumThreads - 1) before = sum;
     __syncthreads();
   }
-  if (threadIdx.x == 0 && a.cumulative != nullptr)
-    a.cumulative[a.segments] = packed_row(before);
+}
+
+template <typename Sum>
+__device__ __forceinline__ void sum_lengths(const PagedCache& cache, int segments, Sum* sums) {
+  __shared__ int64_t wave_total[kThreads / 64];
+  const int thread = static_cast<int>(threadIdx.x);
+  const int64_t sum = running_sum<kThreads>(thread < segments ? cache.rows(thread) : 0, wave_total);
+  if (thread == 0) sums[0] = 0;
+  if (thread < segments) sums[thread + 1] = packed_row<Sum>(sum);
+  __syncthreads();
 }
 
 // ---------------------------------------------------------------------------------------
@@ -278,26 +259,6 @@ __device__ __forceinline__ Eight<T> eight_values(unsigned codes, float scale) {
 }
 
 constexpr int kReadRows = 64;             // of a workgroup
-constexpr int kFusedSegments = kThreads;  // one length a thread
-
-// Cumulative lengths of up to kFusedSegments segments in LDS, by every workgroup for itself.
-__device__ __forceinline__ void sum_lengths(const PagedCache& cache, int segments, int32_t* cumulative) {
-  __shared__ int64_t wave_total[kThreads / 64];
-  const int thread = static_cast<int>(threadIdx.x), lane = thread & 63, wave = thread >> 6;
-  int64_t sum = thread < segments ? cache.rows(thread) : 0;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t other = __shfl_up(sum, d);
-    if (lane >= d) sum += other;
-  }
-  if (lane == 63) wave_total[wave] = sum;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) sum += wave_total[w];
-  if (thread == 0) cumulative[0] = 0;
-  if (thread < segments) cumulative[thread + 1] = packed_row(sum);
-  __syncthreads();
-}
-
 // The segment that packed row `row` < cumulative[segments] belongs to: the largest s with
 // cumulative[s] <= row.
 __device__ __forceinline__ int segment_of(const int32_t* cumulative, int segments, int row) {
@@ -378,88 +339,129 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(ReadArgs a) {
 struct CompactArgs {
   PagedCache cache;
   int64_t segments;
-  int chunks;                   // row chunks of a segment (each 64 rows)
+  int chunks;                   // of kCompactRows rows of a segment
   const int32_t* target;        // [segments, target_pages]
   int target_pages;
-  const int64_t* removed;
+  const int64_t* removed;       // sorted packed rows
   int64_t removed_count;
-  const int64_t* starts;
-  const int64_t* first_rows;
-  const int32_t* new_lengths;
+  const int64_t* sums;          // [segments + 1], unless the workgroups sum the lengths themselves
+  int32_t* new_lengths;
 };
 
-// A wave moves 64 rows of a segment: lane r finds where row r comes from (row + how many removed
-// rows lie at or before it), then all lanes copy 16 bytes each of the rows' codes.
-template <int D>
+constexpr int kCompactRows = kThreads;  // of a workgroup, 64 a wave
+
+// The first of [low, high) that is not `before` (all of those before it are): 32 lanes look at 32
+// places a round, each half of the wave for a range of its own.
+template <typename F>
+__device__ __forceinline__ int64_t half_search(int64_t low, int64_t high, F before) {
+  const int place = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
+  while (true) {
+    const int64_t step = (high - low + 31) / 32;  // 0 once the range is empty
+    const int64_t at = low + place * step;
+    const bool below = step > 0 && at < high && before(at);
+    const unsigned held = static_cast<unsigned>(__ballot(below) >> (32 * half));
+    const int count = __builtin_popcount(held);  // of the places looked at, the first ones
+    if (step > 0) {
+      const int64_t next = low + count * step;
+      low = count > 0 ? low + (count - 1) * step + 1 : low;
+      high = next < high ? next : high;
+    }
+    if (!__any(high > low)) return low;
+  }
+}
+
+// A wave moves 64 rows of a segment: row r comes from row r + how many removed rows lie at or before
+// it. The wave finds that number for its first and its last row, each lane its own between them;
+// then all lanes copy 16 bytes each of the rows' codes.
+template <int D, bool FUSED>
 __global__ __launch_bounds__(kThreads) void paged_compact_kernel(CompactArgs a) {
-  constexpr int kChunks = D / 32;  // 16-byte pieces of a row's codes
+  constexpr int kPieces = D / 32;  // 16 bytes of a row's codes
   using Scales = std::conditional_t<D == 64, uint16_t, std::conditional_t<D == 128, uint32_t, uint64_t>>;
-  const int lane = threadIdx.x & 63;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
-  const int64_t segment = unit / a.chunks;
-  if (segment >= a.segments) return;
-  const int row0 = static_cast<int>(unit - segment * a.chunks) * 64;
+  __shared__ int64_t lds_sums[FUSED ? kFusedSegments + 1 : 1];
   const PagedCache& cache = a.cache;
-  const int rows = min(a.new_lengths[segment], a.target_pages << cache.shift);
+  const int lane = threadIdx.x & 63;
+  const int64_t segment = blockIdx.x / static_cast<unsigned>(a.chunks);
+  const int chunk = static_cast<int>(blockIdx.x - segment * a.chunks);
+  const int64_t* sums = a.sums;
+  if constexpr (FUSED) {
+    sum_lengths(cache, static_cast<int>(a.segments), lds_sums);
+    sums = lds_sums;
+  }
+  const int64_t first = sums[segment];
+  const int length = cache.rows(segment);
+  const int row0 = chunk * kCompactRows + static_cast<int>(threadIdx.x & ~63u);
+  if (chunk > 0 && row0 >= length) return;  // no row can be left there
+  // the segment's part of the removed rows
+  const int64_t bound = lane < 32 ? first : first + length;
+  const int64_t found = half_search(0, a.removed_count, [&](int64_t i) { return a.removed[i] < bound; });
+  const int64_t low = __shfl(found, 0);
+  const int64_t inside = __shfl(found, 32) - low;  // (negative for rows that are not sorted)
+  const int gone = static_cast<int>(inside < 0 ? 0 : inside < length ? inside : length);
+  const int left = length - gone;
+  if (chunk == 0 && threadIdx.x == 0) a.new_lengths[segment] = left;
+  const int rows = min(left, a.target_pages << cache.shift);
   if (row0 >= rows) return;
-  const int row = row0 + lane;
-  const int mask = (1 << cache.shift) - 1;
-  int64_t from = -1, to = -1;  // byte offsets of the rows' pages; slots apart
-  int from_slot = 0, to_slot = 0;
-  if (row < rows) {
-    const int64_t first = a.first_rows[segment], low = a.starts[segment];
-    const int64_t length = cache.rows(segment);
-    int64_t j = 0, high = min(length - a.new_lengths[segment], a.removed_count - low);
-    while (j < high) {  // removed rows whose index less their rank is at most `row`
-      const int64_t mid = (j + high) / 2;
-      if (a.removed[low + mid] - first - mid <= row) j = mid + 1;
-      else high = mid;
+  const int64_t* removed = a.removed + low;
+  // how many removed rows (of this segment) lie at or before kept row `row`
+  auto lies_before = [&](int row) { return [=](int64_t i) { return removed[i] - first - i <= row; }; };
+  int64_t j = half_search(0, gone, lies_before(lane < 32 ? row0 : row0 + 63));
+  const int row = row0 + lane, mask = (1 << cache.shift) - 1;
+  {
+    int64_t from = __shfl(j, 0), to = __shfl(j, 32);
+    while (from < to) {
+      const int64_t mid = (from + to) / 2;
+      if (lies_before(row)(mid)) from = mid + 1;
+      else to = mid;
     }
-    const int source = static_cast<int>(row + j);
-    if (source < length) {
-      const int64_t id = cache.table[segment * cache.max_pages + (source >> cache.shift)];
-      const int64_t target = a.target[segment * a.target_pages + (row >> cache.shift)];
-      if (id >= 0 && id < cache.page_count && target >= 0 && target < cache.page_count) {
-        from = id * (Page<D>::bytes(1) << cache.shift);
-        to = target * (Page<D>::bytes(1) << cache.shift);
-        from_slot = source & mask;
-        to_slot = row & mask;
-      }
+    j = from;
+  }
+  // byte offsets of the row's old and new pages (-1: none), and its slots there
+  int64_t from = -1, to = -1;
+  const int64_t source = row + j;
+  if (row < rows && source < length) {
+    const int64_t id = cache.table[segment * cache.max_pages + (source >> cache.shift)];
+    const int64_t target = a.target[segment * a.target_pages + (row >> cache.shift)];
+    if (id >= 0 && id < cache.page_count && target >= 0 && target < cache.page_count) {
+      from = id * (Page<D>::bytes(1) << cache.shift);
+      to = target * (Page<D>::bytes(1) << cache.shift);
     }
   }
-  if (from >= 0) {
+  const int from_slot = static_cast<int>(source) & mask, to_slot = row & mask;
+  // All loads before the first store (a row that is not moved reads the pool's first one).
+  const uint8_t* const page = cache.pages + (from >= 0 ? from : 0);
+  const int read_slot = from >= 0 ? from_slot : 0;
+  Scales scales[2];
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+    scales[which] = *reinterpret_cast<const Scales*>(page + Page<D>::scales(cache.shift, which, read_slot));
+  const float position = *reinterpret_cast<const float*>(page + Page<D>::position(cache.shift, read_slot));
+  move_u32x4 data[2][kPieces];
+  int64_t target[kPieces];
+#pragma unroll
+  for (int u = 0; u < kPieces; ++u) {
+    const int piece = u * 64 + lane, r = piece / kPieces, c = piece % kPieces;
+    const int64_t piece_from = __shfl(from, r), piece_to = __shfl(to, r);
+    const int slot = __shfl(read_slot, r), target_slot = __shfl(to_slot, r);
+    const uint8_t* p = cache.pages + (piece_from >= 0 ? piece_from : 0);
 #pragma unroll
     for (int which = 0; which < 2; ++which)
-      *reinterpret_cast<Scales*>(cache.pages + to + Page<D>::scales(cache.shift, which, to_slot)) =
-          *reinterpret_cast<const Scales*>(cache.pages + from +
-                                           Page<D>::scales(cache.shift, which, from_slot));
-    *reinterpret_cast<float*>(cache.pages + to + Page<D>::position(cache.shift, to_slot)) =
-        *reinterpret_cast<const float*>(cache.pages + from + Page<D>::position(cache.shift, from_slot));
-  }
-  move_u32x4 data[2][kChunks];
-  int64_t target[kChunks];
-#pragma unroll
-  for (int u = 0; u < kChunks; ++u) {
-    const int piece = u * 64 + lane, r = piece / kChunks, c = piece % kChunks;
-    const int64_t page = __shfl(from, r);
-    const int slot = __shfl(from_slot, r);
-    target[u] = __shfl(to, r);
-    const int target_slot = __shfl(to_slot, r);
-    if (page < 0) target[u] = -1;
-#pragma unroll
-    for (int which = 0; which < 2; ++which)
-      if (page >= 0)
-        data[which][u] = *reinterpret_cast<const move_u32x4*>(
-            cache.pages + page + Page<D>::codes(cache.shift, which, slot) + 16 * c);
-    if (page >= 0) target[u] += Page<D>::codes(cache.shift, 0, target_slot) + 16 * c;
+      data[which][u] = *reinterpret_cast<const move_u32x4*>(
+          p + Page<D>::codes(cache.shift, which, slot) + 16 * c);
+    target[u] = piece_to < 0 ? -1 : piece_to + Page<D>::codes(cache.shift, 0, target_slot) + 16 * c;
   }
 #pragma unroll
-  for (int u = 0; u < kChunks; ++u)
+  for (int u = 0; u < kPieces; ++u)
+    if (target[u] >= 0)
 #pragma unroll
-    for (int which = 0; which < 2; ++which)
-      if (target[u] >= 0)
-        *reinterpret_cast<move_u32x4*>(cache.pages + target[u] +
-                                       Page<D>::codes(cache.shift, which, 0)) = data[which][u];
+      for (int which = 0; which < 2; ++which)
+        *reinterpret_cast<move_u32x4*>(cache.pages + target[u] + Page<D>::codes(cache.shift, which, 0)) =
+            data[which][u];
+  if (to < 0) return;
+  uint8_t* const out = cache.pages + to;
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+    *reinterpret_cast<Scales*>(out + Page<D>::scales(cache.shift, which, to_slot)) = scales[which];
+  *reinterpret_cast<float*>(out + Page<D>::position(cache.shift, to_slot)) = position;
 }
 
 template <typename F>
@@ -575,16 +577,14 @@ extern "C" int lr_paged_read(const void* pages, int64_t page_count, int64_t page
   // One launch where a workgroup can sum the lengths itself, beside its rows' lookups; calls without
   // rows or pages have only the sums to write.
   const bool fused = segments <= kFusedSegments && total > 0 && page_count > 0;
-  SumArgs sums{};
-  sums.cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
-  sums.segments = segments;
-  sums.cumulative = cumulative;
+  const PagedCache cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
   if (!fused) {
-    hipLaunchKernelGGL(paged_sum_kernel, dim3(1), dim3(kSumThreads), 0, as_stream(stream), sums);
+    hipLaunchKernelGGL(paged_sum_kernel<int32_t>, dim3(1), dim3(kSumThreads), 0, as_stream(stream),
+                       cache, segments, cumulative);
     if (int status = check_launch("paged_read lengths")) return status;
     if (total == 0 || page_count == 0) return LR_OK;
   }
-  const ReadArgs args{sums.cache, segments, total, cumulative, keys, values, positions};
+  const ReadArgs args{cache, segments, total, cumulative, keys, values, positions};
   const int64_t blocks = ceil_div(total, kReadRows);
   return dispatch_type(dtype, [&]<typename T>() {
     return dispatch_dim(dim, [&]<int D>() {
@@ -600,7 +600,7 @@ extern "C" int lr_paged_read(const void* pages, int64_t page_count, int64_t page
 }
 
 extern "C" size_t lr_paged_compact_workspace_bytes(int64_t segments) {
-  return segments > 0 ? static_cast<size_t>(2 * segments) * sizeof(int64_t) : 0;
+  return segments > kFusedSegments ? static_cast<size_t>(segments + 1) * sizeof(int64_t) : 0;
 }
 
 extern "C" int lr_paged_compact(void* pages, int64_t page_count, int64_t page_size,
@@ -616,38 +616,35 @@ extern "C" int lr_paged_compact(void* pages, int64_t page_count, int64_t page_si
                  target_pages >= 0 && target_pages <= INT32_MAX / 2 / page_size &&
                  (target || target_pages == 0),
              "Invalid compaction");
-  LR_REQUIRE(workspace && workspace_size >= lr_paged_compact_workspace_bytes(segments) &&
+  const size_t needed = lr_paged_compact_workspace_bytes(segments);
+  LR_REQUIRE(workspace_size >= needed && (needed == 0 || workspace) &&
                  reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
              "Compaction workspace too small");
-  SumArgs sums{};
-  sums.cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
-  sums.segments = segments;
-  sums.removed = removed;
-  sums.removed_count = removed_count;
-  sums.starts = static_cast<int64_t*>(workspace);
-  sums.first_rows = sums.starts + segments;
-  sums.new_lengths = new_lengths;
-  hipLaunchKernelGGL(paged_sum_kernel, dim3(1), dim3(kSumThreads), 0, as_stream(stream), sums);
-  if (int status = check_launch("paged_compact lengths")) return status;
   CompactArgs args{};
-  args.cache = sums.cache;
+  args.cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
   args.segments = segments;
-  // rows that a segment can keep: what both tables hold
-  const int64_t rows = std::min(max_pages, target_pages) * page_size;
-  if (rows == 0) return LR_OK;
-  args.chunks = static_cast<int>(ceil_div(rows, 64));
+  // a segment's rows, kept or not, are at most what its table holds
+  args.chunks = static_cast<int>(std::max<int64_t>(1, ceil_div(max_pages * page_size, kCompactRows)));
   args.target = target;
-  args.target_pages = static_cast<int>(target_pages);
+  // (without a page there is nothing to move: the lengths alone)
+  args.target_pages = page_count == 0 ? 0 : static_cast<int>(target_pages);
   args.removed = removed;
   args.removed_count = removed_count;
-  args.starts = sums.starts;
-  args.first_rows = sums.first_rows;
+  args.sums = static_cast<int64_t*>(workspace);
   args.new_lengths = new_lengths;
-  const int64_t blocks = ceil_div(segments * args.chunks, kThreads / 64);
-  LR_REQUIRE(blocks < (int64_t{1} << 31), "Compaction grid too large");
+  LR_REQUIRE(segments <= INT32_MAX / args.chunks, "Compaction grid too large");
+  if (needed) {
+    hipLaunchKernelGGL(paged_sum_kernel<int64_t>, dim3(1), dim3(kSumThreads), 0, as_stream(stream),
+                       args.cache, segments, static_cast<int64_t*>(workspace));
+    if (int status = check_launch("paged_compact lengths")) return status;
+  }
   return dispatch_dim(dim, [&]<int D>() {
-    hipLaunchKernelGGL((paged_compact_kernel<D>), dim3(static_cast<unsigned>(blocks)),
-                       dim3(kThreads), 0, as_stream(stream), args);
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(segments * args.chunks)), dim3(kThreads),
+                         0, as_stream(stream), args);
+    };
+    if (needed) launch(paged_compact_kernel<D, false>);
+    else launch(paged_compact_kernel<D, true>);
     return check_launch("paged_compact");
   });
 }

@@ -275,12 +275,10 @@ def test_lengths_past_the_table_are_cut(device):
     assert np.array_equal(got[0].double().cpu().numpy(), cache.rows(0, 16)[0])
 
 
-@pytest.mark.parametrize("dim,page_size", [(64, 16), (128, 32), (256, 64)])
-@pytest.mark.parametrize("share", [0.0, 0.1, 0.6, 1.0])
-def test_compact(device, dim, page_size, share):
-    rng = np.random.default_rng(int(100 * share) + dim)
-    lengths = np.array([0, 1, 16, 33, 64, 65, 200, 150])
-    cache = Cache(device, lengths, 2, dim, page_size, seed=dim)
+def check_compact(device, lengths, dim, page_size, share, seed=0):
+    rng = np.random.default_rng(seed)
+    lengths = np.asarray(lengths)
+    cache = Cache(device, lengths, 1, dim, page_size, seed=dim)
     keep = [np.sort(rng.permutation(n)[:n - int(round(share * n))]) for n in lengths]
     starts = np.concatenate([[0], np.cumsum(lengths)])
     removed = np.concatenate([starts[s] + np.setdiff1d(np.arange(n), keep[s])
@@ -298,16 +296,31 @@ def test_compact(device, dim, page_size, share):
     torch.cuda.synchronize()
     assert got.lengths.cpu().tolist() == [len(k) for k in keep]
     assert cache.layer.lengths.cpu().tolist() == lengths.tolist()
-    for s in range(len(lengths)):  # the rows' bytes, section by section
-        widths = [dim // 2, dim // 2, dim // 32, dim // 32, 4]
-        offset = 0
-        for w in widths:
-            for to, source in enumerate(keep[s]):
-                a = cache.table[s, source // page_size], offset + source % page_size * w
-                b = target[s, to // page_size], offset + to % page_size * w
-                cache.pages[b[0], b[1]:b[1] + w] = cache.pages[a[0], a[1]:a[1] + w]
-            offset += page_size * w
+    for s, kept in enumerate(keep):  # the rows' bytes, section by section
+        to, offset = np.arange(len(kept)), 0
+        for width in (dim // 2, dim // 2, dim // 32, dim // 32, 4):
+            place = lambda table, row: (  # noqa: E731
+                table[s, row // page_size][:, None],
+                offset + (row % page_size)[:, None] * width + np.arange(width))
+            cache.pages[place(target, to)] = cache.pages[place(cache.table, kept)]
+            offset += page_size * width
     cache.check_pages()
+
+
+@pytest.mark.parametrize("dim,page_size", [(64, 16), (128, 32), (256, 64)])
+@pytest.mark.parametrize("share", [0.0, 0.1, 0.6, 1.0])
+def test_compact(device, dim, page_size, share):
+    check_compact(device, [0, 1, 16, 33, 64, 65, 200, 150], dim, page_size, share)
+
+
+def test_compact_long_and_many_segments(device):
+    """Searches of several rounds; more segments than a workgroup sums for itself."""
+    check_compact(device, [3000, 0, 5, 2600], 64, 128, 0.4, seed=1)
+    check_compact(device, [3000, 0, 5, 2600], 128, 16, 0.02, seed=2)
+    lengths = np.random.default_rng(3).integers(0, 12, 700)
+    check_compact(device, lengths, 64, 16, 0.5, seed=4)
+    check_compact(device, lengths[:256], 64, 16, 0.3, seed=5)
+    check_compact(device, lengths[:257], 64, 16, 0.3, seed=6)
 
 
 def test_compact_into_a_short_table_and_missing_pages(device):

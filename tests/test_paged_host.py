@@ -132,17 +132,21 @@ def test_read_and_compact_refusals():
                           (dict(keys=264), "16-byte aligned")]:
         assert read(**over) == 1 and message in _lib.last_error(), over
     compact = lambda **o: library.lr_paged_compact(  # noqa: E731
-        256, 4, 32, 8, 2, 8, 2, 128, o.get("removed", 8), o.get("count", 3), o.get("target", 8),
+        256, 4, 32, 8, 2, 8, o.get("segments", 2), 128, o.get("removed", 8), o.get("count", 3),
+        o.get("target", 8),
         o.get("width", 2), o.get("lengths", 8), o.get("workspace", 256), o.get("size", 64), None)
     for over, message in [(dict(removed=None), "Invalid compaction"),
                           (dict(count=-1), "Invalid compaction"),
                           (dict(target=None), "Invalid compaction"),
                           (dict(width=2 ** 30), "Invalid compaction"),
                           (dict(lengths=None), "Invalid compaction"),
-                          (dict(workspace=None), "workspace too small"),
-                          (dict(size=16), "workspace too small")]:
+                          (dict(segments=0), "Invalid page table"),
+                          (dict(segments=300, workspace=None), "workspace too small"),
+                          (dict(segments=300, size=64), "workspace too small"),
+                          (dict(segments=300, size=1 << 20, workspace=8), "workspace too small")]:
         assert compact(**over) == 1 and message in _lib.last_error(), over
-    assert library.lr_paged_compact_workspace_bytes(2) <= 64
+    assert library.lr_paged_compact_workspace_bytes(256) == 0
+    assert library.lr_paged_compact_workspace_bytes(257) == 258 * 8
 
 
 def cpu_layer():
