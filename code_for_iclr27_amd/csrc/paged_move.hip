@@ -85,7 +85,7 @@ struct AppendArgs {
   const float* sin;
   int64_t table_rows;
   int half;
-  unsigned kv_heads, query_heads, added;
+  unsigned batch, kv_heads, query_heads, added;
   unsigned kv_rows, query_rows;  // batch * heads * added
   unsigned kv_blocks;            // workgroups of the keys, and of the values
   const int32_t* counts;         // [batch] rows of `added` that are there, or NULL
@@ -97,6 +97,66 @@ template <int BIT>
 __device__ __forceinline__ float quad_max(float x) {
   return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
                       0, __builtin_bit_cast(int, x), BIT == 0 ? 0xB1 : 0x4E, 0xF, 0xF, false)));
+}
+
+// Eight of a block's elements as codes, with the block's scale byte; four consecutive lanes call it
+// with the block's elements.
+struct Quantised {
+  unsigned codes, scale;
+};
+__device__ __forceinline__ Quantised quantise(const float (&x)[8], ScaleRange range) {
+  float top = 0.0f, sum = 0.0f;  // sum: NaN if an element is not finite
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    top = fmaxf(top, __builtin_fabsf(x[e]));
+    sum = __builtin_fmaf(x[e], 0.0f, sum);
+  }
+  top = sum == sum ? top : __builtin_huge_valf();
+  top = quad_max<1>(quad_max<0>(top));
+  const bool finite = top < __builtin_huge_valf();
+  // 2^(floor(log2 top) - 2), one more where the significand is at least 1.75 (a carry into the exponent)
+  int exponent = static_cast<int>((__builtin_bit_cast(unsigned, top) + 0x200000u) >> 23) - 129;
+  exponent = exponent < range.low ? range.low : exponent > range.high ? range.high : exponent;
+  const unsigned byte = finite ? static_cast<unsigned>(exponent + 127) : kScaleNaN;
+  const float scale = scale_of(finite ? byte : 127u);
+  unsigned codes = 0;
+  if (finite) {
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], scale, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], scale, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], scale, 2);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], scale, 3);
+  }
+  return {codes, byte};
+}
+
+// The page of row lengths[segment] + i, and its slot; NULL where there is none.
+struct Spot {
+  uint8_t* page;
+  int slot;
+};
+template <int D>
+__device__ __forceinline__ Spot new_row(const PagedCache& cache, int64_t segment, unsigned i) {
+  const int n = cache.lengths[segment];
+  const int64_t at = static_cast<int64_t>(n) + i;
+  if (n < 0 || at >= static_cast<int64_t>(cache.max_pages) << cache.shift) return {nullptr, 0};
+  const int64_t id = cache.table[segment * cache.max_pages + (at >> cache.shift)];
+  if (id < 0 || id >= cache.page_count) return {nullptr, 0};
+  return {cache.pages + id * (Page<D>::bytes(1) << cache.shift),
+          static_cast<int>(at) & ((1 << cache.shift) - 1)};
+}
+
+// Chunk c (eight channels) of a K (what 0) or V (1) row.
+template <int D>
+__device__ __forceinline__ void store_eight(const PagedCache& cache, const Spot& spot, int what, int c,
+                                            const Quantised& q) {
+  *reinterpret_cast<unsigned*>(spot.page + Page<D>::codes(cache.shift, what, spot.slot) + 4 * c) = q.codes;
+  if (c % 4 == 0)
+    spot.page[Page<D>::scales(cache.shift, what, spot.slot) + c / 4] = static_cast<uint8_t>(q.scale);
+}
+template <int D>
+__device__ __forceinline__ void store_position(const PagedCache& cache, const Spot& spot, int64_t position) {
+  *reinterpret_cast<float*>(spot.page + Page<D>::position(cache.shift, spot.slot)) =
+      static_cast<float>(position);
 }
 
 template <typename T, int D>
@@ -144,44 +204,83 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs a) {
     return;
   }
 
-  float top = 0.0f, sum = 0.0f;  // sum: NaN if an element is not finite
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    top = fmaxf(top, __builtin_fabsf(x[e]));
-    sum = __builtin_fmaf(x[e], 0.0f, sum);
-  }
-  top = sum == sum ? top : __builtin_huge_valf();
-  top = quad_max<1>(quad_max<0>(top));
-  const bool finite = top < __builtin_huge_valf();
-  int exponent = static_cast<int>((__builtin_bit_cast(unsigned, top) + 0x200000u) >> 23) - 129;
-  exponent = exponent < a.range.low ? a.range.low : exponent > a.range.high ? a.range.high : exponent;
-  const unsigned byte = finite ? static_cast<unsigned>(exponent + 127) : kScaleNaN;
-  const float scale = scale_of(finite ? byte : 127u);
-  unsigned codes = 0;
-  if (finite) {
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], scale, 0);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], scale, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], scale, 2);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], scale, 3);
-  }
-
-  const PagedCache& cache = a.cache;
-  const int n = cache.lengths[segment];
-  const int64_t at = static_cast<int64_t>(n) + i;
-  if (n < 0 || at >= static_cast<int64_t>(cache.max_pages) << cache.shift) return;
-  const int to = static_cast<int>(at);
-  const int64_t id = cache.table[static_cast<int64_t>(segment) * cache.max_pages + (to >> cache.shift)];
-  if (id < 0 || id >= cache.page_count) return;
-  const int slot = to & ((1 << cache.shift) - 1);
-  uint8_t* page = cache.pages + id * (Page<D>::bytes(1) << cache.shift);
-  *reinterpret_cast<unsigned*>(page + Page<D>::codes(cache.shift, what, slot) + 4 * c) = codes;
-  if (c % 4 == 0) page[Page<D>::scales(cache.shift, what, slot) + c / 4] = static_cast<uint8_t>(byte);
-  if (what == 0 && c == 0)
-    *reinterpret_cast<float*>(page + Page<D>::position(cache.shift, slot)) =
-        static_cast<float>(position);
+  const Quantised q = quantise(x, a.range);
+  const Spot spot = new_row<D>(a.cache, segment, i);
+  if (spot.page == nullptr) return;
+  store_eight<D>(a.cache, spot, what, c, q);
+  if (what == 0 && c == 0) store_position<D>(a.cache, spot, position);
 }
 
-// ---------------------------------------------------------------------------------------
+// The same where whole blocks are rotated (half a multiple of 32): D / 16 threads a row, each with a
+// chunk and its partner (rotated: channels c and c + half; the others: half of them apart), so that
+// a cosine and sine are loaded once for both, and for the same chunks of HEADS heads, whose loads
+// are in flight together.
+template <typename T, int D, int HEADS>
+__global__ __launch_bounds__(kThreads) void paged_append_pairs_kernel(AppendArgs a) {
+  constexpr int kRowThreads = D / 16, kUnits = kThreads / kRowThreads;
+  const int what = blockIdx.x < a.kv_blocks ? 0 : blockIdx.x < 2 * a.kv_blocks ? 1 : 2;
+  const unsigned unit = (blockIdx.x - what * a.kv_blocks) * kUnits + threadIdx.x / kRowThreads;
+  const unsigned heads = what == 2 ? a.query_heads : a.kv_heads;
+  const unsigned head_groups = (heads + HEADS - 1) / HEADS;
+  const unsigned place = unit / head_groups, h0 = (unit - place * head_groups) * HEADS;
+  const unsigned b = place / a.added, i = place - b * a.added;
+  if (b >= a.batch) return;  // whole rows are in or out: the exchanges below stay within a row
+  if (what != 2 && a.counts != nullptr && static_cast<int64_t>(i) >= a.counts[b]) return;
+  const int t = threadIdx.x % kRowThreads, pairs = what == 1 ? 0 : a.half / 8;
+  const bool rotated = t < pairs;
+  const int lo = rotated ? t : t + pairs, hi = lo + (rotated ? pairs : D / 16 - pairs);
+
+  const Rows& rows = what == 0 ? a.keys : what == 1 ? a.values : a.queries;
+  const T* source = static_cast<const T*>(rows.base) + b * rows.batch + i * rows.row;
+  Eight<T> first[HEADS], second[HEADS];
+#pragma unroll
+  for (int n = 0; n < HEADS; ++n) {
+    const T* p = source + min(h0 + n, heads - 1) * rows.head;
+    first[n] = *reinterpret_cast<const Eight<T>*>(p + 8 * lo);
+    second[n] = *reinterpret_cast<const Eight<T>*>(p + 8 * hi);
+  }
+  const int64_t position = what == 1 ? 0 : a.positions[static_cast<int64_t>(b) * a.added + i];
+  const bool known = position >= 0 && position < a.table_rows;
+  float cosine[8], sine[8];
+  if (rotated) {
+    const int64_t at = (known ? position : 0) * a.half + 8 * t;
+    reinterpret_cast<const Eight<float>*>(a.cos + at)->get(cosine);
+    reinterpret_cast<const Eight<float>*>(a.sin + at)->get(sine);
+  }
+#pragma unroll
+  for (int n = 0; n < HEADS; ++n) {
+    if (h0 + n >= heads) break;
+    float x[8], y[8];
+    first[n].get(x);
+    second[n].get(y);
+    if (rotated) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float xc = x[e] * cosine[e], ys = y[e] * sine[e], yc = y[e] * cosine[e], xs = x[e] * sine[e];
+        x[e] = known ? xc - ys : __builtin_nanf("");
+        y[e] = known ? yc + xs : __builtin_nanf("");
+      }
+    }
+    if (what == 2) {
+      T* out = static_cast<T*>(a.out_queries) +
+               ((static_cast<int64_t>(b) * heads + h0 + n) * a.added + i) * D;
+      Eight<T> result;
+      result.set(x);
+      *reinterpret_cast<Eight<T>*>(out + 8 * lo) = result;
+      result.set(y);
+      *reinterpret_cast<Eight<T>*>(out + 8 * hi) = result;
+      continue;
+    }
+    const Quantised p = quantise(x, a.range), q = quantise(y, a.range);
+    const Spot spot = new_row<D>(a.cache, static_cast<int64_t>(b) * heads + h0 + n, i);
+    if (spot.page == nullptr) continue;
+    store_eight<D>(a.cache, spot, what, lo, p);
+    store_eight<D>(a.cache, spot, what, hi, q);
+    if (what == 0 && t == 0) store_position<D>(a.cache, spot, position);
+  }
+}
+
+
 // Rows of the segments before each one, sums[s], and of all, sums[segments]: by one workgroup in a launch
 // of its own, or (up to kFusedSegments segments, a length a thread) by every workgroup for itself.
 constexpr int kSumThreads = 1024;
@@ -547,15 +646,26 @@ extern "C" int lr_paged_append(const void* keys, const int64_t* key_strides, con
   args.counts = counts;
   args.range = dtype == LR_DTYPE_F16 ? kHalfRange : kWideRange;
   args.cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
-  const int64_t per_block = kThreads / (dim / 8);
-  const int64_t kv_blocks = ceil_div(args.kv_rows, per_block);
-  const int64_t blocks = 2 * kv_blocks + ceil_div(args.query_rows, per_block);
+  args.batch = static_cast<unsigned>(batch);
+  // Rotated blocks whole: the pairs kernel, four heads a thread where there are enough rows to fill
+  // the chip with them.
+  const bool pairs = half % kBlock == 0;
+  const int64_t all_rows = 2 * static_cast<int64_t>(args.kv_rows) + args.query_rows;
+  const int64_t heads = pairs && all_rows >= 32768 ? 4 : 1;
+  const int64_t per_block = kThreads / (dim / (pairs ? 16 : 8));
+  const int64_t kv_blocks = ceil_div(batch * added * ceil_div(kv_heads, heads), per_block);
+  const int64_t blocks = 2 * kv_blocks + ceil_div(batch * added * ceil_div(query_heads, heads), per_block);
   LR_REQUIRE(blocks < (int64_t{1} << 31), "Appended grid too large");
   args.kv_blocks = static_cast<unsigned>(kv_blocks);
   return dispatch_type(dtype, [&]<typename T>() {
     return dispatch_dim(dim, [&]<int D>() {
-      hipLaunchKernelGGL((paged_append_kernel<T, D>), dim3(static_cast<unsigned>(blocks)),
-                         dim3(kThreads), 0, as_stream(stream), args);
+      auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                           as_stream(stream), args);
+      };
+      if (!pairs) launch(paged_append_kernel<T, D>);
+      else if (heads == 1) launch(paged_append_pairs_kernel<T, D, 1>);
+      else launch(paged_append_pairs_kernel<T, D, 4>);
       return check_launch("paged_append");
     });
   });

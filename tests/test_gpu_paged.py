@@ -151,6 +151,13 @@ def test_append_many_rows(device):
     check_append(device, [100, 3], 2, 2, 500, 128, 64, BF16, 64, seed=4)
 
 
+@pytest.mark.parametrize("dtype,dim,half", [(BF16, 64, 32), (F32, 128, 32), (F16, 128, 64),
+                                            (BF16, 256, 0)])
+def test_append_of_many_rows_takes_several_heads_a_thread(device, dtype, dim, half):
+    """From 32,768 rows on; three and six heads are no multiple of the four that a thread takes."""
+    check_append(device, [100, 3, 0], 3, 2, 2800, dim, 64, dtype, half, counts=[2799], seed=dim)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 def test_append_edge_values(device, dtype):
     top = float(torch.finfo(dtype).max)
