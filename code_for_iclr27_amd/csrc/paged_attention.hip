@@ -597,20 +597,30 @@ void paged_tile_kernel(PagedAttnArgs a) {
   struct Codes {
     unsigned w[KS], scales;
   };
-  auto load = [&](Codes& u, int which, int key, int id0, int id1) {
-    const int id = col < 16 ? id0 : id1, slot = (key + col) & mask;
-    const PagedBytes page = (PagedBytes)(cache.pages + (id < 0 ? 0 : id) * page_bytes);
-    const PagedBytes codes = page + (Page<D>::codes(cache.shift, which, slot) + half * (D / 4));
+  // Lanes 0 .. 15 and 16 .. 31 read 16 rows each; only pages of 16 rows make them two pages.
+  const unsigned lane_slot = col & mask;
+  const unsigned lane_codes = lane_slot * Page<D>::kCodes + half * (D / 4);
+  const unsigned lane_scales = lane_slot * Page<D>::kScales + half * (DT / 2);
+  auto load = [&](Codes& k, Codes& v, int key, int id0, int id1) {
+    const PagedBytes page0 = (PagedBytes)(cache.pages + (id0 < 0 ? 0 : id0) * page_bytes);
+    const PagedBytes page1 = (PagedBytes)(cache.pages + (id1 < 0 ? 0 : id1) * page_bytes);
+    const PagedBytes page = col < 16 ? page0 : page1;
+    const int slot = key & mask;
 #pragma unroll
-    for (int n = 0; n < KS / 4; ++n) {
-      const attn_u32x4 x = *(const __attribute__((address_space(1))) attn_u32x4*)(codes + 16 * n);
+    for (int which = 0; which < 2; ++which) {
+      Codes& u = which == 0 ? k : v;
+      const PagedBytes codes = page + (Page<D>::codes(cache.shift, which, slot) + lane_codes);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) u.w[4 * n + e] = x[e];
+      for (int n = 0; n < KS / 4; ++n) {
+        const attn_u32x4 x = *(const __attribute__((address_space(1))) attn_u32x4*)(codes + 16 * n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u.w[4 * n + e] = x[e];
+      }
+      const PagedBytes scales = page + (Page<D>::scales(cache.shift, which, slot) + lane_scales);
+      if constexpr (D == 64) u.scales = *scales;
+      else if constexpr (D == 128) u.scales = *(const __attribute__((address_space(1))) uint16_t*)scales;
+      else u.scales = *(const __attribute__((address_space(1))) unsigned*)scales;
     }
-    const PagedBytes scales = page + (Page<D>::scales(cache.shift, which, slot) + half * (DT / 2));
-    if constexpr (D == 64) u.scales = *scales;
-    else if constexpr (D == 128) u.scales = *(const __attribute__((address_space(1))) uint16_t*)scales;
-    else u.scales = *(const __attribute__((address_space(1))) unsigned*)scales;
   };
   auto scale = [&](const Codes& u, int ks) {
     return scale_of(D == 64 ? u.scales : u.scales >> (8 * (ks / 4)) & 255u);
@@ -651,8 +661,7 @@ void paged_tile_kernel(PagedAttnArgs a) {
     if (key >= end) return;
     Codes k, v;
     int id0 = page_id(key), id1 = page_id(key + 16);
-    load(k, 0, key, id0, id1);
-    load(v, 1, key, id0, id1);
+    load(k, v, key, id0, id1);
     int next0 = page_id(key + kStep), next1 = page_id(key + kStep + 16);
     while (true) {
       const int later0 = page_id(key + 2 * kStep), later1 = page_id(key + 2 * kStep + 16);
@@ -690,10 +699,7 @@ void paged_tile_kernel(PagedAttnArgs a) {
       for (int r = 0; r < 16; ++r) s[r] = 0.0f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(expand8<T>(k.w[ks], scale(k, ks)), q_lds[ks][lane], s);
-      if (more) {
-        load(k, 0, key + kStep, next0, next1);
-        load(v, 1, key + kStep, next0, next1);
-      }
+      if (more) load(k, v, key + kStep, next0, next1);
       if (key + kUnit - 1 > all_see || id0 < 0 || id1 < 0) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -940,6 +946,18 @@ extern "C" size_t lr_paged_attention_workspace_bytes(int64_t segments, int64_t g
                                                      int64_t dim) {
   if (segments <= 0 || groups <= 0 || length <= 0 || max_keys < 0 || dim <= 0) return 0;
   return plan_bytes(plan_paged(segments, groups, length, max_keys), dim);
+}
+
+extern "C" int lr_paged_attention_plan(int64_t segments, int64_t groups, int64_t length,
+                                       int64_t max_keys, int64_t* plan) {
+  clear_error();
+  LR_REQUIRE(segments > 0 && groups > 0 && length > 0 && max_keys >= 0 && plan,
+             "Empty attention dimensions");
+  const PagedPlan p = plan_paged(segments, groups, length, max_keys);
+  plan[0] = p.tile_kernel ? kTileRows : kSmallRows;
+  plan[1] = p.waves;
+  plan[2] = p.splits;
+  return LR_OK;
 }
 
 extern "C" int lr_paged_attention(const void* queries, const int64_t* query_strides,

@@ -440,8 +440,44 @@ def test_prefill(device, dim, groups):
     attend(device, [0, 60], 2, groups, 250, dim, 32, seed=dim, layout="heads")
 
 
+def plan(segments, groups, length, max_keys):
+    from code_for_iclr27_amd import _lib
+    out = np.zeros(3, np.int64)
+    _lib.call("lr_paged_attention_plan", segments, groups, length, max_keys, out.ctypes.data)
+    return out.tolist()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim,page_size,groups,length", [(64, 16, 4, 32), (128, 32, 3, 43),
+                                                         (256, 64, 4, 32), (128, 16, 7, 19),
+                                                         (64, 256, 1, 120), (256, 16, 6, 22)])
+def test_tiles_of_32_rows(device, dtype, dim, page_size, groups, length):
+    lengths = np.random.default_rng(dim).integers(0, 150, 48)
+    lengths[:6] = [0, 1, 31, 32, 33, 200]
+    assert plan(48, groups, length, int(lengths.max()) + length)[::2] == [32, 1]
+    attend(device, lengths, 24, groups, length, dim, page_size, dtype, seed=length, layout="heads")
+
+
+@pytest.mark.parametrize("dim,page_size", [(64, 32), (128, 16), (256, 128)])
+def test_tiles_of_32_rows_with_split_keys(device, dim, page_size):
+    lengths = np.random.default_rng(dim).integers(0, 60, 48)
+    lengths[[3, 17, 47]] = [700, 513, 1030]
+    assert plan(48, 4, 29, 1059)[::2] == [32, 2]
+    attend(device, lengths, 24, 4, 29, dim, page_size, seed=dim)
+    attend(device, lengths, 24, 4, 29, dim, page_size, seed=dim, counts=[29, 11])
+
+
+@pytest.mark.parametrize("dim,page_size", [(64, 16), (128, 64), (256, 32)])
+def test_eight_waves(device, dim, page_size):
+    lengths = np.random.default_rng(dim).integers(0, 30, 260)
+    lengths[[0, 5, 100, 259]] = [600, 255, 256, 999]
+    assert plan(260, 3, 1, 1000) == [16, 8, 1]
+    attend(device, lengths, 10, 3, 1, dim, page_size, seed=dim)
+
+
 def test_padded_batch(device):
-    for length in (1, 5, 40):
+    for length in (1, 5, 40, 500):
+        assert plan(8, 4, length, 800)[0] == (32 if length == 500 else 16)
         attend(device, [0, 5, 100, 33, 64, 0, 7, 300], 2, 4, length, 128, 16,
                counts=[length, 0, length // 2 + 1, -1], seed=length)
 
@@ -497,11 +533,12 @@ def test_keys_in_missing_pages_do_not_count(device):
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
-@pytest.mark.parametrize("length,groups", [(1, 4), (6, 2), (40, 3)])
+@pytest.mark.parametrize("length,groups", [(1, 4), (6, 2), (40, 3), (128, 24)])
 def test_nan_blocks_reach_only_the_rows_that_see_them(device, dim, length, groups):
-    """NaN blocks of V (one each in the cached rows, at the diagonal and past the last row), and of
-    K: a row that sees a NaN key is NaN, one that sees a NaN block of V is NaN in its channels."""
+    """NaN blocks of V (in the last key of all and at the diagonal), and of K: a row that sees a NaN
+    key is NaN, one that sees a NaN block of V is NaN in its channels."""
     lengths = [45, 130]
+    assert plan(2, groups, length, 300)[0] == (32 if length == 128 else 16)
     grown = np.asarray(lengths) + length
     cache = Cache(device, grown, 2, dim, 16)
     cache.lengths = np.asarray(lengths, np.int32)
@@ -526,6 +563,53 @@ def test_nan_blocks_reach_only_the_rows_that_see_them(device, dim, length, group
     assert np.array_equal(np.isnan(got), np.isnan(expect))
     fine = ~np.isnan(expect)
     np.testing.assert_allclose(got[fine], expect[fine], rtol=2.0 ** -8, atol=1e-3)
+
+
+@pytest.mark.parametrize("length,groups", [(1, 4), (5, 3), (300, 4)])
+def test_a_non_finite_query_reaches_its_own_row_only(device, length, groups):
+    cache = Cache(device, [90 + length] * 6, 6, 64, 16)
+    cache.lengths[:] = 90
+    cache.upload()
+    queries = randn(cache.rng, (1, 6 * groups, length, 64), BF16)
+    spoiled = queries.clone()
+    spoiled[0, 1, 0, 3], spoiled[0, groups, length - 1, 60] = float("nan"), float("inf")
+    clean = paged.attention(cache.layer, queries.to(device), 90 + length).view(length, -1, 64)
+    got = paged.attention(cache.layer, spoiled.to(device), 90 + length).view(length, -1, 64)
+    bad = torch.zeros(length, 6 * groups, dtype=torch.bool)
+    bad[0, 1] = bad[length - 1, groups] = True
+    assert got.isnan().any(-1).cpu().equal(bad) and got.isnan().all(-1).cpu().equal(bad)
+    keep = ~bad.to(device)
+    assert ((got - clean)[keep].abs() <= 2.0 ** -7 * clean[keep].abs() + 1e-5).all()
+
+
+def test_shared_pages_and_wide_tables(device):
+    """Requests that share a prefix's pages read the same rows; tables far wider than their segments
+    change nothing."""
+    cache = Cache(device, [70, 100], 1, 128, 32)
+    cache.table[0, :2] = cache.table[1, :2]  # the first 64 rows are one prefix
+    cache.lengths = np.array([69, 99], np.int32)
+    cache.upload()
+    queries = randn(cache.rng, (2, 4, 1, 128), BF16)
+    rows = [cache.rows(s, n)[:2] for s, n in enumerate((70, 100))]
+    first = paged.attention(cache.layer, queries.to(device), 100)
+    check_attention(first, queries, rows, [69, 99], [1, 1], 1)
+    wide = torch.full((2, 5000), 10 ** 9, dtype=torch.int32, device=device)
+    wide[:, :cache.table.shape[1]] = cache.layer.table
+    import dataclasses
+    layer = dataclasses.replace(cache.layer, table=wide)
+    for bound in (100, 5000 * 32):
+        check_attention(paged.attention(layer, queries.to(device), bound), queries, rows, [69, 99],
+                        [1, 1], 1)
+    grown = layer.with_lengths(layer.lengths + 1)
+    for a, b in zip(paged.read(grown, 170), paged.read(cache.layer.with_lengths(grown.lengths), 170)):
+        assert torch.equal(a, b)
+    target = torch.full_like(wide, -1)
+    target[0, 0], target[1, 0] = (int(p) for p in cache.spare[:2])
+    removed = torch.arange(60, 160, device=device)  # ten of the first stay out, ninety of the other
+    moved = paged.compact(grown, removed, target)
+    assert moved.lengths.cpu().tolist() == [60, 10]
+    k = paged.read(moved.with_lengths(moved.lengths.clamp(max=32)), 42)[0].double().cpu().numpy()
+    assert np.array_equal(k, np.concatenate((rows[0][0][:32], rows[1][0][90:])))
 
 
 def test_attention_equals_packed_attention_over_the_rows_read(device):
