@@ -98,7 +98,7 @@ SIGNATURES = {
     "lr_paged_append": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P, _P, _P,
                         _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P],
     "lr_paged_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64],
-    "lr_paged_attention_plan": [_I64, _I64, _I64, _I64, _P],
+    "lr_paged_attention_plan": [_I64, _I64, _I64, _I64, _I64, _P],
     "lr_paged_attention": [_P, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I,
                            _I64, _P, _F, _P, _P, _SZ, _P],
     "lr_paged_read": [_P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I, _I64, _P, _P, _P, _P, _P],

@@ -273,9 +273,7 @@ void paged_attention_kernel(PagedAttnArgs a) {
   using X8 = typename Vec::x8;
   using Codes = UnitCodes<D>;
   constexpr int KW = D / 32, DT = D / 16;
-  constexpr int DH = D == 256 ? 128 : D;  // channels of V in LDS at a time
-  constexpr int kHalves = D / DH, kHalfWords = DH / 32;
-  __shared__ __align__(1024) uint16_t v_lds[WAVES][kUnit * DH];
+  __shared__ __align__(1024) uint16_t v_lds[WAVES][kUnit * D];
   __shared__ float wave_ml[WAVES][kSmallRows][2];
   __shared__ __align__(16) attn_u32x4 q_lds[KW][64];
 
@@ -346,17 +344,16 @@ void paged_attention_kernel(PagedAttnArgs a) {
   uint32_t read_at;  // of the lane's transposed reads: row 4 j + m / 4, columns 4 (m % 4) .. + 3
   {
     const int r = 4 * j + (m >> 2), chunk = (m & 3) >> 1;
-    read_at = lds_address(my_values) + r * (2 * DH) + 16 * (chunk ^ value_swizzle<DH>(r)) + 8 * (m & 1);
+    read_at = lds_address(my_values) + r * (2 * D) + 16 * (chunk ^ value_swizzle<D>(r)) + 8 * (m & 1);
   }
-  auto write_values = [&](const Codes& u, int half) {
+  auto write_values = [&](const Codes& u) {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      char* to = my_values + (16 * blk + m) * (2 * DH);
+      char* to = my_values + (16 * blk + m) * (2 * D);
 #pragma unroll
-      for (int w = 0; w < kHalfWords; ++w)
-        *reinterpret_cast<attn_u32x4*>(to + 16 * (word_chunk<DH>(j, w) ^ value_swizzle<DH>(m))) =
-            expand8<__bf16>(u.v[blk][kHalfWords * half + w],
-                            scale_of(u.vs[blk][Codes::kBytes == 2 ? half : 0]));
+      for (int w = 0; w < KW; ++w)
+        *reinterpret_cast<attn_u32x4*>(to + 16 * (word_chunk<D>(j, w) ^ value_swizzle<D>(m))) =
+            expand8<__bf16>(u.v[blk][w], scale_of(u.vs[blk][Codes::kBytes == 2 ? w / 4 : 0]));
     }
   };
 
@@ -413,7 +410,7 @@ void paged_attention_kernel(PagedAttnArgs a) {
             }
       }
       // V rows to LDS (the last unit's reads are done: a wave's LDS accesses stay in order)
-      write_values(u, 0);
+      write_values(u);
       // S^T
       attn_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -424,8 +421,6 @@ void paged_attention_kernel(PagedAttnArgs a) {
           s[blk] = Vec::mfma(__builtin_bit_cast(X8, expand8<T>(u.k[blk][w], scale_of(
                                  u.ks[blk][Codes::kBytes == 2 ? w / 4 : 0]))), q, s[blk]);
       }
-      Codes here;  // d256: the second half's codes of V outlive the next unit's loads
-      if constexpr (kHalves == 2) here = u;
       if (more) load(u, key + kStep, next0, next1);
       if (key + kUnit - 1 > all_see || id0 < 0 || id1 < 0) {
 #pragma unroll
@@ -461,24 +456,15 @@ void paged_attention_kernel(PagedAttnArgs a) {
         split_bf16(x, y, piece, n);
       }
       // O^T += V^T P^T
+      wave_fence();
 #pragma unroll
-      for (int half = 0; half < kHalves; ++half) {
-        if constexpr (kHalves == 2)
-          if (half > 0) {
-            wave_fence();
-            write_values(here, 1);
-          }
-        wave_fence();
+      for (int ct = 0; ct < DT; ++ct) {
+        const uint32_t at = read_at ^ (32 * ct);
+        const paged_u32x2 lo = read_transposed(at), hi = read_transposed(at + 16 * (2 * D));
+        const attn_bf16x8 v = __builtin_bit_cast(attn_bf16x8, attn_u32x4{lo[0], lo[1], hi[0], hi[1]});
 #pragma unroll
-        for (int c = 0; c < DH / 16; ++c) {
-          const uint32_t at = read_at ^ (32 * c);
-          const paged_u32x2 lo = read_transposed(at), hi = read_transposed(at + 16 * (2 * DH));
-          const attn_bf16x8 v = __builtin_bit_cast(attn_bf16x8, attn_u32x4{lo[0], lo[1], hi[0], hi[1]});
-          attn_f32x4& o = out[DH / 16 * half + c];
-#pragma unroll
-          for (int i = 0; i < kPieces; ++i)
-            o = AttnVec<__bf16>::mfma(v, __builtin_bit_cast(attn_bf16x8, piece[i]), o);
-        }
+        for (int i = 0; i < kPieces; ++i)
+          out[ct] = AttnVec<__bf16>::mfma(v, __builtin_bit_cast(attn_bf16x8, piece[i]), out[ct]);
       }
       wave_fence();
       if (!more) break;
@@ -501,32 +487,26 @@ void paged_attention_kernel(PagedAttnArgs a) {
     sum = pair.first + pair.second;
   }
 
-  // Wave states to LDS, DH channels at a time: 16-byte chunk c of row r in slot c ^ r.
-  constexpr int kItems = kSmallRows * (DH / 8);
+  // Wave states to LDS: 16-byte chunk c of row r in slot c ^ r.
+  __syncthreads();
+  float* const mine = reinterpret_cast<float*>(my_values) + m * D;
+#pragma unroll
+  for (int ct = 0; ct < DT; ++ct) *reinterpret_cast<attn_f32x4*>(mine + 4 * ((4 * ct + j) ^ m)) = out[ct];
+  if (j == 0) {
+    wave_ml[wave][m][0] = reference;
+    wave_ml[wave][m][1] = sum;
+  }
+  __syncthreads();
   const int64_t slot = (static_cast<int64_t>(place.unit) * a.splits + place.split) * a.tile_rows;
-#pragma unroll
-  for (int half = 0; half < kHalves; ++half) {
-    __syncthreads();
-    float* const mine = reinterpret_cast<float*>(my_values) + m * DH;
-#pragma unroll
-    for (int c = 0; c < DH / 16; ++c)
-      *reinterpret_cast<attn_f32x4*>(mine + 4 * ((4 * c + j) ^ m)) = out[DH / 16 * half + c];
-    if (j == 0 && half == 0) {
-      wave_ml[wave][m][0] = reference;
-      wave_ml[wave][m][1] = sum;
-    }
-    __syncthreads();
-    for (int item = threadIdx.x; item < kItems; item += 64 * WAVES) {
-      const int r = item / (DH / 8), c = item - r * (DH / 8);
-      if (r >= rows_here) break;
-      auto state = [&](int w, attn_f32x4& lo, attn_f32x4& hi) {
-        const float* wo = reinterpret_cast<const float*>(&v_lds[w][0]) + r * DH;
-        lo = *reinterpret_cast<const attn_f32x4*>(wo + 4 * ((2 * c) ^ r));
-        hi = *reinterpret_cast<const attn_f32x4*>(wo + 4 * ((2 * c + 1) ^ r));
-      };
-      finish_item<T, D, WAVES>(a, seg, row0 + r, DH * half + 8 * c, slot + r, keys.needed == 1,
-                               [&](int w, int i) { return wave_ml[w][r][i]; }, state);
-    }
+  for (int item = threadIdx.x; item < rows_here * (D / 8); item += 64 * WAVES) {
+    const int r = item / (D / 8), c = item - r * (D / 8);
+    auto state = [&](int w, attn_f32x4& lo, attn_f32x4& hi) {
+      const float* wo = reinterpret_cast<const float*>(&v_lds[w][0]) + r * D;
+      lo = *reinterpret_cast<const attn_f32x4*>(wo + 4 * ((2 * c) ^ r));
+      hi = *reinterpret_cast<const attn_f32x4*>(wo + 4 * ((2 * c + 1) ^ r));
+    };
+    finish_item<T, D, WAVES>(a, seg, row0 + r, 8 * c, slot + r, keys.needed == 1,
+                             [&](int w, int i) { return wave_ml[w][r][i]; }, state);
   }
 }
 
@@ -877,9 +857,10 @@ struct PagedPlan {
 // against 155 in tiles of 16, 64 queries 19 either way. Decode and short calls: chunks until there are
 // 512 workgroups (256 in tiles of 32 rows: 300 queries of d256, G6, 67 against 82 with 512), at most
 // 32 a tile, whose states a merge takes in one round of loads (8,000 rows: 9.4 against 11.6 with 63);
-// none where four units a wave reach (500 rows: 7.1 against 8.0), and in the place of two chunks one
-// workgroup of eight waves (256 segments of 2,000 rows: 16.0 against 18.8).
-PagedPlan plan_paged(int64_t segments, int64_t groups, int64_t length, int64_t max_keys) {
+// none where a few units a wave reach (five at d64: 630 rows 6.8 against 7.8; four: 500 rows 7.1
+// against 7.5, five 8.0 for 7.5; two at d256: 250 rows 7.9 for 8.4, 380 rows 9.6 against 9.2); and in
+// the place of two chunks one workgroup of eight waves (256 segments of 2,000 rows: 16.0 against 18.8).
+PagedPlan plan_paged(int64_t segments, int64_t groups, int64_t length, int64_t max_keys, int64_t dim) {
   PagedPlan p{};
   const int64_t rows = length * groups;
   p.tile_kernel = rows > kSmallRows && segments * ceil_div(rows, int64_t{kTileRows}) >= 192;
@@ -890,7 +871,7 @@ PagedPlan plan_paged(int64_t segments, int64_t groups, int64_t length, int64_t m
   p.units = segments * p.tiles;
   int64_t step = kUnit * kAttnWaves, steps = std::max<int64_t>(1, ceil_div(max_keys, step));
   int64_t wanted = std::min({steps, int64_t{32}, ceil_div(p.tile_kernel ? 256 : 512, p.units)});
-  if (steps <= 4) wanted = 1;
+  if (steps <= (dim == 64 ? 5 : dim == 128 ? 4 : 2)) wanted = 1;
   if (wanted == 2 && !p.tile_kernel) {
     p.waves = 2 * kAttnWaves;
     step *= 2;
@@ -945,15 +926,16 @@ extern "C" size_t lr_paged_attention_workspace_bytes(int64_t segments, int64_t g
                                                      int64_t length, int64_t max_keys,
                                                      int64_t dim) {
   if (segments <= 0 || groups <= 0 || length <= 0 || max_keys < 0 || dim <= 0) return 0;
-  return plan_bytes(plan_paged(segments, groups, length, max_keys), dim);
+  return plan_bytes(plan_paged(segments, groups, length, max_keys, dim), dim);
 }
 
 extern "C" int lr_paged_attention_plan(int64_t segments, int64_t groups, int64_t length,
-                                       int64_t max_keys, int64_t* plan) {
+                                       int64_t max_keys, int64_t dim, int64_t* plan) {
   clear_error();
+  LR_REQUIRE(dim == 64 || dim == 128 || dim == 256, "Head dimension must be 64, 128 or 256");
   LR_REQUIRE(segments > 0 && groups > 0 && length > 0 && max_keys >= 0 && plan,
              "Empty attention dimensions");
-  const PagedPlan p = plan_paged(segments, groups, length, max_keys);
+  const PagedPlan p = plan_paged(segments, groups, length, max_keys, dim);
   plan[0] = p.tile_kernel ? kTileRows : kSmallRows;
   plan[1] = p.waves;
   plan[2] = p.splits;
@@ -986,7 +968,7 @@ extern "C" int lr_paged_attention(const void* queries, const int64_t* query_stri
   LR_REQUIRE(alignment % 16 == 0, "Attention operands must be 16-byte aligned");
   // keys there can be: what a table holds, of a pool that has pages
   max_keys = page_count == 0 ? 0 : std::min(max_keys, max_pages * page_size);
-  const PagedPlan plan = plan_paged(segments, groups, length, max_keys);
+  const PagedPlan plan = plan_paged(segments, groups, length, max_keys, dim);
   const size_t needed = plan_bytes(plan, dim);
   LR_REQUIRE(workspace_size >= needed && (needed == 0 || workspace != nullptr),
              "Attention workspace too small");

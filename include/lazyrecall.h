@@ -583,7 +583,7 @@ size_t lr_paged_attention_workspace_bytes(int64_t segments, int64_t groups, int6
 /* How a call of these sizes runs (host only): plan[0] query rows of a tile (16 or 32), plan[1] waves
  * of a workgroup, plan[2] the parts its keys are split into. */
 int lr_paged_attention_plan(int64_t segments, int64_t groups, int64_t length, int64_t max_keys,
-                            int64_t* plan);
+                            int64_t dim, int64_t* plan);
 int lr_paged_attention(const void* queries, const int64_t* query_strides, const void* pages,
                        int64_t page_count, int64_t page_size, const int32_t* table,
                        int64_t max_pages, const int32_t* lengths, int64_t batch, int64_t kv_heads,

@@ -440,10 +440,10 @@ def test_prefill(device, dim, groups):
     attend(device, [0, 60], 2, groups, 250, dim, 32, seed=dim, layout="heads")
 
 
-def plan(segments, groups, length, max_keys):
+def plan(segments, groups, length, max_keys, dim=128):
     from code_for_iclr27_amd import _lib
     out = np.zeros(3, np.int64)
-    _lib.call("lr_paged_attention_plan", segments, groups, length, max_keys, out.ctypes.data)
+    _lib.call("lr_paged_attention_plan", segments, groups, length, max_keys, dim, out.ctypes.data)
     return out.tolist()
 
 
@@ -454,7 +454,7 @@ def plan(segments, groups, length, max_keys):
 def test_tiles_of_32_rows(device, dtype, dim, page_size, groups, length):
     lengths = np.random.default_rng(dim).integers(0, 150, 48)
     lengths[:6] = [0, 1, 31, 32, 33, 200]
-    assert plan(48, groups, length, int(lengths.max()) + length)[::2] == [32, 1]
+    assert plan(48, groups, length, int(lengths.max()) + length, dim)[::2] == [32, 1]
     attend(device, lengths, 24, groups, length, dim, page_size, dtype, seed=length, layout="heads")
 
 
@@ -462,7 +462,7 @@ def test_tiles_of_32_rows(device, dtype, dim, page_size, groups, length):
 def test_tiles_of_32_rows_with_split_keys(device, dim, page_size):
     lengths = np.random.default_rng(dim).integers(0, 60, 48)
     lengths[[3, 17, 47]] = [700, 513, 1030]
-    assert plan(48, 4, 29, 1059)[::2] == [32, 2]
+    assert plan(48, 4, 29, 1059, dim)[::2] == [32, 2]
     attend(device, lengths, 24, 4, 29, dim, page_size, seed=dim)
     attend(device, lengths, 24, 4, 29, dim, page_size, seed=dim, counts=[29, 11])
 
@@ -471,7 +471,7 @@ def test_tiles_of_32_rows_with_split_keys(device, dim, page_size):
 def test_eight_waves(device, dim, page_size):
     lengths = np.random.default_rng(dim).integers(0, 30, 260)
     lengths[[0, 5, 100, 259]] = [600, 255, 256, 999]
-    assert plan(260, 3, 1, 1000) == [16, 8, 1]
+    assert plan(260, 3, 1, 1000, dim) == [16, 8, 1]
     attend(device, lengths, 10, 3, 1, dim, page_size, seed=dim)
 
 
@@ -538,7 +538,7 @@ def test_nan_blocks_reach_only_the_rows_that_see_them(device, dim, length, group
     """NaN blocks of V (in the last key of all and at the diagonal), and of K: a row that sees a NaN
     key is NaN, one that sees a NaN block of V is NaN in its channels."""
     lengths = [45, 130]
-    assert plan(2, groups, length, 300)[0] == (32 if length == 128 else 16)
+    assert plan(2, groups, length, 300, dim)[0] == (32 if length == 128 else 16)
     grown = np.asarray(lengths) + length
     cache = Cache(device, grown, 2, dim, 16)
     cache.lengths = np.asarray(lengths, np.int32)

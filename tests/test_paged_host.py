@@ -117,9 +117,9 @@ def test_attention_workspace_grows_with_the_splits():
     assert size(0, 4, 1, 4096, 128) == 0
 
 
-def plan(segments, groups, length, max_keys):
+def plan(segments, groups, length, max_keys, dim=128):
     out = np.zeros(3, np.int64)
-    assert _lib.load().lr_paged_attention_plan(segments, groups, length, max_keys,
+    assert _lib.load().lr_paged_attention_plan(segments, groups, length, max_keys, dim,
                                                out.ctypes.data) == 0
     return out.tolist()
 
@@ -127,17 +127,20 @@ def plan(segments, groups, length, max_keys):
 def test_attention_plans():
     """Short calls in one launch, long ones in up to 32 parts, eight waves in the place of two parts,
     tiles of 32 rows where they fill most of the chip."""
-    assert plan(8, 4, 1, 512) == [16, 4, 1]
+    assert plan(8, 4, 1, 512) == plan(8, 4, 1, 640, 64) == plan(8, 6, 1, 256, 256) == [16, 4, 1]
+    assert plan(8, 4, 1, 513)[2] > 1 and plan(8, 4, 1, 641, 64)[2] > 1 and plan(8, 6, 1, 257, 256)[2] > 1
     assert plan(8, 4, 1, 2250) == [16, 4, 18]
     assert plan(8, 4, 1, 34000)[2] <= 32
     assert plan(256, 4, 1, 2000) == [16, 8, 1]
     assert plan(512, 4, 1, 2000) == [16, 4, 1]
     assert plan(8, 4, 1000, 5000) == [32, 4, 1]
-    assert plan(4, 6, 300, 4300) == [32, 4, 2]
+    assert plan(4, 6, 300, 4300, 256) == [32, 4, 2]
     assert plan(8, 4, 8, 4000)[0] == 16
-    library = _lib.load()
-    assert library.lr_paged_attention_plan(0, 4, 1, 5, np.zeros(3, np.int64).ctypes.data) == 1
+    library, out = _lib.load(), np.zeros(3, np.int64)
+    assert library.lr_paged_attention_plan(0, 4, 1, 5, 128, out.ctypes.data) == 1
     assert "Empty attention dimensions" in _lib.last_error()
+    assert library.lr_paged_attention_plan(1, 4, 1, 5, 96, out.ctypes.data) == 1
+    assert "Head dimension must be" in _lib.last_error()
     # the workspace holds the parts' states
     for shape in [(8, 4, 1, 2250), (4, 6, 300, 4300), (3, 5, 7, 30000), (64, 4, 1, 2250)]:
         rows, _, splits = plan(*shape)
