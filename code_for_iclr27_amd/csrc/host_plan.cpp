@@ -1530,9 +1530,9 @@ torch::Tensor paged_attention_launch(const torch::Tensor& pages, const torch::Te
   torch::Tensor out = torch::empty({batch, length, heads * dim},
                                    queries.options().memory_format(c10::MemoryFormat::Contiguous));
   if (length == 0) return out;
-  max_keys = std::min(max_keys, table.size(1) * page_size);
+  max_keys = pages.size(0) ? std::min(max_keys, table.size(1) * page_size) : 0;
   const size_t size = library.paged_attention_workspace_bytes(
-      batch * kv_heads, heads / kv_heads, length, pages.size(0) ? max_keys : 0, dim);
+      batch * kv_heads, heads / kv_heads, length, max_keys, dim);
   torch::Tensor workspace;
   if (size)
     workspace = torch::empty({static_cast<int64_t>(size)}, queries.options().dtype(torch::kUInt8));

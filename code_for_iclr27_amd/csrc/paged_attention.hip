@@ -959,15 +959,13 @@ extern "C" int lr_paged_attention(const void* queries, const int64_t* query_stri
   const int64_t segments = batch * kv_heads;
   if (int status = check_paged(pages, page_count, page_size, dim, table, max_pages, lengths, segments))
     return status;
-  LR_REQUIRE(max_keys >= 0, "Invalid key lengths");
+  LR_REQUIRE(max_keys >= 0 && max_keys <= INT32_MAX / 2, "Invalid key lengths");
   LR_REQUIRE(scale > 0.0f && std::isfinite(scale), "Softmax scale must be positive");
   LR_REQUIRE(queries && query_strides && out, "Invalid attention buffers");
   const uintptr_t alignment =
       reinterpret_cast<uintptr_t>(queries) | reinterpret_cast<uintptr_t>(out) |
       static_cast<uintptr_t>((query_strides[0] | query_strides[1] | query_strides[2]) * 2);
   LR_REQUIRE(alignment % 16 == 0, "Attention operands must be 16-byte aligned");
-  // keys there can be: what a table holds, of a pool that has pages
-  max_keys = page_count == 0 ? 0 : std::min(max_keys, max_pages * page_size);
   const PagedPlan plan = plan_paged(segments, groups, length, max_keys, dim);
   const size_t needed = plan_bytes(plan, dim);
   LR_REQUIRE(workspace_size >= needed && (needed == 0 || workspace != nullptr),
@@ -988,7 +986,8 @@ extern "C" int lr_paged_attention(const void* queries, const int64_t* query_stri
   args.kv_heads = static_cast<int>(kv_heads);
   args.groups = static_cast<int>(groups);
   args.length = static_cast<int>(length);
-  args.max_keys = static_cast<int>(max_keys);
+  // keys there can be: what a table holds, of a pool that has pages
+  args.max_keys = page_count == 0 ? 0 : static_cast<int>(std::min(max_keys, max_pages * page_size));
   args.segments = static_cast<unsigned>(segments);
   args.tiles = static_cast<unsigned>(plan.tiles);
   args.splits = static_cast<unsigned>(plan.splits);
@@ -997,8 +996,8 @@ extern "C" int lr_paged_attention(const void* queries, const int64_t* query_stri
   args.to_log2 = scale * kAttnLog2e;
   args.out = out;
   if (needed) {
-    args.part_ml = static_cast<float*>(workspace);
-    args.part_o = args.part_ml + plan.units * plan.splits * plan.tile_rows * 2;
+    args.part_o = static_cast<float*>(workspace);  // first, as it is accessed 16 bytes at a time
+    args.part_ml = args.part_o + plan.units * plan.splits * plan.tile_rows * dim;
   }
   return dispatch_dim(dim, [&]<int D>() {
     return dtype == LR_DTYPE_BF16 ? launch_paged<__bf16, D>(args, plan, as_stream(stream))

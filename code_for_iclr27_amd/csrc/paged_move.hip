@@ -736,6 +736,9 @@ extern "C" int lr_paged_compact(void* pages, int64_t page_count, int64_t page_si
   LR_REQUIRE(workspace_size >= needed && (needed == 0 || workspace) &&
                  reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
              "Compaction workspace too small");
+  // rows move while other workgroups still read theirs, and the lengths
+  LR_REQUIRE((target != table || target_pages == 0 || page_count == 0) && new_lengths != lengths,
+             "Compaction needs other pages and lengths than the cache's");
   CompactArgs args{};
   args.cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
   args.segments = segments;

@@ -45,7 +45,8 @@ class PagedLayer:
     """A layer's rows: ``pages`` uint8 [pages, page_bytes(page_size, dim)], ``table`` int32
     [batch * kv_heads, max_pages] (row i of a segment: slot i % page_size of page i // page_size),
     ``lengths`` int32 [batch * kv_heads], on one device. ``compact`` and ``read`` take the segments
-    of several layers in one table as well."""
+    of several layers in one table as well. A page that is appended to belongs to one segment;
+    segments that only read may share pages."""
 
     pages: torch.Tensor
     table: torch.Tensor
@@ -163,8 +164,8 @@ def attention(layer, queries, max_length, counts=None, scale=None):
     ``packed_attention`` returns it; rows of padding queries (at or past ``counts[b]``) are zero.
 
     ``max_length``: a bound on every segment's cached rows plus ``length`` (host int; rows past it
-    are not visited). ``scale`` defaults to dim^-0.5. The rows must have been appended as bf16, or
-    in the queries' dtype (f16 queries read larger values as infinities)."""
+    are not visited). ``scale`` defaults to dim^-0.5. f16 queries are for rows appended as f16 (of
+    others, keys outside f16's range read as infinities and zeros)."""
     if queries.requires_grad and torch.is_grad_enabled():
         _forward_only("attention")
     return (_native_module or _native()).paged_attention(

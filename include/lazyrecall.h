@@ -574,10 +574,11 @@ int lr_paged_append(const void* keys, const int64_t* key_strides, const void* va
 /* Attention of a step's queries [batch, kv_heads * groups, length, dim] (bf16 or f16) over each
  * segment's lengths[s] rows and the rows appended behind them in this step: query i < counts[b]
  * (i < length without counts) sees rows j <= lengths[s] + i; other queries, and those that see no
- * row, give zeros. out [batch, length, kv_heads * groups, dim], contiguous. max_keys bounds
- * lengths[s] + length (rows at or past it are not visited). scale is positive. Products, softmax
+ * row, give zeros. out [batch, length, kv_heads * groups, dim], contiguous. max_keys (below
+ * 2^30; no more than max_pages * page_size is of use) bounds lengths[s] + length: rows at or past it
+ * are not visited. scale is positive. Products, softmax
  * and sums are f32 (the probabilities enter as exact sums of bf16 pieces). workspace: as for
- * lr_packed_attention; 0 bytes and one launch when the keys are not split. */
+ * lr_packed_attention, of the same max_keys; 0 bytes and one launch when the keys are not split. */
 size_t lr_paged_attention_workspace_bytes(int64_t segments, int64_t groups, int64_t length,
                                           int64_t max_keys, int64_t dim);
 /* How a call of these sizes runs (host only): plan[0] query rows of a tile (16 or 32), plan[1] waves
@@ -602,7 +603,8 @@ int lr_paged_read(const void* pages, int64_t page_count, int64_t page_size, cons
 /* Moves the rows that stay, in order, to the pages of `target` [segments, target_pages], which
  * share none with `table`; removed: i64, sorted, unique row numbers in the packed order of
  * lr_paged_read. new_lengths [segments]: the rows that stay. Rows past the target table's end are
- * dropped, and table, lengths and the source pages stay as they are. */
+ * dropped, and table, lengths and the source pages stay as they are (target and new_lengths are
+ * other arrays). */
 size_t lr_paged_compact_workspace_bytes(int64_t segments);
 int lr_paged_compact(void* pages, int64_t page_count, int64_t page_size, const int32_t* table,
                      int64_t max_pages, const int32_t* lengths, int64_t segments, int64_t dim,

@@ -699,6 +699,7 @@ def test_refusals(device):
         (lambda: paged.read(layer, 5, torch.float64), "bf16, f16 or f32"),
         (lambda: paged.compact(layer, at.int()[0], layer.table), "Removed indices must be int64"),
         (lambda: paged.compact(layer, at[0], layer.table.long()), "Page table must"),
+        (lambda: paged.compact(layer, at[0], layer.table), "other pages"),
     ]
     for call, message in refused:
         if message is None:

@@ -102,7 +102,9 @@ def attend(**over):
     (dict(queries=None), "Invalid attention buffers"),
     (dict(out=None), "Invalid attention buffers"),
     (dict(queries=264), "16-byte aligned"),
+    (dict(max_keys=2 ** 30), "Invalid key lengths"),
     (dict(max_pages=2 ** 15, max_keys=2 ** 20), "Attention workspace too small"),
+    (dict(max_pages=2, max_keys=4096), "Attention workspace too small"),  # as its size was asked for
     (dict(max_pages=2 ** 15, max_keys=2 ** 20, workspace=128, size=1 << 40), "256-byte aligned"),
 ])
 def test_attention_refusals(over, message):
@@ -176,7 +178,9 @@ def test_read_and_compact_refusals():
                           (dict(segments=0), "Invalid page table"),
                           (dict(segments=300, workspace=None), "workspace too small"),
                           (dict(segments=300, size=64), "workspace too small"),
-                          (dict(segments=300, size=1 << 20, workspace=8), "workspace too small")]:
+                          (dict(segments=300, size=1 << 20, workspace=8), "workspace too small"),
+                          (dict(), "other pages"),
+                          (dict(target=16), "other pages")]:
         assert compact(**over) == 1 and message in _lib.last_error(), over
     assert library.lr_paged_compact_workspace_bytes(256) == 0
     assert library.lr_paged_compact_workspace_bytes(257) == 258 * 8
