@@ -5,8 +5,12 @@ a run of them together as a decode loop with evictions uses them.
 Attention's tolerance. Products of a 16-bit query element and a stored value are exact in f32, as
 are those of the probabilities' pieces, so the errors are: D f32 additions of a score (each at most
 2^-24 of the sum A of the score's absolute terms), the scaled exponent's rounding and the
-exponential (a few 2^-24 of A + 1), n additions of the sums, and the output's rounding, half a step:
-|got - ref| <= eps / 2 |ref| + 2 max|V| 2^-24 ((D + 8) (A + 1) + n + 64).
+exponential (a few 2^-24 of A + 1), n additions of the sums, the rounding of a probability (one f16
+piece for bf16 queries: 2^-11 of it; two f16 or bf16 pieces else: at most 2^-16; and, below f16's
+normal numbers, a row's largest being 2^11 at least, 2^-25 / 2^11 of the largest), and the output's
+rounding, half a step of the value and of its error. All but the last weigh in with E, the same
+average of |V|: |got - ref| <= eps / 2 |ref| + (1 + eps) (piece E + 2^-36 n max|V| +
+2 E 2^-24 ((D + 8) (A + 1) + n + 64)), piece = 2^-11 or 2^-16.
 """
 
 import numpy as np
@@ -348,33 +352,38 @@ def test_compact_into_a_short_table_and_missing_pages(device):
 
 
 def reference(queries, rows, lengths, counts, kv_heads, scale):
-    """The oracle's output and, per output row, the tolerance's A and n."""
+    """The oracle's output, the tolerance's E, its max|V| of a channel and, per row, its A."""
     q = queries.double().numpy()
     with np.errstate(all="ignore"):
         out = opaged.attention(q, rows, lengths, counts, kv_heads, scale)
+        average = opaged.attention(q, [(k, np.abs(v)) for k, v in rows], lengths, counts, kv_heads,
+                                   scale)
     batch, heads, length, dim = q.shape
-    a = np.zeros((batch, length, heads))
-    for s, (keys, _) in enumerate(rows):
+    a, top = np.zeros((batch, length, heads)), np.zeros((batch, 1, heads, dim))
+    for s, (keys, values) in enumerate(rows):
         b, h = divmod(s, kv_heads)
         groups = heads // kv_heads
         mine = np.abs(q[b, h * groups:(h + 1) * groups])  # [G, L, D]
         terms = mine @ np.abs(np.nan_to_num(keys)).T * scale
         if terms.shape[-1]:
             a[b, :, h * groups:(h + 1) * groups] = terms.max(-1).T
-    return out, a
+            top[b, 0, h * groups:(h + 1) * groups] = np.abs(values).max(0)
+    return out, average, top, a
 
 
 def check_attention(got, queries, rows, lengths, counts, kv_heads, scale=None):
     batch, heads, length, dim = queries.shape
     scale = dim ** -0.5 if scale is None else scale
-    expect, a = reference(queries, rows, lengths, counts, kv_heads, scale)
+    expect, average, top, a = reference(queries, rows, lengths, counts, kv_heads, scale)
     assert got.shape == expect.shape and got.dtype == queries.dtype
     got = got.double().cpu().numpy().reshape(batch, length, heads, dim)
-    expect = expect.reshape(got.shape)
-    top = max((float(np.abs(v).max(initial=0.0)) for _, v in rows), default=0.0)
+    expect, average = expect.reshape(got.shape), average.reshape(got.shape)
     most = max((len(k) for k, _ in rows), default=0)
-    bound = (torch.finfo(queries.dtype).eps / 2 * np.abs(expect)
-             + 2 * top * 2.0 ** -24 * ((dim + 8) * (a[..., None] + 1) + most + 64))
+    eps = torch.finfo(queries.dtype).eps
+    piece = 2.0 ** -11 if queries.dtype == BF16 else 2.0 ** -16
+    bound = (eps / 2 * np.abs(expect) + (1 + eps)
+             * (piece * average + 2.0 ** -36 * most * top
+                + 2 * average * 2.0 ** -24 * ((dim + 8) * (a[..., None] + 1) + most + 64)))
     error = np.abs(got - expect)
     assert np.all(error <= bound), float((error - bound).max())
     return expect
@@ -504,6 +513,31 @@ def test_scores_that_rise_key_by_key(device):
     check_attention(got, queries, [cache.rows(0, 500)[:2]], [499], [1], 1)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("length,groups", [(1, 4), (5, 3), (128, 24)])
+def test_values_of_every_size(device, dim, length, groups):
+    """Blocks of V that f16 holds as normal or subnormal numbers, that it does not hold, of zeros,
+    and all of these in one segment."""
+    sizes = [1.0, 2e-4, 3e-6, 1e-9, 1e-30, 4e4, 1e30, 0.0, None, None]
+    lengths = np.asarray([0, 33, 75, 75, 75, 75, 75, 90, 140, 300])
+    assert plan(10, groups, length, 300 + length, dim)[0] == (32 if length == 128 else 16)
+    cache = Cache(device, lengths + length, 10, dim, 16)
+    for s, size in enumerate(sizes):
+        n = int(lengths[s]) + length
+        keys, values = cache.rng.standard_normal((2, n, dim))
+        if size is None:
+            drawn = cache.rng.choice(sizes[:7], (n, dim // 32), p=[.94, .01, .01, .01, .01, .01, .01])
+            size = np.repeat(drawn * (cache.rng.random(drawn.shape) < 0.9), 32, 1)
+        cache.store(s, 0, keys, values * size, np.arange(n))
+    cache.lengths = lengths.astype(np.int32)
+    cache.upload()
+    queries = randn(cache.rng, (1, 10 * groups, length, dim), BF16)
+    got = paged.attention(cache.layer, queries.to(device), 300 + length)
+    rows = [cache.rows(s, int(n) + length)[:2] for s, n in enumerate(lengths)]
+    check_attention(got, queries, rows, lengths, [length], 10)
+    assert not got[..., 7 * groups * dim:8 * groups * dim].any()
+
+
 def test_max_length_bounds_the_keys(device):
     cache = Cache(device, [200, 90], 2, 128, 32)
     queries = randn(cache.rng, (1, 4, 1, 128), BF16)
@@ -613,7 +647,9 @@ def test_shared_pages_and_wide_tables(device):
 
 
 def test_attention_equals_packed_attention_over_the_rows_read(device):
-    """Both hold f32 throughout: the same rows give the same output but for the order of sums."""
+    """The same rows give the same output but for the order of sums, half a step of either output
+    and the paged kernel's f16 probabilities, 2^-11 of the average of |V| (from the packed kernel,
+    rounded once)."""
     for length, dim in ((1, 128), (4, 64), (90, 128)):
         got, cache, queries = attend(device, [300, 411, 90, 1000], 2, 4, length, dim, 32)
         grown = cache.layer.lengths + length
@@ -622,8 +658,10 @@ def test_attention_equals_packed_attention_over_the_rows_read(device):
         meta = SimpleNamespace(cu_seqlens_k=cu, max_seqlen_k=int(grown.max()),
                                decoding_cu_seqlens_q=torch.arange(5, device=device))
         other = packed.packed_attention(queries.to(device), keys, values, meta, length, 2)
+        average = packed.packed_attention(queries.to(device), keys, values.abs(), meta, length, 2)
         a, b = got.float(), other.float()
-        assert ((a - b).abs() <= 2.0 ** -7 * b.abs() + 1e-5).all()
+        bound = 2.0 ** -7 * b.abs() + 2.0 ** -11 * (1 + 2.0 ** -6) * average.float() + 1e-5
+        assert ((a - b).abs() <= bound).all()
 
 
 def test_empty_pool_and_empty_table(device):
