@@ -886,36 +886,93 @@ struct PagedPlan {
   int64_t tiles, units, splits, chunk;
 };
 
-// Which kernel runs and how many chunks the keys get. Both sides measured, us (8 segments, G4, d128
-// unless said). Tiles of 32 rows where they fill most of the chip: 1000 queries onto 4,000 rows 128
-// against 155 in tiles of 16, 64 queries 19 either way. Decode and short calls: chunks until there are
-// 512 workgroups (256 in tiles of 32 rows: 300 queries of d256, G6, 67 against 82 with 512), at most
-// 32 a tile, whose states a merge takes in one round of loads (8,000 rows: 9.4 against 11.6 with 63);
-// none where a few units a wave reach (five at d64: 630 rows 6.8 against 7.8; four: 500 rows 7.1
-// against 7.5, five 8.0 for 7.5; two at d256: 250 rows 7.9 for 8.4, 380 rows 9.6 against 9.2); and in
-// the place of two chunks one workgroup of eight waves (256 segments of 2,000 rows: 16.0 against 18.8).
-PagedPlan plan_paged(int64_t segments, int64_t groups, int64_t length, int64_t max_keys, int64_t dim) {
-  PagedPlan p{};
+// Which kernel runs and how many chunks the keys get: the choice with the least estimated time,
+//   call + round R + p (step R + share S) [+ merge + megabyte M + state N, when the keys are split],
+// where a chunk is p steps (a unit of 32 keys a wave), S workgroups share a compute unit, R rounds of
+// them follow one another (`resident` fit at once), M is the MB of partial states written and read,
+// and a thread of the merge loads N states. The constants (us) are a least-squares fit to 9,654 calls
+// (1 to 1,000 queries of 1 to 64 segments onto 100 to 130,000 rows, each kernel, 1 to 64 chunks),
+// within 6 to 8% of them; over the 1,077 shapes the choice takes 0.6% longer than the best one, 13%
+// at most. (Rules by the number of workgroups alone took 8% longer, up to 2.2 times: 8 queries of 16
+// requests onto 300 rows, 4 heads, G6, d256, 20 us against 10.8; 192 queries onto 9,000 rows 164
+// against 83.)
+struct PagedCost {
+  bool tile_kernel;
+  int waves, resident;
+  double call, round, step, share;
+};
+struct MergeCost {
+  double call, megabyte, state;
+};
+constexpr PagedCost kPagedCosts[3][3] = {  // d64, d128, d256
+    {{false, 4, 4, 4.2, 0.08, 0.467, 0.20}, {false, 8, 2, 3.7, 1.5, 0.35, 0.46}, {true, 4, 4, 5.15, 0.0, 0.486, 0.265}},
+    {{false, 4, 3, 3.6, 0.8, 0.467, 0.34}, {false, 8, 2, 1.8, 3.6, 0.0, 1.06}, {true, 4, 3, 5.9, 0.0, 0.477, 0.48}},
+    {{false, 4, 2, 4.95, 1.15, 0.245, 1.04}, {false, 8, 1, 3.15, 2.95, 2.19, 0.0}, {true, 4, 2, 8.4, 0.0, 1.12, 0.805}}};
+constexpr MergeCost kMergeCosts[3] = {{2.0, 0.34, 0.23}, {2.2, 0.26, 0.23}, {2.4, 0.26, 0.23}};
+constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+constexpr unsigned kComputeUnits = 256, kMostSplitGroups = 4096;  // (more of them need no splitting)
+
+// Chunks' states that a thread of the merge loads together.
+int merge_loads(int64_t splits) {
+  return splits <= 2 * kMergeParts ? 2 : splits <= 5 * kMergeParts ? 5 : 8;
+}
+
+PagedPlan least_cost(int64_t segments, int64_t groups, int64_t length, int64_t max_keys, int64_t dim) {
+  const int row = dim == 64 ? 0 : dim == 128 ? 1 : 2;
   const int64_t rows = length * groups;
-  p.tile_kernel = rows > kSmallRows && segments * ceil_div(rows, int64_t{kTileRows}) >= 192;
-  const int64_t tile = p.tile_kernel ? kTileRows : kSmallRows;
-  p.waves = kAttnWaves;
-  p.tile_rows = static_cast<int>(std::min(rows, tile));
-  p.tiles = ceil_div(rows, tile);
-  p.units = segments * p.tiles;
-  int64_t step = kUnit * kAttnWaves, steps = std::max<int64_t>(1, ceil_div(max_keys, step));
-  int64_t wanted = std::min({steps, int64_t{32}, ceil_div(p.tile_kernel ? 256 : 512, p.units)});
-  if (steps <= (dim == 64 ? 5 : dim == 128 ? 4 : 2)) wanted = 1;
-  if (wanted == 2 && !p.tile_kernel) {
-    p.waves = 2 * kAttnWaves;
-    step *= 2;
-    steps = ceil_div(max_keys, step);
-    wanted = 1;
+  const MergeCost& merge = kMergeCosts[row];
+  PagedPlan best{};
+  double least = HUGE_VAL;
+  for (const PagedCost& cost : kPagedCosts[row]) {
+    if (cost.tile_kernel && rows <= kSmallRows) continue;
+    PagedPlan p{};
+    p.tile_kernel = cost.tile_kernel;
+    p.waves = cost.waves;
+    const int64_t tile = p.tile_kernel ? kTileRows : kSmallRows;
+    p.tile_rows = static_cast<int>(std::min(rows, tile));
+    p.tiles = ceil_div(rows, tile);
+    p.units = segments * p.tiles;
+    const unsigned units = static_cast<unsigned>(std::min<int64_t>(p.units, INT32_MAX));
+    const unsigned step = static_cast<unsigned>(kUnit * p.waves);
+    const unsigned steps = std::max(1u, (static_cast<unsigned>(max_keys) + step - 1) / step);
+    const double state_megabytes = 8e-6 * static_cast<double>(p.tile_rows * dim);
+    for (const unsigned wanted : kSplits) {
+      const unsigned parts = std::min(steps, wanted), per = (steps + parts - 1) / parts;
+      const unsigned splits = (steps + per - 1) / per;
+      if (splits > 1 && units > kMostSplitGroups / splits) break;
+      if (splits > 4 && p.waves > kAttnWaves) break;  // (never the best, and past the fit)
+      const unsigned workgroups = units * splits, resident = kComputeUnits * cost.resident;
+      const unsigned rounds = (workgroups + resident - 1) / resident;
+      const unsigned shares = (workgroups + kComputeUnits - 1) / kComputeUnits;
+      double time = cost.call + cost.round * rounds + per * (cost.step * rounds + cost.share * shares);
+      if (splits > 1) {
+        const int loads = merge_loads(splits);
+        time += merge.call + merge.megabyte * state_megabytes * workgroups +
+                merge.state * static_cast<double>(ceil_div(splits, loads * kMergeParts) * loads);
+      }
+      if (time < least) {
+        least = time;
+        p.splits = splits;
+        p.chunk = static_cast<int64_t>(per) * step;
+        best = p;
+      }
+      if (wanted >= steps) break;
+    }
   }
-  const int64_t per = ceil_div(steps, wanted);
-  p.splits = ceil_div(steps, per);
-  p.chunk = per * step;
-  return p;
+  return best;
+}
+
+// The query for the workspace's size and the launch behind it plan the same sizes: the second takes
+// the thread's last plan (0.15 us of a call's 7 us of host work).
+PagedPlan plan_paged(int64_t segments, int64_t groups, int64_t length, int64_t max_keys, int64_t dim) {
+  thread_local int64_t sizes[5] = {};
+  thread_local PagedPlan plan;
+  const int64_t now[5] = {segments, groups, length, max_keys, dim};
+  if (!std::equal(now, now + 5, sizes)) {
+    plan = least_cost(segments, groups, length, max_keys, dim);
+    std::copy(now, now + 5, sizes);
+  }
+  return plan;
 }
 
 size_t plan_bytes(const PagedPlan& p, int64_t dim) {
@@ -932,8 +989,9 @@ int launch_merge(const PagedAttnArgs& args, const PagedPlan& plan, hipStream_t s
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.units) * blocks), dim3(kAttnThreads),
                        0, stream, args, blocks);
   };
-  if (plan.splits <= 2 * kMergeParts) merge(paged_merge_kernel<T, D, 2>);
-  else if (plan.splits <= 5 * kMergeParts) merge(paged_merge_kernel<T, D, 5>);
+  const int loads = merge_loads(plan.splits);
+  if (loads == 2) merge(paged_merge_kernel<T, D, 2>);
+  else if (loads == 5) merge(paged_merge_kernel<T, D, 5>);
   else merge(paged_merge_kernel<T, D, 8>);
   return check_launch("paged_attention merge");
 }
@@ -959,7 +1017,8 @@ using namespace lr;
 extern "C" size_t lr_paged_attention_workspace_bytes(int64_t segments, int64_t groups,
                                                      int64_t length, int64_t max_keys,
                                                      int64_t dim) {
-  if (segments <= 0 || groups <= 0 || length <= 0 || max_keys < 0 || dim <= 0) return 0;
+  if (segments <= 0 || groups <= 0 || length <= 0 || max_keys < 0 || max_keys > INT32_MAX / 2 || dim <= 0)
+    return 0;
   return plan_bytes(plan_paged(segments, groups, length, max_keys, dim), dim);
 }
 
@@ -967,7 +1026,8 @@ extern "C" int lr_paged_attention_plan(int64_t segments, int64_t groups, int64_t
                                        int64_t max_keys, int64_t dim, int64_t* plan) {
   clear_error();
   LR_REQUIRE(dim == 64 || dim == 128 || dim == 256, "Head dimension must be 64, 128 or 256");
-  LR_REQUIRE(segments > 0 && groups > 0 && length > 0 && max_keys >= 0 && plan,
+  LR_REQUIRE(segments > 0 && groups > 0 && length > 0 && max_keys >= 0 &&
+                 max_keys <= INT32_MAX / 2 && plan,
              "Empty attention dimensions");
   const PagedPlan p = plan_paged(segments, groups, length, max_keys, dim);
   plan[0] = p.tile_kernel ? kTileRows : kSmallRows;

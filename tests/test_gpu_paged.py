@@ -461,27 +461,39 @@ def plan(segments, groups, length, max_keys, dim=128):
                                                          (256, 64, 4, 32), (128, 16, 7, 19),
                                                          (64, 256, 1, 120), (256, 16, 6, 22)])
 def test_tiles_of_32_rows(device, dtype, dim, page_size, groups, length):
-    lengths = np.random.default_rng(dim).integers(0, 150, 48)
+    lengths = np.random.default_rng(dim).integers(0, 150, 144)
     lengths[:6] = [0, 1, 31, 32, 33, 200]
-    assert plan(48, groups, length, int(lengths.max()) + length, dim)[::2] == [32, 1]
+    assert plan(144, groups, length, int(lengths.max()) + length, dim)[::2] == [32, 1]
     attend(device, lengths, 24, groups, length, dim, page_size, dtype, seed=length, layout="heads")
 
 
 @pytest.mark.parametrize("dim,page_size", [(64, 32), (128, 16), (256, 128)])
 def test_tiles_of_32_rows_with_split_keys(device, dim, page_size):
-    lengths = np.random.default_rng(dim).integers(0, 60, 48)
-    lengths[[3, 17, 47]] = [700, 513, 1030]
-    assert plan(48, 4, 29, 1059, dim)[::2] == [32, 2]
-    attend(device, lengths, 24, 4, 29, dim, page_size, seed=dim)
-    attend(device, lengths, 24, 4, 29, dim, page_size, seed=dim, counts=[29, 11])
+    lengths = np.random.default_rng(dim).integers(0, 60, 36)
+    lengths[[3, 17, 35]] = [1700, 1013, 2471]
+    rows, _, splits = plan(36, 4, 29, 2500, dim)
+    assert rows == 32 and splits > 1
+    attend(device, lengths, 12, 4, 29, dim, page_size, seed=dim)
+    attend(device, lengths, 12, 4, 29, dim, page_size, seed=dim, counts=[29, 11, 0])
 
 
 @pytest.mark.parametrize("dim,page_size", [(64, 16), (128, 64), (256, 32)])
 def test_eight_waves(device, dim, page_size):
-    lengths = np.random.default_rng(dim).integers(0, 30, 260)
-    lengths[[0, 5, 100, 259]] = [600, 255, 256, 999]
-    assert plan(260, 3, 1, 1000, dim) == [16, 8, 1]
+    lengths = np.random.default_rng(dim).integers(0, 30, 140)
+    lengths[[0, 5, 100, 139]] = [600, 255, 256, 999]
+    assert plan(140, 3, 1, 1000, dim) == [16, 8, 1]
     attend(device, lengths, 10, 3, 1, dim, page_size, seed=dim)
+
+
+@pytest.mark.parametrize("dim,segments,groups,length,rows", [(64, 36, 7, 5, 3000),
+                                                             (128, 24, 7, 5, 1500),
+                                                             (256, 48, 1, 1, 800)])
+def test_eight_waves_with_split_keys(device, dim, segments, groups, length, rows):
+    lengths = np.random.default_rng(dim).integers(0, 90, segments)
+    lengths[[1, 9, 22]] = [rows - length, rows // 2, rows // 3]
+    assert plan(segments, groups, length, rows, dim)[1] == 8
+    assert plan(segments, groups, length, rows, dim)[2] > 1
+    attend(device, lengths, 12, groups, length, dim, 32, seed=dim)
 
 
 def test_padded_batch(device):
@@ -571,10 +583,11 @@ def test_keys_in_missing_pages_do_not_count(device):
 def test_nan_blocks_reach_only_the_rows_that_see_them(device, dim, length, groups):
     """NaN blocks of V (in the last key of all and at the diagonal), and of K: a row that sees a NaN
     key is NaN, one that sees a NaN block of V is NaN in its channels."""
-    lengths = [45, 130]
-    assert plan(2, groups, length, 300, dim)[0] == (32 if length == 128 else 16)
+    lengths = [45, 130] + [20] * (6 if length == 128 else 0)
+    heads, most = len(lengths), 130 + length
+    assert plan(heads, groups, length, most, dim)[0] == (32 if length == 128 else 16)
     grown = np.asarray(lengths) + length
-    cache = Cache(device, grown, 2, dim, 16)
+    cache = Cache(device, grown, heads, dim, 16)
     cache.lengths = np.asarray(lengths, np.int32)
     blocks = dim // 32
     scales = lambda which, s, row: (  # noqa: E731
@@ -586,12 +599,12 @@ def test_nan_blocks_reach_only_the_rows_that_see_them(device, dim, length, group
         page, at = scales(which, s, row)
         cache.pages[page, at + block] = 255
     cache.upload()
-    queries = randn(cache.rng, (1, 2 * groups, length, dim), BF16)
-    got = paged.attention(cache.layer, queries.to(device), int(grown.max()))
-    got = got.view(length, 2, groups, dim).double().cpu().numpy()
+    queries = randn(cache.rng, (1, heads * groups, length, dim), BF16)
+    got = paged.attention(cache.layer, queries.to(device), most)
+    got = got.view(length, heads, groups, dim).double().cpu().numpy()
     rows = [cache.rows(s, int(n))[:2] for s, n in enumerate(grown)]
     with np.errstate(invalid="ignore"):
-        expect = opaged.attention(queries.double().numpy(), rows, lengths, [length], 2)
+        expect = opaged.attention(queries.double().numpy(), rows, lengths, [length], heads)
     expect = expect.reshape(got.shape)
     assert np.isnan(expect).any() and (length == 1 or not np.isnan(expect).all())
     assert np.array_equal(np.isnan(got), np.isnan(expect))

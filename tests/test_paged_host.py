@@ -127,19 +127,21 @@ def plan(segments, groups, length, max_keys, dim=128):
 
 
 def test_attention_plans():
-    """Short calls in one launch, long ones in up to 32 parts, eight waves in the place of two parts,
-    tiles of 32 rows where they fill most of the chip."""
-    assert plan(8, 4, 1, 512) == plan(8, 4, 1, 640, 64) == plan(8, 6, 1, 256, 256) == [16, 4, 1]
-    assert plan(8, 4, 1, 513)[2] > 1 and plan(8, 4, 1, 641, 64)[2] > 1 and plan(8, 6, 1, 257, 256)[2] > 1
-    assert plan(8, 4, 1, 2250) == [16, 4, 18]
-    assert plan(8, 4, 1, 34000)[2] <= 32
-    assert plan(256, 4, 1, 2000) == [16, 8, 1]
-    assert plan(512, 4, 1, 2000) == [16, 4, 1]
-    assert plan(8, 4, 1000, 5000) == [32, 4, 1]
-    assert plan(4, 6, 300, 4300, 256) == [32, 4, 2]
-    assert plan(8, 4, 8, 4000)[0] == 16
+    """Short calls in one launch, a few rows onto long caches in up to 64 parts, no parts where the
+    rows fill the chip, tiles of 32 rows for many."""
+    for dim in (64, 128, 256):
+        assert plan(8, 4, 1, 0, dim) == plan(8, 4, 1, 100, dim) == [16, 4, 1]
+        assert plan(8, 4, 1, 2250, dim) == [16, 4, 18]
+        assert plan(8, 4, 1, 130000, dim) == [16, 4, 64]
+        assert plan(8, 4, 1, 2 ** 30 - 1, dim)[2] == 64
+        assert plan(2048, 4, 1, 2000, dim) == [16, 4, 1]
+        assert plan(140, 3, 1, 1000, dim) == [16, 8, 1]
+        assert plan(8, 4, 1000, 5000, dim) == [32, 4, 1]
+        assert plan(36, 4, 29, 2500, dim)[0] == 32 and plan(36, 4, 29, 2500, dim)[2] > 1
     library, out = _lib.load(), np.zeros(3, np.int64)
     assert library.lr_paged_attention_plan(0, 4, 1, 5, 128, out.ctypes.data) == 1
+    assert "Empty attention dimensions" in _lib.last_error()
+    assert library.lr_paged_attention_plan(1, 4, 1, 2 ** 30, 128, out.ctypes.data) == 1
     assert "Empty attention dimensions" in _lib.last_error()
     assert library.lr_paged_attention_plan(1, 4, 1, 5, 96, out.ctypes.data) == 1
     assert "Head dimension must be" in _lib.last_error()
