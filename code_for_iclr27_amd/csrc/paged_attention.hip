@@ -13,28 +13,33 @@
 //                 of 4 + 4 keys.
 //   O^T += V^T P^T  B: the probabilities where S^T left them (the key order is free as well); A: the
 //                 same keys of one channel, read transposed from the wave's V rows in LDS.
-// The values are exact in the 16-bit type. P enters as the sum of two bf16 pieces, whose products
-// with V are exact: 8 bits by truncation and 8 of the rest by rounding, within 2^-17 of P and without
-// a bias, against an output step of 2^-8 or 2^-11 (a third piece, all of P's bits, cost a third more
-// products: 1000 queries onto 4,000 rows 158 us against 136). Scores, exponentials, their sum and the
-// products' sums are f32 throughout.
+// The values are exact in the 16-bit type, and their products exact in f32. P enters as f16, rounded
+// to nearest: for bf16 queries as one piece, within 2^-11 of P where the output's own rounding is
+// 2^-8, for f16 queries as the sum of two, within 2^-22 (one piece for bf16 in the place of two bf16
+// ones, within 2^-16: 1000 queries onto 4,450 rows 113 us against 132). P is lifted by 2^kPagedLift,
+// so that all of a row down to 2^-25 of its largest are normal numbers of f16, and the reference of
+// its exponentials moves when a row's maximum has outgrown it by 2^kPagedSlack (as in
+// attention_tile.hip): P stays at or below 2^15. Scores, exponentials, their sum and the products'
+// sums are f32 throughout.
 //
-// The exponentials' reference moves when a row's maximum has outgrown it by 2^kPagedSlack (as in
-// attention_tile.hip). The waves' states meet in LDS; tiles whose keys span several chunks leave
-// partial states, which a second launch merges.
+// The waves' states meet in LDS; tiles whose keys span several chunks leave partial states, which a
+// second launch merges.
 //
-// A masked key contributes nothing: its score becomes -inf, its P 0. As 0 * NaN is NaN, a wave that
-// ends with a non-finite sum takes its keys again, with the blocks of V that read as NaN kept out of
-// the product and added to the rows that see their key.
+// A masked key contributes nothing: its score becomes -inf, its P 0. But 0 * NaN is NaN, and rows
+// appended as bf16 can lie outside f16's range. So a wave that met a block of V with a scale that f16
+// does not hold takes its keys again (SAFE): V and P, in two pieces, as bf16, without a lift or
+// slack, so that no sum overflows before its row does; blocks that read as NaN are kept out of the
+// product and added to the rows that see their key. Blocks of zeros, whatever their scale, need none
+// of it. (Where every wave does: 1000 queries onto 4,450 rows 265 us, eight requests of 36k rows 114.)
 //
 // What bounds it. Decode of a long cache: memory (eight requests of 36k rows, 8 heads, G4, d128: 312 MB
 // of codes in 62 us, 5.0 TB/s; a large copy reaches 5.2). Short ones: the two launches (8 segments of
-// 2,250 rows: 8 us, 2,250 rows of eight requests 11 us). Prefill: the vector instructions, 233 a unit
-// of 32 keys and 32 rows beside 24 MFMAs (a quarter each for the values, the exponentials and the
-// pieces), 71% of a SIMD's issue slots: 1000 queries onto 4,000 rows 128 us, where the packed kernel
-// on the same rows in 16 bits takes 171. Tried and no faster: units in flight two ahead, the
-// exponentials laid between the MFMAs of the last unit's product by hand, a raised wave priority for
-// the products, tiles of 64 rows.
+// 2,250 rows: 8 us, 2,250 rows of eight requests 11 us). Prefill: the vector instructions, 189 a unit
+// of 32 keys and 32 rows beside 16 MFMAs (a third each for the values and the exponentials), 60% of a
+// SIMD's issue slots with 2.3 waves of it on average: 1000 queries onto 4,450 rows 113 us, where the
+// packed kernel on the same rows in 16 bits takes 171. Tried and no faster: units in flight two ahead,
+// the exponentials laid between the MFMAs of the last unit's product by hand, a raised wave priority
+// for the products, tiles of 64 rows, four waves a SIMD (11 registers spilled).
 
 #include <algorithm>
 #include <cmath>
@@ -121,15 +126,11 @@ __device__ __forceinline__ bool outside_f16(unsigned byte) {
   return byte - (127 + kHalfRange.low) > static_cast<unsigned>(kHalfRange.high - kHalfRange.low);
 }
 
-// V rows in LDS: 16-byte chunk c of row r in slot c ^ x(r). Eight lanes that write one chunk of
-// eight rows, and 32 lanes that read 16 columns of eight rows transposed, touch every bank once:
-// four consecutive rows go to the four 64-byte quarters of a bank cycle (a d64 row is half of one),
-// and groups of four rows to different 16-byte places of a quarter.
-template <int D>
-__device__ __forceinline__ int value_swizzle(int row) {
-  const int quarter = D == 64 ? (row >> 1) & 1 : row & 3, group = (row >> 2) & 3;
-  return quarter << 2 ^ ((group & 1) << 1 | group >> 1);
-}
+// V rows in LDS: 16-byte chunk c of row r in slot c ^ x(r). The eight rows that eight lanes write one
+// chunk of lie in different 16-byte places of 128, and the 32 bytes of four rows that 16 lanes read
+// transposed in different quarters of it. (Slots that differ in the four rows' 64-byte places alone
+// had twice the bank conflicts; the prefill kernel as a whole took 0.6% longer.)
+__device__ __forceinline__ int value_swizzle(int row) { return (row & 3) << 1 | ((row >> 2) & 1); }
 
 typedef const __attribute__((address_space(4))) int32_t* PageIds;  // read by scalar loads
 __device__ __forceinline__ PageIds page_table(const PagedCache& cache, unsigned seg) {
@@ -138,7 +139,7 @@ __device__ __forceinline__ PageIds page_table(const PagedCache& cache, unsigned 
 
 // A block's segment, tile and split. Consecutive blocks take consecutive segments, so with 8 segments
 // (or a divisor or multiple of it) each XCD's L2 serves its own segments' rows (1000 queries onto
-// 4,000 rows: 125 us against 135 with consecutive tiles); within a segment the tiles with the most
+// 4,000 rows: 7% less than with consecutive tiles); within a segment the tiles with the most
 // visible keys come first, so that the launch's tail is short.
 struct Place {
   unsigned seg, tile, split, unit;
@@ -353,7 +354,7 @@ void paged_attention_kernel(PagedAttnArgs a) {
   uint32_t read_at;  // of the lane's transposed reads: row 4 j + m / 4, columns 4 (m % 4) .. + 3
   {
     const int r = 4 * j + (m >> 2), chunk = (m & 3) >> 1;
-    read_at = lds_address(my_values) + r * (2 * D) + 16 * (chunk ^ value_swizzle<D>(r)) + 8 * (m & 1);
+    read_at = lds_address(my_values) + r * (2 * D) + 16 * (chunk ^ value_swizzle(r)) + 8 * (m & 1);
   }
   auto write_values = [&]<typename P>(const Codes& u) {
 #pragma unroll
@@ -361,7 +362,7 @@ void paged_attention_kernel(PagedAttnArgs a) {
       char* to = my_values + (16 * blk + m) * (2 * D);
 #pragma unroll
       for (int w = 0; w < KW; ++w)
-        *reinterpret_cast<attn_u32x4*>(to + 16 * (word_chunk<D>(j, w) ^ value_swizzle<D>(m))) =
+        *reinterpret_cast<attn_u32x4*>(to + 16 * (word_chunk<D>(j, w) ^ value_swizzle(m))) =
             expand8<P>(u.v[blk][w], scale_of(u.vs[blk][Codes::kBytes == 2 ? w / 4 : 0]));
     }
   };
@@ -396,30 +397,37 @@ void paged_attention_kernel(PagedAttnArgs a) {
         }
       }
       if constexpr (SAFE) {
-#pragma unroll 1
-        for (int left = 0; left < kUnit; ++left) {
-#pragma unroll
-          for (int i = 0; i < Codes::kBytes; ++i)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {  // the lane that holds block b + 4 i of row `left`
-              if (D == 64 && b >= 2) continue;
-              const int from = (D == 64 ? 2 * b : b) * 16 + (left & 15);
-              const unsigned byte = __shfl(left < 16 ? u.vs[0][i] : u.vs[1][i], from);
-              if (byte == kScaleNaN && key + left <= limit)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  out[2 * (b + 4 * i)][r] = out[2 * (b + 4 * i) + 1][r] = __builtin_nanf("");
-            }
-        }
+        bool invalid = false;
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-          for (int i = 0; i < Codes::kBytes; ++i)
-            if (u.vs[blk][i] == kScaleNaN) {
-              u.vs[blk][i] = 127u;
+          for (int i = 0; i < Codes::kBytes; ++i) invalid |= u.vs[blk][i] == kScaleNaN;
+        if (__any(invalid)) {
+#pragma unroll 1
+          for (int left = 0; left < kUnit; ++left) {
 #pragma unroll
-              for (int w = 0; w < KW / Codes::kBytes; ++w) u.v[blk][i * 4 + w] = 0u;
-            }
+            for (int i = 0; i < Codes::kBytes; ++i)
+#pragma unroll
+              for (int b = 0; b < 4; ++b) {  // the lane that holds block b + 4 i of row `left`
+                if (D == 64 && b >= 2) continue;
+                const int from = (D == 64 ? 2 * b : b) * 16 + (left & 15);
+                const unsigned byte = __shfl(left < 16 ? u.vs[0][i] : u.vs[1][i], from);
+                if (byte == kScaleNaN && key + left <= limit)
+#pragma unroll
+                  for (int r = 0; r < 4; ++r)
+                    out[2 * (b + 4 * i)][r] = out[2 * (b + 4 * i) + 1][r] = __builtin_nanf("");
+              }
+          }
+#pragma unroll
+          for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+            for (int i = 0; i < Codes::kBytes; ++i)
+              if (u.vs[blk][i] == kScaleNaN) {
+                u.vs[blk][i] = 127u;
+#pragma unroll
+                for (int w = 0; w < KW / Codes::kBytes; ++w) u.v[blk][i * 4 + w] = 0u;
+              }
+        }
       } else {
         bool odd = false;
 #pragma unroll
@@ -638,7 +646,7 @@ void paged_tile_kernel(PagedAttnArgs a) {
     char* row = my_values + col * (2 * D);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
-      *reinterpret_cast<attn_u32x4*>(row + 16 * ((half * KS + ks) ^ value_swizzle<D>(col))) =
+      *reinterpret_cast<attn_u32x4*>(row + 16 * ((half * KS + ks) ^ value_swizzle(col))) =
           expand8<P>(v.w[ks], scale(v, ks));
   };
   // Transposed reads: row 4 half + (lane % 16) / 4 of eight, columns 16 (lane / 16 % 2) +
@@ -646,13 +654,13 @@ void paged_tile_kernel(PagedAttnArgs a) {
   uint32_t read_at;
   {
     const int row = 4 * half + ((lane & 15) >> 2), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    read_at = lds_address(my_values) + row * (2 * D) + 16 * (chunk ^ value_swizzle<D>(row)) +
+    read_at = lds_address(my_values) + row * (2 * D) + 16 * (chunk ^ value_swizzle(row)) +
               8 * (lane & 1);
   }
   auto read_column = [&](int k, int dt) {  // A operand: keys 16 k .. 16 k + 15 of 32 channels
-    // (eight rows on, value_swizzle differs in one bit)
+    // (eight rows on, value_swizzle is the same)
     const uint32_t at = (read_at ^ (64 * dt)) + 16 * k * (2 * D);
-    const paged_u32x2 lo = read_transposed(at), hi = read_transposed((at ^ 16) + 8 * (2 * D));
+    const paged_u32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * (2 * D));
     return attn_u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
 
@@ -681,23 +689,28 @@ void paged_tile_kernel(PagedAttnArgs a) {
         v.scales = there ? v.scales : 0x7f7f7f7fu;
       }
       if constexpr (SAFE) {
+        bool invalid = false;
+#pragma unroll
+        for (int b = 0; b < DT / 2; ++b) invalid |= (v.scales >> (8 * b) & 255u) == kScaleNaN;
+        if (__any(invalid)) {
 #pragma unroll 1
-        for (int left = 0; left < kUnit; ++left) {
+          for (int left = 0; left < kUnit; ++left) {
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const unsigned bytes = __shfl(v.scales, left + 32 * (dt / (DT / 2)));
-            if ((bytes >> (8 * (dt % (DT / 2))) & 255u) == kScaleNaN && key + left <= limit)
+            for (int dt = 0; dt < DT; ++dt) {
+              const unsigned bytes = __shfl(v.scales, left + 32 * (dt / (DT / 2)));
+              if ((bytes >> (8 * (dt % (DT / 2))) & 255u) == kScaleNaN && key + left <= limit)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) out[dt][r] = __builtin_nanf("");
+                for (int r = 0; r < 16; ++r) out[dt][r] = __builtin_nanf("");
+            }
           }
+#pragma unroll
+          for (int b = 0; b < DT / 2; ++b)
+            if ((v.scales >> (8 * b) & 255u) == kScaleNaN) {
+              v.scales &= ~(0x80u << (8 * b));  // 127
+#pragma unroll
+              for (int w = 0; w < 4; ++w) v.w[4 * b + w] = 0u;
+            }
         }
-#pragma unroll
-        for (int b = 0; b < DT / 2; ++b)
-          if ((v.scales >> (8 * b) & 255u) == kScaleNaN) {
-            v.scales &= ~(0x80u << (8 * b));  // 127
-#pragma unroll
-            for (int w = 0; w < 4; ++w) v.w[4 * b + w] = 0u;
-          }
       } else {
         bool odd = false;
 #pragma unroll
@@ -905,9 +918,15 @@ struct MergeCost {
   double call, megabyte, state;
 };
 constexpr PagedCost kPagedCosts[3][3] = {  // d64, d128, d256
-    {{false, 4, 4, 4.2, 0.08, 0.467, 0.20}, {false, 8, 2, 3.7, 1.5, 0.35, 0.46}, {true, 4, 4, 5.15, 0.0, 0.486, 0.265}},
-    {{false, 4, 3, 3.6, 0.8, 0.467, 0.34}, {false, 8, 2, 1.8, 3.6, 0.0, 1.06}, {true, 4, 3, 5.9, 0.0, 0.477, 0.48}},
-    {{false, 4, 2, 4.95, 1.15, 0.245, 1.04}, {false, 8, 1, 3.15, 2.95, 2.19, 0.0}, {true, 4, 2, 8.4, 0.0, 1.12, 0.805}}};
+    {{false, 4, 4, 4.2, 0.08, 0.467, 0.20},
+     {false, 8, 2, 3.7, 1.5, 0.35, 0.46},
+     {true, 4, 4, 5.15, 0.0, 0.486, 0.265}},
+    {{false, 4, 3, 3.6, 0.8, 0.467, 0.34},
+     {false, 8, 2, 1.8, 3.6, 0.0, 1.06},
+     {true, 4, 3, 5.9, 0.0, 0.477, 0.48}},
+    {{false, 4, 2, 4.95, 1.15, 0.245, 1.04},
+     {false, 8, 1, 3.15, 2.95, 2.19, 0.0},
+     {true, 4, 2, 8.4, 0.0, 1.12, 0.805}}};
 constexpr MergeCost kMergeCosts[3] = {{2.0, 0.34, 0.23}, {2.2, 0.26, 0.23}, {2.4, 0.26, 0.23}};
 constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
 constexpr unsigned kComputeUnits = 256, kMostSplitGroups = 4096;  // (more of them need no splitting)
