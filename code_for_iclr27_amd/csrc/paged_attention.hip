@@ -13,24 +13,21 @@
 //                 of 4 + 4 keys.
 //   O^T += V^T P^T  B: the probabilities where S^T left them (the key order is free as well); A: the
 //                 same keys of one channel, read transposed from the wave's V rows in LDS.
-// The values are exact in the 16-bit type, and their products exact in f32. P enters as f16, rounded
-// to nearest: for bf16 queries as one piece, within 2^-11 of P where the output's own rounding is
-// 2^-8, for f16 queries as the sum of two, within 2^-22 (one piece for bf16 in the place of two bf16
-// ones, within 2^-16: 1000 queries onto 4,450 rows 113 us against 132). P is lifted by 2^kPagedLift,
-// so that all of a row down to 2^-25 of its largest are normal numbers of f16, and the reference of
-// its exponentials moves when a row's maximum has outgrown it by 2^kPagedSlack (as in
-// attention_tile.hip): P stays at or below 2^15. Scores, exponentials, their sum and the products'
-// sums are f32 throughout.
+// The values are exact in the 16-bit type, and their products exact in f32. P enters as the sum of two
+// bf16 pieces, whose products with V are exact: 8 bits and 8 of the rest, within 2^-16 of P at every
+// size, as the cached rows' packed attention keeps to. (One f16 piece, within 2^-11 down to 2^-25 of
+// a row's largest, took 113 us in the place of 131 for 1000 queries onto 4,450 rows: an eighth of a
+// bf16 output's own step, but sixteen halves of an f16 one's beside a dominant key whose V is 0. A
+// third bf16 piece, all of P's bits, costs a third more products.) Scores, exponentials, their sum
+// and the products' sums are f32 throughout.
 //
-// The waves' states meet in LDS; tiles whose keys span several chunks leave partial states, which a
-// second launch merges.
+// The exponentials' reference moves when a row's maximum has outgrown it by 2^kPagedSlack (as in
+// attention_tile.hip). The waves' states meet in LDS; tiles whose keys span several chunks leave
+// partial states, which a second launch merges.
 //
-// A masked key contributes nothing: its score becomes -inf, its P 0. But 0 * NaN is NaN, and rows
-// appended as bf16 can lie outside f16's range. So a wave that met a block of V with a scale that f16
-// does not hold takes its keys again (SAFE): V and P, in two pieces, as bf16, without a lift or
-// slack, so that no sum overflows before its row does; blocks that read as NaN are kept out of the
-// product and added to the rows that see their key. Blocks of zeros, whatever their scale, need none
-// of it. (Where every wave does: 1000 queries onto 4,450 rows 265 us, eight requests of 36k rows 114.)
+// A masked key contributes nothing: its score becomes -inf, its P 0. As 0 * NaN is NaN, a wave that
+// ends with a non-finite sum takes its keys again, with the blocks of V that read as NaN kept out of
+// the product and added to the rows that see their key.
 //
 // What bounds it. Decode of a long cache: memory (eight requests of 36k rows, 8 heads, G4, d128: 312 MB
 // of codes in 62 us, 5.0 TB/s; a large copy reaches 5.2). Short ones: the two launches (8 segments of
@@ -57,9 +54,8 @@ typedef unsigned paged_u32x2 __attribute__((ext_vector_type(2)));
 constexpr int kUnit = 32;       // keys of a wave's step
 constexpr int kSmallRows = 16;  // rows of a tile: decode and a few query rows
 constexpr int kTileRows = 32;   // many query rows
-constexpr float kPagedSlack = 4.0f, kPagedLift = 11.0f;
-template <typename T, bool SAFE>
-constexpr int kPieces = SAFE || std::is_same<T, _Float16>::value ? 2 : 1;  // of a probability
+constexpr float kPagedSlack = 4.0f;
+constexpr int kPieces = 2;      // of a probability
 
 struct PagedAttnArgs {
   const void* queries;  // element strides below; the last dimension is contiguous
@@ -107,23 +103,16 @@ __device__ __forceinline__ T* paged_output(const PagedAttnArgs& a, unsigned seg,
           h * groups + g) * D;
 }
 
-// Two f32 values as sums of P type's pieces, word `w` of the piece vectors: the values rounded to
-// nearest, and (of two pieces) the rest, an exact difference, as well.
-template <typename P, int PIECES>
-__device__ __forceinline__ void split(float x, float y, attn_u32x4 (&piece)[PIECES], int w) {
-  typedef P pair __attribute__((ext_vector_type(2)));
-  const pair top = {static_cast<P>(x), static_cast<P>(y)};
-  piece[0][w] = __builtin_bit_cast(unsigned, top);
-  if constexpr (PIECES == 2) {
-    const pair rest = {static_cast<P>(__builtin_fmaf(static_cast<float>(top[0]), -1.0f, x)),
-                       static_cast<P>(__builtin_fmaf(static_cast<float>(top[1]), -1.0f, y))};
-    piece[1][w] = __builtin_bit_cast(unsigned, rest);
-  }
-}
-
-// A scale whose values (nonzero ones) f16 does not hold exactly, NaN among them.
-__device__ __forceinline__ bool outside_f16(unsigned byte) {
-  return byte - (127 + kHalfRange.low) > static_cast<unsigned>(kHalfRange.high - kHalfRange.low);
+// Two f32 values as sums of two bf16 pieces each, word `w` of the piece vectors: the values rounded to
+// nearest, and the rest, an exact difference, as well.
+__device__ __forceinline__ void split_bf16(float x, float y, attn_u32x4 (&piece)[kPieces], int w) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 near = {static_cast<__bf16>(x), static_cast<__bf16>(y)};
+  const unsigned both = __builtin_bit_cast(unsigned, near);
+  piece[0][w] = both;
+  const bf16x2 rest = {static_cast<__bf16>(x - __builtin_bit_cast(float, both << 16)),
+                       static_cast<__bf16>(y - __builtin_bit_cast(float, both & 0xffff0000u))};
+  piece[1][w] = __builtin_bit_cast(unsigned, rest);
 }
 
 // V rows in LDS: 16-byte chunk c of row r in slot c ^ x(r). The eight rows that eight lanes write one
@@ -356,23 +345,20 @@ void paged_attention_kernel(PagedAttnArgs a) {
     const int r = 4 * j + (m >> 2), chunk = (m & 3) >> 1;
     read_at = lds_address(my_values) + r * (2 * D) + 16 * (chunk ^ value_swizzle(r)) + 8 * (m & 1);
   }
-  auto write_values = [&]<typename P>(const Codes& u) {
+  auto write_values = [&](const Codes& u) {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
       char* to = my_values + (16 * blk + m) * (2 * D);
 #pragma unroll
       for (int w = 0; w < KW; ++w)
         *reinterpret_cast<attn_u32x4*>(to + 16 * (word_chunk<D>(j, w) ^ value_swizzle(m))) =
-            expand8<P>(u.v[blk][w], scale_of(u.vs[blk][Codes::kBytes == 2 ? w / 4 : 0]));
+            expand8<__bf16>(u.v[blk][w], scale_of(u.vs[blk][Codes::kBytes == 2 ? w / 4 : 0]));
     }
   };
 
   // The wave's units of the chunk. SAFE: blocks of V that read as NaN are kept out of the product and
-  // added to the rows that see their key, V is bf16, and no exponential exceeds one.
-  bool unusual = false;  // a block of V needs that
+  // added to the rows that see their key, and no exponential exceeds one.
   auto pass = [&]<bool SAFE>() {
-    using P = std::conditional_t<SAFE, __bf16, _Float16>;
-    constexpr float kLift = SAFE ? 0.0f : kPagedLift, kSlack = SAFE ? 0.0f : kPagedSlack;
     reference = kNegInf, sum = 0.0f;
 #pragma unroll
     for (int ct = 0; ct < DT; ++ct) out[ct] = attn_f32x4{0.f, 0.f, 0.f, 0.f};
@@ -428,26 +414,9 @@ void paged_attention_kernel(PagedAttnArgs a) {
                 for (int w = 0; w < KW / Codes::kBytes; ++w) u.v[blk][i * 4 + w] = 0u;
               }
         }
-      } else {
-        bool odd = false;
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-          for (int i = 0; i < Codes::kBytes; ++i) odd |= outside_f16(u.vs[blk][i]);
-        if (__any(odd))  // blocks of zeros are harmless
-#pragma unroll
-          for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-            for (int i = 0; i < Codes::kBytes; ++i) {
-              unsigned some = 0;
-#pragma unroll
-              for (int w = 0; w < KW / Codes::kBytes; ++w) some |= u.v[blk][i * 4 + w];
-              unusual |= outside_f16(u.vs[blk][i]) &&
-                         ((some & 0x77777777u) != 0 || u.vs[blk][i] == kScaleNaN);
-            }
       }
       // V rows to LDS (the last unit's reads are done: a wave's LDS accesses stay in order)
-      write_values.template operator()<P>(u);
+      write_values(u);
       // S^T
       attn_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -472,8 +441,8 @@ void paged_attention_kernel(PagedAttnArgs a) {
       LanePair pair = lane_pair<16>(top);
       pair = lane_pair<32>(fmaxf(pair.first, pair.second));
       top = fmaxf(pair.first, pair.second) * a.to_log2;
-      if (__any(top > reference + (kLift + kSlack))) {
-        const float raised = fmaxf(reference, top - kLift);
+      if (__any(top > reference + (SAFE ? 0.0f : kPagedSlack))) {
+        const float raised = fmaxf(reference, top);
         const float factor = reference == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(reference - raised);
         sum *= factor;
 #pragma unroll
@@ -483,14 +452,14 @@ void paged_attention_kernel(PagedAttnArgs a) {
         reference = raised;
       }
       const float base = reference == kNegInf ? 0.0f : reference;
-      attn_u32x4 piece[kPieces<T, SAFE>];
+      attn_u32x4 piece[kPieces];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n / 2][2 * (n % 2)], a.to_log2, -base));
         const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n / 2][2 * (n % 2) + 1], a.to_log2, -base));
         sum += x;
         sum += y;
-        split<P>(x, y, piece, n);
+        split_bf16(x, y, piece, n);
       }
       // O^T += V^T P^T
       wave_fence();
@@ -498,11 +467,10 @@ void paged_attention_kernel(PagedAttnArgs a) {
       for (int ct = 0; ct < DT; ++ct) {
         const uint32_t at = read_at ^ (32 * ct);
         const paged_u32x2 lo = read_transposed(at), hi = read_transposed(at + 16 * (2 * D));
-        using P8 = typename AttnVec<P>::x8;
-        const P8 v = __builtin_bit_cast(P8, attn_u32x4{lo[0], lo[1], hi[0], hi[1]});
+        const attn_bf16x8 v = __builtin_bit_cast(attn_bf16x8, attn_u32x4{lo[0], lo[1], hi[0], hi[1]});
 #pragma unroll
-        for (int i = 0; i < kPieces<T, SAFE>; ++i)
-          out[ct] = AttnVec<P>::mfma(v, __builtin_bit_cast(P8, piece[i]), out[ct]);
+        for (int i = 0; i < kPieces; ++i)
+          out[ct] = AttnVec<__bf16>::mfma(v, __builtin_bit_cast(attn_bf16x8, piece[i]), out[ct]);
       }
       wave_fence();
       if (!more) break;
@@ -513,7 +481,12 @@ void paged_attention_kernel(PagedAttnArgs a) {
   };
   __syncthreads();
   pass.template operator()<false>();
-  if (__any(unusual)) pass.template operator()<true>();
+  float poison = 0.0f;  // 0 * NaN is NaN: a wave with a sum that is not finite takes its keys again
+#pragma unroll
+  for (int ct = 0; ct < DT; ++ct)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) poison = __builtin_fmaf(out[ct][r], 0.0f, poison);
+  if (__any(poison != poison)) pass.template operator()<true>();
   {
     LanePair pair = lane_pair<16>(sum);
     pair = lane_pair<32>(pair.first + pair.second);
@@ -642,12 +615,12 @@ void paged_tile_kernel(PagedAttnArgs a) {
   float reference = kNegInf, sum = 0.0f;  // in exponents of two; the same in both halves
   paged_f32x16 out[DT];
   char* const my_values = reinterpret_cast<char*>(&v_lds[wave][0]);
-  auto write_values = [&]<typename P>(const Codes& v) {
+  auto write_values = [&](const Codes& v) {
     char* row = my_values + col * (2 * D);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
       *reinterpret_cast<attn_u32x4*>(row + 16 * ((half * KS + ks) ^ value_swizzle(col))) =
-          expand8<P>(v.w[ks], scale(v, ks));
+          expand8<__bf16>(v.w[ks], scale(v, ks));
   };
   // Transposed reads: row 4 half + (lane % 16) / 4 of eight, columns 16 (lane / 16 % 2) +
   // 4 (lane % 4) .. + 3 of 32.
@@ -664,10 +637,7 @@ void paged_tile_kernel(PagedAttnArgs a) {
     return attn_u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
 
-  bool unusual = false;  // a block of V needs the SAFE pass (as above)
   auto pass = [&]<bool SAFE>() {
-    using P = std::conditional_t<SAFE, __bf16, _Float16>;
-    constexpr float kLift = SAFE ? 0.0f : kPagedLift, kSlack = SAFE ? 0.0f : kPagedSlack;
     reference = kNegInf, sum = 0.0f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -711,20 +681,9 @@ void paged_tile_kernel(PagedAttnArgs a) {
               for (int w = 0; w < 4; ++w) v.w[4 * b + w] = 0u;
             }
         }
-      } else {
-        bool odd = false;
-#pragma unroll
-        for (int b = 0; b < DT / 2; ++b) odd |= outside_f16(v.scales >> (8 * b) & 255u);
-        if (__any(odd))  // blocks of zeros are harmless
-#pragma unroll
-          for (int b = 0; b < DT / 2; ++b) {
-            const unsigned byte = v.scales >> (8 * b) & 255u;
-            const unsigned some = v.w[4 * b] | v.w[4 * b + 1] | v.w[4 * b + 2] | v.w[4 * b + 3];
-            unusual |= outside_f16(byte) && ((some & 0x77777777u) != 0 || byte == kScaleNaN);
-          }
       }
       // V rows to LDS (the last unit's reads are done: a wave's LDS accesses stay in order)
-      write_values.template operator()<P>(v);
+      write_values(v);
       // S^T
       paged_f32x16 s;
 #pragma unroll
@@ -742,8 +701,8 @@ void paged_tile_kernel(PagedAttnArgs a) {
       for (int r = 0; r < 8; ++r) top = fmaxf(fmaxf(top, s[2 * r]), s[2 * r + 1]);
       const LanePair pair = lane_pair<32>(top);
       top = fmaxf(pair.first, pair.second) * a.to_log2;
-      if (__any(top > reference + (kLift + kSlack))) {
-        const float raised = fmaxf(reference, top - kLift);
+      if (__any(top > reference + (SAFE ? 0.0f : kPagedSlack))) {
+        const float raised = fmaxf(reference, top);
         const float factor = reference == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(reference - raised);
         sum *= factor;
 #pragma unroll
@@ -753,14 +712,14 @@ void paged_tile_kernel(PagedAttnArgs a) {
         reference = raised;
       }
       const float base = reference == kNegInf ? 0.0f : reference;
-      attn_u32x4 piece[2][kPieces<T, SAFE>];
+      attn_u32x4 piece[2][kPieces];
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * n], a.to_log2, -base));
         const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * n + 1], a.to_log2, -base));
         sum += x;
         sum += y;
-        split<P>(x, y, piece[n / 4], n % 4);
+        split_bf16(x, y, piece[n / 4], n % 4);
       }
       // O^T += V^T P^T
       wave_fence();
@@ -770,7 +729,7 @@ void paged_tile_kernel(PagedAttnArgs a) {
         for (int dt = 0; dt < DT; ++dt) {
           const attn_u32x4 x = read_column(kk, dt);
 #pragma unroll
-          for (int n = 0; n < kPieces<T, SAFE>; ++n) out[dt] = mfma32<P>(x, piece[kk][n], out[dt]);
+          for (int n = 0; n < kPieces; ++n) out[dt] = mfma32<__bf16>(x, piece[kk][n], out[dt]);
         }
       wave_fence();
       if (!more) break;
@@ -781,7 +740,12 @@ void paged_tile_kernel(PagedAttnArgs a) {
   };
   __syncthreads();
   pass.template operator()<false>();
-  if (__any(unusual)) pass.template operator()<true>();
+  float poison = 0.0f;  // 0 * NaN is NaN: a wave with a sum that is not finite takes its keys again
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) poison = __builtin_fmaf(out[dt][r], 0.0f, poison);
+  if (__any(poison != poison)) pass.template operator()<true>();
   {
     const LanePair pair = lane_pair<32>(sum);
     sum = pair.first + pair.second;

@@ -5,12 +5,11 @@ a run of them together as a decode loop with evictions uses them.
 Attention's tolerance. Products of a 16-bit query element and a stored value are exact in f32, as
 are those of the probabilities' pieces, so the errors are: D f32 additions of a score (each at most
 2^-24 of the sum A of the score's absolute terms), the scaled exponent's rounding and the
-exponential (a few 2^-24 of A + 1), n additions of the sums, the rounding of a probability (one f16
-piece for bf16 queries: 2^-11 of it; two f16 or bf16 pieces else: at most 2^-16; and, below f16's
-normal numbers, a row's largest being 2^11 at least, 2^-25 / 2^11 of the largest), and the output's
-rounding, half a step of the value and of its error. All but the last weigh in with E, the same
-average of |V|: |got - ref| <= eps / 2 |ref| + (1 + eps) (piece E + 2^-36 n max|V| +
-2 E 2^-24 ((D + 8) (A + 1) + n + 64)), piece = 2^-11 or 2^-16.
+exponential (a few 2^-24 of A + 1), n additions of the sums, the rounding of a probability to two
+bf16 pieces (2^-16 of it), and the output's rounding, half a step of the value and of its error. All
+but the last weigh in with E, the same average of |V|: |got - ref| <= eps / 2 |ref| +
+(1 + eps) (E (2^-16 + 2 2^-24 ((D + 8) (A + 1) + n + 64)) + 2^-126 n max(1, |V|)); the last term
+for exponentials (of which a row's largest is 1 at least) and products below f32's normal numbers.
 """
 
 import numpy as np
@@ -359,7 +358,7 @@ def reference(queries, rows, lengths, counts, kv_heads, scale):
         average = opaged.attention(q, [(k, np.abs(v)) for k, v in rows], lengths, counts, kv_heads,
                                    scale)
     batch, heads, length, dim = q.shape
-    a, top = np.zeros((batch, length, heads)), np.zeros((batch, 1, heads, dim))
+    a, top = np.zeros((batch, length, heads)), np.ones((batch, 1, heads, dim))
     for s, (keys, values) in enumerate(rows):
         b, h = divmod(s, kv_heads)
         groups = heads // kv_heads
@@ -367,7 +366,7 @@ def reference(queries, rows, lengths, counts, kv_heads, scale):
         terms = mine @ np.abs(np.nan_to_num(keys)).T * scale
         if terms.shape[-1]:
             a[b, :, h * groups:(h + 1) * groups] = terms.max(-1).T
-            top[b, 0, h * groups:(h + 1) * groups] = np.abs(values).max(0)
+            top[b, 0, h * groups:(h + 1) * groups] = np.abs(values).max(0).clip(min=1.0)
     return out, average, top, a
 
 
@@ -380,10 +379,8 @@ def check_attention(got, queries, rows, lengths, counts, kv_heads, scale=None):
     expect, average = expect.reshape(got.shape), average.reshape(got.shape)
     most = max((len(k) for k, _ in rows), default=0)
     eps = torch.finfo(queries.dtype).eps
-    piece = 2.0 ** -11 if queries.dtype == BF16 else 2.0 ** -16
-    bound = (eps / 2 * np.abs(expect) + (1 + eps)
-             * (piece * average + 2.0 ** -36 * most * top
-                + 2 * average * 2.0 ** -24 * ((dim + 8) * (a[..., None] + 1) + most + 64)))
+    bound = eps / 2 * np.abs(expect) + (1 + eps) * (2.0 ** -126 * most * top + average * (
+        2.0 ** -16 + 2 * 2.0 ** -24 * ((dim + 8) * (a[..., None] + 1) + most + 64)))
     error = np.abs(got - expect)
     assert np.all(error <= bound), float((error - bound).max())
     return expect
@@ -550,6 +547,32 @@ def test_values_of_every_size(device, dim, length, groups):
     assert not got[..., 7 * groups * dim:8 * groups * dim].any()
 
 
+@pytest.mark.parametrize("dtype,margins", [(BF16, (6, 18, 30, 55)), (F16, (6, 12, 18))])
+@pytest.mark.parametrize("segments,groups,length,most", [(2, 3, 1, 90), (8, 4, 1, 2250), (140, 3, 1, 1000),
+                                                         (144, 4, 32, 150)])
+def test_a_dominant_key_of_no_value(device, dtype, margins, segments, groups, length, most):
+    """All of the output is small probabilities on large values, on one side of zero and on both."""
+    forms = {2: [16, 4, 1], 140: [16, 8, 1], 144: [32, 4, 1]}
+    assert plan(segments, groups, length, most) == forms.get(segments, [16, 4, 18])
+    lengths = np.random.default_rng(segments).integers(5, 40, segments)
+    lengths[0], lengths[-1] = most - length, (most - length) // 2
+    cache = Cache(device, lengths + length, 2, 128, 16, dtype=dtype)
+    for s in range(segments):
+        n = int(lengths[s]) + length
+        keys, values = np.zeros((n, 128)), 8e3 * cache.rng.random((n, 128)) + 1e3
+        keys[n // 3], values[n // 3] = 1.5, 0.0
+        values[:, 64:] *= cache.rng.choice([-1, 1], (n, 64))
+        cache.store(s, 0, keys, values, np.arange(n))
+    cache.lengths = lengths.astype(np.int32)
+    cache.upload()
+    queries = torch.ones(segments // 2, 2 * groups, length, 128, dtype=dtype)
+    rows = [cache.rows(s, int(n) + length)[:2] for s, n in enumerate(lengths)]
+    for margin in margins:
+        scale = margin / 192
+        got = paged.attention(cache.layer, queries.to(device), most, scale=scale)
+        check_attention(got, queries, rows, lengths, [length] * (segments // 2), 2, scale)
+
+
 def test_max_length_bounds_the_keys(device):
     cache = Cache(device, [200, 90], 2, 128, 32)
     queries = randn(cache.rng, (1, 4, 1, 128), BF16)
@@ -661,7 +684,7 @@ def test_shared_pages_and_wide_tables(device):
 
 def test_attention_equals_packed_attention_over_the_rows_read(device):
     """The same rows give the same output but for the order of sums, half a step of either output
-    and the paged kernel's f16 probabilities, 2^-11 of the average of |V| (from the packed kernel,
+    and the paged kernel's probabilities, within 2^-16 of the average of |V| (from the packed kernel,
     rounded once)."""
     for length, dim in ((1, 128), (4, 64), (90, 128)):
         got, cache, queries = attend(device, [300, 411, 90, 1000], 2, 4, length, dim, 32)
@@ -673,7 +696,7 @@ def test_attention_equals_packed_attention_over_the_rows_read(device):
         other = packed.packed_attention(queries.to(device), keys, values, meta, length, 2)
         average = packed.packed_attention(queries.to(device), keys, values.abs(), meta, length, 2)
         a, b = got.float(), other.float()
-        bound = 2.0 ** -7 * b.abs() + 2.0 ** -11 * (1 + 2.0 ** -6) * average.float() + 1e-5
+        bound = 2.0 ** -7 * b.abs() + 2.0 ** -16 * (1 + 2.0 ** -6) * average.float() + 1e-5
         assert ((a - b).abs() <= bound).all()
 
 
