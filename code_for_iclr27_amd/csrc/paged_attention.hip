@@ -867,12 +867,12 @@ struct PagedPlan {
 //   call + round R + p (step R + share S) [+ merge + megabyte M + state N, when the keys are split],
 // where a chunk is p steps (a unit of 32 keys a wave), S workgroups share a compute unit, R rounds of
 // them follow one another (`resident` fit at once), M is the MB of partial states written and read,
-// and a thread of the merge loads N states. The constants (us) are a least-squares fit to 9,654 calls
-// (1 to 1,000 queries of 1 to 64 segments onto 100 to 130,000 rows, each kernel, 1 to 64 chunks),
-// within 6 to 8% of them; over the 1,077 shapes the choice takes 0.6% longer than the best one, 13%
-// at most. (Rules by the number of workgroups alone took 8% longer, up to 2.2 times: 8 queries of 16
-// requests onto 300 rows, 4 heads, G6, d256, 20 us against 10.8; 192 queries onto 9,000 rows 164
-// against 83.)
+// and a thread of the merge loads N states. The constants (us) are a least-squares fit to 17,944
+// calls (1 to 1,000 queries of 1 to 128 segments onto 100 to 130,000 rows, each kernel, 1 to 64
+// chunks), within 6 to 7% of them; over the 1,077 shapes the choice takes 0.7% longer than the best
+// one, 14% at most. (Rules by the number of workgroups alone took 10% longer, up to 2.2 times: 8
+// queries of 16 requests onto 300 rows, 4 heads, G6, d256, 21 us against 11.5; 192 queries onto 9,000
+// rows 170 against 87.)
 struct PagedCost {
   bool tile_kernel;
   int waves, resident;
@@ -882,16 +882,16 @@ struct MergeCost {
   double call, megabyte, state;
 };
 constexpr PagedCost kPagedCosts[3][3] = {  // d64, d128, d256
-    {{false, 4, 4, 4.2, 0.08, 0.467, 0.20},
-     {false, 8, 2, 3.7, 1.5, 0.35, 0.46},
-     {true, 4, 4, 5.15, 0.0, 0.486, 0.265}},
-    {{false, 4, 3, 3.6, 0.8, 0.467, 0.34},
-     {false, 8, 2, 1.8, 3.6, 0.0, 1.06},
-     {true, 4, 3, 5.9, 0.0, 0.477, 0.48}},
-    {{false, 4, 2, 4.95, 1.15, 0.245, 1.04},
-     {false, 8, 1, 3.15, 2.95, 2.19, 0.0},
-     {true, 4, 2, 8.4, 0.0, 1.12, 0.805}}};
-constexpr MergeCost kMergeCosts[3] = {{2.0, 0.34, 0.23}, {2.2, 0.26, 0.23}, {2.4, 0.26, 0.23}};
+    {{false, 4, 4, 4.2, 0.0, 0.446, 0.226},
+     {false, 8, 2, 4.5, 0.66, 0.375, 0.48},
+     {true, 4, 4, 5.1, 0.0, 0.455, 0.353}},
+    {{false, 4, 3, 4.4, 0.0, 0.545, 0.344},
+     {false, 8, 2, 4.4, 1.1, 0.2, 0.94},
+     {true, 4, 3, 6.0, 0.0, 0.415, 0.62}},
+    {{false, 4, 2, 5.1, 1.1, 0.624, 0.88},
+     {false, 8, 1, 3.3, 3.3, 2.27, 0.0},
+     {true, 4, 2, 8.75, 0.0, 0.632, 1.12}}};
+constexpr MergeCost kMergeCosts[3] = {{2.1, 0.34, 0.23}, {2.3, 0.26, 0.24}, {2.45, 0.27, 0.21}};
 constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
 constexpr unsigned kComputeUnits = 256, kMostSplitGroups = 4096;  // (more of them need no splitting)
 

@@ -484,7 +484,7 @@ def test_eight_waves(device, dim, page_size):
 
 @pytest.mark.parametrize("dim,segments,groups,length,rows", [(64, 36, 7, 5, 3000),
                                                              (128, 24, 7, 5, 1500),
-                                                             (256, 48, 1, 1, 800)])
+                                                             (256, 24, 3, 9, 2200)])
 def test_eight_waves_with_split_keys(device, dim, segments, groups, length, rows):
     lengths = np.random.default_rng(dim).integers(0, 90, segments)
     lengths[[1, 9, 22]] = [rows - length, rows // 2, rows // 3]
@@ -549,7 +549,7 @@ def test_values_of_every_size(device, dim, length, groups):
 
 @pytest.mark.parametrize("dtype,margins", [(BF16, (6, 18, 30, 55)), (F16, (6, 12, 18))])
 @pytest.mark.parametrize("segments,groups,length,most", [(2, 3, 1, 90), (8, 4, 1, 2250), (140, 3, 1, 1000),
-                                                         (144, 4, 32, 150)])
+                                                         (144, 3, 43, 243)])
 def test_a_dominant_key_of_no_value(device, dtype, margins, segments, groups, length, most):
     """All of the output is small probabilities on large values, on one side of zero and on both."""
     forms = {2: [16, 4, 1], 140: [16, 8, 1], 144: [32, 4, 1]}
