@@ -15,9 +15,9 @@
 //                 same keys of one channel, read transposed from the wave's V rows in LDS.
 // The values are exact in the 16-bit type, and their products exact in f32. P enters as the sum of two
 // bf16 pieces, whose products with V are exact: 8 bits and 8 of the rest, within 2^-16 of P at every
-// size, as the cached rows' packed attention keeps to. (One f16 piece, within 2^-11 down to 2^-25 of
-// a row's largest, took 113 us in the place of 131 for 1000 queries onto 4,450 rows: an eighth of a
-// bf16 output's own step, but sixteen halves of an f16 one's beside a dominant key whose V is 0. A
+// size, as attention over packed rows keeps to. (One f16 piece took 113 us in the place of 134 for 1000
+// queries onto 4,450 rows. It is within 2^-11 of P, an eighth of a bf16 output's own step, but only
+// down to 2^-25 of a row's largest: beside a dominant key whose V is 0, smaller ones are the output. A
 // third bf16 piece, all of P's bits, costs a third more products.) Scores, exponentials, their sum
 // and the products' sums are f32 throughout.
 //
@@ -30,13 +30,14 @@
 // the product and added to the rows that see their key.
 //
 // What bounds it. Decode of a long cache: memory (eight requests of 36k rows, 8 heads, G4, d128: 312 MB
-// of codes in 62 us, 5.0 TB/s; a large copy reaches 5.2). Short ones: the two launches (8 segments of
-// 2,250 rows: 8 us, 2,250 rows of eight requests 11 us). Prefill: the vector instructions, 189 a unit
-// of 32 keys and 32 rows beside 16 MFMAs (a third each for the values and the exponentials), 60% of a
-// SIMD's issue slots with 2.3 waves of it on average: 1000 queries onto 4,450 rows 113 us, where the
-// packed kernel on the same rows in 16 bits takes 171. Tried and no faster: units in flight two ahead,
-// the exponentials laid between the MFMAs of the last unit's product by hand, a raised wave priority
-// for the products, tiles of 64 rows, four waves a SIMD (11 registers spilled).
+// of codes in 63 us, 4.9 TB/s; a large copy reaches 5.2). Short ones: the two launches (8 segments of
+// 2,250 rows: 8 us, 2,250 rows of eight requests 11 us). Prefill: the vector instructions, 236 a unit
+// of 32 keys and 32 rows beside 24 MFMAs (a quarter each for the values, the exponentials and the
+// pieces), 66% of a SIMD's issue slots with 2.3 waves on average: 1000 queries onto 4,450 rows 134 us,
+// where the packed kernel on the same rows in 16 bits takes 171. Tried and no faster: units in flight
+// two ahead, the exponentials laid between the MFMAs of the last unit's product by hand, a raised wave
+// priority for the products, tiles of 64 rows, four waves a SIMD (registers spilled), the pieces' rests
+// by two-element dot products.
 
 #include <algorithm>
 #include <cmath>
