@@ -433,6 +433,13 @@ def test_decode_long(device):
     attend(device, [20001, 17], 2, 2, 1, 64, 128)
 
 
+@pytest.mark.parametrize("dim,length,groups", [(64, 1, 3), (128, 2, 1), (256, 1, 16)])
+def test_decode_of_many_parts(device, dim, length, groups):
+    """More parts than the merge loads in one round; of the second segment's, most see no key."""
+    assert plan(2, groups, length, 24000, dim)[2] > 32
+    attend(device, [24000 - length, 9000], 2, groups, length, dim, 64, seed=dim)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("length,groups,dim", [(2, 1, 64), (3, 4, 128), (8, 6, 256), (8, 4, 128),
                                                (17, 2, 64), (5, 3, 256), (16, 4, 64), (33, 4, 128),
