@@ -164,8 +164,9 @@ def attention(layer, queries, max_length, counts=None, scale=None):
     ``packed_attention`` returns it; rows of padding queries (at or past ``counts[b]``) are zero.
 
     ``max_length``: a bound on every segment's cached rows plus ``length`` (host int; rows past it
-    are not visited). ``scale`` defaults to dim^-0.5. f16 queries are for rows appended as f16 (of
-    others, keys outside f16's range read as infinities and zeros)."""
+    are not visited, and the keys are split over the chip by it). ``scale`` defaults to dim^-0.5.
+    f16 queries are for rows appended as f16 (of others, keys outside f16's range read as infinities
+    and zeros)."""
     if queries.requires_grad and torch.is_grad_enabled():
         _forward_only("attention")
     return (_native_module or _native()).paged_attention(
