@@ -13,13 +13,12 @@
 //                 of 4 + 4 keys.
 //   O^T += V^T P^T  B: the probabilities where S^T left them (the key order is free as well); A: the
 //                 same keys of one channel, read transposed from the wave's V rows in LDS.
-// The values are exact in the 16-bit type, and their products exact in f32. P enters as the sum of two
-// bf16 pieces, whose products with V are exact: 8 bits and 8 of the rest, within 2^-16 of P at every
-// size, as attention over packed rows keeps to. (One f16 piece took 113 us in the place of 134 for 1000
-// queries onto 4,450 rows. It is within 2^-11 of P, an eighth of a bf16 output's own step, but only
-// down to 2^-25 of a row's largest: beside a dominant key whose V is 0, smaller ones are the output. A
-// third bf16 piece, all of P's bits, costs a third more products.) Scores, exponentials, their sum
-// and the products' sums are f32 throughout.
+// The values are exact in the 16-bit type, and their products exact in f32. P is f32 and stays f32: it
+// enters as the sum of three bf16 pieces by truncation, 3 x 8 bits = the whole 24-bit significand, whose
+// products with V are exact (a P below 2^-110 keeps what lies above 2^-133, bf16's smallest number), as
+// attention over packed rows has it. (Two pieces took 133 us in the place of 157 for 1000 queries onto
+// 4,450 rows and 64 in the place of 65 for a long decode, and left 2^-18 to 2^-16 of P out. Three by
+// rounding: 161.) Scores, exponentials, their sum and the products' sums are f32 throughout.
 //
 // The exponentials' reference moves when a row's maximum has outgrown it by 2^kPagedSlack (as in
 // attention_tile.hip). The waves' states meet in LDS; tiles whose keys span several chunks leave
@@ -30,11 +29,10 @@
 // the product and added to the rows that see their key.
 //
 // What bounds it. Decode of a long cache: memory (eight requests of 36k rows, 8 heads, G4, d128: 312 MB
-// of codes in 63 us, 4.9 TB/s; a large copy reaches 5.2). Short ones: the two launches (8 segments of
-// 2,250 rows: 8 us, 2,250 rows of eight requests 11 us). Prefill: the vector instructions, 236 a unit
-// of 32 keys and 32 rows beside 24 MFMAs (a quarter each for the values, the exponentials and the
-// pieces), 66% of a SIMD's issue slots with 2.3 waves on average: 1000 queries onto 4,450 rows 134 us,
-// where the packed kernel on the same rows in 16 bits takes 171. Tried and no faster: units in flight
+// of codes in 65 us, 4.8 TB/s; a large copy reaches 5.2). Short ones: the two launches (8 segments of
+// 2,250 rows: 8 us, 2,250 rows of eight requests 11 us). Prefill: the vector instructions, for the
+// values, the exponentials and most of all the pieces: 1000 queries onto 4,450 rows 157 us, where the
+// packed kernel on the same rows in 16 bits takes 171. Tried and no faster: units in flight
 // two ahead, the exponentials laid between the MFMAs of the last unit's product by hand, a raised wave
 // priority for the products, tiles of 64 rows, four waves a SIMD (registers spilled), the pieces' rests
 // by two-element dot products.
@@ -56,7 +54,7 @@ constexpr int kUnit = 32;       // keys of a wave's step
 constexpr int kSmallRows = 16;  // rows of a tile: decode and a few query rows
 constexpr int kTileRows = 32;   // many query rows
 constexpr float kPagedSlack = 4.0f;
-constexpr int kPieces = 2;      // of a probability
+constexpr int kPieces = 3;      // of a probability
 
 struct PagedAttnArgs {
   const void* queries;  // element strides below; the last dimension is contiguous
@@ -104,16 +102,17 @@ __device__ __forceinline__ T* paged_output(const PagedAttnArgs& a, unsigned seg,
           h * groups + g) * D;
 }
 
-// Two f32 values as sums of two bf16 pieces each, word `w` of the piece vectors: the values rounded to
-// nearest, and the rest, an exact difference, as well.
+// Two f32 values as sums of three bf16 pieces each, word `w` of the piece vectors: the top halves of x,
+// of x minus that, and of what is left (each difference is exact, the last has at most 8 significant
+// bits).
 __device__ __forceinline__ void split_bf16(float x, float y, attn_u32x4 (&piece)[kPieces], int w) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  const bf16x2 near = {static_cast<__bf16>(x), static_cast<__bf16>(y)};
-  const unsigned both = __builtin_bit_cast(unsigned, near);
-  piece[0][w] = both;
-  const bf16x2 rest = {static_cast<__bf16>(x - __builtin_bit_cast(float, both << 16)),
-                       static_cast<__bf16>(y - __builtin_bit_cast(float, both & 0xffff0000u))};
-  piece[1][w] = __builtin_bit_cast(unsigned, rest);
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const unsigned a = __builtin_bit_cast(unsigned, x), b = __builtin_bit_cast(unsigned, y);
+    piece[i][w] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    x -= __builtin_bit_cast(float, a & 0xffff0000u);
+    y -= __builtin_bit_cast(float, b & 0xffff0000u);
+  }
 }
 
 // V rows in LDS: 16-byte chunk c of row r in slot c ^ x(r). The eight rows that eight lanes write one

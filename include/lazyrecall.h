@@ -577,7 +577,7 @@ int lr_paged_append(const void* keys, const int64_t* key_strides, const void* va
  * row, give zeros. out [batch, length, kv_heads * groups, dim], contiguous. max_keys (below
  * 2^30; no more than max_pages * page_size is of use) bounds lengths[s] + length: rows at or past it
  * are not visited. scale is positive. Products, softmax
- * and sums are f32 (the probabilities enter as sums of two bf16 pieces, within 2^-16). workspace: as
+ * and sums are f32 (the probabilities enter as sums of three bf16 pieces, all of their bits). workspace: as
  * for lr_packed_attention, of the same max_keys; 0 bytes and one launch when the keys are not
  * split. */
 size_t lr_paged_attention_workspace_bytes(int64_t segments, int64_t groups, int64_t length,

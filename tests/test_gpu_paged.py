@@ -962,3 +962,45 @@ def test_offsets_past_32_bits(device):
     k, _, p, _ = paged.read(moved, 598)
     assert np.array_equal(k.double().cpu().numpy(), np.concatenate((rows[0][0][1:], rows[1][0][:-1])))
     assert p.view(-1).cpu().tolist() == list(range(1, 300)) + list(range(299))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("segments,groups,length,most", [(8, 4, 1, 90), (8, 4, 1, 2250),
+                                                         (140, 3, 1, 1000), (144, 3, 43, 243)])
+def test_probabilities_keep_all_of_their_bits(device, dtype, dim, segments, groups, length, most):
+    """Two keys of nearly the same score whose values cancel: the output, 2^-12 of the average of
+    |V|, is what their probabilities differ by. Scores are exact (two channels), and of the others
+    P is below 2^-69 and V 0, so errors are counted without the scores' additions, in units of 2^-24 of the
+    average: 7 for the exponents (their products, references and differences, 10 2^-24 in all, times
+    ln 2), 6 for three exponentials, 12 for the additions and the weights that join three keys, 3 for
+    the division. (Probabilities of 16 to 18 bits miss it by 2 to 3 times.)"""
+    forms = {140: [16, 8, 1], 144: [32, 4, 1]}
+    assert plan(segments, groups, length, most, dim) == forms.get(
+        segments, [16, 4, 1] if most == 90 else [16, 4, 18])
+    lengths = np.random.default_rng(segments).integers(5, 40, segments)
+    lengths[0], lengths[-1] = most - length, (most - length) // 2
+    cache = Cache(device, lengths + length, 2, dim, 16, dtype=dtype)
+    for s in range(segments):
+        n = int(lengths[s])
+        keys, values = np.zeros((n + length, dim)), np.zeros((n + length, dim))
+        keys[:, 0] = -192.0
+        places = cache.rng.permutation(n)[:3]
+        keys[places, 0] = 6.0, 4.0, 4.0
+        keys[places[2], 32] = 6 * 2.0 ** -12
+        values[places[1]], values[places[2]] = 96.0, -96.0
+        cache.store(s, 0, keys, values, np.arange(n + length))
+    cache.lengths = lengths.astype(np.int32)
+    cache.upload()
+    queries = torch.zeros(segments // 2, 2 * groups, length, dim, dtype=dtype)
+    rows = torch.arange(queries[..., 0].numel()).view(queries.shape[:3])
+    queries[..., 0], queries[..., 32] = 1 + rows % 97 / 128.0, 1.0
+    got = paged.attention(cache.layer, queries.to(device), most, scale=0.25)
+    held = [cache.rows(s, int(n) + length)[:2] for s, n in enumerate(lengths)]
+    counts = [length] * (segments // 2)
+    expect, average = (opaged.attention(queries.double().numpy(), [(k, f(v)) for k, v in held],
+                                        lengths, counts, 2, 0.25) for f in (np.asarray, np.abs))
+    eps = torch.finfo(dtype).eps
+    bound = eps / 2 * np.abs(expect) + (1 + eps) * 28 * 2.0 ** -24 * average
+    error = np.abs(got.double().cpu().numpy() - expect)
+    assert np.all(error <= bound), float((error / bound).max())
