@@ -26,7 +26,8 @@
 //
 // A masked key contributes nothing: its score becomes -inf, its P 0. As 0 * NaN is NaN, a wave that
 // ends with a non-finite sum takes its keys again, with the blocks of V that read as NaN kept out of
-// the product and added to the rows that see their key.
+// the product and added to the rows that see their key. So does one whose scores are so large that the
+// reference's own rounding would show in the exponentials (kLargeReference).
 //
 // What bounds it. Decode of a long cache: memory (eight requests of 36k rows, 8 heads, G4, d128: 312 MB
 // of codes in 65 us, 4.8 TB/s; a large copy reaches 5.2). Short ones: the two launches (8 segments of
@@ -55,6 +56,10 @@ constexpr int kSmallRows = 16;  // rows of a tile: decode and a few query rows
 constexpr int kTileRows = 32;   // many query rows
 constexpr float kPagedSlack = 4.0f;
 constexpr int kPieces = 3;      // of a probability
+// A row's largest exponent (of two) up to which score * to_log2 - reference is one multiply-add: the
+// reference is a rounded product, off by half at most, so the largest P stays within 2^(slack + 1/2). (From
+// 2^31 on it can be off by more than f32's exponents hold.)
+constexpr float kLargeReference = 0x1p24f;
 
 struct PagedAttnArgs {
   const void* queries;  // element strides below; the last dimension is contiguous
@@ -113,6 +118,21 @@ __device__ __forceinline__ void split_bf16(float x, float y, attn_u32x4 (&piece)
     x -= __builtin_bit_cast(float, a & 0xffff0000u);
     y -= __builtin_bit_cast(float, b & 0xffff0000u);
   }
+}
+
+// The exponential of a score against its row's reference, the rounded product of its largest score and
+// to_log2 (or 0). SAFE: for references of any size; the score's product is rounded as well, so that
+// the largest one's exponent is 0.
+template <bool SAFE>
+__device__ __forceinline__ float probability(float score, float to_log2, float base) {
+  return __builtin_amdgcn_exp2f(SAFE ? score * to_log2 - base : __builtin_fmaf(score, to_log2, -base));
+}
+
+// Whether a wave has to take its keys again: a sum that is not finite (`poison` is NaN) or a reference
+// past kLargeReference (-inf: the row has seen no key).
+__device__ __forceinline__ bool take_again(float poison, float reference) {
+  return __any(poison != poison || reference > kLargeReference ||
+               (reference < -kLargeReference && reference != kNegInf));
 }
 
 // V rows in LDS: 16-byte chunk c of row r in slot c ^ x(r). The eight rows that eight lanes write one
@@ -357,7 +377,7 @@ void paged_attention_kernel(PagedAttnArgs a) {
   };
 
   // The wave's units of the chunk. SAFE: blocks of V that read as NaN are kept out of the product and
-  // added to the rows that see their key, and no exponential exceeds one.
+  // added to the rows that see their key, and no exponential exceeds one, however large the scores.
   auto pass = [&]<bool SAFE>() {
     reference = kNegInf, sum = 0.0f;
 #pragma unroll
@@ -455,8 +475,8 @@ void paged_attention_kernel(PagedAttnArgs a) {
       attn_u32x4 piece[kPieces];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n / 2][2 * (n % 2)], a.to_log2, -base));
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n / 2][2 * (n % 2) + 1], a.to_log2, -base));
+        const float x = probability<SAFE>(s[n / 2][2 * (n % 2)], a.to_log2, base);
+        const float y = probability<SAFE>(s[n / 2][2 * (n % 2) + 1], a.to_log2, base);
         sum += x;
         sum += y;
         split_bf16(x, y, piece, n);
@@ -481,12 +501,12 @@ void paged_attention_kernel(PagedAttnArgs a) {
   };
   __syncthreads();
   pass.template operator()<false>();
-  float poison = 0.0f;  // 0 * NaN is NaN: a wave with a sum that is not finite takes its keys again
+  float poison = 0.0f;  // 0 * NaN is NaN
 #pragma unroll
   for (int ct = 0; ct < DT; ++ct)
 #pragma unroll
     for (int r = 0; r < 4; ++r) poison = __builtin_fmaf(out[ct][r], 0.0f, poison);
-  if (__any(poison != poison)) pass.template operator()<true>();
+  if (take_again(poison, reference)) pass.template operator()<true>();
   {
     LanePair pair = lane_pair<16>(sum);
     pair = lane_pair<32>(pair.first + pair.second);
@@ -715,8 +735,8 @@ void paged_tile_kernel(PagedAttnArgs a) {
       attn_u32x4 piece[2][kPieces];
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * n], a.to_log2, -base));
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * n + 1], a.to_log2, -base));
+        const float x = probability<SAFE>(s[2 * n], a.to_log2, base);
+        const float y = probability<SAFE>(s[2 * n + 1], a.to_log2, base);
         sum += x;
         sum += y;
         split_bf16(x, y, piece[n / 4], n % 4);
@@ -740,12 +760,12 @@ void paged_tile_kernel(PagedAttnArgs a) {
   };
   __syncthreads();
   pass.template operator()<false>();
-  float poison = 0.0f;  // 0 * NaN is NaN: a wave with a sum that is not finite takes its keys again
+  float poison = 0.0f;  // 0 * NaN is NaN
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) poison = __builtin_fmaf(out[dt][r], 0.0f, poison);
-  if (__any(poison != poison)) pass.template operator()<true>();
+  if (take_again(poison, reference)) pass.template operator()<true>();
   {
     const LanePair pair = lane_pair<32>(sum);
     sum = pair.first + pair.second;

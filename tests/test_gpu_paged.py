@@ -1004,3 +1004,53 @@ def test_probabilities_keep_all_of_their_bits(device, dtype, dim, segments, grou
     bound = eps / 2 * np.abs(expect) + (1 + eps) * 28 * 2.0 ** -24 * average
     error = np.abs(got.double().cpu().numpy() - expect)
     assert np.all(error <= bound), float((error / bound).max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("segments,groups,length,most", [(8, 4, 1, 90), (8, 4, 1, 2250),
+                                                         (140, 3, 1, 1000), (144, 3, 43, 243)])
+def test_scores_of_every_finite_size(device, dtype, dim, segments, groups, length, most):
+    """Scores of 2^27 to 2^59, whose rounded products with the scale are off by up to 2^35: the keys
+    of a row's largest score share the output, the others lie far below. Scores are exact (equal
+    channels of a few bits each), so the largest one's probability is one, the output the mean of
+    their values: off by its rounding and, in units of 2^-24 of the average of |V|, one for each of up to
+    `most` additions to the sum and the products' sum and 64 for the rest."""
+    forms = {140: [16, 8, 1], 144: [32, 4, 1]}
+    assert plan(segments, groups, length, most, dim) == forms.get(
+        segments, [16, 4, 1] if most == 90 else [16, 4, 18])
+    lengths = np.random.default_rng(segments).integers(5, 40, segments)
+    lengths[0], lengths[-1] = most - length, (most - length) // 2
+    cache = Cache(device, lengths + length, 2, dim, 16, dtype=dtype)
+    codes = np.array([0, .5, 1, 1.5, 2, 3, 4, 6, -.5, -1, -1.5, -2, -3, -4, -6]) * 2.0 ** 13
+    for s in range(segments):
+        n = int(lengths[s]) + length
+        keys = np.repeat(cache.rng.choice(codes, (n, 1)), dim, 1)
+        if s % 4 == 3:  # all scores of one sign, growing to the end
+            keys = np.sort(np.abs(keys), 0)
+        cache.store(s, 0, keys, cache.rng.standard_normal((n, dim)), np.arange(n))
+    cache.lengths = lengths.astype(np.int32)
+    cache.upload()
+    sizes = 2.0 ** 12 * torch.tensor([1.0, -1.125, 8.0, -8.0, 1.875, -15.0, 13.0])
+    queries = torch.ones(segments // 2, 2 * groups, length, dim, dtype=dtype)
+    rows = torch.arange(queries[..., 0].numel()).view(queries.shape[:3])
+    queries *= sizes[rows % 7].unsqueeze(-1).to(dtype)
+    held = [cache.rows(s, int(n) + length)[:2] for s, n in enumerate(lengths)]
+    expect, average = np.zeros((2, segments // 2, length, 2 * groups, dim))
+    for s, (keys, values) in enumerate(held):
+        b, h = divmod(s, 2)
+        for i in range(length):
+            n = int(lengths[s]) + i + 1
+            for sign in (1, -1):
+                scores = sign * keys[:n, 0]
+                top = scores == scores.max()
+                heads = [g for g in range(h * groups, (h + 1) * groups)
+                         if float(queries[b, g, i, 0]) * sign > 0]
+                expect[b, i, heads] = values[:n][top].mean(0)
+                average[b, i, heads] = np.abs(values[:n][top]).mean(0)
+    eps = torch.finfo(dtype).eps
+    bound = eps / 2 * np.abs(expect) + (1 + eps) * average * 2.0 ** -24 * (2 * most + 64)
+    for scale in (2.0 ** -3, 1.0, 2.0 ** 20):
+        got = paged.attention(cache.layer, queries.to(device), most, scale=scale)
+        error = np.abs(got.double().cpu().numpy().reshape(expect.shape) - expect)
+        assert np.all(error <= bound), (scale, np.argwhere(~(error <= bound))[:3].tolist())
