@@ -38,7 +38,8 @@
 //
 // A masked key never contributes: scores past a query's limit become -inf. Their P is 0, and as
 // 0 * V is NaN for a non-finite V, a wave that ends with a non-finite accumulator recomputes its
-// rows key by key over the visible keys only.
+// rows key by key over the visible keys only. So does one whose scores are so large that the
+// reference's own rounding would show in the exponentials (kLargeReference).
 
 #include <algorithm>
 #include <cmath>
@@ -57,6 +58,10 @@ typedef unsigned tile_u32x2 __attribute__((ext_vector_type(2)));
 constexpr int kTileWaves = 4;
 constexpr int kWaveRows = 32;
 constexpr float kSlack = 4.0f;  // exponents of two a row maximum may exceed its reference by
+// A row's largest exponent (of two) up to which score * to_log2 - reference is one multiply-add: the
+// reference is a rounded product, off by 2 at most. (From 2^31 on it can be off by more than f32's
+// exponents hold.)
+constexpr float kLargeReference = 0x1p26f;
 
 constexpr int kStageKeys = 32;
 constexpr int kBuffers = 2;     // K and V stages in LDS
@@ -460,8 +465,12 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) poison = __builtin_fmaf(out[dt][r], 0.0f, poison);
-  if (__any(row_valid && poison != poison)) {
-    // Non-finite inputs (or sums past f32): this wave's rows again over their visible keys only.
+  const bool large = reference > kLargeReference ||
+                     (reference < -kLargeReference && reference != kNegInf);
+  if (__any(row_valid && (poison != poison || large))) {
+    // Non-finite inputs (or sums past f32, or very large scores): this wave's rows again over their
+    // visible keys only. (The score's product with the scale is rounded as the reference is: the
+    // largest score's exponent is the same whatever their size.)
     const int stop = min(end, limit + 1);
     auto score = [&](int key) {
       const T* k_row = reinterpret_cast<const T*>(keys) + static_cast<int64_t>(key) * D;
@@ -488,7 +497,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(
       for (int r = 0; r < 16; ++r) out[dt][r] = 0.0f;
 #pragma unroll 1
     for (int key = begin; key < stop; ++key) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(score(key), to_log2, -base));
+      const float p = __builtin_amdgcn_exp2f(score(key) * to_log2 - base);
       sum += p;
       const T* v = reinterpret_cast<const T*>(values) + static_cast<int64_t>(key) * D + 4 * half;
 #pragma unroll

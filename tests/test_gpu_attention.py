@@ -471,3 +471,46 @@ def test_decode_step_with_appends_deferred_to_one_launch(device):
         assert torch.equal(keys[rows], k) and torch.equal(values[rows], v)
         assert torch.equal(positions[rows].reshape(-1), p.reshape(-1))
         assert torch.equal(cumulative[l], cu)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [*TILE_FORMS, (2, 4, 11, 300, 128), (2, 1, 1, 400, 64)])
+def test_scores_of_every_finite_size(device, dtype, shape):
+    """Scores of 2^27 to 2^59, whose rounded products with the scale are off by up to 2^35: the keys
+    of a row's largest score share the output, the others lie far below. Scores are exact (equal
+    channels of a few bits each), so the largest one's probability is one, the output the mean of
+    their values: off by its rounding and, in units of 2^-24 of the average of |V|, one for each of up to
+    `keys` additions to the sum and the products' sum and 64 for the rest."""
+    segments, groups, length, keys, dim = shape
+    if shape in TILE_FORMS:
+        assert plan(*shape, dtype)[0] == TILE_FORMS[shape][0]
+    q, k, v, cu, meta = make(device, 1, segments, groups, length, dim, [keys] * segments, dtype,
+                             seed=31)
+    rng = np.random.default_rng(32)
+    codes = np.array([0, .5, 1, 1.5, 2, 3, 4, 6, -.5, -1, -1.5, -2, -3, -4, -6]) * 2.0 ** 13
+    drawn = rng.choice(codes, (segments, keys))
+    drawn[1::4] = np.sort(np.abs(drawn[1::4]), 1)  # scores of one sign, growing to the end
+    k[:] = torch.from_numpy(drawn.reshape(-1, 1)).to(dtype)
+    sizes = 2.0 ** 12 * torch.tensor([1.0, -1.125, 8.0, -8.0, 1.875, -15.0, 13.0])
+    size = sizes[torch.arange(segments * groups * length).view(q.shape[:3]) % 7]
+    q[:] = size.unsqueeze(-1).to(dtype)
+    values = v.double().numpy().reshape(segments, keys, dim)
+    first, signs = keys - length, size[0].sign().numpy().reshape(segments, groups, length)
+    means = np.zeros((2, 2, segments, length, dim))  # of the values, of their magnitudes
+    for s in range(segments):
+        for n, sign in enumerate((1, -1)):
+            scores = sign * drawn[s]
+            for i in range(length):
+                seen = scores[:first + i + 1]
+                top = seen == seen.max()
+                means[0, n, s, i] = values[s, :first + i + 1][top].mean(0)
+                means[1, n, s, i] = np.abs(values[s, :first + i + 1][top]).mean(0)
+    eps = torch.finfo(dtype).eps
+    for scale in (2.0 ** -3, -1.0, 2.0 ** 20):
+        at = (signs * scale < 0).astype(int).transpose(2, 0, 1)  # [length, segments, groups]
+        place = (at, np.arange(segments)[None, :, None], np.arange(length)[:, None, None])
+        expect, average = means[0][place], means[1][place]
+        got = through_the_abi(device, "lr_packed_attention", q, k, v, meta, length, segments, scale)
+        error = np.abs(got.double().cpu().numpy().reshape(expect.shape) - expect)
+        bound = eps / 2 * np.abs(expect) + (1 + eps) * average * 2.0 ** -24 * (2 * keys + 64)
+        assert np.all(error <= bound), (scale, np.argwhere(~(error <= bound))[:3].tolist())
