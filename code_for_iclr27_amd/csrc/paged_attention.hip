@@ -91,6 +91,7 @@ __device__ __forceinline__ TileKeys tile_keys(const PagedAttnArgs& a, unsigned s
     const int c = a.counts[seg / static_cast<unsigned>(a.kv_heads)];
     t.count = c < 0 ? 0 : c < a.length ? c : a.length;
   }
+  if (a.cache.lengths[seg] < 0) t.count = 0;  // (append has stored nothing there)
   const int first = static_cast<int>(row0 / groups), last = static_cast<int>(last_row / groups);
   const int most = min(a.cache.max_pages << a.cache.shift, a.max_keys);
   t.key_end = first < t.count ? min(most, t.cached + min(last, t.count - 1) + 1) : 0;

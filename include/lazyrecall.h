@@ -535,7 +535,8 @@ int lr_packed_attention_noalloc(const void* queries, int64_t q_batch_stride,
  *
  * Layout. Segment s = request b * kv_heads + KV head h. Its row i lies in page
  * table[s * max_pages + i / page_size], slot i % page_size; it has lengths[s] rows (clamped to
- * [0, max_pages * page_size]). A page is lr_paged_page_bytes(page_size, dim) bytes: the keys'
+ * [0, max_pages * page_size]; a segment of a negative length takes no new ones). A page is
+ * lr_paged_page_bytes(page_size, dim) bytes: the keys'
  * codes [page_size, dim / 2], the values' codes, the keys' scales [page_size, dim / 32], the
  * values' scales, the rows' positions (f32). Channels 32 k .. 32 k + 31 of a row form a block of
  * OCP MX FP4: E2M1 codes (the even channel in the low nibble) times 2^(scale - 127); scale 255:

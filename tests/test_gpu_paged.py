@@ -1054,3 +1054,18 @@ def test_scores_of_every_finite_size(device, dtype, dim, segments, groups, lengt
         got = paged.attention(cache.layer, queries.to(device), most, scale=scale)
         error = np.abs(got.double().cpu().numpy().reshape(expect.shape) - expect)
         assert np.all(error <= bound), (scale, np.argwhere(~(error <= bound))[:3].tolist())
+
+
+@pytest.mark.parametrize("length,groups,most", [(1, 4, 90), (5, 3, 2250), (128, 24, 300)])
+def test_a_segment_of_negative_length_has_no_rows_to_attend_to(device, length, groups, most):
+    """Appends store nothing behind a negative length, so its queries see nothing either: not the
+    rows that lie in its pages' first slots."""
+    cache = Cache(device, [60, 200, 70, 90], 2, 64, 16)
+    cache.lengths = np.array([40, -1, -(2 ** 31), 60], np.int32)
+    cache.upload()
+    queries = randn(cache.rng, (2, 2 * groups, length, 64), BF16)
+    got = paged.attention(cache.layer, queries.to(device), most)
+    got = got.view(2, length, 2, groups * 64)
+    assert not got[0, :, 1].any() and not got[1, :, 0].any()
+    assert got[0, :, 0].any(-1).all() and got[1, :, 1].any(-1).all()
+    assert paged.read(cache.layer, 100)[3].cpu().tolist() == [0, 40, 40, 40, 100]
