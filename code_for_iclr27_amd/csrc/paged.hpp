@@ -90,6 +90,9 @@ inline int64_t paged_bytes(int64_t page_size, int64_t dim) {
   return page_size * (dim + dim / 16 + 4);
 }
 
+// A launch has fewer than 2^32 threads.
+inline bool launchable(int64_t blocks, int64_t threads) { return blocks < (int64_t{1} << 32) / threads; }
+
 // The checks every entry point makes of the cache.
 int check_paged(const void* pages, int64_t page_count, int64_t page_size, int64_t dim,
                 const int32_t* table, int64_t max_pages, const int32_t* lengths, int64_t segments);

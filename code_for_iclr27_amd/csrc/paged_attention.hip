@@ -1070,9 +1070,8 @@ extern "C" int lr_paged_attention(const void* queries, const int64_t* query_stri
              "Attention workspace too small");
   LR_REQUIRE(needed == 0 || reinterpret_cast<uintptr_t>(workspace) % 256 == 0,
              "Attention workspace must be 256-byte aligned");
-  LR_REQUIRE(plan.units <= INT32_MAX / plan.splits &&
-                 plan.units <= INT32_MAX / ceil_div(int64_t{plan.tile_rows} * dim / 8, kMergeItems),
-             "Attention grid too large");
+  // (the merge of a split call, of at most kMostSplitGroups parts, has fewer)
+  LR_REQUIRE(launchable(plan.units * plan.splits, 64 * plan.waves), "Attention grid too large");
 
   PagedAttnArgs args{};
   args.queries = queries;

@@ -661,7 +661,7 @@ extern "C" int lr_paged_append(const void* keys, const int64_t* key_strides, con
   const int64_t per_block = kThreads / (dim / (pairs ? 16 : 8));
   const int64_t kv_blocks = ceil_div(batch * added * ceil_div(kv_heads, heads), per_block);
   const int64_t blocks = 2 * kv_blocks + ceil_div(batch * added * ceil_div(query_heads, heads), per_block);
-  LR_REQUIRE(blocks < (int64_t{1} << 31), "Appended grid too large");
+  LR_REQUIRE(launchable(blocks, kThreads), "Appended grid too large");
   args.kv_blocks = static_cast<unsigned>(kv_blocks);
   return dispatch_type(dtype, [&]<typename T>() {
     return dispatch_dim(dim, [&]<int D>() {
@@ -690,6 +690,8 @@ extern "C" int lr_paged_read(const void* pages, int64_t page_count, int64_t page
              "Invalid packed buffers");
   LR_REQUIRE(((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) % 16) == 0,
              "Packed buffers must be 16-byte aligned");
+  const int64_t blocks = ceil_div(total, kReadRows);
+  LR_REQUIRE(launchable(blocks, kThreads), "Packed rows' grid too large");
   // One launch where a workgroup can sum the lengths itself, beside its rows' lookups; calls without
   // rows or pages have only the sums to write.
   const bool fused = segments <= kFusedSegments && total > 0 && page_count > 0;
@@ -701,7 +703,6 @@ extern "C" int lr_paged_read(const void* pages, int64_t page_count, int64_t page
     if (total == 0 || page_count == 0) return LR_OK;
   }
   const ReadArgs args{cache, segments, total, cumulative, keys, values, positions};
-  const int64_t blocks = ceil_div(total, kReadRows);
   return dispatch_type(dtype, [&]<typename T>() {
     return dispatch_dim(dim, [&]<int D>() {
       auto launch = [&](auto kernel) {
@@ -751,7 +752,7 @@ extern "C" int lr_paged_compact(void* pages, int64_t page_count, int64_t page_si
   args.removed_count = removed_count;
   args.sums = static_cast<int64_t*>(workspace);
   args.new_lengths = new_lengths;
-  LR_REQUIRE(segments <= INT32_MAX / args.chunks, "Compaction grid too large");
+  LR_REQUIRE(launchable(segments * args.chunks, kThreads), "Compaction grid too large");
   if (needed) {
     hipLaunchKernelGGL(paged_sum_kernel<int64_t>, dim3(1), dim3(kSumThreads), 0, as_stream(stream),
                        args.cache, segments, static_cast<int64_t*>(workspace));

@@ -242,3 +242,23 @@ def test_pool():
     assert not layer.lengths.any() and layer.kv_heads == 3 and layer.dim == 128
     wide, none = pool.table([0, 0], width=3)
     assert wide.shape == (2, 3) and none == []
+
+
+def test_launches_of_2_to_the_32_threads_are_refused():
+    """A launch has fewer: larger calls are refused before anything is enqueued."""
+    for over in (dict(kv_heads=1, added=2 ** 28, dim=256),
+                 dict(kv_heads=1, added=2 ** 27, dim=256, half=8, cos=256, sin=256, table_rows=9)):
+        assert append(**over) == 1 and "Appended grid too large" in _lib.last_error(), over
+    for over in (dict(batch=2 ** 24, kv_heads=1, groups=1), dict(batch=2 ** 23, kv_heads=1, groups=40),
+                 dict(kv_heads=1, batch=1, groups=2 ** 6, length=2 ** 23)):
+        assert attend(max_keys=32, **over) == 1, over
+        assert "Attention grid too large" in _lib.last_error(), over
+    library = _lib.load()
+    assert library.lr_paged_read(256, 4, 32, 8, 2, 8, 2, 128, _lib.LR_DTYPE_BF16, 2 ** 30, 256, 256,
+                                 8, 8, None) == 1
+    assert "Packed rows' grid too large" in _lib.last_error()
+    for segments, pages in ((2 ** 24, 1), (5, 2 ** 22 - 1)):
+        size = library.lr_paged_compact_workspace_bytes(segments)
+        assert library.lr_paged_compact(256, 4, 256, 8, pages, 8, segments, 128, 8, 3, 16, 1, 16,
+                                        256, size, None) == 1
+        assert "Compaction grid too large" in _lib.last_error(), segments
