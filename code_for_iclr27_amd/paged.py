@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import dataclasses
 from collections import deque
+from itertools import islice
 from typing import Sequence
 
 import torch
@@ -86,13 +87,16 @@ class PagePool:
             raise RuntimeError(f"Page pool exhausted: {sum(needed)} pages wanted, "
                                f"{len(self._free)} free")
         host = torch.full((len(needed), width), -1, dtype=torch.int32)
-        ids = []
+        ids = list(islice(self._free, sum(needed)))
+        first = 0
         for segment, count in enumerate(needed):
-            mine = [self._free.popleft() for _ in range(count)]
-            host[segment, :count] = torch.tensor(mine, dtype=torch.int32)
-            ids += mine
+            host[segment, :count] = torch.tensor(ids[first:first + count], dtype=torch.int32)
+            first += count
+        table = host.to(self.pages.device)
+        for _ in ids:  # taken once the table is there: an upload that fails takes none
+            self._free.popleft()
         self._taken.update(ids)
-        return host.to(self.pages.device), ids
+        return table, ids
 
     def release(self, ids: Sequence[int]) -> None:
         """Takes pages back. Work that reads them has been enqueued on the stream that their next
@@ -106,8 +110,8 @@ class PagePool:
     def layer(self, batch: int, kv_heads: int, rows: int):
         """An empty layer with room for ``rows`` rows a segment: (PagedLayer, its pages' ids)."""
         segments = int(batch) * int(kv_heads)
-        table, ids = self.table([rows] * segments)
         lengths = torch.zeros(segments, dtype=torch.int32, device=self.pages.device)
+        table, ids = self.table([rows] * segments)
         return PagedLayer(self.pages, table, lengths, int(kv_heads), self.dim, self.page_size), ids
 
 

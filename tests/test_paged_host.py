@@ -262,3 +262,27 @@ def test_launches_of_2_to_the_32_threads_are_refused():
         assert library.lr_paged_compact(256, 4, 256, 8, pages, 8, segments, 128, 8, 3, 16, 1, 16,
                                         256, size, None) == 1
         assert "Compaction grid too large" in _lib.last_error(), segments
+
+
+def test_a_failed_upload_takes_no_pages(monkeypatch):
+    """A table that cannot be put on the device leaves the pool as it was."""
+    pool = paged.PagePool(10, 128, 32, device="cpu")
+    _, ids = pool.table([40])
+
+    def refuse(*args, **kwargs):
+        raise RuntimeError("out of memory")
+
+    with monkeypatch.context() as m:
+        m.setattr(torch.Tensor, "to", refuse)
+        with pytest.raises(RuntimeError, match="out of memory"):
+            pool.table([32, 64])
+    assert pool.free_pages == 8
+    with monkeypatch.context() as m:
+        m.setattr(torch, "zeros", refuse)
+        with pytest.raises(RuntimeError, match="out of memory"):
+            pool.layer(1, 2, 64)
+    assert pool.free_pages == 8
+    pool.release(ids)
+    table, all_pages = pool.table([320])
+    assert pool.free_pages == 0 and sorted(all_pages) == list(range(10))
+    assert table.tolist() == [all_pages]
