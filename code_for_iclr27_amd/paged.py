@@ -152,10 +152,11 @@ def append(layer, keys, values, positions, rotary=None, queries=None, counts=Non
     the tables gives NaN. ``counts`` int32 [batch] on the device: request b brings its first
     counts[b] rows only (a padded batch, or a request that has ended). Rows that the table has no
     page for are not stored."""
-    if torch.is_grad_enabled() and (keys.requires_grad or values.requires_grad
-                                    or queries is not None and queries.requires_grad):
-        _forward_only("append")
     cos, sin = (None, None) if rotary is None else rotary
+    if torch.is_grad_enabled() and (
+            keys.requires_grad or values.requires_grad or queries is not None and queries.requires_grad
+            or cos is not None and cos.requires_grad or sin is not None and sin.requires_grad):
+        _forward_only("append")
     return (_native_module or _native()).paged_append(
         layer.pages, layer.table, layer.lengths, layer.kv_heads, layer.dim, layer.page_size, keys,
         values, positions, cos, sin, queries, counts)

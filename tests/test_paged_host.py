@@ -286,3 +286,13 @@ def test_a_failed_upload_takes_no_pages(monkeypatch):
     table, all_pages = pool.table([320])
     assert pool.free_pages == 0 and sorted(all_pages) == list(range(10))
     assert table.tolist() == [all_pages]
+
+
+def test_gradients_of_the_rotation_tables_are_refused():
+    rows = torch.zeros(1, 2, 1, 128, dtype=torch.bfloat16)
+    position, angles = torch.zeros(1, 1, dtype=torch.int64), torch.zeros(4, 64, requires_grad=True)
+    for rotary in ((angles.cos(), angles.sin()), (angles.detach(), angles), (angles, angles.detach())):
+        with pytest.raises(RuntimeError, match="forward only"):
+            paged.append(cpu_layer(), rows, rows, position, rotary=rotary)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="Expected contiguous CUDA tensor"):
+            paged.append(cpu_layer(), rows, rows, position, rotary=rotary)
