@@ -1069,3 +1069,108 @@ def test_a_segment_of_negative_length_has_no_rows_to_attend_to(device, length, g
     assert not got[0, :, 1].any() and not got[1, :, 0].any()
     assert got[0, :, 0].any(-1).all() and got[1, :, 1].any(-1).all()
     assert paged.read(cache.layer, 100)[3].cpu().tolist() == [0, 40, 40, 40, 100]
+
+
+NAN_FORMS = {  # (segments, groups, queries, longest): rows of a tile, waves, split
+    (8, 4, 1, 90): (16, 4, False), (8, 4, 1, 2250): (16, 4, True), (140, 3, 1, 1000): (16, 8, False),
+    (36, 7, 5, 3000): (16, 8, True), (144, 3, 43, 243): (32, 4, False), (36, 4, 29, 2500): (32, 4, True)}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("shape", NAN_FORMS)
+def test_nan_blocks_in_every_form(device, dtype, dim, shape):
+    """NaN blocks of V and K in the first rows, in the middle of the cache (a part of its own where
+    the keys are split), at the diagonal and at the last key: a row that sees a NaN key is NaN, one
+    that sees a NaN block of V is NaN in its channels, and all others are within the tolerance."""
+    segments, groups, length, most = shape
+    rows, waves, split = NAN_FORMS[shape]
+    chosen = plan(segments, groups, length, most, dim)
+    assert chosen[:2] == [rows, waves] and (chosen[2] > 1) == split
+    lengths = np.random.default_rng(segments).integers(3, 40, segments)
+    lengths[0], lengths[3], lengths[4], lengths[5], lengths[-1] = [most - length] * 5
+    grown = lengths + length
+    cache = Cache(device, grown, 2, dim, 16, dtype=dtype, seed=dim)
+    cache.lengths = lengths.astype(np.int32)
+    blocks = dim // 32
+    marks = [(0, 1, most // 2, 0), (1, 1, int(grown[1]) - 1, blocks - 1), (2, 0, 1, 0),
+             (3, 1, most - 1 - length // 2, 1), (3, 1, 0, blocks - 1), (4, 0, most - 1, 1),
+             (5, 0, most - 1 - length // 2, 0), (5, 1, most // 3, 0)]
+    for s, which, row, block in marks:
+        at = 16 * dim + which * 16 * blocks + row % 16 * blocks + block
+        cache.pages[cache.table[s, row // 16], at] = 255
+    cache.upload()
+    queries = randn(cache.rng, (segments // 2, 2 * groups, length, dim), dtype)
+    got = paged.attention(cache.layer, queries.to(device), most)
+    held = [cache.rows(s, int(n))[:2] for s, n in enumerate(grown)]
+    counts = [length] * (segments // 2)
+    with np.errstate(invalid="ignore"):
+        expect, average, _, a = reference(queries, held, lengths, counts, 2, dim ** -0.5)
+    got = got.double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(expect))
+    assert np.isnan(expect).any() and not np.isnan(expect).all()
+    shape = (segments // 2, length, 2 * groups, dim)
+    got, expect, average = (x.reshape(shape) for x in (got, expect, average))
+    eps = torch.finfo(dtype).eps
+    # (2^-25: half of f16's subnormal step)
+    bound = eps / 2 * np.abs(expect) + (1 + eps) * average * (
+        2.0 ** -22 * ((dim + 8) * (a[..., None] + 1) + most + 64)) + 2.0 ** -25
+    fine = ~np.isnan(expect)
+    assert np.all(np.abs(got - expect)[fine] <= bound[fine])
+
+
+def test_an_audit_of_the_rows_read_back_evicts_the_same_rows(device):
+    """Prompt and decode steps in two layers, the rows read back into an audit (scores, selection,
+    its own compaction of the packed rows), and the rows that it removes taken out of the cache: the
+    pages hold what the audit's compacted layers hold, bit for bit. Twice, so that the second audit
+    meets ragged heads."""
+    from code_for_iclr27_amd import audit, scoring
+    rng = np.random.default_rng(21)
+    layers, kv_heads, groups, dim, window, budget = 2, 2, 4, 128, 16, 40
+    pool = paged.PagePool(200, dim, 16, device)
+    held = [pool.layer(1, kv_heads, 300) for _ in range(layers)]
+    lengths = [[0] * kv_heads for _ in range(layers)]
+    _, rotary = tables(1000, dim // 2, device)
+    position = 0
+    for _ in range(2):
+        for length in (150, 1, 1, 1):
+            at = torch.arange(position, position + length, device=device)[None]
+            for n, (layer, _) in enumerate(held):
+                k, v = (randn(rng, (1, kv_heads, length, dim), BF16).to(device) for _ in range(2))
+                q = randn(rng, (1, kv_heads * groups, length, dim), BF16).to(device)
+                q = paged.append(layer, k, v, at, rotary=rotary, queries=q)
+                out = paged.attention(layer, q, max(lengths[n]) + length)
+                assert out.isfinite().all()
+                layer.lengths += length
+                lengths[n] = [r + length for r in lengths[n]]
+            position += length
+        states = []
+        for n, (layer, _) in enumerate(held):
+            keys, values, where, cu = paged.read(layer, sum(lengths[n]))
+            assert cu.cpu().tolist() == np.concatenate([[0], np.cumsum(lengths[n])]).tolist()
+            states.append(scoring.LayerState(
+                keys, values, where.view(-1), lengths[n], None,
+                randn(rng, (kv_heads * groups, window, dim), BF16).to(device),
+                randn(rng, (kv_heads * groups, dim), F32).to(device)))
+        outcome = audit.AuditStep().run(
+            states, torch.arange(position - window, position, device=device),
+            torch.ones(1, device=device), layers * kv_heads * budget + 3, protect_recent=8)
+        chosen, offsets = (t.cpu().numpy() for t in (outcome.selection.removed_positions,
+                                                     outcome.selection.offsets))
+        gone = {(s.layer, s.head): chosen[offsets[i]:offsets[i + 1]]
+                for i, s in enumerate(outcome.segments)}
+        assert sum(len(g) for g in gone.values()) == layers * kv_heads * budget + 3
+        for n, (layer, pages) in enumerate(held):
+            starts = np.concatenate([[0], np.cumsum(lengths[n])])
+            removed = np.concatenate([starts[h] + gone[n, h] for h in range(kv_heads)])
+            lengths[n] = [lengths[n][h] - len(gone[n, h]) for h in range(kv_heads)]
+            target, fresh = pool.table([r + 160 for r in lengths[n]])
+            layer = paged.compact(layer, torch.from_numpy(removed).to(device), target)
+            pool.release(pages)
+            held[n] = layer, fresh
+            kept = outcome.layers[n]
+            assert list(kept.head_lens) == lengths[n] and layer.lengths.cpu().tolist() == lengths[n]
+            got = paged.read(layer, sum(lengths[n]))
+            for a, b in zip(got, (kept.keys, kept.values, kept.positions)):
+                assert torch.equal(a.view(-1), b.reshape(-1))
+    assert len({*map(tuple, lengths)}) > 1 or len(set(lengths[0])) > 1
