@@ -31,12 +31,13 @@
 //
 // What bounds it. Decode of a long cache: memory (eight requests of 36k rows, 8 heads, G4, d128: 312 MB
 // of codes in 65 us, 4.8 TB/s; a large copy reaches 5.2). Short ones: the two launches (8 segments of
-// 2,250 rows: 8 us, 2,250 rows of eight requests 11 us). Prefill: the vector instructions, for the
-// values, the exponentials and most of all the pieces: 1000 queries onto 4,450 rows 157 us, where the
-// packed kernel on the same rows in 16 bits takes 171. Tried and no faster: units in flight
-// two ahead, the exponentials laid between the MFMAs of the last unit's product by hand, a raised wave
-// priority for the products, tiles of 64 rows, four waves a SIMD (registers spilled), the pieces' rests
-// by two-element dot products.
+// 2,250 rows: 8.8 us, 2,250 rows of eight requests 11.6 us). Prefill: the vector instructions, 268 a
+// unit of 32 keys and 32 rows beside 32 MFMAs (a third for the pieces, a quarter for the values), 65% of
+// a SIMD's issue slots with 2.3 waves on average: 1000 queries onto 4,450 rows 158 us, where the packed
+// kernel on the same rows in 16 bits, with P in as many pieces, takes 206. Tried with two pieces and no
+// faster: units in flight two ahead, the exponentials laid between the MFMAs of the last unit's product
+// by hand, a raised wave priority for the products, tiles of 64 rows, four waves a SIMD (registers
+// spilled), the pieces' rests by two-element dot products.
 
 #include <algorithm>
 #include <cmath>
@@ -887,13 +888,16 @@ struct PagedPlan {
 // Which kernel runs and how many chunks the keys get: the choice with the least estimated time,
 //   call + round R + p (step R + share S) [+ merge + megabyte M + state N, when the keys are split],
 // where a chunk is p steps (a unit of 32 keys a wave), S workgroups share a compute unit, R rounds of
-// them follow one another (`resident` fit at once), M is the MB of partial states written and read,
-// and a thread of the merge loads N states. The constants (us) are a least-squares fit to 17,944
-// calls (1 to 1,000 queries of 1 to 128 segments onto 100 to 130,000 rows, each kernel, 1 to 64
-// chunks), within 6 to 7% of them; over the 1,077 shapes the choice takes 0.7% longer than the best
-// one, 14% at most. (Rules by the number of workgroups alone took 10% longer, up to 2.2 times: 8
-// queries of 16 requests onto 300 rows, 4 heads, G6, d256, 21 us against 11.5; 192 queries onto 9,000
-// rows 170 against 87.)
+// them follow one another (`resident` to a compute unit), M is the MB of partial states written and
+// read, and a thread of the merge loads N states. The constants (us) are a least-squares fit to measured
+// calls (1 to 1,000 queries of 1 to 128 segments onto 100 to 130,000 rows, each kernel, 1 to 64 chunks),
+// made when P had two pieces. With three, 17,944 such calls take 6 to 9% longer than estimated (median),
+// 7% about that; over their 1,077 shapes the choice takes 0.6% longer than the best one, 15% at most.
+// Constants fitted anew choose no better (0.5%). `resident` is a parameter of the fit like the others:
+// the registers let five workgroups of four waves share a compute unit at d64 and four at d128, and a
+// fit with these numbers comes to 0.6% too. (Rules by the number of workgroups alone take 9% longer,
+// up to twice as long: 8 queries of 16 requests onto 300 rows, 4 heads, G6, d256, 21 us against 12; 192
+// queries of one onto 9,000 rows 175 against 99.)
 struct PagedCost {
   bool tile_kernel;
   int waves, resident;

@@ -13,11 +13,13 @@
 // its cumulative lengths. Bound by memory: 155,000 rows of d256 as f16, 203 MB in 46.6 us (4.4 TB/s;
 // 78 with D / 8 threads a row that each searched for its segment); 19,000 rows of d128 5.9 us.
 //
-// compact: the rows that stay, in order, into other pages, in one launch. Bound by memory and a chain
-// of about ten dependent loads (the lengths, the searches, the tables) ahead of it: 537,000 rows of
-// d128, 150 MB read and written in 51 us (3.0 TB/s; 35 where the last-level cache holds them), 256,000
-// of d64 12.5 us. Two 64-row rounds a wave (one round of workgroups instead of one and a bit) and
-// non-temporal accesses are no faster with the read that follows.
+// compact: the rows that stay, in order, into other pages, in one launch. A wave has a chain of about ten
+// dependent loads (the lengths, the searches, the tables) ahead of its copies, then reads all of its
+// rows and writes them; as nearly all workgroups are resident at once, reads and writes hardly overlap.
+// 537,000 rows of d128, 150 MB read and written in 51 us (3.0 TB/s; 35 with the same chain where the
+// last-level cache holds them), 256,000 of d64 12.5 us. Two 64-row rounds a wave, one after the other
+// (one round of workgroups instead of one and a bit), and non-temporal accesses are no faster with the
+// read that follows.
 
 #include <algorithm>
 

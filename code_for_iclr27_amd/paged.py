@@ -16,8 +16,9 @@ One decode step of a layer::
 
 (one ``lengths`` tensor for every layer, each layer holding its row of it, makes that one launch a
 step). An audit reads the rows back (``read``), scores them as before and removes rows with
-``compact``. Every call runs on torch's current stream and waits for nothing; all of them can be
-captured into a HIP graph. There is no CPU path and no backward pass.
+``compact``. ``append``, ``attention``, ``read`` and ``compact`` run on torch's current stream and wait
+for nothing; all of them can be captured into a HIP graph. (A ``PagePool`` uploads its tables with a copy
+that the host waits for, outside of graphs.) There is no CPU path and no backward pass.
 """
 
 from __future__ import annotations
@@ -76,7 +77,9 @@ class PagePool:
 
     def table(self, rows: Sequence[int], width: int | None = None):
         """Pages for ``rows[s]`` rows of each segment: (table int32 [segments, width] on the
-        pool's device, the pages' ids for ``release``). Entries past a segment's pages are -1."""
+        pool's device, the pages' ids for ``release``). Entries past a segment's pages are -1. The
+        room is the table's for good: a segment that needs more moves to another one (``compact``),
+        or the caller writes further pages' ids into the table itself."""
         needed = [-(-int(n) // self.page_size) for n in rows]
         if any(int(n) < 0 for n in rows):
             raise RuntimeError("A segment's rows cannot be negative")
@@ -171,7 +174,7 @@ def attention(layer, queries, max_length, counts=None, scale=None):
     ``max_length``: a bound on every segment's cached rows plus ``length`` (host int; rows past it
     are not visited, and the keys are split over the chip by it). ``scale`` defaults to dim^-0.5.
     f16 queries are for rows appended as f16 (of others, keys outside f16's range read as infinities
-    and zeros)."""
+    and zeros). Finite scores may be of any size that f32 holds."""
     if queries.requires_grad and torch.is_grad_enabled():
         _forward_only("attention")
     return (_native_module or _native()).paged_attention(
@@ -182,7 +185,9 @@ def attention(layer, queries, max_length, counts=None, scale=None):
 def read(layer, total, dtype=torch.bfloat16):
     """The ``total`` rows the cache holds (the host's sum of the lengths), packed by segment:
     (keys [total, dim], values, positions float32 [total, 1], cu_seqlens_k int32 [segments + 1])
-    in ``dtype`` (bf16, f16 or f32): what ``scoring.LayerState`` and ``_C`` take."""
+    in ``dtype`` (bf16, f16 or f32): what ``scoring.LayerState`` and ``_C`` take. Rows of the outputs
+    that the cache does not hold (``total`` past its rows, or a table entry outside the pool) are not
+    written: they hold whatever their memory held."""
     return tuple((_native_module or _native()).paged_read(
         layer.pages, layer.table, layer.lengths, layer.dim, layer.page_size, int(total), dtype))
 

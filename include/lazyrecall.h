@@ -577,10 +577,11 @@ int lr_paged_append(const void* keys, const int64_t* key_strides, const void* va
  * (i < length without counts) sees rows j <= lengths[s] + i; other queries, and those that see no
  * row, give zeros. out [batch, length, kv_heads * groups, dim], contiguous. max_keys (below
  * 2^30; no more than max_pages * page_size is of use) bounds lengths[s] + length: rows at or past it
- * are not visited. scale is positive. Products, softmax
- * and sums are f32 (the probabilities enter as sums of three bf16 pieces, all of their bits). workspace: as
- * for lr_packed_attention, of the same max_keys; 0 bytes and one launch when the keys are not
- * split. */
+ * are not visited. scale is positive. Products, softmax and sums are f32 (the probabilities enter as
+ * sums of three bf16 pieces, all of their bits). A score whose product with the scale passes f32's
+ * range counts as infinite (-inf: as a masked key), and values whose weighted sum, against a largest
+ * weight of one, passes it give infinities or NaN. workspace: as for lr_packed_attention, of the same
+ * max_keys; 0 bytes and one launch when the keys are not split. */
 size_t lr_paged_attention_workspace_bytes(int64_t segments, int64_t groups, int64_t length,
                                           int64_t max_keys, int64_t dim);
 /* How a call of these sizes runs (host only): plan[0] query rows of a tile (16 or 32), plan[1] waves
