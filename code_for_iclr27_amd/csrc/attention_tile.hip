@@ -59,9 +59,9 @@ constexpr int kTileWaves = 4;
 constexpr int kWaveRows = 32;
 constexpr float kSlack = 4.0f;  // exponents of two a row maximum may exceed its reference by
 // A row's largest exponent (of two) up to which score * to_log2 - reference is one multiply-add: the
-// reference is a rounded product, off by 2 at most. (From 2^31 on it can be off by more than f32's
-// exponents hold.)
-constexpr float kLargeReference = 0x1p26f;
+// reference is a rounded product, and the multiply-add keeps the scores' differences exact, but the
+// largest P is 2^32 or 2^-32 here, and from 2^31 on f32's exponents do not hold it.
+constexpr float kLargeReference = 0x1p30f;
 
 constexpr int kStageKeys = 32;
 constexpr int kBuffers = 2;     // K and V stages in LDS
@@ -469,8 +469,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(
                      (reference < -kLargeReference && reference != kNegInf);
   if (__any(row_valid && (poison != poison || large))) {
     // Non-finite inputs (or sums past f32, or very large scores): this wave's rows again over their
-    // visible keys only. (The score's product with the scale is rounded as the reference is: the
-    // largest score's exponent is the same whatever their size.)
+    // visible keys only. (Past kLargeReference the scores' products are rounded as the reference is:
+    // the largest one's exponent is the same whatever their size.)
     const int stop = min(end, limit + 1);
     auto score = [&](int key) {
       const T* k_row = reinterpret_cast<const T*>(keys) + static_cast<int64_t>(key) * D;
@@ -497,7 +497,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(
       for (int r = 0; r < 16; ++r) out[dt][r] = 0.0f;
 #pragma unroll 1
     for (int key = begin; key < stop; ++key) {
-      const float p = __builtin_amdgcn_exp2f(score(key) * to_log2 - base);
+      const float x = score(key);
+      const float p = __builtin_amdgcn_exp2f(__builtin_fabsf(reference) > kLargeReference
+                                                 ? x * to_log2 - base : __builtin_fmaf(x, to_log2, -base));
       sum += p;
       const T* v = reinterpret_cast<const T*>(values) + static_cast<int64_t>(key) * D + 4 * half;
 #pragma unroll

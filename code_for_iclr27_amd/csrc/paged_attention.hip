@@ -58,9 +58,9 @@ constexpr int kTileRows = 32;   // many query rows
 constexpr float kPagedSlack = 4.0f;
 constexpr int kPieces = 3;      // of a probability
 // A row's largest exponent (of two) up to which score * to_log2 - reference is one multiply-add: the
-// reference is a rounded product, off by half at most, so the largest P stays within 2^(slack + 1/2). (From
-// 2^31 on it can be off by more than f32's exponents hold.)
-constexpr float kLargeReference = 0x1p24f;
+// reference is a rounded product, and the multiply-add keeps the scores' differences exact, but the
+// largest P is 2^32 or 2^-32 here, and from 2^31 on f32's exponents do not hold it.
+constexpr float kLargeReference = 0x1p30f;
 
 struct PagedAttnArgs {
   const void* queries;  // element strides below; the last dimension is contiguous
@@ -123,11 +123,13 @@ __device__ __forceinline__ void split_bf16(float x, float y, attn_u32x4 (&piece)
 }
 
 // The exponential of a score against its row's reference, the rounded product of its largest score and
-// to_log2 (or 0). SAFE: for references of any size; the score's product is rounded as well, so that
-// the largest one's exponent is 0.
+// to_log2 (or 0). SAFE: for references of any size; past kLargeReference the score's product is rounded
+// as well, so that the largest one's exponent is 0.
 template <bool SAFE>
 __device__ __forceinline__ float probability(float score, float to_log2, float base) {
-  return __builtin_amdgcn_exp2f(SAFE ? score * to_log2 - base : __builtin_fmaf(score, to_log2, -base));
+  if (SAFE && __builtin_fabsf(base) > kLargeReference)
+    return __builtin_amdgcn_exp2f(score * to_log2 - base);
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(score, to_log2, -base));
 }
 
 // Whether a wave has to take its keys again: a sum that is not finite (`poison` is NaN) or a reference
@@ -379,7 +381,7 @@ void paged_attention_kernel(PagedAttnArgs a) {
   };
 
   // The wave's units of the chunk. SAFE: blocks of V that read as NaN are kept out of the product and
-  // added to the rows that see their key, and no exponential exceeds one, however large the scores.
+  // added to the rows that see their key, and no exponential exceeds its row's largest.
   auto pass = [&]<bool SAFE>() {
     reference = kNegInf, sum = 0.0f;
 #pragma unroll

@@ -514,3 +514,36 @@ def test_scores_of_every_finite_size(device, dtype, shape):
         error = np.abs(got.double().cpu().numpy().reshape(expect.shape) - expect)
         bound = eps / 2 * np.abs(expect) + (1 + eps) * average * 2.0 ** -24 * (2 * keys + 64)
         assert np.all(error <= bound), (scale, np.argwhere(~(error <= bound))[:3].tolist())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+@pytest.mark.parametrize("shape", [*TILE_FORMS, (2, 4, 11, 300, 128), (2, 1, 1, 400, 64)])
+def test_large_scores_keep_their_differences(device, dtype, shape):
+    """Exact scores of 2^27 on either side of zero, that differ by one to eight of f32's steps there: with
+    scale 1/8 by factors of e^2 of the probabilities, by e^16 and e^128 with larger ones. An exponent is
+    exact but for the scale's rounding and its own (of at most 24: 3 2^-24 24 ln 2), so that in units
+    of 2^-24 of the average of |V| the sums' additions count, 2 `keys`, and 128 for the rest. Where that average is next to
+    nothing: half of f16's smallest step, and what lies below f32's normal numbers (of exponentials whose
+    largest is 2^-8 at least, as the reference's rounding is 8 at most at 2^28). (The split-key
+    kernel rounds each score's product with the scale: scales are powers of two.)"""
+    segments, groups, length, keys, dim = shape
+    if shape in TILE_FORMS:
+        assert plan(*shape, dtype)[0] == TILE_FORMS[shape][0]
+    q, k, v, cu, meta = make(device, 1, segments, groups, length, dim, [keys] * segments, dtype,
+                             seed=33)
+    rng = np.random.default_rng(34)
+    k[:], q[:] = 0.0, 0.0
+    k[:, 0] = 2.0 ** 15
+    k[:, 32] = torch.from_numpy(rng.choice([0, .5, 1, 1.5, 2, 3, -.5, -1], segments * keys)).to(dtype)
+    sign = 1 - 2 * (torch.arange(q[..., 0].numel()).view(q.shape[:3]) % 2)
+    q[..., 0], q[..., 32] = 4096.0 * sign, 32.0
+    arrays = [t.double().numpy() for t in (q, k, v)]
+    eps = torch.finfo(dtype).eps
+    for scale in (0.125, 1.0, 8.0):
+        expect, average = (oattention.packed_attention(*arrays[:2], f(arrays[2]), cu, segments, scale)
+                           for f in (np.asarray, np.abs))
+        got = through_the_abi(device, "lr_packed_attention", q, k, v, meta, length, segments, scale)
+        error = np.abs(got.double().cpu().numpy() - expect)
+        bound = eps / 2 * np.abs(expect) + (1 + eps) * average * 2.0 ** -24 * (2 * keys + 128)
+        bound += 2.0 ** -25 * (dtype == torch.float16) + 2.0 ** -118 * keys * 8
+        assert np.all(error <= bound), (scale, float((error / bound).max()))

@@ -1174,3 +1174,43 @@ def test_an_audit_of_the_rows_read_back_evicts_the_same_rows(device):
             for a, b in zip(got, (kept.keys, kept.values, kept.positions)):
                 assert torch.equal(a.view(-1), b.reshape(-1))
     assert len({*map(tuple, lengths)}) > 1 or len(set(lengths[0])) > 1
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("segments,groups,length,most", [(8, 4, 1, 90), (8, 4, 1, 2250),
+                                                         (140, 3, 1, 1000), (144, 3, 43, 243)])
+def test_large_scores_keep_their_differences(device, dtype, dim, segments, groups, length, most):
+    """Exact scores of 2^27 on either side of zero, that differ by one to eight of f32's steps there: with
+    scale 1/8 by factors of e^2 of the probabilities, by e^16 and e^128 with larger ones. An exponent is
+    exact but for the scale's rounding and its own (of at most 24: 3 2^-24 24 ln 2), so that in units
+    of 2^-24 of the average of |V| the sums' additions count, 2 `most`, and 128 for the rest. Where that average is next to
+    nothing: half of f16's smallest step, and what lies below f32's normal numbers (of exponentials whose
+    largest is 2^-8 at least, as the reference's rounding is 8 at most at 2^28)."""
+    forms = {140: [16, 8, 1], 144: [32, 4, 1]}
+    assert plan(segments, groups, length, most, dim) == forms.get(
+        segments, [16, 4, 1] if most == 90 else [16, 4, 18])
+    lengths = np.random.default_rng(segments).integers(5, 40, segments)
+    lengths[0], lengths[-1] = most - length, (most - length) // 2
+    cache = Cache(device, lengths + length, 2, dim, 16, dtype=dtype)
+    for s in range(segments):
+        n = int(lengths[s]) + length
+        keys = np.zeros((n, dim))
+        keys[:, 0], keys[:, 32] = 2.0 ** 15, cache.rng.choice([0, .5, 1, 1.5, 2, 3, -.5, -1], n)
+        cache.store(s, 0, keys, cache.rng.standard_normal((n, dim)), np.arange(n))
+    cache.lengths = lengths.astype(np.int32)
+    cache.upload()
+    queries = torch.zeros(segments // 2, 2 * groups, length, dim, dtype=dtype)
+    rows = torch.arange(queries[..., 0].numel()).view(queries.shape[:3])
+    queries[..., 0], queries[..., 32] = 4096.0 * (1 - 2 * (rows % 2)), 32.0
+    held = [cache.rows(s, int(n) + length)[:2] for s, n in enumerate(lengths)]
+    eps = torch.finfo(dtype).eps
+    for scale in (0.125, 1.0, 8.0):
+        got = paged.attention(cache.layer, queries.to(device), most, scale=scale)
+        expect, average = (opaged.attention(
+            queries.double().numpy(), [(k, f(v)) for k, v in held], lengths,
+            [length] * (segments // 2), 2, scale) for f in (np.asarray, np.abs))
+        bound = eps / 2 * np.abs(expect) + (1 + eps) * average * 2.0 ** -24 * (2 * most + 128)
+        bound += 2.0 ** -25 * (dtype == F16) + 2.0 ** -118 * most * 8
+        error = np.abs(got.double().cpu().numpy() - expect)
+        assert np.all(error <= bound), (scale, float((error / bound).max()))
