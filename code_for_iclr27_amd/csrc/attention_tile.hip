@@ -301,7 +301,10 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(
     top = both_halves_max(top) * to_log2;
     if (__any(top > reference + kSlack)) {
       const float raised = fmaxf(reference, top);
-      const float factor = reference == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(reference - raised);
+      // (between the bases that the exponentials were and will be taken against: past 2^24 a reference
+      // less kRaise is rounded)
+      const float factor = reference == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(
+          (reference - Vec::kRaise) - (raised - Vec::kRaise));
       sum *= factor;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)

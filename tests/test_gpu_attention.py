@@ -516,7 +516,7 @@ def test_scores_of_every_finite_size(device, dtype, shape):
         assert np.all(error <= bound), (scale, np.argwhere(~(error <= bound))[:3].tolist())
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("shape", [*TILE_FORMS, (2, 4, 11, 300, 128), (2, 1, 1, 400, 64)])
 def test_large_scores_keep_their_differences(device, dtype, shape):
     """Exact scores of 2^27 on either side of zero, that differ by one to eight of f32's steps there: with
