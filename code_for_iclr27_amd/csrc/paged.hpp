@@ -19,6 +19,7 @@
 namespace lr {
 
 typedef unsigned paged_u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned paged_u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kBlock = 32;  // channels that share a scale
 constexpr unsigned kScaleNaN = 255;

@@ -21,9 +21,7 @@
 // (one round of workgroups instead of one and a bit), and non-temporal accesses are no faster with the
 // read that follows.
 
-#include <algorithm>
-
-#include "paged.hpp"
+#include "paged_move.hpp"
 
 namespace lr {
 
@@ -43,62 +41,6 @@ int check_paged(const void* pages, int64_t page_count, int64_t page_size, int64_
 }
 
 namespace {
-
-constexpr int kThreads = 256;
-
-typedef float move_f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned move_u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned move_u32x2 __attribute__((ext_vector_type(2)));
-
-template <typename T>
-struct Eight;  // eight elements in memory
-template <>
-struct Eight<float> {
-  move_f32x4 lo, hi;
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
-  }
-  __device__ __forceinline__ void set(const float (&v)[8]) {
-    lo = move_f32x4{v[0], v[1], v[2], v[3]};
-    hi = move_f32x4{v[4], v[5], v[6], v[7]};
-  }
-};
-template <typename T>
-struct Eight {
-  typedef T vec __attribute__((ext_vector_type(8)));
-  vec x;
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(x[e]);
-  }
-  __device__ __forceinline__ void set(const float (&v)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = static_cast<T>(v[e]);  // round to nearest even
-  }
-};
-
-// Rows [batch, heads, added, D] with the strides (elements) of the first three dimensions.
-struct Rows {
-  const void* base;
-  int64_t batch, head, row;
-};
-
-struct AppendArgs {
-  Rows keys, values, queries;
-  void* out_queries;          // [batch, query_heads, added, D], contiguous
-  const int64_t* positions;   // [batch, added]
-  const float* cos;           // [table_rows, half], or half = 0
-  const float* sin;
-  int64_t table_rows;
-  int half;
-  unsigned batch, kv_heads, query_heads, added;
-  unsigned kv_rows, query_rows;  // batch * heads * added
-  unsigned kv_blocks;            // workgroups of the keys, and of the values
-  const int32_t* counts;         // [batch] rows of `added` that are there, or NULL
-  ScaleRange range;
-  PagedCache cache;
-};
 
 template <int BIT>
 __device__ __forceinline__ float quad_max(float x) {
@@ -287,70 +229,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_pairs_kernel(AppendArgs
   }
 }
 
-
-// Rows of the segments before each one, sums[s], and of all, sums[segments]: by one workgroup in a launch
-// of its own, or (up to kFusedSegments segments, a length a thread) by every workgroup for itself.
-constexpr int kSumThreads = 1024;
-constexpr int kFusedSegments = kThreads;
-
-// A packed row number as the i32 of the packed layout (rows past 2^31 - 1 are not read).
-template <typename Sum>
-__device__ __forceinline__ Sum packed_row(int64_t row) {
-  if constexpr (sizeof(Sum) == 4) return static_cast<Sum>(row < INT32_MAX ? row : INT32_MAX);
-  else return row;
-}
-
-// The sum of `n` over the workgroup's threads up to and with this one.
-template <int THREADS>
-__device__ __forceinline__ int64_t running_sum(int64_t n, int64_t (&wave_total)[THREADS / 64]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t sum = n;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t other = __shfl_up(sum, d);
-    if (lane >= d) sum += other;
-  }
-  if (lane == 63) wave_total[wave] = sum;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) sum += wave_total[w];
-  return sum;
-}
-
-template <typename Sum>
-__global__ __launch_bounds__(kSumThreads) void paged_sum_kernel(PagedCache cache, int64_t segments, Sum* sums) {
-  __shared__ int64_t wave_total[kSumThreads / 64];
-  __shared__ int64_t before;  // rows of the segments of earlier rounds
-  if (threadIdx.x == 0) before = 0, sums[0] = 0;
-  for (int64_t s0 = 0; s0 < segments; s0 += kSumThreads) {
-    const int64_t s = s0 + threadIdx.x;
-    const int64_t sum = running_sum<kSumThreads>(s < segments ? cache.rows(s) : 0, wave_total) + before;
-    if (s < segments) sums[s + 1] = packed_row<Sum>(sum);
-    __syncthreads();
-    if (threadIdx.x == kSumThreads - 1) before = sum;
-    __syncthreads();
-  }
-}
-
-template <typename Sum>
-__device__ __forceinline__ void sum_lengths(const PagedCache& cache, int segments, Sum* sums) {
-  __shared__ int64_t wave_total[kThreads / 64];
-  const int thread = static_cast<int>(threadIdx.x);
-  const int64_t sum = running_sum<kThreads>(thread < segments ? cache.rows(thread) : 0, wave_total);
-  if (thread == 0) sums[0] = 0;
-  if (thread < segments) sums[thread + 1] = packed_row<Sum>(sum);
-  __syncthreads();
-}
-
 // ---------------------------------------------------------------------------------------
-struct ReadArgs {
-  PagedCache cache;
-  int64_t segments, total;
-  int32_t* cumulative;  // [segments + 1]: written by the fused form, read by the other
-  void* keys;
-  void* values;
-  float* positions;
-};
-
 template <typename T>
 __device__ __forceinline__ Eight<T> eight_values(unsigned codes, float scale) {
   if constexpr (std::is_same<T, float>::value) {
@@ -362,19 +241,6 @@ __device__ __forceinline__ Eight<T> eight_values(unsigned codes, float scale) {
   } else {
     return {__builtin_bit_cast(typename Eight<T>::vec, expand8<T>(codes, scale))};
   }
-}
-
-constexpr int kReadRows = 64;             // of a workgroup
-// The segment that packed row `row` < cumulative[segments] belongs to: the largest s with
-// cumulative[s] <= row.
-__device__ __forceinline__ int segment_of(const int32_t* cumulative, int segments, int row) {
-  int low = 0, high = segments;
-  while (high - low > 1) {
-    const int mid = (low + high) >> 1;
-    if (cumulative[mid] <= row) low = mid;
-    else high = mid;
-  }
-  return low;
 }
 
 // A workgroup takes 64 packed rows: the first wave finds each one's page and slot, then D / 8 threads
@@ -442,40 +308,6 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(ReadArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------
-struct CompactArgs {
-  PagedCache cache;
-  int64_t segments;
-  int chunks;                   // of kCompactRows rows of a segment
-  const int32_t* target;        // [segments, target_pages]
-  int target_pages;
-  const int64_t* removed;       // sorted packed rows
-  int64_t removed_count;
-  const int64_t* sums;          // [segments + 1], unless the workgroups sum the lengths themselves
-  int32_t* new_lengths;
-};
-
-constexpr int kCompactRows = kThreads;  // of a workgroup, 64 a wave
-
-// The first of [low, high) that is not `before` (all of those before it are): 32 lanes look at 32
-// places a round, each half of the wave for a range of its own.
-template <typename F>
-__device__ __forceinline__ int64_t half_search(int64_t low, int64_t high, F before) {
-  const int place = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
-  while (true) {
-    const int64_t step = (high - low + 31) / 32;  // 0 once the range is empty
-    const int64_t at = low + place * step;
-    const bool below = step > 0 && at < high && before(at);
-    const unsigned held = static_cast<unsigned>(__ballot(below) >> (32 * half));
-    const int count = __builtin_popcount(held);  // of the places looked at, the first ones
-    if (step > 0) {
-      const int64_t next = low + count * step;
-      low = count > 0 ? low + (count - 1) * step + 1 : low;
-      high = next < high ? next : high;
-    }
-    if (!__any(high > low)) return low;
-  }
-}
-
 // A wave moves 64 rows of a segment: row r comes from row r + how many removed rows lie at or before
 // it. The wave finds that number for its first and its last row, each lane its own between them;
 // then all lanes copy 16 bytes each of the rows' codes.
@@ -570,19 +402,6 @@ __global__ __launch_bounds__(kThreads) void paged_compact_kernel(CompactArgs a) 
   *reinterpret_cast<float*>(out + Page<D>::position(cache.shift, to_slot)) = position;
 }
 
-template <typename F>
-int dispatch_type(int dtype, F&& f) {
-  switch (dtype) {
-    case LR_DTYPE_BF16: return f.template operator()<__bf16>();
-    case LR_DTYPE_F16: return f.template operator()<_Float16>();
-    default: return f.template operator()<float>();
-  }
-}
-
-bool paged_type(int dtype) {
-  return dtype == LR_DTYPE_BF16 || dtype == LR_DTYPE_F16 || dtype == LR_DTYPE_F32;
-}
-
 }  // namespace
 }  // namespace lr
 
@@ -601,125 +420,60 @@ extern "C" int lr_paged_append(const void* keys, const int64_t* key_strides, con
                                const int32_t* counts, void* pages, int64_t page_count,
                                int64_t page_size, const int32_t* table, int64_t max_pages,
                                const int32_t* lengths, void* stream) {
-  clear_error();
-  LR_REQUIRE(paged_type(dtype), "Appended rows must be bf16, f16 or f32");
-  LR_REQUIRE(batch > 0 && kv_heads > 0 && added >= 0 && query_heads >= 0 &&
-                 (query_heads > 0) == (queries != nullptr),
-             "Invalid appended shape");
-  LR_REQUIRE(batch <= INT32_MAX / kv_heads, "Invalid appended shape");
-  if (int status = check_paged(pages, page_count, page_size, dim, table, max_pages, lengths,
-                               batch * kv_heads))
-    return status;
-  if (added == 0) return LR_OK;
-  LR_REQUIRE(keys && values && positions && key_strides && value_strides &&
-                 (queries == nullptr) == (out_queries == nullptr) &&
-                 (queries == nullptr || query_strides != nullptr),
-             "Invalid appended KV");
-  LR_REQUIRE(half >= 0 && half % 8 == 0 && 2 * half <= dim && table_rows >= 0 &&
-                 (half == 0 || (cos && sin && table_rows > 0)),
-             "Rotated channels must be a multiple of 16, at most the head dimension, with tables");
-  LR_REQUIRE(added <= INT32_MAX / (batch * kv_heads) &&
-                 (query_heads == 0 || added <= INT32_MAX / batch / query_heads),
-             "Appended grid too large");
-  uintptr_t alignment = reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values) |
-                        reinterpret_cast<uintptr_t>(queries) |
-                        reinterpret_cast<uintptr_t>(out_queries) | reinterpret_cast<uintptr_t>(cos) |
-                        reinterpret_cast<uintptr_t>(sin);
-  const int64_t elem = dtype == LR_DTYPE_F32 ? 4 : 2;
-  for (int i = 0; i < 3; ++i) {
-    alignment |= static_cast<uintptr_t>((key_strides[i] | value_strides[i]) * elem);
-    if (queries != nullptr) alignment |= static_cast<uintptr_t>(query_strides[i] * elem);
-  }
-  LR_REQUIRE(alignment % 16 == 0, "Appended operands must be 16-byte aligned");
-
-  AppendArgs args{};
-  auto rows = [](const void* base, const int64_t* strides) {
-    return base ? Rows{base, strides[0], strides[1], strides[2]} : Rows{};
-  };
-  args.keys = rows(keys, key_strides);
-  args.values = rows(values, value_strides);
-  args.queries = rows(queries, query_strides);
-  args.out_queries = out_queries;
-  args.positions = positions;
-  args.cos = cos;
-  args.sin = sin;
-  args.table_rows = table_rows;
-  args.half = static_cast<int>(half);
-  args.kv_heads = static_cast<unsigned>(kv_heads);
-  args.query_heads = static_cast<unsigned>(query_heads);
-  args.added = static_cast<unsigned>(added);
-  args.kv_rows = static_cast<unsigned>(batch * kv_heads * added);
-  args.query_rows = static_cast<unsigned>(batch * query_heads * added);
-  args.counts = counts;
-  args.range = dtype == LR_DTYPE_F16 ? kHalfRange : kWideRange;
-  args.cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
-  args.batch = static_cast<unsigned>(batch);
-  // Rotated blocks whole: the pairs kernel, four heads a thread where there are enough rows to fill
-  // the chip with them (8,192 tokens, 393,000 rows: 36 us against 47 with a row's D / 8 threads and
-  // one head; a step of eight requests, 384 rows, 3.4 either way).
-  const bool pairs = half % kBlock == 0;
-  const int64_t all_rows = 2 * static_cast<int64_t>(args.kv_rows) + args.query_rows;
-  const int64_t heads = pairs && all_rows >= 32768 ? 4 : 1;
-  const int64_t per_block = kThreads / (dim / (pairs ? 16 : 8));
-  const int64_t kv_blocks = ceil_div(batch * added * ceil_div(kv_heads, heads), per_block);
-  const int64_t blocks = 2 * kv_blocks + ceil_div(batch * added * ceil_div(query_heads, heads), per_block);
-  LR_REQUIRE(launchable(blocks, kThreads), "Appended grid too large");
-  args.kv_blocks = static_cast<unsigned>(kv_blocks);
-  return dispatch_type(dtype, [&]<typename T>() {
-    return dispatch_dim(dim, [&]<int D>() {
-      auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
-                           as_stream(stream), args);
-      };
-      if (!pairs) launch(paged_append_kernel<T, D>);
-      else if (heads == 1) launch(paged_append_pairs_kernel<T, D, 1>);
-      else launch(paged_append_pairs_kernel<T, D, 4>);
-      return check_launch("paged_append");
+  auto launch = [&](AppendArgs& args) {
+    args.range = dtype == LR_DTYPE_F16 ? kHalfRange : kWideRange;
+    // Rotated blocks whole: the pairs kernel, four heads a thread where there are enough rows to fill
+    // the chip with them (8,192 tokens, 393,000 rows: 36 us against 47 with a row's D / 8 threads and
+    // one head; a step of eight requests, 384 rows, 3.4 either way).
+    const bool pairs = half % kBlock == 0;
+    const int64_t all_rows = 2 * static_cast<int64_t>(args.kv_rows) + args.query_rows;
+    const int64_t heads = pairs && all_rows >= 32768 ? 4 : 1;
+    const int64_t per_block = kThreads / (dim / (pairs ? 16 : 8));
+    const int64_t kv_blocks = ceil_div(batch * added * ceil_div(kv_heads, heads), per_block);
+    const int64_t blocks = 2 * kv_blocks + ceil_div(batch * added * ceil_div(query_heads, heads), per_block);
+    LR_REQUIRE(launchable(blocks, kThreads), "Appended grid too large");
+    args.kv_blocks = static_cast<unsigned>(kv_blocks);
+    return dispatch_type(dtype, [&]<typename T>() {
+      return dispatch_dim(dim, [&]<int D>() {
+        auto enqueue = [&](auto kernel) {
+          hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                             as_stream(stream), args);
+        };
+        if (!pairs) enqueue(paged_append_kernel<T, D>);
+        else if (heads == 1) enqueue(paged_append_pairs_kernel<T, D, 1>);
+        else enqueue(paged_append_pairs_kernel<T, D, 4>);
+        return check_launch("paged_append");
+      });
     });
-  });
+  };
+  return append_paged(keys, key_strides, values, value_strides, queries, query_strides, out_queries,
+                      batch, kv_heads, query_heads, added, dim, dtype, positions, cos, sin, table_rows,
+                      half, counts, pages, page_count, page_size, table, max_pages, lengths, launch);
 }
 
 extern "C" int lr_paged_read(const void* pages, int64_t page_count, int64_t page_size,
                              const int32_t* table, int64_t max_pages, const int32_t* lengths,
                              int64_t segments, int64_t dim, int dtype, int64_t total, void* keys,
                              void* values, float* positions, int32_t* cumulative, void* stream) {
-  clear_error();
-  LR_REQUIRE(paged_type(dtype), "Rows are read as bf16, f16 or f32");
-  if (int status = check_paged(pages, page_count, page_size, dim, table, max_pages, lengths, segments))
-    return status;
-  LR_REQUIRE(total >= 0 && total <= INT32_MAX && cumulative &&
-                 (total == 0 || (keys && values && positions)),
-             "Invalid packed buffers");
-  LR_REQUIRE(((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) % 16) == 0,
-             "Packed buffers must be 16-byte aligned");
-  const int64_t blocks = ceil_div(total, kReadRows);
-  LR_REQUIRE(launchable(blocks, kThreads), "Packed rows' grid too large");
-  // One launch where a workgroup can sum the lengths itself, beside its rows' lookups; calls without
-  // rows or pages have only the sums to write.
-  const bool fused = segments <= kFusedSegments && total > 0 && page_count > 0;
-  const PagedCache cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
-  if (!fused) {
-    hipLaunchKernelGGL(paged_sum_kernel<int32_t>, dim3(1), dim3(kSumThreads), 0, as_stream(stream),
-                       cache, segments, cumulative);
-    if (int status = check_launch("paged_read lengths")) return status;
-    if (total == 0 || page_count == 0) return LR_OK;
-  }
-  const ReadArgs args{cache, segments, total, cumulative, keys, values, positions};
-  return dispatch_type(dtype, [&]<typename T>() {
-    return dispatch_dim(dim, [&]<int D>() {
-      auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
-                           as_stream(stream), args);
-      };
-      if (fused) launch(paged_read_kernel<T, D, true>);
-      else launch(paged_read_kernel<T, D, false>);
-      return check_launch("paged_read");
+  auto launch = [&](const ReadArgs& args, int64_t blocks, bool fused) {
+    return dispatch_type(dtype, [&]<typename T>() {
+      return dispatch_dim(dim, [&]<int D>() {
+        auto enqueue = [&](auto kernel) {
+          hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                             as_stream(stream), args);
+        };
+        if (fused) enqueue(paged_read_kernel<T, D, true>);
+        else enqueue(paged_read_kernel<T, D, false>);
+        return check_launch("paged_read");
+      });
     });
-  });
+  };
+  return read_paged(pages, page_count, page_size, table, max_pages, lengths, segments, dim, dtype, total,
+                    keys, values, positions, cumulative, stream, launch);
 }
 
 extern "C" size_t lr_paged_compact_workspace_bytes(int64_t segments) {
-  return segments > kFusedSegments ? static_cast<size_t>(segments + 1) * sizeof(int64_t) : 0;
+  return compact_paged_workspace(segments);
 }
 
 extern "C" int lr_paged_compact(void* pages, int64_t page_count, int64_t page_size,
@@ -728,45 +482,17 @@ extern "C" int lr_paged_compact(void* pages, int64_t page_count, int64_t page_si
                                 int64_t removed_count, const int32_t* target, int64_t target_pages,
                                 int32_t* new_lengths, void* workspace, size_t workspace_size,
                                 void* stream) {
-  clear_error();
-  if (int status = check_paged(pages, page_count, page_size, dim, table, max_pages, lengths, segments))
-    return status;
-  LR_REQUIRE(removed_count >= 0 && (removed_count == 0 || removed) && new_lengths &&
-                 target_pages >= 0 && target_pages <= INT32_MAX / 2 / page_size &&
-                 (target || target_pages == 0),
-             "Invalid compaction");
-  const size_t needed = lr_paged_compact_workspace_bytes(segments);
-  LR_REQUIRE(workspace_size >= needed && (needed == 0 || workspace) &&
-                 reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
-             "Compaction workspace too small");
-  // rows move while other workgroups still read theirs, and the lengths
-  LR_REQUIRE((target != table || target_pages == 0 || page_count == 0) && new_lengths != lengths,
-             "Compaction needs other pages and lengths than the cache's");
-  CompactArgs args{};
-  args.cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
-  args.segments = segments;
-  // a segment's rows, kept or not, are at most what its table holds
-  args.chunks = static_cast<int>(std::max<int64_t>(1, ceil_div(max_pages * page_size, kCompactRows)));
-  args.target = target;
-  // (without a page there is nothing to move: the lengths alone)
-  args.target_pages = page_count == 0 ? 0 : static_cast<int>(target_pages);
-  args.removed = removed;
-  args.removed_count = removed_count;
-  args.sums = static_cast<int64_t*>(workspace);
-  args.new_lengths = new_lengths;
-  LR_REQUIRE(launchable(segments * args.chunks, kThreads), "Compaction grid too large");
-  if (needed) {
-    hipLaunchKernelGGL(paged_sum_kernel<int64_t>, dim3(1), dim3(kSumThreads), 0, as_stream(stream),
-                       args.cache, segments, static_cast<int64_t*>(workspace));
-    if (int status = check_launch("paged_compact lengths")) return status;
-  }
-  return dispatch_dim(dim, [&]<int D>() {
-    auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(segments * args.chunks)), dim3(kThreads),
-                         0, as_stream(stream), args);
-    };
-    if (needed) launch(paged_compact_kernel<D, false>);
-    else launch(paged_compact_kernel<D, true>);
-    return check_launch("paged_compact");
-  });
+  auto launch = [&](const CompactArgs& args, unsigned blocks, bool fused) {
+    return dispatch_dim(dim, [&]<int D>() {
+      auto enqueue = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, as_stream(stream), args);
+      };
+      if (fused) enqueue(paged_compact_kernel<D, true>);
+      else enqueue(paged_compact_kernel<D, false>);
+      return check_launch("paged_compact");
+    });
+  };
+  return compact_paged(pages, page_count, page_size, table, max_pages, lengths, segments, dim, removed,
+                       removed_count, target, target_pages, new_lengths, workspace, workspace_size,
+                       stream, launch);
 }
