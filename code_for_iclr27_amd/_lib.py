@@ -105,6 +105,17 @@ SIGNATURES = {
     "lr_paged_compact_workspace_bytes": [_I64],
     "lr_paged_compact": [_P, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _SZ,
                          _P],
+    "lr_paged8_page_bytes": [_I64, _I64],
+    "lr_paged8_append": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P, _P, _P,
+                        _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P],
+    "lr_paged8_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64],
+    "lr_paged8_attention_plan": [_I64, _I64, _I64, _I64, _I64, _P],
+    "lr_paged8_attention": [_P, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64,
+                            _I, _I64, _P, _F, _P, _P, _SZ, _P],
+    "lr_paged8_read": [_P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I, _I64, _P, _P, _P, _P, _P],
+    "lr_paged8_compact_workspace_bytes": [_I64],
+    "lr_paged8_compact": [_P, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _SZ,
+                         _P],
     "lr_head_logits": [_P, _I64, _P, _P, _I64, _I64, _I, _P, _P],
     "lr_margin_stats_workspace_bytes": [_I64, _I64],
     "lr_margin_stats": [_P, _I64, _I64, _P, _P, _P, _P, _P, _SZ, _P],
@@ -122,6 +133,9 @@ _RESTYPES = {"lr_last_error": ctypes.c_char_p, "lr_score_workspace_bytes": ctype
              "lr_paged_page_bytes": ctypes.c_int64,
              "lr_paged_attention_workspace_bytes": ctypes.c_size_t,
              "lr_paged_compact_workspace_bytes": ctypes.c_size_t,
+             "lr_paged8_page_bytes": ctypes.c_int64,
+             "lr_paged8_attention_workspace_bytes": ctypes.c_size_t,
+             "lr_paged8_compact_workspace_bytes": ctypes.c_size_t,
              "lr_row_sum_workspace_bytes": ctypes.c_size_t,
              "lr_margin_stats_workspace_bytes": ctypes.c_size_t,
              "lr_pre_gradient_layers_workspace_bytes": ctypes.c_size_t}

@@ -244,13 +244,15 @@ struct Library {
   decltype(&lr_packed_attention_workspace_bytes) attention_workspace_bytes = nullptr;
   decltype(&lr_packed_attention_pending) packed_attention_pending = nullptr;
   decltype(&lr_packed_attention_pending_workspace_bytes) pending_workspace_bytes = nullptr;
-  decltype(&lr_paged_append) paged_append = nullptr;
-  decltype(&lr_paged_attention) paged_attention = nullptr;
-  decltype(&lr_paged_attention_workspace_bytes) paged_attention_workspace_bytes = nullptr;
-  decltype(&lr_paged_read) paged_read = nullptr;
-  decltype(&lr_paged_compact) paged_compact = nullptr;
-  decltype(&lr_paged_compact_workspace_bytes) paged_compact_workspace_bytes = nullptr;
-  decltype(&lr_paged_page_bytes) paged_page_bytes = nullptr;
+  struct Paged {  // the paged caches': 4 bits, 8 bits
+    decltype(&lr_paged_append) append = nullptr;
+    decltype(&lr_paged_attention) attention = nullptr;
+    decltype(&lr_paged_attention_workspace_bytes) attention_workspace_bytes = nullptr;
+    decltype(&lr_paged_read) read = nullptr;
+    decltype(&lr_paged_compact) compact = nullptr;
+    decltype(&lr_paged_compact_workspace_bytes) compact_workspace_bytes = nullptr;
+    decltype(&lr_paged_page_bytes) page_bytes = nullptr;
+  } paged[2];
   decltype(&lr_last_error) last_error = nullptr;
   decltype(&lr_staging_alloc) staging_alloc = nullptr;
   decltype(&lr_staging_free) staging_free = nullptr;
@@ -321,16 +323,18 @@ void bind_attention(int64_t packed_attention, int64_t workspace_bytes, int64_t p
   bind_one(library.pending_workspace_bytes, pending_workspace_bytes);
 }
 
-void bind_paged(int64_t append, int64_t attention, int64_t attention_workspace_bytes, int64_t read,
-                int64_t compact, int64_t compact_workspace_bytes, int64_t page_bytes,
+void bind_paged(int64_t bits, int64_t append, int64_t attention, int64_t attention_workspace_bytes,
+                int64_t read, int64_t compact, int64_t compact_workspace_bytes, int64_t page_bytes,
                 int64_t last_error) {
-  bind_one(library.paged_append, append);
-  bind_one(library.paged_attention, attention);
-  bind_one(library.paged_attention_workspace_bytes, attention_workspace_bytes);
-  bind_one(library.paged_read, read);
-  bind_one(library.paged_compact, compact);
-  bind_one(library.paged_compact_workspace_bytes, compact_workspace_bytes);
-  bind_one(library.paged_page_bytes, page_bytes);
+  require(bits == 4 || bits == 8, "A paged cache holds 4 or 8 bits");
+  auto& paged = library.paged[bits == 8];
+  bind_one(paged.append, append);
+  bind_one(paged.attention, attention);
+  bind_one(paged.attention_workspace_bytes, attention_workspace_bytes);
+  bind_one(paged.read, read);
+  bind_one(paged.compact, compact);
+  bind_one(paged.compact_workspace_bytes, compact_workspace_bytes);
+  bind_one(paged.page_bytes, page_bytes);
   bind_one(library.last_error, last_error);
 }
 
@@ -1391,31 +1395,36 @@ torch::Tensor attention_launch(const torch::Tensor& queries, const torch::Tensor
 }
 
 // ---------------------------------------------------------------------------------------
-// The paged 4-bit KV cache's operators (paged.py): checks, output and workspace allocation and
+// The paged KV caches' operators (paged.py): checks, output and workspace allocation and
 // launch on torch's current stream.
 
 void* current_stream(const torch::Device& device);
 
 struct PagedOperands {
   const torch::Tensor &pages, &table, &lengths;
-  int64_t dim, page_size;
+  int64_t dim, page_size, bits;
 };
 
-void check_paged_layer(const PagedOperands& p) {
-  require(library.paged_append != nullptr, "library entry points are not bound");
-  const int64_t bytes = library.paged_page_bytes(p.page_size, p.dim);
+// The entry points of the layer's format, the layer checked.
+const auto& check_paged_layer(const PagedOperands& p) {
+  require(p.bits == 4 || p.bits == 8, "A paged cache holds 4 or 8 bits");
+  const auto& paged = library.paged[p.bits == 8];
+  require(paged.append != nullptr, "library entry points are not bound");
+  const int64_t bytes = paged.page_bytes(p.page_size, p.dim);
   require(bytes > 0, "Head dimension must be 64, 128 or 256 and page size 16, 32, 64, 128 or 256");
   for (const torch::Tensor* t : {&p.pages, &p.table, &p.lengths}) {
     require(t->is_cuda() && t->is_contiguous(), "Expected contiguous CUDA tensor");
     require(t->device() == p.pages.device(), "CUDA devices differ");
   }
   require(p.pages.scalar_type() == torch::kUInt8 && p.pages.dim() == 2 && p.pages.size(1) == bytes,
-          "Pages must be uint8 [pages, page_bytes(page_size, dim)]");
+          p.bits == 8 ? "Pages must be uint8 [pages, page_bytes(page_size, dim, 8)]"
+                      : "Pages must be uint8 [pages, page_bytes(page_size, dim)]");
   require(p.lengths.scalar_type() == torch::kInt32 && p.lengths.dim() == 1 && p.lengths.numel() > 0,
           "Lengths must be int32 [segments]");
   require(p.table.scalar_type() == torch::kInt32 && p.table.dim() == 2 &&
               p.table.size(0) == p.lengths.numel(),
           "Page table must be int32 [segments, max_pages]");
+  return paged;
 }
 
 const int32_t* paged_counts(const py::object& counts_in, int64_t batch, const torch::Device& device,
@@ -1443,11 +1452,11 @@ const void* address_or_null(const torch::Tensor& t) { return t.numel() ? t.data_
 
 py::object paged_append_launch(const torch::Tensor& pages, const torch::Tensor& table,
                                const torch::Tensor& lengths, int64_t kv_heads, int64_t dim,
-                               int64_t page_size, const torch::Tensor& keys,
+                               int64_t page_size, int64_t bits, const torch::Tensor& keys,
                                const torch::Tensor& values, const torch::Tensor& positions,
                                const py::object& cos_in, const py::object& sin_in,
                                const py::object& queries_in, const py::object& counts_in) {
-  check_paged_layer({pages, table, lengths, dim, page_size});
+  const auto& paged = check_paged_layer({pages, table, lengths, dim, page_size, bits});
   require(keys.dim() == 4 && keys.sizes() == values.sizes(),
           "New keys and values must be [batch, kv_heads, length, dim]");
   const int64_t batch = keys.size(0), added = keys.size(2);
@@ -1494,7 +1503,7 @@ py::object paged_append_launch(const torch::Tensor& pages, const torch::Tensor& 
     row_strides(queries, query_strides);
   }
   if (added > 0)
-    check_call(library.paged_append(
+    check_call(paged.append(
         keys.data_ptr(), key_strides, values.data_ptr(), value_strides,
         queries.defined() ? queries.data_ptr() : nullptr, query_strides,
         out.defined() ? out.data_ptr() : nullptr, batch, kv_heads,
@@ -1509,9 +1518,9 @@ py::object paged_append_launch(const torch::Tensor& pages, const torch::Tensor& 
 
 torch::Tensor paged_attention_launch(const torch::Tensor& pages, const torch::Tensor& table,
                                      const torch::Tensor& lengths, int64_t kv_heads, int64_t dim,
-                                     int64_t page_size, const torch::Tensor& queries,
+                                     int64_t page_size, int64_t bits, const torch::Tensor& queries,
                                      int64_t max_keys, const py::object& counts_in, double scale) {
-  check_paged_layer({pages, table, lengths, dim, page_size});
+  const auto& paged = check_paged_layer({pages, table, lengths, dim, page_size, bits});
   require(queries.dim() == 4 && kv_heads > 0 && queries.size(3) == dim &&
               queries.size(0) * kv_heads == lengths.numel(),
           "Queries must be [batch, query_heads, length, dim]");
@@ -1531,14 +1540,14 @@ torch::Tensor paged_attention_launch(const torch::Tensor& pages, const torch::Te
                                    queries.options().memory_format(c10::MemoryFormat::Contiguous));
   if (length == 0) return out;
   max_keys = pages.size(0) ? std::min(max_keys, table.size(1) * page_size) : 0;
-  const size_t size = library.paged_attention_workspace_bytes(
+  const size_t size = paged.attention_workspace_bytes(
       batch * kv_heads, heads / kv_heads, length, max_keys, dim);
   torch::Tensor workspace;
   if (size)
     workspace = torch::empty({static_cast<int64_t>(size)}, queries.options().dtype(torch::kUInt8));
   int64_t strides[3];
   row_strides(queries, strides);
-  check_call(library.paged_attention(
+  check_call(paged.attention(
       queries.data_ptr(), strides, address_or_null(pages), pages.size(0), page_size,
       table.numel() ? table.data_ptr<int32_t>() : nullptr, table.size(1),
       lengths.data_ptr<int32_t>(), batch, kv_heads, heads / kv_heads, length, dim,
@@ -1550,9 +1559,9 @@ torch::Tensor paged_attention_launch(const torch::Tensor& pages, const torch::Te
 
 std::vector<torch::Tensor> paged_read_launch(const torch::Tensor& pages, const torch::Tensor& table,
                                              const torch::Tensor& lengths, int64_t dim,
-                                             int64_t page_size, int64_t total,
+                                             int64_t page_size, int64_t bits, int64_t total,
                                              const py::object& type_in) {
-  check_paged_layer({pages, table, lengths, dim, page_size});
+  const auto& paged = check_paged_layer({pages, table, lengths, dim, page_size, bits});
   require(total >= 0 && total <= INT32_MAX, "Invalid packed rows");
   const auto type = torch::python::detail::py_object_to_dtype(type_in);
   const int dtype = paged_type(type);
@@ -1561,7 +1570,7 @@ std::vector<torch::Tensor> paged_read_launch(const torch::Tensor& pages, const t
   torch::Tensor keys = torch::empty({total, dim}, options), values = torch::empty({total, dim}, options);
   torch::Tensor positions = torch::empty({total, 1}, pages.options().dtype(torch::kFloat32));
   torch::Tensor cumulative = torch::empty({lengths.numel() + 1}, lengths.options());
-  check_call(library.paged_read(
+  check_call(paged.read(
       address_or_null(pages), pages.size(0), page_size,
       table.numel() ? table.data_ptr<int32_t>() : nullptr, table.size(1),
       lengths.data_ptr<int32_t>(), lengths.numel(), dim, dtype, total,
@@ -1573,8 +1582,9 @@ std::vector<torch::Tensor> paged_read_launch(const torch::Tensor& pages, const t
 
 torch::Tensor paged_compact_launch(const torch::Tensor& pages, const torch::Tensor& table,
                                    const torch::Tensor& lengths, int64_t dim, int64_t page_size,
-                                   const torch::Tensor& removed, const torch::Tensor& target) {
-  check_paged_layer({pages, table, lengths, dim, page_size});
+                                   int64_t bits, const torch::Tensor& removed,
+                                   const torch::Tensor& target) {
+  const auto& paged = check_paged_layer({pages, table, lengths, dim, page_size, bits});
   for (const torch::Tensor* t : {&removed, &target}) {
     require(t->is_cuda() && t->is_contiguous(), "Expected contiguous CUDA tensor");
     require(t->device() == pages.device(), "CUDA devices differ");
@@ -1585,10 +1595,10 @@ torch::Tensor paged_compact_launch(const torch::Tensor& pages, const torch::Tens
           "Page table must be int32 [segments, max_pages]");
   const c10::DeviceGuard guard(pages.device());
   torch::Tensor new_lengths = torch::empty_like(lengths);
-  const size_t size = library.paged_compact_workspace_bytes(lengths.numel());
+  const size_t size = paged.compact_workspace_bytes(lengths.numel());
   torch::Tensor workspace;
   if (size) workspace = torch::empty({static_cast<int64_t>(size)}, pages.options());
-  check_call(library.paged_compact(
+  check_call(paged.compact(
       const_cast<void*>(address_or_null(pages)), pages.size(0), page_size,
       table.numel() ? table.data_ptr<int32_t>() : nullptr, table.size(1),
       lengths.data_ptr<int32_t>(), lengths.numel(), dim,

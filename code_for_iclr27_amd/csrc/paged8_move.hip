@@ -1,0 +1,703 @@
+// Rows into, out of and within the paged 8-bit KV cache (paged8.hpp states its layout and its codes).
+//
+// append: new K and V rows behind each segment's rows, K (and the step's queries) rotated to their
+// positions on the way. The rotation pairs channels c and c + half; its products are rounded one by
+// one (no fused multiply-add), in f32. A wave owns a token block's keys or values, as their scale
+// depends on all of the block's rows: it has the new rows in registers, takes their largest magnitude
+// over its lanes, and where that outgrows the scale of rows that are there already, moves these to the
+// new one. (A scale a row would spare the decode step that, and cost attention a multiplication for
+// each key in the place of one for sixteen, and 2 bytes a row.)
+//
+// read: the rows as 16- or 32-bit rows packed by segment, the layout of the other operators, with
+// its cumulative lengths.
+//
+// compact: the rows that stay, in order, into other pages, in one launch. The rows of a block come
+// from several; it takes the largest of their scales.
+
+#include "attention_common.hpp"
+#include "paged8.hpp"
+#include "paged_move.hpp"
+
+namespace lr {
+namespace {
+
+template <int CONTROL>
+__device__ __forceinline__ float dpp_max(float x) {
+  return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                      0, __builtin_bit_cast(int, x), CONTROL, 0xF, 0xF, false)));
+}
+// The largest of each 16 lanes' values, and of the wave's, in all of them.
+__device__ __forceinline__ float row_max(float x) {
+  return dpp_max<0x140>(dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(x))));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  LanePair pair = lane_pair<16>(row_max(x));
+  pair = lane_pair<32>(fmaxf(pair.first, pair.second));
+  return fmaxf(pair.first, pair.second);
+}
+
+// log2 of the scale for a largest magnitude.
+__device__ __forceinline__ int scale_exponent(float top, ScaleRange range) {
+  const int exponent = static_cast<int>((__builtin_bit_cast(unsigned, top) + 0x180000u) >> 23) - 135;
+  return exponent < range.low ? range.low : exponent > range.high ? range.high : exponent;
+}
+
+// The largest finite magnitude of N elements.
+template <int N>
+__device__ __forceinline__ float finite_max(const float (&x)[N]) {
+  float top = 0.0f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) top = fmaxf(top, __builtin_fabsf(x[e]));  // (takes no NaN)
+  if (top == __builtin_huge_valf()) {
+    top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      top = __builtin_fabsf(x[e]) < __builtin_huge_valf() ? fmaxf(top, __builtin_fabsf(x[e])) : top;
+  }
+  return top;
+}
+
+// An element's code at scale 2^exponent. Times 2^(-exponent - 120) a code is the exponent and the top
+// three bits of the significand of an f32, with the small codes among its subnormal numbers, and the
+// cut to whole codes drops the bits below.
+__device__ __forceinline__ unsigned encode(float x, int exponent) {
+  const unsigned bits = __builtin_bit_cast(unsigned, x), size = bits & 0x7fffffffu;
+  const unsigned four = (size + 0x7ffffu + ((size >> 20) & 1u)) & 0xfff00000u;
+  const float scaled = __builtin_ldexpf(__builtin_bit_cast(float, four), -exponent - 120);
+  unsigned code = min(__builtin_bit_cast(unsigned, scaled) >> 20, kCodeNaN - 1);
+  code = size >= 0x7f800000u ? kCodeNaN : code;
+  return code | (bits >> 24 & 0x80u);
+}
+__device__ __forceinline__ unsigned encode4(const float* x, int exponent) {
+  return encode(x[0], exponent) | encode(x[1], exponent) << 8 | encode(x[2], exponent) << 16 |
+         encode(x[3], exponent) << 24;
+}
+
+// Four codes at a scale 2^by times theirs.
+__device__ __forceinline__ unsigned shift_codes(unsigned codes, int by) {
+  unsigned result = codes & 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned size = codes >> (8 * i) & 0x7fu;
+    const unsigned moved =
+        __builtin_bit_cast(unsigned, __builtin_ldexpf(__builtin_bit_cast(float, size << 20), -by)) >> 20;
+    result |= (size == kCodeNaN ? kCodeNaN : moved) << (8 * i);
+  }
+  return result;
+}
+
+// Four words of four codes, each word's bytes of one row, as words of one byte of each: a 4 x 4
+// transposition.
+__device__ __forceinline__ void transpose4(const unsigned (&in)[4], unsigned (&out)[4]) {
+  const unsigned a = __builtin_amdgcn_perm(in[1], in[0], 0x05010400u);  // 0.0 1.0 0.1 1.1
+  const unsigned b = __builtin_amdgcn_perm(in[1], in[0], 0x07030602u);
+  const unsigned c = __builtin_amdgcn_perm(in[3], in[2], 0x05010400u);
+  const unsigned d = __builtin_amdgcn_perm(in[3], in[2], 0x07030602u);
+  out[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+  out[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  out[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+  out[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+// A token block that rows are appended to: rows [from, to) of it are new, `first` is the number of its
+// row 0 among the new ones (negative where it has older rows), `page` NULL where there is none.
+struct Target {
+  uint8_t* page;
+  int slot, from, to, first;  // slot: of the block's row 0
+};
+template <int D>
+__device__ __forceinline__ Target target_block(const AppendArgs& a, unsigned segment, unsigned b, unsigned n) {
+  Target t{nullptr, 0, 0, 0, 0};
+  const PagedCache& cache = a.cache;
+  const int length = cache.lengths[segment];
+  if (length < 0) return t;
+  int count = static_cast<int>(a.added);
+  if (a.counts != nullptr) count = max(0, min(count, a.counts[b]));
+  const int64_t row = (static_cast<int64_t>(length) & ~int64_t{15}) + 16 * static_cast<int64_t>(n);
+  const int64_t behind = static_cast<int64_t>(length) + count - row;  // past the last new row
+  t.first = static_cast<int>(row - length);
+  t.from = max(0, -t.first);
+  t.to = behind < kTokens ? static_cast<int>(behind) : kTokens;
+  if (t.to <= t.from || row >= static_cast<int64_t>(cache.max_pages) << cache.shift) return t;
+  const int64_t id = cache.table[static_cast<int64_t>(segment) * cache.max_pages + (row >> cache.shift)];
+  if (id < 0 || id >= cache.page_count) return t;
+  t.page = cache.pages + id * (Page8<D>::bytes(1) << cache.shift);
+  t.slot = static_cast<int>(row) & ((1 << cache.shift) - 1);
+  return t;
+}
+
+// The exponent of a block's scale, written to its byte, and by how much older rows' codes move.
+struct Scale {
+  int exponent, by;
+};
+template <int D>
+__device__ __forceinline__ Scale grow_scale(const AppendArgs& a, const Target& t, int which, float top) {
+  uint8_t* const byte = t.page + Page8<D>::scales(a.cache.shift, t.slot) + which;
+  Scale s{scale_exponent(wave_max(top), a.range), 0};
+  if (t.from > 0) {
+    const int was = static_cast<int>(*byte) - 127;
+    s.by = max(0, s.exponent - was);
+    s.exponent = max(s.exponent, was);
+  }
+  if ((threadIdx.x & 63) == 0) *byte = static_cast<uint8_t>(s.exponent + 127);
+  return s;
+}
+
+// A chunk's eight channels rotated with its partner's.
+__device__ __forceinline__ void rotate_pair(float (&x)[8], float (&y)[8], const float (&cosine)[8],
+                                            const float (&sine)[8], bool known) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float xc = x[e] * cosine[e], ys = y[e] * sine[e], yc = y[e] * cosine[e], xs = x[e] * sine[e];
+    x[e] = known ? xc - ys : __builtin_nanf("");
+    y[e] = known ? yc + xs : __builtin_nanf("");
+  }
+}
+
+// The keys of a token block: a lane has eight channels and their partners (rotated: channels c and
+// c + half; the others: half of them apart) of D / 64 rows.
+template <typename T, int D>
+__device__ __forceinline__ void append_keys(const AppendArgs& a, unsigned segment, unsigned b, unsigned h,
+                                            const Target& t) {
+  constexpr int kPairs = D / 16, kGroups = 64 / kPairs, kRows = kTokens / kGroups;
+  const int lane = threadIdx.x & 63, c = lane % kPairs, group = lane / kPairs;
+  const int pairs = a.half / 8;
+  const bool rotated = c < pairs;
+  const int chunk[2] = {rotated ? c : c + pairs, rotated ? c + pairs : c + kPairs};
+  const T* source = static_cast<const T*>(a.keys.base) + b * a.keys.batch + h * a.keys.head;
+  const int64_t* positions = a.positions + static_cast<int64_t>(b) * a.added;
+  Eight<T> raw[kRows][2];
+  int64_t position[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int row = i * kGroups + group, at = t.first + row;
+    if (row >= t.from && row < t.to) {
+      raw[i][0] = *reinterpret_cast<const Eight<T>*>(source + at * a.keys.row + 8 * chunk[0]);
+      raw[i][1] = *reinterpret_cast<const Eight<T>*>(source + at * a.keys.row + 8 * chunk[1]);
+      position[i] = positions[at];
+    }
+  }
+  float x[kRows][2][8], top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int row = i * kGroups + group;
+    const bool fresh = row >= t.from && row < t.to;
+    if (fresh) {
+      raw[i][0].get(x[i][0]);
+      raw[i][1].get(x[i][1]);
+      if (rotated) {
+        float cosine[8], sine[8];
+        const bool known = position[i] >= 0 && position[i] < a.table_rows;
+        const int64_t at = (known ? position[i] : 0) * a.half + 8 * c;
+        reinterpret_cast<const Eight<float>*>(a.cos + at)->get(cosine);
+        reinterpret_cast<const Eight<float>*>(a.sin + at)->get(sine);
+        rotate_pair(x[i][0], x[i][1], cosine, sine, known);
+      }
+      top = fmaxf(top, fmaxf(finite_max(x[i][0]), finite_max(x[i][1])));
+      if (c == 0)
+        *reinterpret_cast<float*>(t.page + Page8<D>::position(a.cache.shift, t.slot + row)) =
+            static_cast<float>(position[i]);
+    }
+  }
+  const Scale scale = grow_scale<D>(a, t, 0, top);
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int row = i * kGroups + group;
+    if (row >= t.to || (row < t.from && scale.by == 0)) continue;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      move_u32x2* const to = reinterpret_cast<move_u32x2*>(
+          t.page + Page8<D>::key(t.slot + row, chunk[p] >> 1) + 8 * (chunk[p] & 1));
+      if (row >= t.from) {
+        *to = move_u32x2{encode4(&x[i][p][0], scale.exponent), encode4(&x[i][p][4], scale.exponent)};
+      } else {
+        const move_u32x2 old = *to;
+        *to = move_u32x2{shift_codes(old[0], scale.by), shift_codes(old[1], scale.by)};
+      }
+    }
+  }
+}
+
+// The values of a token block: a lane has eight channels of four rows, D / 128 times.
+template <typename T, int D>
+__device__ __forceinline__ void append_values(const AppendArgs& a, unsigned segment, unsigned b, unsigned h,
+                                              const Target& t) {
+  constexpr int kChunks = D / 8, kTimes = D == 256 ? 2 : 1;
+  const int lane = threadIdx.x & 63;
+  const T* source = static_cast<const T*>(a.values.base) + b * a.values.batch + h * a.values.head;
+  Eight<T> raw[kTimes][4];
+  float top = 0.0f;
+#pragma unroll
+  for (int u = 0; u < kTimes; ++u) {
+    const int c = (u * 64 + lane) % kChunks, quad = (u * 64 + lane) / kChunks;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 4 * quad + r;
+      if (row >= t.from && row < t.to)  // (d64: none for the last 32 lanes)
+        raw[u][r] = *reinterpret_cast<const Eight<T>*>(source + (t.first + row) * a.values.row + 8 * c);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kTimes; ++u) {
+    const int quad = (u * 64 + lane) / kChunks;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 4 * quad + r;
+      if (row >= t.from && row < t.to) {
+        float x[8];
+        raw[u][r].get(x);
+        top = fmaxf(top, finite_max(x));
+      }
+    }
+  }
+  const Scale scale = grow_scale<D>(a, t, 1, top);
+#pragma unroll
+  for (int u = 0; u < kTimes; ++u) {
+    const int c = (u * 64 + lane) % kChunks, quad = (u * 64 + lane) / kChunks;
+    const int row0 = 4 * quad;
+    const bool older = row0 < t.from && scale.by > 0;
+    if (quad >= 4 || row0 >= t.to || (row0 + 4 <= t.from && !older)) continue;
+    uint8_t* const to = t.page + Page8<D>::value(a.cache.shift, t.slot + row0) + 32 * c;
+    unsigned word[4][2];  // a row's eight codes
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float x[8] = {};
+      if (row0 + r >= t.from && row0 + r < t.to) raw[u][r].get(x);
+      word[r][0] = encode4(x, scale.exponent);
+      word[r][1] = encode4(x + 4, scale.exponent);
+    }
+    const bool whole = row0 >= t.from && row0 + 4 <= t.to;
+    if (whole || older) {
+      unsigned fresh = 0;  // bytes of the words that are new
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (row0 + r >= t.from && row0 + r < t.to) fresh |= 0xffu << (8 * r);
+      const unsigned old_rows = row0 + 4 <= t.from ? ~0u : row0 >= t.from ? 0u : (1u << (8 * (t.from - row0))) - 1;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const unsigned rows[4] = {word[0][n], word[1][n], word[2][n], word[3][n]};
+        unsigned codes[4];
+        transpose4(rows, codes);
+        move_u32x4* const place = reinterpret_cast<move_u32x4*>(to + 16 * n);
+        if (!whole) {
+          const move_u32x4 was = *place;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            codes[k] = (codes[k] & fresh) | (shift_codes(was[k], scale.by) & old_rows) |
+                       (was[k] & ~(fresh | old_rows));
+        }
+        *place = move_u32x4{codes[0], codes[1], codes[2], codes[3]};
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (row0 + r >= t.from && row0 + r < t.to)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) to[4 * e + r] = static_cast<uint8_t>(word[r][e / 4] >> (8 * (e % 4)));
+    }
+  }
+}
+
+// Queries, rotated: D / 16 threads a row, each with a chunk and its partner, for the same chunks of HEADS
+// heads, so that a cosine and sine are loaded once.
+template <typename T, int D, int HEADS>
+__device__ __forceinline__ void rotate_queries(const AppendArgs& a, unsigned block) {
+  constexpr int kRowThreads = D / 16, kUnits = kThreads / kRowThreads;
+  const unsigned unit = block * kUnits + threadIdx.x / kRowThreads;
+  const unsigned groups = (a.query_heads + HEADS - 1) / HEADS;
+  const unsigned place = unit / groups, h0 = (unit - place * groups) * HEADS;
+  const unsigned b = place / a.added, i = place - b * a.added;
+  if (b >= a.batch) return;
+  const int c = threadIdx.x % kRowThreads, pairs = a.half / 8;
+  const bool rotated = c < pairs;
+  const int lo = rotated ? c : c + pairs, hi = rotated ? c + pairs : c + kRowThreads;
+  const T* source = static_cast<const T*>(a.queries.base) + b * a.queries.batch + i * a.queries.row;
+  Eight<T> first[HEADS], second[HEADS];
+#pragma unroll
+  for (int n = 0; n < HEADS; ++n) {
+    const T* p = source + min(h0 + n, a.query_heads - 1) * a.queries.head;
+    first[n] = *reinterpret_cast<const Eight<T>*>(p + 8 * lo);
+    second[n] = *reinterpret_cast<const Eight<T>*>(p + 8 * hi);
+  }
+  const int64_t position = a.positions[static_cast<int64_t>(b) * a.added + i];
+  const bool known = position >= 0 && position < a.table_rows;
+  float cosine[8], sine[8];
+  if (rotated) {
+    const int64_t at = (known ? position : 0) * a.half + 8 * c;
+    reinterpret_cast<const Eight<float>*>(a.cos + at)->get(cosine);
+    reinterpret_cast<const Eight<float>*>(a.sin + at)->get(sine);
+  }
+#pragma unroll
+  for (int n = 0; n < HEADS; ++n) {
+    if (h0 + n >= a.query_heads) break;
+    float x[8], y[8];
+    first[n].get(x);
+    second[n].get(y);
+    if (rotated) rotate_pair(x, y, cosine, sine, known);
+    T* out = static_cast<T*>(a.out_queries) +
+             ((static_cast<int64_t>(b) * a.query_heads + h0 + n) * a.added + i) * D;
+    Eight<T> result;
+    result.set(x);
+    *reinterpret_cast<Eight<T>*>(out + 8 * lo) = result;
+    result.set(y);
+    *reinterpret_cast<Eight<T>*>(out + 8 * hi) = result;
+  }
+}
+
+// blocks: the keys', the values', the queries'. A wave takes a token block of one segment, consecutive
+// ones those of consecutive heads.
+template <typename T, int D, int HEADS>
+__global__ __launch_bounds__(kThreads) void paged8_append_kernel(AppendArgs a, unsigned blocks) {
+  if (blockIdx.x >= 2 * a.kv_blocks) return rotate_queries<T, D, HEADS>(a, blockIdx.x - 2 * a.kv_blocks);
+  const bool keys = blockIdx.x < a.kv_blocks;
+  const unsigned unit = __builtin_amdgcn_readfirstlane(
+      (blockIdx.x - (keys ? 0 : a.kv_blocks)) * (kThreads / 64) + (threadIdx.x >> 6));
+  const unsigned place = unit / a.kv_heads, h = unit - place * a.kv_heads;
+  const unsigned b = place / blocks, n = place - b * blocks;
+  if (b >= a.batch) return;
+  const unsigned segment = b * a.kv_heads + h;
+  const Target t = target_block<D>(a, segment, b, n);
+  if (t.page == nullptr) return;
+  if (keys) append_keys<T, D>(a, segment, b, h, t);
+  else append_values<T, D>(a, segment, b, h, t);
+}
+
+// ---------------------------------------------------------------------------------------
+// Eight codes times 2^exponent, rounded once to T (codes are exact in f32).
+template <typename T>
+__device__ __forceinline__ Eight<T> eight_values(move_u32x2 codes, unsigned scale) {
+  const float power = scale_of(scale);
+  float x[8];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes[w], power, false);
+    const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes[w], power, true);
+    x[4 * w] = lo[0], x[4 * w + 1] = lo[1], x[4 * w + 2] = hi[0], x[4 * w + 3] = hi[1];
+  }
+  Eight<T> result;
+  result.set(x);
+  return result;
+}
+
+// Byte `row` of each of eight words.
+__device__ __forceinline__ move_u32x2 gather_bytes(move_u32x4 lo, move_u32x4 hi, int row) {
+  const unsigned two = 0x0c0c0400u + 0x0101u * static_cast<unsigned>(row);
+  move_u32x2 result;
+  result[0] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(lo[3], lo[2], two),
+                                    __builtin_amdgcn_perm(lo[1], lo[0], two), 0x05040100u);
+  result[1] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(hi[3], hi[2], two),
+                                    __builtin_amdgcn_perm(hi[1], hi[0], two), 0x05040100u);
+  return result;
+}
+
+// A workgroup takes 64 packed rows: the first wave finds each one's page and slot, then D / 8 threads
+// a row expand eight channels each, four rows' loads in flight. (Of a value's word a row uses one byte:
+// the rows beside it take the others from the same cache lines.)
+template <typename T, int D, bool FUSED>
+__global__ __launch_bounds__(kThreads) void paged8_read_kernel(ReadArgs a) {
+  constexpr int kRowThreads = D / 8, kRowsAtOnce = kThreads / kRowThreads;
+  constexpr int kRounds = kReadRows / kRowsAtOnce, kTogether = kRounds < 4 ? kRounds : 4;
+  __shared__ int32_t sums[FUSED ? kFusedSegments + 1 : 1];
+  __shared__ int64_t row_page[kReadRows];  // byte offset of the row's page, or -1
+  __shared__ int row_slot[kReadRows];
+  const PagedCache& cache = a.cache;
+  const int segments = static_cast<int>(a.segments);
+  const int32_t* cumulative = a.cumulative;
+  if constexpr (FUSED) {
+    sum_lengths(cache, segments, sums);
+    if (blockIdx.x == 0)
+      for (int s = threadIdx.x; s <= segments; s += kThreads) a.cumulative[s] = sums[s];
+    cumulative = sums;
+  }
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kReadRows;
+  if (threadIdx.x < kReadRows) {
+    const int64_t row = row0 + threadIdx.x;
+    int64_t page = -1;
+    int slot = 0;
+    if (row < a.total && row < cumulative[segments]) {
+      const int segment = segment_of(cumulative, segments, static_cast<int>(row));
+      const int at = static_cast<int>(row) - cumulative[segment];
+      const int64_t id = cache.table[static_cast<int64_t>(segment) * cache.max_pages + (at >> cache.shift)];
+      if (id >= 0 && id < cache.page_count) {
+        page = id * (Page8<D>::bytes(1) << cache.shift);
+        slot = at & ((1 << cache.shift) - 1);
+        a.positions[row] = *reinterpret_cast<const float*>(cache.pages + page +
+                                                           Page8<D>::position(cache.shift, slot));
+      }
+    }
+    row_page[threadIdx.x] = page;
+    row_slot[threadIdx.x] = slot;
+  }
+  __syncthreads();
+  const int c = threadIdx.x % kRowThreads, first = threadIdx.x / kRowThreads;
+#pragma unroll
+  for (int r0 = 0; r0 < kRounds; r0 += kTogether) {
+    move_u32x2 keys[kTogether];
+    move_u32x4 values[kTogether][2];
+    unsigned scales[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const int r = (r0 + i) * kRowsAtOnce + first, slot = row_slot[r];
+      // (a row that is not there reads the pool's first one, and is not written)
+      const uint8_t* p = cache.pages + (row_page[r] >= 0 ? row_page[r] : 0);
+      keys[i] = *reinterpret_cast<const move_u32x2*>(p + Page8<D>::key(slot, c >> 1) + 8 * (c & 1));
+      const uint8_t* q = p + Page8<D>::value(cache.shift, slot & ~3) + 32 * c;
+      values[i][0] = *reinterpret_cast<const move_u32x4*>(q);
+      values[i][1] = *reinterpret_cast<const move_u32x4*>(q + 16);
+      scales[i] = *reinterpret_cast<const uint16_t*>(p + Page8<D>::scales(cache.shift, slot));
+    }
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const int r = (r0 + i) * kRowsAtOnce + first;
+      if (row_page[r] < 0) continue;
+      const int64_t at = (row0 + r) * D + 8 * c;
+      *reinterpret_cast<Eight<T>*>(static_cast<T*>(a.keys) + at) = eight_values<T>(keys[i], scales[i] & 255u);
+      *reinterpret_cast<Eight<T>*>(static_cast<T*>(a.values) + at) =
+          eight_values<T>(gather_bytes(values[i][0], values[i][1], row_slot[r] & 3), scales[i] >> 8);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// A wave moves 64 rows of a segment: row r comes from row r + how many removed rows lie at or before
+// it. The wave finds that number for its first and its last row, each lane its own between them;
+// then all lanes move the codes, a token block of 16 rows after the other.
+template <int D, bool FUSED>
+__global__ __launch_bounds__(kThreads) void paged8_compact_kernel(CompactArgs a) {
+  __shared__ int64_t lds_sums[FUSED ? kFusedSegments + 1 : 1];
+  const PagedCache& cache = a.cache;
+  const int lane = threadIdx.x & 63;
+  const int64_t segment = blockIdx.x / static_cast<unsigned>(a.chunks);
+  const int chunk = static_cast<int>(blockIdx.x - segment * a.chunks);
+  const int64_t* sums = a.sums;
+  if constexpr (FUSED) {
+    sum_lengths(cache, static_cast<int>(a.segments), lds_sums);
+    sums = lds_sums;
+  }
+  const int64_t first = sums[segment];
+  const int length = cache.rows(segment);
+  const int row0 = chunk * kCompactRows + static_cast<int>(threadIdx.x & ~63u);
+  if (chunk > 0 && row0 >= length) return;  // no row can be left there
+  // the segment's part of the removed rows
+  const int64_t bound = lane < 32 ? first : first + length;
+  const int64_t found = half_search(0, a.removed_count, [&](int64_t i) { return a.removed[i] < bound; });
+  const int64_t low = __shfl(found, 0);
+  const int64_t inside = __shfl(found, 32) - low;  // (negative for rows that are not sorted)
+  const int gone = static_cast<int>(inside < 0 ? 0 : inside < length ? inside : length);
+  const int left = length - gone;
+  if (chunk == 0 && threadIdx.x == 0) a.new_lengths[segment] = left;
+  const int rows = min(left, a.target_pages << cache.shift);
+  if (row0 >= rows) return;
+  const int64_t* removed = a.removed + low;
+  // how many removed rows (of this segment) lie at or before kept row `row`
+  auto lies_before = [&](int row) { return [=](int64_t i) { return removed[i] - first - i <= row; }; };
+  int64_t j = half_search(0, gone, lies_before(lane < 32 ? row0 : row0 + 63));
+  const int row = row0 + lane, mask = (1 << cache.shift) - 1;
+  {
+    int64_t from = __shfl(j, 0), to = __shfl(j, 32);
+    while (from < to) {
+      const int64_t mid = (from + to) / 2;
+      if (lies_before(row)(mid)) from = mid + 1;
+      else to = mid;
+    }
+    j = from;
+  }
+  // byte offsets of the row's old and new pages (-1: none), and its slots there
+  int64_t from = -1, to = -1;
+  const int64_t source = row + j;
+  if (row < rows && source < length) {
+    const int64_t id = cache.table[segment * cache.max_pages + (source >> cache.shift)];
+    const int64_t target = a.target[segment * a.target_pages + (row >> cache.shift)];
+    if (id >= 0 && id < cache.page_count && target >= 0 && target < cache.page_count) {
+      from = id * (Page8<D>::bytes(1) << cache.shift);
+      to = target * (Page8<D>::bytes(1) << cache.shift);
+    }
+  }
+  const bool moves = to >= 0;
+  const int from_slot = moves ? static_cast<int>(source) & mask : 0;
+  if (!moves) from = 0;  // (reads the pool's first row)
+  // a block's scales, and by how much the row's codes move to them
+  const unsigned bytes = *reinterpret_cast<const uint16_t*>(cache.pages + from +
+                                                            Page8<D>::scales(cache.shift, from_slot));
+  int by[2];
+  unsigned largest[2];
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const unsigned mine = bytes >> (8 * which) & 255u;
+    largest[which] = static_cast<unsigned>(row_max(moves ? static_cast<float>(mine) : 0.0f));
+    by[which] = moves ? static_cast<int>(largest[which] - mine) : 0;
+  }
+  const float position = *reinterpret_cast<const float*>(cache.pages + from +
+                                                         Page8<D>::position(cache.shift, from_slot));
+  if (moves) {
+    uint8_t* const out = cache.pages + to;
+    *reinterpret_cast<float*>(out + Page8<D>::position(cache.shift, row & mask)) = position;
+    // (any of the block's rows that moves: they write the same)
+    *reinterpret_cast<uint16_t*>(out + Page8<D>::scales(cache.shift, row & mask)) =
+        static_cast<uint16_t>(largest[0] | largest[1] << 8);
+  }
+  const bool shifts = __any(by[0] > 0 || by[1] > 0);
+  constexpr int kKeyLoads = D / 64, kTimes = D == 256 ? 2 : 1, kChunks = D / 8;
+#pragma unroll 2
+  for (int block = 0; block < 4; ++block) {
+    if (row0 + 16 * block >= rows) break;
+    // keys: lane (row, 16 channels)
+    {
+      const int r = 16 * block + (lane & 15);
+      const int64_t key_from = __shfl(from, r), key_to = __shfl(to, r);
+      const int slot = __shfl(from_slot, r), target_slot = (row0 + r) & mask, shift = __shfl(by[0], r);
+      move_u32x4 data[kKeyLoads];
+#pragma unroll
+      for (int u = 0; u < kKeyLoads; ++u)
+        data[u] = *reinterpret_cast<const move_u32x4*>(cache.pages + key_from +
+                                                       Page8<D>::key(slot, 4 * u + (lane >> 4)));
+      if (shifts)
+#pragma unroll
+        for (int u = 0; u < kKeyLoads; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) data[u][e] = shift_codes(data[u][e], shift);
+      if (key_to >= 0)
+#pragma unroll
+        for (int u = 0; u < kKeyLoads; ++u)
+          *reinterpret_cast<move_u32x4*>(cache.pages + key_to +
+                                         Page8<D>::key(target_slot, 4 * u + (lane >> 4))) = data[u];
+    }
+    // values: lane (four rows, eight channels)
+#pragma unroll
+    for (int u = 0; u < kTimes; ++u) {
+      const int c = (u * 64 + lane) % kChunks, quad = (u * 64 + lane) / kChunks & 3;  // (d64: twice)
+      move_u32x4 data[4][2];
+      int64_t row_to[4];
+      int slot[4], shift[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * block + 4 * quad + i;
+        row_to[i] = __shfl(to, r);
+        slot[i] = __shfl(from_slot, r);
+        shift[i] = __shfl(by[1], r);
+        const uint8_t* p = cache.pages + __shfl(from, r) + Page8<D>::value(cache.shift, slot[i] & ~3) + 32 * c;
+        data[i][0] = *reinterpret_cast<const move_u32x4*>(p);
+        data[i][1] = *reinterpret_cast<const move_u32x4*>(p + 16);
+      }
+      unsigned word[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const move_u32x2 codes = gather_bytes(data[i][0], data[i][1], slot[i] & 3);
+        word[i][0] = codes[0], word[i][1] = codes[1];
+        if (shifts) word[i][0] = shift_codes(word[i][0], shift[i]), word[i][1] = shift_codes(word[i][1], shift[i]);
+      }
+      if (D == 64 && lane >= 32) continue;
+      const int target_slot = (row0 + 16 * block + 4 * quad) & mask;
+      const int at = Page8<D>::value(cache.shift, target_slot) + 32 * c;
+      if (row_to[0] >= 0 && row_to[1] >= 0 && row_to[2] >= 0 && row_to[3] >= 0) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const unsigned in[4] = {word[0][n], word[1][n], word[2][n], word[3][n]};
+          unsigned codes[4];
+          transpose4(in, codes);
+          *reinterpret_cast<move_u32x4*>(cache.pages + row_to[0] + at + 16 * n) =
+              move_u32x4{codes[0], codes[1], codes[2], codes[3]};
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (row_to[i] >= 0)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              cache.pages[row_to[i] + at + 4 * e + i] = static_cast<uint8_t>(word[i][e / 4] >> (8 * (e % 4)));
+      }
+    }
+  }
+}
+
+}  // namespace
+}  // namespace lr
+
+using namespace lr;
+
+extern "C" int64_t lr_paged8_page_bytes(int64_t page_size, int64_t dim) {
+  return paged8_bytes(page_size, dim);
+}
+
+extern "C" int lr_paged8_append(const void* keys, const int64_t* key_strides, const void* values,
+                                const int64_t* value_strides, const void* queries,
+                                const int64_t* query_strides, void* out_queries, int64_t batch,
+                                int64_t kv_heads, int64_t query_heads, int64_t added, int64_t dim,
+                                int dtype, const int64_t* positions, const float* cos,
+                                const float* sin, int64_t table_rows, int64_t half,
+                                const int32_t* counts, void* pages, int64_t page_count,
+                                int64_t page_size, const int32_t* table, int64_t max_pages,
+                                const int32_t* lengths, void* stream) {
+  auto launch = [&](AppendArgs& args) {
+    args.range = dtype == LR_DTYPE_F16 ? kHalfRange8 : kWideRange8;
+    // token blocks that a segment's new rows can touch, from any row of the first one on
+    const int64_t token_blocks = (added + 2 * kTokens - 2) / kTokens;
+    const int64_t kv_blocks = ceil_div(batch * kv_heads * token_blocks, kThreads / 64);
+    // four heads a thread where there are enough rows to fill the chip with them
+    const int64_t heads = static_cast<int64_t>(args.query_rows) >= 32768 ? 4 : 1;
+    const int64_t per_block = kThreads / (dim / 16);
+    const int64_t blocks = 2 * kv_blocks + ceil_div(batch * added * ceil_div(query_heads, heads), per_block);
+    LR_REQUIRE(launchable(blocks, kThreads), "Appended grid too large");
+    args.kv_blocks = static_cast<unsigned>(kv_blocks);
+    return dispatch_type(dtype, [&]<typename T>() {
+      return dispatch_dim(dim, [&]<int D>() {
+        auto enqueue = [&](auto kernel) {
+          hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                             as_stream(stream), args, static_cast<unsigned>(token_blocks));
+        };
+        if (heads == 1) enqueue(paged8_append_kernel<T, D, 1>);
+        else enqueue(paged8_append_kernel<T, D, 4>);
+        return check_launch("paged8_append");
+      });
+    });
+  };
+  return append_paged(keys, key_strides, values, value_strides, queries, query_strides, out_queries,
+                      batch, kv_heads, query_heads, added, dim, dtype, positions, cos, sin, table_rows,
+                      half, counts, pages, page_count, page_size, table, max_pages, lengths, launch);
+}
+
+extern "C" int lr_paged8_read(const void* pages, int64_t page_count, int64_t page_size,
+                              const int32_t* table, int64_t max_pages, const int32_t* lengths,
+                              int64_t segments, int64_t dim, int dtype, int64_t total, void* keys,
+                              void* values, float* positions, int32_t* cumulative, void* stream) {
+  auto launch = [&](const ReadArgs& args, int64_t blocks, bool fused) {
+    return dispatch_type(dtype, [&]<typename T>() {
+      return dispatch_dim(dim, [&]<int D>() {
+        auto enqueue = [&](auto kernel) {
+          hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                             as_stream(stream), args);
+        };
+        if (fused) enqueue(paged8_read_kernel<T, D, true>);
+        else enqueue(paged8_read_kernel<T, D, false>);
+        return check_launch("paged8_read");
+      });
+    });
+  };
+  return read_paged(pages, page_count, page_size, table, max_pages, lengths, segments, dim, dtype, total,
+                    keys, values, positions, cumulative, stream, launch);
+}
+
+extern "C" size_t lr_paged8_compact_workspace_bytes(int64_t segments) {
+  return compact_paged_workspace(segments);
+}
+
+extern "C" int lr_paged8_compact(void* pages, int64_t page_count, int64_t page_size,
+                                 const int32_t* table, int64_t max_pages, const int32_t* lengths,
+                                 int64_t segments, int64_t dim, const int64_t* removed,
+                                 int64_t removed_count, const int32_t* target, int64_t target_pages,
+                                 int32_t* new_lengths, void* workspace, size_t workspace_size,
+                                 void* stream) {
+  auto launch = [&](const CompactArgs& args, unsigned blocks, bool fused) {
+    return dispatch_dim(dim, [&]<int D>() {
+      auto enqueue = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, as_stream(stream), args);
+      };
+      if (fused) enqueue(paged8_compact_kernel<D, true>);
+      else enqueue(paged8_compact_kernel<D, false>);
+      return check_launch("paged8_compact");
+    });
+  };
+  return compact_paged(pages, page_count, page_size, table, max_pages, lengths, segments, dim, removed,
+                       removed_count, target, target_pages, new_lengths, workspace, workspace_size,
+                       stream, launch);
+}

@@ -1,12 +1,21 @@
-"""A paged KV cache held in 4 bits: append with the position rotation, attention, compaction, and
-the way back to packed rows.
+"""A paged KV cache held in 4 or 8 bits: append with the position rotation, attention, compaction,
+and the way back to packed rows.
 
 The reference keeps its cache as packed 16-bit rows and copies all of them at every append
-(cache.py:33-52). Here a layer's rows lie in pages of a pool, quantised in blocks of 32 channels
-(OCP MX FP4: E2M1 codes times a power of two, which the matrix cores' 16-bit types hold exactly),
-and an append writes the step's rows only. A (request, KV head) segment keeps its own rows, so
-heads may be ragged, as an eviction leaves them. A d128 row takes 140 bytes, its position
-included, in the place of 516.
+(cache.py:33-52). Here a layer's rows lie in pages of a pool, quantised, and an append writes the
+step's rows only. A (request, KV head) segment keeps its own rows, so heads may be ragged, as an
+eviction leaves them. A pool holds one of two formats (``bits``), and every call takes either:
+
+4  blocks of 32 channels of a row share a scale (OCP MX FP4: E2M1 codes times a power of two). A
+   d128 row takes 140 bytes, its position included, in the place of 516; elements are off by up to
+   a quarter.
+8  16 rows of a head share one scale for their keys and one for their values (E4M3 codes times a
+   power of two). A d128 row takes 264 bytes; elements are off by up to 2^-4. An append whose rows
+   have larger elements than those in their block moves the block to a larger scale: which bits are
+   lost then, all below 2^-17 of the block's largest element, does not depend on the calls that the
+   rows came in.
+
+Either's values are exact in the matrix cores' bf16.
 
 One decode step of a layer::
 
@@ -33,9 +42,16 @@ import torch
 from . import _lib
 
 
-def page_bytes(page_size: int, dim: int) -> int:
+def _format(bits) -> str:
+    """The prefix of a format's entry points."""
+    if bits not in (4, 8):
+        raise RuntimeError("A paged cache holds 4 or 8 bits")
+    return "lr_paged_" if bits == 4 else "lr_paged8_"
+
+
+def page_bytes(page_size: int, dim: int, bits: int = 4) -> int:
     """Bytes of a page: ``page_size`` rows of K and V codes, scales and positions."""
-    size = int(_lib.load().lr_paged_page_bytes(int(page_size), int(dim)))
+    size = int(getattr(_lib.load(), _format(bits) + "page_bytes")(int(page_size), int(dim)))
     if size == 0:
         raise RuntimeError("Head dimension must be 64, 128 or 256 and page size 16, 32, 64, 128 "
                            "or 256")
@@ -44,7 +60,7 @@ def page_bytes(page_size: int, dim: int) -> int:
 
 @dataclasses.dataclass
 class PagedLayer:
-    """A layer's rows: ``pages`` uint8 [pages, page_bytes(page_size, dim)], ``table`` int32
+    """A layer's rows: ``pages`` uint8 [pages, page_bytes(page_size, dim, bits)], ``table`` int32
     [batch * kv_heads, max_pages] (row i of a segment: slot i % page_size of page i // page_size),
     ``lengths`` int32 [batch * kv_heads], on one device. ``compact`` and ``read`` take the segments
     of several layers in one table as well. A page that is appended to belongs to one segment;
@@ -56,6 +72,7 @@ class PagedLayer:
     kv_heads: int
     dim: int
     page_size: int = 32
+    bits: int = 4
 
     def with_lengths(self, lengths: torch.Tensor) -> "PagedLayer":
         return dataclasses.replace(self, lengths=lengths)
@@ -64,10 +81,11 @@ class PagedLayer:
 class PagePool:
     """The pages of one device and the host's list of free ones."""
 
-    def __init__(self, page_count: int, dim: int, page_size: int = 32, device="cuda") -> None:
-        self.dim, self.page_size = int(dim), int(page_size)
-        self.pages = torch.empty((int(page_count), page_bytes(page_size, dim)), dtype=torch.uint8,
-                                 device=device)
+    def __init__(self, page_count: int, dim: int, page_size: int = 32, device="cuda",
+                 bits: int = 4) -> None:
+        self.dim, self.page_size, self.bits = int(dim), int(page_size), int(bits)
+        self.pages = torch.empty((int(page_count), page_bytes(page_size, dim, bits)),
+                                 dtype=torch.uint8, device=device)
         self._free = deque(range(int(page_count)))
         self._taken = set()
 
@@ -115,7 +133,8 @@ class PagePool:
         segments = int(batch) * int(kv_heads)
         lengths = torch.zeros(segments, dtype=torch.int32, device=self.pages.device)
         table, ids = self.table([rows] * segments)
-        return PagedLayer(self.pages, table, lengths, int(kv_heads), self.dim, self.page_size), ids
+        return PagedLayer(self.pages, table, lengths, int(kv_heads), self.dim, self.page_size,
+                          self.bits), ids
 
 
 _native_module = None
@@ -130,17 +149,16 @@ def _native():
         planner = _planner()
         library = _lib.load()
         address = lambda name: ctypes.cast(getattr(library, name), ctypes.c_void_p).value
-        planner.bind_paged(address("lr_paged_append"), address("lr_paged_attention"),
-                           address("lr_paged_attention_workspace_bytes"), address("lr_paged_read"),
-                           address("lr_paged_compact"),
-                           address("lr_paged_compact_workspace_bytes"),
-                           address("lr_paged_page_bytes"), address("lr_last_error"))
+        for bits in (4, 8):
+            planner.bind_paged(bits, *(address(_format(bits) + name) for name in (
+                "append", "attention", "attention_workspace_bytes", "read", "compact",
+                "compact_workspace_bytes", "page_bytes")), address("lr_last_error"))
         _native_module = planner
     return _native_module
 
 
 def _forward_only(name):
-    raise RuntimeError(f"paged.{name}: the 4-bit cache has no backward pass (forward only)")
+    raise RuntimeError(f"paged.{name}: the cache has no backward pass (forward only)")
 
 
 def append(layer, keys, values, positions, rotary=None, queries=None, counts=None):
@@ -154,15 +172,16 @@ def append(layer, keys, values, positions, rotary=None, queries=None, counts=Non
     dim], which are returned (contiguous, rounded once; None without queries). A position outside
     the tables gives NaN. ``counts`` int32 [batch] on the device: request b brings its first
     counts[b] rows only (a padded batch, or a request that has ended). Rows that the table has no
-    page for are not stored."""
+    page for are not stored. In 8 bits, rows written over later ones that were given up (a draft's)
+    leave their block's scale at what these needed."""
     cos, sin = (None, None) if rotary is None else rotary
     if torch.is_grad_enabled() and (
             keys.requires_grad or values.requires_grad or queries is not None and queries.requires_grad
             or cos is not None and cos.requires_grad or sin is not None and sin.requires_grad):
         _forward_only("append")
     return (_native_module or _native()).paged_append(
-        layer.pages, layer.table, layer.lengths, layer.kv_heads, layer.dim, layer.page_size, keys,
-        values, positions, cos, sin, queries, counts)
+        layer.pages, layer.table, layer.lengths, layer.kv_heads, layer.dim, layer.page_size,
+        layer.bits, keys, values, positions, cos, sin, queries, counts)
 
 
 def attention(layer, queries, max_length, counts=None, scale=None):
@@ -173,13 +192,13 @@ def attention(layer, queries, max_length, counts=None, scale=None):
 
     ``max_length``: a bound on every segment's cached rows plus ``length`` (host int; rows past it
     are not visited, and the keys are split over the chip by it). ``scale`` defaults to dim^-0.5.
-    f16 queries are for rows appended as f16 (of others, keys outside f16's range read as infinities
-    and zeros). Finite scores may be of any size that f32 holds."""
+    f16 queries are for rows appended as f16, in 4 bits (of others, keys outside f16's range read as
+    infinities and zeros); in 8 bits for any. Finite scores may be of any size that f32 holds."""
     if queries.requires_grad and torch.is_grad_enabled():
         _forward_only("attention")
     return (_native_module or _native()).paged_attention(
         layer.pages, layer.table, layer.lengths, layer.kv_heads, layer.dim, layer.page_size,
-        queries, int(max_length), counts, float(layer.dim ** -0.5 if scale is None else scale))
+        layer.bits, queries, int(max_length), counts, float(layer.dim ** -0.5 if scale is None else scale))
 
 
 def read(layer, total, dtype=torch.bfloat16):
@@ -189,14 +208,17 @@ def read(layer, total, dtype=torch.bfloat16):
     that the cache does not hold (``total`` past its rows, or a table entry outside the pool) are not
     written: they hold whatever their memory held."""
     return tuple((_native_module or _native()).paged_read(
-        layer.pages, layer.table, layer.lengths, layer.dim, layer.page_size, int(total), dtype))
+        layer.pages, layer.table, layer.lengths, layer.dim, layer.page_size, layer.bits, int(total),
+        dtype))
 
 
 def compact(layer, removed, target):
     """Evicts rows: ``removed`` int64 [count] on the device, sorted, unique row numbers in the
     packed order of ``read`` (as for ``_C.compact``). The rows that stay are moved, in order, to the
     pages of ``target`` int32 [segments, max_pages] (pages that the layer does not use, such as
-    ``PagePool.table`` gives); the old pages stay as they are. -> the layer in its new pages."""
+    ``PagePool.table`` gives); the old pages stay as they are. In 8 bits a block of 16 rows takes the
+    largest scale of the rows that come together in it. -> the layer in its new pages."""
     lengths = (_native_module or _native()).paged_compact(
-        layer.pages, layer.table, layer.lengths, layer.dim, layer.page_size, removed, target)
+        layer.pages, layer.table, layer.lengths, layer.dim, layer.page_size, layer.bits, removed,
+        target)
     return dataclasses.replace(layer, table=target, lengths=lengths)

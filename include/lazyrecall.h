@@ -616,6 +616,67 @@ int lr_paged_compact(void* pages, int64_t page_count, int64_t page_size, const i
                      size_t workspace_size, void* stream);
 
 /* ---------------------------------------------------------------------------------------
+ * A paged KV cache held in 8 bits: the same operators on pages of another format, for a cache of half
+ * the packed rows' size. Arguments, tables, lengths, counts and workspaces are those of the 4-bit
+ * cache's calls above, and what is said there of rows without a page holds here.
+ *
+ * Layout. Rows 16 k .. 16 k + 15 of a segment are a token block, whose keys share a scale and whose
+ * values share another. A page is lr_paged8_page_bytes(page_size, dim) = page_size * (2 dim + 8) bytes:
+ * the keys' codes [page_size / 16, dim / 16, 16 rows, 16 channels], the values' codes
+ * [page_size / 4, dim, 4 rows], the rows' positions (f32), and for each token block the keys' scale
+ * byte and the values', in room for 4 * page_size bytes of which page_size / 8 are used. Codes are OCP
+ * E4M3 (448 the largest, a magnitude of 127 NaN) times 2^(scale - 127). A block's scale is 2^e, e =
+ * floor(log2 amax) - 8 for its largest finite magnitude, one more from a significand of 1.8125 on, kept
+ * within [-117, 119], or [-117, 7] for rows appended as f16 (larger magnitudes saturate at 448 * 2^e).
+ * Elements are rounded to four significant bits, ties to even (a subnormal f32 to a multiple of 2^-129),
+ * and then cut, toward zero, to multiples of the smallest code, 2^(e - 9); an infinite element or NaN is
+ * stored as NaN. A block that gets rows of larger elements takes their scale, and its older codes are
+ * cut to multiples of the new smallest one: its bytes do not depend on how its rows were divided over
+ * calls. A scale grows with the rows that are written, and does not shrink when they are written over.
+ * ------------------------------------------------------------------------------------- */
+
+/* Bytes of a page (host only); 0 for a page size or head dimension that is not taken. */
+int64_t lr_paged8_page_bytes(int64_t page_size, int64_t dim);
+
+/* As lr_paged_append. Of a page that is appended to, the block that the first new row lies in is
+ * rewritten where its scale grows. One launch. */
+int lr_paged8_append(const void* keys, const int64_t* key_strides, const void* values,
+                     const int64_t* value_strides, const void* queries,
+                     const int64_t* query_strides, void* out_queries, int64_t batch,
+                     int64_t kv_heads, int64_t query_heads, int64_t added, int64_t dim, int dtype,
+                     const int64_t* positions, const float* cos, const float* sin,
+                     int64_t table_rows, int64_t half, const int32_t* counts, void* pages,
+                     int64_t page_count, int64_t page_size, const int32_t* table, int64_t max_pages,
+                     const int32_t* lengths, void* stream);
+
+/* As lr_paged_attention. Queries of either type are for rows of any type. */
+size_t lr_paged8_attention_workspace_bytes(int64_t segments, int64_t groups, int64_t length,
+                                           int64_t max_keys, int64_t dim);
+int lr_paged8_attention_plan(int64_t segments, int64_t groups, int64_t length, int64_t max_keys,
+                             int64_t dim, int64_t* plan);
+int lr_paged8_attention(const void* queries, const int64_t* query_strides, const void* pages,
+                        int64_t page_count, int64_t page_size, const int32_t* table,
+                        int64_t max_pages, const int32_t* lengths, int64_t batch, int64_t kv_heads,
+                        int64_t groups, int64_t length, int64_t dim, int dtype, int64_t max_keys,
+                        const int32_t* counts, float scale, void* out, void* workspace,
+                        size_t workspace_size, void* stream);
+
+/* As lr_paged_read; a value outside the output type's range is rounded to it once. */
+int lr_paged8_read(const void* pages, int64_t page_count, int64_t page_size, const int32_t* table,
+                   int64_t max_pages, const int32_t* lengths, int64_t segments, int64_t dim,
+                   int dtype, int64_t total, void* keys, void* values, float* positions,
+                   int32_t* cumulative, void* stream);
+
+/* As lr_paged_compact. The rows of a new block come from several old ones: it takes the largest of
+ * their scales, and the codes are cut to it. */
+size_t lr_paged8_compact_workspace_bytes(int64_t segments);
+int lr_paged8_compact(void* pages, int64_t page_count, int64_t page_size, const int32_t* table,
+                      int64_t max_pages, const int32_t* lengths, int64_t segments, int64_t dim,
+                      const int64_t* removed, int64_t removed_count, const int32_t* target,
+                      int64_t target_pages, int32_t* new_lengths, void* workspace,
+                      size_t workspace_size, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Audit vector-Jacobian helpers (the margin objective and its gradients)
  * ------------------------------------------------------------------------------------- */
 
