@@ -25,8 +25,8 @@
 
 namespace lr {
 
-constexpr int kTokens = 16;           // rows that share a scale
-constexpr unsigned kCodeNaN = 0x7f;   // magnitude
+constexpr int kTokens = 16;          // rows that share a scale
+constexpr unsigned kCodeNaN = 0xff;  // the NaN that is written (the conversion instruction's)
 
 // Exponents of the scales that append writes: 2^-9 times the smallest is a normal number in f32 and
 // bf16, 448 times the largest is finite there, or (rows appended as f16) in f16.

@@ -34,14 +34,70 @@
 namespace lr {
 namespace {
 
-// A wave's loads of codes: a uniform address and the lane's offset.
-__device__ __forceinline__ attn_u32x4 load_piece(PagedBytes p) {
-  return *(const __attribute__((address_space(1))) attn_u32x4*)p;
-}
-// The scales of the token block at `slot`: the keys' in the low byte, the values' in the next.
-__device__ __forceinline__ unsigned block_scales(const uint8_t* page, int offset) {
-  typedef const __attribute__((address_space(4))) unsigned* Words;
-  return *(Words)(page + (offset & ~3)) >> (8 * (offset & 2));
+// Pages of a unit of 32 keys from a multiple of 32 on: one, or (TWO: pages of 16 rows) two.
+template <bool TWO>
+struct UnitPages {
+  int id[TWO ? 2 : 1];  // as the table has them
+
+  __device__ __forceinline__ bool in_pool(int blk, unsigned page_count) const {
+    return static_cast<unsigned>(id[TWO ? blk : 0]) < page_count;
+  }
+};
+
+// What a wave needs to find its units: addresses are scalar, but for a lane's offset.
+template <int D, bool TWO>
+struct UnitSource {
+  PageIds table;
+  const uint8_t* pages;
+  unsigned page_count, page_bytes;
+  int shift, last;  // last: of the rows that a lookup may name
+
+  __device__ __forceinline__ UnitSource(const PagedCache& cache, unsigned seg, int last_row)
+      : table(page_table(cache, seg)), pages(cache.pages), page_count(static_cast<unsigned>(cache.page_count)),
+        page_bytes(static_cast<unsigned>(Page8<D>::bytes(1) << cache.shift)), shift(cache.shift), last(last_row) {}
+
+  __device__ __forceinline__ UnitPages<TWO> find(int key) const {
+    UnitPages<TWO> u;
+    u.id[0] = table[min(key, last) >> shift];
+    if constexpr (TWO) u.id[1] = table[min(key + 16, last) >> shift];
+    return u;
+  }
+  // The page of a unit's token block (a page outside the pool: the first one, which is not used).
+  __device__ __forceinline__ PagedBytes page(const UnitPages<TWO>& u, int blk) const {
+    const unsigned id = u.in_pool(blk, page_count) ? static_cast<unsigned>(u.id[TWO ? blk : 0]) : 0u;
+    return (PagedBytes)uniform_address(pages + static_cast<uint64_t>(id) * page_bytes);
+  }
+  // The slot of a unit's token block.
+  __device__ __forceinline__ unsigned slot(int key, int blk) const {
+    return TWO ? 0u : (static_cast<unsigned>(key) & ((1u << shift) - 1)) + 16 * blk;
+  }
+};
+
+// The scales of a unit's token blocks, read by scalar loads (they are taken apart where they are used,
+// so that nothing waits for them before).
+template <int D, bool TWO>
+struct UnitScales {
+  unsigned word[TWO ? 2 : 1];
+
+  __device__ __forceinline__ void load(const UnitSource<D, TWO>& source, const UnitPages<TWO>& u, int key) {
+    typedef const __attribute__((address_space(4))) unsigned* Words;
+#pragma unroll
+    for (int blk = 0; blk < (TWO ? 2 : 1); ++blk) {
+      const PagedBytes p = source.page(u, blk);  // (a unit's two pairs of bytes are an aligned word)
+      word[blk] = *(Words)(p + Page8<D>::scales(source.shift, static_cast<int>(source.slot(key, 0))));
+    }
+  }
+  __device__ __forceinline__ float key(int blk) const {
+    return scale_of((TWO ? word[blk] : word[0] >> (16 * blk)) & 255u);
+  }
+  __device__ __forceinline__ float value(int blk) const {
+    return scale_of((TWO ? word[blk] : word[0] >> (16 * blk)) >> 8 & 255u);
+  }
+};
+
+// 16 bytes of a lane from a uniform address on.
+__device__ __forceinline__ attn_u32x4 load_piece(PagedBytes p, unsigned lane_offset) {
+  return *(const __attribute__((address_space(1))) attn_u32x4*)(p + lane_offset);
 }
 
 // The rows of a quad of keys from `key` on that lie before `end`, as bytes of a word.
@@ -64,13 +120,14 @@ __device__ __forceinline__ attn_u32x4 take_out_nan(attn_u32x4& v) {
 }
 
 // Tiles of 16 rows: decode, and a few query rows.
-template <typename T, int D, int WAVES>
+template <typename T, int D, int WAVES, bool TWO>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(
     WAVES == 8 || D == 256 ? 2 : D == 64 ? 4 : 3)))
 void paged8_attention_kernel(PagedAttnArgs a) {
   constexpr int kStep = kUnit * WAVES;  // keys of the workgroup's step
   constexpr int KL = D / 64;            // 16-byte loads of a lane for a token block's keys, or values
   constexpr int DT = D / 16;            // column tiles of the output
+  constexpr bool kFoldScale = std::is_same<T, __bf16>::value;  // the keys' scale into the conversion
   using Vec = AttnVec<T>;
   using X8 = typename Vec::x8;
   __shared__ __align__(16) float state_lds[WAVES][kSmallRows * D];
@@ -83,25 +140,18 @@ void paged8_attention_kernel(PagedAttnArgs a) {
   const int rows_here = rows_of_tile(a, row0, kSmallRows);
   // The pages of the wave's first unit, looked up beside the segment's length (an entry past the
   // segment's last page is not used): the two memory round trips overlap.
-  const PagedCache& cache = a.cache;
-  const PageIds table = page_table(cache, seg);
-  auto in_pool = [&](int id) { return id >= 0 && id < cache.page_count ? id : -1; };
-  int first0 = -1, first1 = -1;
-  if (a.max_keys > 0) {
-    const int key = static_cast<int>(place.split) * a.chunk + kUnit * wave;
-    first0 = table[min(key >> cache.shift, cache.max_pages - 1)];
-    first1 = table[min((key + 16) >> cache.shift, cache.max_pages - 1)];
-  }
+  UnitSource<D, TWO> source(a.cache, seg, (a.cache.max_pages << a.cache.shift) - 1);
+  const int begin = static_cast<int>(place.split) * a.chunk;
+  UnitPages<TWO> first{};
+  if (a.max_keys > 0) first = source.find(begin + kUnit * wave);
   const TileKeys keys = tile_keys(a, seg, row0, row0 + rows_here - 1);
   if (keys.needed == 0) {  // no visible key for any row of this tile
     if (place.split == 0) zero_rows<T, D>(a, seg, row0, rows_here);
     return;
   }
   if (static_cast<int>(place.split) >= keys.needed) return;  // uniform across the workgroup
-  const int begin = static_cast<int>(place.split) * a.chunk;
   const int end = min(begin + a.chunk, keys.key_end);
-  first0 = in_pool(first0);
-  first1 = in_pool(first1);
+  source.last = keys.key_end - 1;
 
   // Queries (B operand of step 2 n + h: channels 16 (4 n + j) + 8 h of row m), and the last key that
   // the lane's row sees.
@@ -113,37 +163,24 @@ void paged8_attention_kernel(PagedAttnArgs a) {
   for (int s = 0; s < 2 * KL; ++s)
     q[s] = load16(static_cast<const T*>(a.queries) + row.offset + 16 * (4 * (s >> 1) + j) + 8 * (s & 1));
 
-  const int64_t page_bytes = Page8<D>::bytes(1) << cache.shift;
-  const int mask = (1 << cache.shift) - 1;
-  // Page of 16 rows from `key` on (one page: page sizes are multiples of 16); -1: outside the pool.
-  auto page_id = [&](int key) { return in_pool(table[min(key, keys.key_end - 1) >> cache.shift]); };
-  auto page_of = [&](int id) {
-    return reinterpret_cast<const uint8_t*>(uniform_address(cache.pages + (id < 0 ? 0 : id) * page_bytes));
-  };
-  // A page and a slot are the wave's, so addresses are scalar but for the lane's place in 16 rows.
   attn_u32x4 k[2][KL], v[2][KL];
-  unsigned scales[2];  // of the unit whose keys are loaded
-  auto load_keys = [&](int key0, int id0, int id1) {
+  UnitScales<D, TWO> scales;  // of the unit whose keys are loaded
+  auto load_keys = [&](const UnitPages<TWO>& u, int key0) {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      const uint8_t* page = page_of(blk == 0 ? id0 : id1);
-      const int slot = (key0 + 16 * blk) & mask;
+      const PagedBytes block = source.page(u, blk) + D * source.slot(key0, blk);
 #pragma unroll
-      for (int n = 0; n < KL; ++n)
-        k[blk][n] = load_piece((PagedBytes)page + (Page8<D>::key(slot, 4 * n) + 16 * lane));
-      scales[blk] = block_scales(page, Page8<D>::scales(cache.shift, slot));
+      for (int n = 0; n < KL; ++n) k[blk][n] = load_piece(block + 1024 * n, 16u * lane);
     }
+    scales.load(source, u, key0);
   };
   // (words 4 n + e: channels 64 n + 4 m + e of keys 4 j .. 4 j + 3)
-  auto load_values = [&](int key0, int id0, int id1) {
+  auto load_values = [&](const UnitPages<TWO>& u, int key0) {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      const uint8_t* page = page_of(blk == 0 ? id0 : id1);
-      const int slot = (key0 + 16 * blk) & mask;
+      const PagedBytes block = source.page(u, blk) + ((D << source.shift) + D * source.slot(key0, blk));
 #pragma unroll
-      for (int n = 0; n < KL; ++n)
-        v[blk][n] = load_piece((PagedBytes)page + (Page8<D>::value(cache.shift, slot) + 256 * n) +
-                               (j * 4 * D + 16 * m));
+      for (int n = 0; n < KL; ++n) v[blk][n] = load_piece(block + 256 * n, 4u * D * j + 16u * m);
     }
   };
 
@@ -157,43 +194,54 @@ void paged8_attention_kernel(PagedAttnArgs a) {
     for (int ct = 0; ct < DT; ++ct) out[ct] = attn_f32x4{0.f, 0.f, 0.f, 0.f};
     int key = begin + kUnit * wave;
     if (key >= end) return;
-    int id0 = SAFE ? page_id(key) : first0, id1 = SAFE ? page_id(key + 16) : first1;
-    load_keys(key, id0, id1);
-    load_values(key, id0, id1);
-    int next0 = page_id(key + kStep), next1 = page_id(key + kStep + 16);
+    UnitPages<TWO> now = SAFE ? source.find(key) : first;
+    load_keys(now, key);
+    load_values(now, key);
+    UnitPages<TWO> next = source.find(key + kStep);
     while (true) {
       // the unit after the next: its pages' ids arrive while this one is worked on
-      const int later0 = page_id(key + 2 * kStep), later1 = page_id(key + 2 * kStep + 16);
+      const UnitPages<TWO> later = source.find(key + 2 * kStep);
       const bool more = key + kStep < end;
-      const bool whole = key + kUnit <= keys.key_end && id0 >= 0 && id1 >= 0;
-      const bool there1 = key + 16 < keys.key_end && id1 >= 0;
-      const float key_scale[2] = {scale_of(scales[0] & 255u), scale_of(scales[1] & 255u)};
-      const float value_scale[2] = {id0 >= 0 ? scale_of(scales[0] >> 8 & 255u) : 1.0f,
-                                    there1 ? scale_of(scales[1] >> 8 & 255u) : 1.0f};
+      const bool there[2] = {now.in_pool(0, source.page_count), now.in_pool(1, source.page_count)};
       // S^T
       attn_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      const float key_scale[2] = {scales.key(0), scales.key(1)};
+      float value_scale[2] = {scales.value(0), scales.value(1)};
 #pragma unroll
       for (int n = 0; n < 2 * KL; ++n)
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
-          const float scale = std::is_same<T, __bf16>::value ? key_scale[blk] : 1.0f;
+          const float scale = kFoldScale ? key_scale[blk] : 1.0f;
           const paged_u32x2 lo = expand4<T>(k[blk][n >> 1][2 * (n & 1)], scale);
           const paged_u32x2 hi = expand4<T>(k[blk][n >> 1][2 * (n & 1) + 1], scale);
           s[blk] = Vec::mfma(__builtin_bit_cast(X8, attn_u32x4{lo[0], lo[1], hi[0], hi[1]}),
                              __builtin_bit_cast(X8, q[n]), s[blk]);
         }
-      if (more) load_keys(key + kStep, next0, next1);
-      if constexpr (!std::is_same<T, __bf16>::value)
+      if (more) load_keys(next, key + kStep);
+      if constexpr (!kFoldScale)
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[blk][r] *= key_scale[blk];
-      if (key + kUnit - 1 > all_see || id0 < 0 || id1 < 0) {
+      if (key + kUnit - 1 > all_see || !there[0] || !there[1]) {
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
+        for (int blk = 0; blk < 2; ++blk) {
+          const int lane_limit = there[blk] ? limit - (key + 16 * blk + 4 * j) : -1;
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (key + 16 * blk + 4 * j + r > limit || (blk == 0 ? id0 : id1) < 0) s[blk][r] = kNegInf;
+          for (int r = 0; r < 4; ++r) s[blk][r] = r > lane_limit ? kNegInf : s[blk][r];
+        }
+        // rows that are not there: zeros for V
+        if (key + kUnit > keys.key_end || !there[0] || !there[1]) {
+#pragma unroll
+          for (int blk = 0; blk < 2; ++blk) {
+            const unsigned rows = there[blk] ? quad_mask(key + 16 * blk + 4 * j, keys.key_end) : 0u;
+#pragma unroll
+            for (int n = 0; n < KL; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[blk][n][e] &= rows;
+            if (!there[blk] || key + 16 * blk >= keys.key_end) value_scale[blk] = 1.0f;
+          }
+        }
       }
       float top = kNegInf;
 #pragma unroll
@@ -221,16 +269,6 @@ void paged8_attention_kernel(PagedAttnArgs a) {
         sum += y;
         split_bf16(x, y, piece, n);
       }
-      if (!whole) {  // rows that are not there: zeros for V
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-          const unsigned rows = (blk == 0 ? id0 : id1) < 0 ? 0u : quad_mask(key + 16 * blk + 4 * j, keys.key_end);
-#pragma unroll
-          for (int n = 0; n < KL; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[blk][n][e] &= rows;
-        }
-      }
       // SAFE: ones for the lane's keys that its row sees
       attn_u32x4 seen{0u, 0u, 0u, 0u};
       if constexpr (SAFE)
@@ -257,10 +295,10 @@ void paged8_attention_kernel(PagedAttnArgs a) {
                                           __builtin_bit_cast(attn_bf16x8, piece[i]), out[ct]);
       }
       if (!more) break;
-      load_values(key + kStep, next0, next1);
+      load_values(next, key + kStep);
       key += kStep;
-      id0 = next0, id1 = next1;
-      next0 = later0, next1 = later1;
+      now = next;
+      next = later;
     }
   };
   pass.template operator()<false>();
@@ -303,30 +341,37 @@ void paged8_attention_kernel(PagedAttnArgs a) {
   }
 }
 
-// ---- Tiles of 32 rows -------------------------------------------------------------------------
-// The same with v_mfma_f32_32x32x16 for calls of many rows: a lane holds one query's scores of 16
-// keys, and an MFMA of twice the work takes no more of the wave's issue slots.
+// Groups of 32 rows in a tile of the kernel for many rows, and its waves on a SIMD.
+template <int D>
+constexpr int kGroups = 1;
+constexpr int tile_waves(int dim, int groups) { return dim * groups > 128 ? 2 : dim * groups == 128 ? 3 : 4; }
 
-template <typename T, int D>
-__global__ __launch_bounds__(kAttnThreads) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : D == 128 ? 3 : 2)))
+// ---- Tiles of 32 or 64 rows -------------------------------------------------------------------
+// The same with v_mfma_f32_32x32x16 for calls of many rows: a lane holds one query's scores of 16
+// keys for each 32 rows, and an MFMA of twice the work takes no more of the wave's issue slots.
+
+template <typename T, int D, int GROUPS, bool TWO>
+__global__ __launch_bounds__(kAttnThreads) __attribute__((amdgpu_waves_per_eu(tile_waves(D, GROUPS))))
 void paged8_tile_kernel(PagedAttnArgs a) {
+  constexpr int kRows = 32 * GROUPS;
   constexpr int KS = D / 16;      // MFMA steps over the head dimension
   constexpr int KL = D / 32;      // 16-byte loads of a lane for the unit's keys
   constexpr int DT = D / 32;      // column tiles of the output
   constexpr int VW = D == 64 ? 2 : 4;     // channels of a lane's load of values
   constexpr int VL = DT / VW;             // loads of a quad's values
   constexpr int kStep = kUnit * kAttnWaves;
-  __shared__ __align__(16) attn_u32x4 q_lds[KS][64];
-  __shared__ __align__(16) float state_lds[kAttnWaves][kTileRows * D / 2];
+  constexpr bool kFoldScale = std::is_same<T, __bf16>::value;  // the keys' scale into the conversion
+  __shared__ __align__(16) attn_u32x4 q_lds[GROUPS][KS][64];
+  __shared__ __align__(16) float state_lds[kAttnWaves][16 * D];
   // the waves' softmax states at the end, in the place of the queries
-  float(*const wave_ml)[kTileRows][2] = reinterpret_cast<float(*)[kTileRows][2]>(&q_lds[0][0]);
-  static_assert(sizeof(q_lds) >= sizeof(float) * kAttnWaves * kTileRows * 2, "room for the states");
+  float(*const wave_ml)[kRows][2] = reinterpret_cast<float(*)[kRows][2]>(&q_lds[0][0][0]);
+  static_assert(sizeof(q_lds) >= sizeof(float) * kAttnWaves * kRows * 2, "room for the states");
 
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = static_cast<int>(wave_index());
   const Place place = block_place(a);
-  const unsigned seg = place.seg, row0 = place.tile * kTileRows;
-  const int rows_here = rows_of_tile(a, row0, kTileRows);
+  const unsigned seg = place.seg, row0 = place.tile * kRows;
+  const int rows_here = rows_of_tile(a, row0, kRows);
   const TileKeys keys = tile_keys(a, seg, row0, row0 + rows_here - 1);
   if (keys.needed == 0) {  // no visible key for any row of this tile
     if (place.split == 0) zero_rows<T, D>(a, seg, row0, rows_here);
@@ -336,60 +381,57 @@ void paged8_tile_kernel(PagedAttnArgs a) {
   const int begin = static_cast<int>(place.split) * a.chunk;
   const int end = min(begin + a.chunk, keys.key_end);
 
-  // Queries (B operand of step 2 n + h: channels 16 (2 n + half) + 8 h of row `col`) in LDS for every
-  // wave, and the last key that the lane's row sees.
-  const TileRow row = tile_row(a, seg, row0 + (col < rows_here ? col : 0));
-  const int limit = col < rows_here ? last_key(keys, row.query) : -1;
+  // Queries (B operand of step 2 n + h: channels 16 (2 n + half) + 8 h of row `col` of a group) in LDS
+  // for every wave, and the last key that the lane's rows see.
+  int limit[GROUPS];
   const int all_see = all_rows_see(a, keys, row0, rows_here);
 #pragma unroll
-  for (int n = 0; n < KS / kAttnWaves; ++n) {
-    const int ks = n * kAttnWaves + wave;
-    q_lds[ks][lane] = load16(static_cast<const T*>(a.queries) + row.offset + 16 * (2 * (ks >> 1) + half) +
-                             8 * (ks & 1));
+  for (int g = 0; g < GROUPS; ++g) {
+    const int r = 32 * g + col;
+    const TileRow row = tile_row(a, seg, row0 + (r < rows_here ? r : 0));
+    limit[g] = r < rows_here ? last_key(keys, row.query) : -1;
+#pragma unroll
+    for (int n = 0; n < KS / kAttnWaves; ++n) {
+      const int ks = n * kAttnWaves + wave;
+      q_lds[g][ks][lane] = load16(static_cast<const T*>(a.queries) + row.offset +
+                                  16 * (2 * (ks >> 1) + half) + 8 * (ks & 1));
+    }
   }
 
-  const PagedCache& cache = a.cache;
-  const PageIds table = page_table(cache, seg);
-  const int64_t page_bytes = Page8<D>::bytes(1) << cache.shift;
-  const int mask = (1 << cache.shift) - 1;
-  auto page_id = [&](int key) {
-    const int id = table[min(key, keys.key_end - 1) >> cache.shift];
-    return id >= 0 && id < cache.page_count ? id : -1;
-  };
-  auto page_of = [&](int id) {
-    return reinterpret_cast<const uint8_t*>(uniform_address(cache.pages + (id < 0 ? 0 : id) * page_bytes));
-  };
+  const UnitSource<D, TWO> source(a.cache, seg, keys.key_end - 1);
   // Lane (key, half): 16 channels of every 32, chunks 2 n + half.
   attn_u32x4 k[KL];
   unsigned v[2][2][DT];  // a token block's quads half and 2 + half: the lane's channels
-  unsigned scales[2];
-  auto load_keys = [&](int key0, int id0, int id1) {
-    const uint8_t *const page0 = page_of(id0), *const page1 = page_of(id1);
-    const int slot0 = key0 & mask, slot1 = (key0 + 16) & mask;
-    const PagedBytes block = col < 16 ? (PagedBytes)page0 + Page8<D>::key(slot0, 0)
-                                      : (PagedBytes)page1 + Page8<D>::key(slot1, 0);
+  UnitScales<D, TWO> scales;
+  auto load_keys = [&](const UnitPages<TWO>& u, int key0) {
+    const unsigned lane_offset = 256u * half + 16u * (col & 15);
+    if constexpr (TWO) {
+      const PagedBytes block = col < 16 ? source.page(u, 0) : source.page(u, 1);
 #pragma unroll
-    for (int n = 0; n < KL; ++n) k[n] = load_piece(block + (512 * n + 256 * half + 16 * (col & 15)));
-    scales[0] = block_scales(page0, Page8<D>::scales(cache.shift, slot0));
-    scales[1] = block_scales(page1, Page8<D>::scales(cache.shift, slot1));
+      for (int n = 0; n < KL; ++n) k[n] = load_piece(block + 512 * n, lane_offset);
+    } else {
+      const PagedBytes block = source.page(u, 0) + D * source.slot(key0, 0);
+#pragma unroll
+      for (int n = 0; n < KL; ++n) k[n] = load_piece(block + 512 * n, lane_offset + 16u * D * (col >> 4));
+    }
+    scales.load(source, u, key0);
   };
   // (word VW n + e: channel 32 VW n + VW col + e)
-  auto load_values = [&](int key0, int id0, int id1) {
+  auto load_values = [&](const UnitPages<TWO>& u, int key0) {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      const uint8_t* page = page_of(blk == 0 ? id0 : id1);
-      const int slot = (key0 + 16 * blk) & mask;
+      const PagedBytes block = source.page(u, blk) + ((D << source.shift) + D * source.slot(key0, blk));
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int n = 0; n < VL; ++n) {
-          const PagedBytes p = (PagedBytes)page + (Page8<D>::value(cache.shift, slot) + 8 * D * i + 512 * n) +
-                               (4 * D * half + 4 * VW * col);
+          const PagedBytes p = block + (8 * D * i + 512 * n);
+          const unsigned lane_offset = 4u * D * half + 4u * VW * col;
           if constexpr (VW == 2) {
-            const paged_u32x2 x = *(const __attribute__((address_space(1))) paged_u32x2*)p;
+            const paged_u32x2 x = *(const __attribute__((address_space(1))) paged_u32x2*)(p + lane_offset);
             v[blk][i][0] = x[0], v[blk][i][1] = x[1];
           } else {
-            const attn_u32x4 x = load_piece(p);
+            const attn_u32x4 x = load_piece(p, lane_offset);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[blk][i][4 * n + e] = x[e];
           }
@@ -397,139 +439,181 @@ void paged8_tile_kernel(PagedAttnArgs a) {
     }
   };
 
-  float reference = kNegInf, sum = 0.0f;  // in exponents of two; the same in both halves
-  paged_f32x16 out[DT];
+  float reference[GROUPS], sum[GROUPS];  // in exponents of two; the same in both halves
+  paged_f32x16 out[GROUPS][DT];
   auto pass = [&]<bool SAFE>() {
-    reference = kNegInf, sum = 0.0f;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int g = 0; g < GROUPS; ++g) {
+      reference[g] = kNegInf, sum[g] = 0.0f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) out[dt][r] = 0.0f;
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) out[g][dt][r] = 0.0f;
+    }
     int key = begin + kUnit * wave;
     if (key >= end) return;
-    int id0 = page_id(key), id1 = page_id(key + 16);
-    load_keys(key, id0, id1);
-    load_values(key, id0, id1);
-    int next0 = page_id(key + kStep), next1 = page_id(key + kStep + 16);
+    UnitPages<TWO> now = source.find(key);
+    load_keys(now, key);
+    load_values(now, key);
+    UnitPages<TWO> next = source.find(key + kStep);
     while (true) {
-      const int later0 = page_id(key + 2 * kStep), later1 = page_id(key + 2 * kStep + 16);
+      const UnitPages<TWO> later = source.find(key + 2 * kStep);
       const bool more = key + kStep < end;
-      const bool whole = key + kUnit <= keys.key_end && id0 >= 0 && id1 >= 0;
-      const bool there1 = key + 16 < keys.key_end && id1 >= 0;
-      const float key_scale[2] = {scale_of(scales[0] & 255u), scale_of(scales[1] & 255u)};
-      const float value_scale[2] = {id0 >= 0 ? scale_of(scales[0] >> 8 & 255u) : 1.0f,
-                                    there1 ? scale_of(scales[1] >> 8 & 255u) : 1.0f};
+      const bool there[2] = {now.in_pool(0, source.page_count), now.in_pool(1, source.page_count)};
+      const float key_scale[2] = {scales.key(0), scales.key(1)};
+      float value_scale[2] = {scales.value(0), scales.value(1)};
       // S^T
-      paged_f32x16 s;
+      paged_f32x16 s[GROUPS];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = 0.0f;
-      const float lane_scale = !std::is_same<T, __bf16>::value ? 1.0f : col < 16 ? key_scale[0] : key_scale[1];
+      for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[g][r] = 0.0f;
+      const float lane_scale = !kFoldScale ? 1.0f : col < 16 ? key_scale[0] : key_scale[1];
+      asm volatile("" ::: "memory");  // (the queries stay in LDS: as registers they would spill)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const paged_u32x2 lo = expand4<T>(k[ks >> 1][2 * (ks & 1)], lane_scale);
         const paged_u32x2 hi = expand4<T>(k[ks >> 1][2 * (ks & 1) + 1], lane_scale);
-        s = mfma32<T>(attn_u32x4{lo[0], lo[1], hi[0], hi[1]}, q_lds[ks][lane], s);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+          s[g] = mfma32<T>(attn_u32x4{lo[0], lo[1], hi[0], hi[1]}, q_lds[g][ks][lane], s[g]);
       }
-      if (more) load_keys(key + kStep, next0, next1);
-      if constexpr (!std::is_same<T, __bf16>::value)
+      if (more) load_keys(next, key + kStep);
+      if constexpr (!kFoldScale)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= key_scale[r >> 3];
-      if (key + kUnit - 1 > all_see || id0 < 0 || id1 < 0) {
+        for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (key + 8 * (r >> 2) + 4 * half + (r & 3) > limit || (r < 8 ? id0 : id1) < 0) s[r] = kNegInf;
-      }
-      float top = kNegInf;
+          for (int r = 0; r < 16; ++r) s[g][r] *= key_scale[r >> 3];
+      if (key + kUnit - 1 > all_see || !there[0] || !there[1]) {
 #pragma unroll
-      for (int r = 0; r < 8; ++r) top = fmaxf(fmaxf(top, s[2 * r]), s[2 * r + 1]);
-      const LanePair pair = lane_pair<32>(top);
-      top = fmaxf(pair.first, pair.second) * a.to_log2;
-      if (__any(top > reference + (SAFE ? 0.0f : kPagedSlack))) {
-        const float raised = fmaxf(reference, top);
-        const float factor = reference == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(reference - raised);
-        sum *= factor;
+        for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+          for (int blk = 0; blk < 2; ++blk) {
+            const int lane_limit = there[blk] ? limit[g] - (key + 16 * blk + 4 * half) : -1;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) out[dt][r] *= factor;
-        reference = raised;
-      }
-      const float base = reference == kNegInf ? 0.0f : reference;
-      attn_u32x4 piece[2][kPieces];
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const float x = probability<SAFE>(s[2 * n], a.to_log2, base);
-        const float y = probability<SAFE>(s[2 * n + 1], a.to_log2, base);
-        sum += x;
-        sum += y;
-        split_bf16(x, y, piece[n / 4], n % 4);
-      }
-      if (!whole) {  // rows that are not there: zeros for V
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const unsigned rows = (blk == 0 ? id0 : id1) < 0
-                                      ? 0u : quad_mask(key + 16 * blk + 8 * i + 4 * half, keys.key_end);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) v[blk][i][dt] &= rows;
+            for (int r = 0; r < 8; ++r)
+              if (8 * (r >> 2) + (r & 3) > lane_limit) s[g][8 * blk + r] = kNegInf;
           }
+        // rows that are not there: zeros for V
+        if (key + kUnit > keys.key_end || !there[0] || !there[1]) {
+#pragma unroll
+          for (int blk = 0; blk < 2; ++blk) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const unsigned rows = there[blk] ? quad_mask(key + 16 * blk + 8 * i + 4 * half, keys.key_end) : 0u;
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt) v[blk][i][dt] &= rows;
+            }
+            if (!there[blk] || key + 16 * blk >= keys.key_end) value_scale[blk] = 1.0f;
+          }
+        }
       }
-      // O^T += V^T P^T
+      float top[GROUPS], base[GROUPS];
+      bool outgrown = false;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        top[g] = kNegInf;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) top[g] = fmaxf(fmaxf(top[g], s[g][2 * r]), s[g][2 * r + 1]);
+        const LanePair pair = lane_pair<32>(top[g]);
+        top[g] = fmaxf(pair.first, pair.second) * a.to_log2;
+        outgrown |= top[g] > reference[g] + (SAFE ? 0.0f : kPagedSlack);
+      }
+      if (__any(outgrown)) {
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          const float raised = fmaxf(reference[g], top[g]);
+          const float factor = reference[g] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(reference[g] - raised);
+          sum[g] *= factor;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) out[g][dt][r] *= factor;
+          reference[g] = raised;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) base[g] = reference[g] == kNegInf ? 0.0f : reference[g];
+      // O^T += V^T P^T, a token block after the other
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk) {
-        attn_u32x4 seen{0u, 0u, 0u, 0u};
-        if constexpr (SAFE)
+        attn_u32x4 piece[GROUPS][kPieces], seen[GROUPS];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (key + 16 * blk + 8 * (i >> 2) + 4 * half + (i & 3) <= limit) seen[i >> 1] |= 0x3f80u << (16 * (i & 1));
+        for (int g = 0; g < GROUPS; ++g) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float x = probability<SAFE>(s[g][8 * blk + 2 * n], a.to_log2, base[g]);
+            const float y = probability<SAFE>(s[g][8 * blk + 2 * n + 1], a.to_log2, base[g]);
+            sum[g] += x;
+            sum[g] += y;
+            split_bf16(x, y, piece[g], n);
+          }
+          if constexpr (SAFE) {  // ones for the lane's keys that its row sees
+            seen[g] = attn_u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (key + 16 * blk + 8 * (i >> 2) + 4 * half + (i & 3) <= limit[g])
+                seen[g][i >> 1] |= 0x3f80u << (16 * (i & 1));
+          }
+        }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           const paged_u32x2 lo = expand4<__bf16>(v[blk][0][dt], value_scale[blk]);
           const paged_u32x2 hi = expand4<__bf16>(v[blk][1][dt], value_scale[blk]);
           attn_u32x4 x{lo[0], lo[1], hi[0], hi[1]};
           if constexpr (SAFE) {
-            paged_f32x16 count;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) count[r] = 0.0f;
             const attn_u32x4 ones = take_out_nan(x);
-            count = mfma32<__bf16>(ones, seen, count);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) out[dt][r] = count[r] > 0.0f ? __builtin_nanf("") : out[dt][r];
+            for (int g = 0; g < GROUPS; ++g) {
+              paged_f32x16 count;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) count[r] = 0.0f;
+              count = mfma32<__bf16>(ones, seen[g], count);
+#pragma unroll
+              for (int r = 0; r < 16; ++r) out[g][dt][r] = count[r] > 0.0f ? __builtin_nanf("") : out[g][dt][r];
+            }
           }
 #pragma unroll
-          for (int n = 0; n < kPieces; ++n) out[dt] = mfma32<__bf16>(x, piece[blk][n], out[dt]);
+          for (int n = 0; n < kPieces; ++n)
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) out[g][dt] = mfma32<__bf16>(x, piece[g][n], out[g][dt]);
         }
       }
       if (!more) break;
-      load_values(key + kStep, next0, next1);
+      load_values(next, key + kStep);
       key += kStep;
-      id0 = next0, id1 = next1;
-      next0 = later0, next1 = later1;
+      now = next;
+      next = later;
     }
   };
   __syncthreads();
   pass.template operator()<false>();
-  float poison = 0.0f;  // 0 * NaN is NaN
+  bool again = false;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+  for (int g = 0; g < GROUPS; ++g) {
+    float poison = 0.0f;  // 0 * NaN is NaN
 #pragma unroll
-    for (int r = 0; r < 16; ++r) poison = __builtin_fmaf(out[dt][r], 0.0f, poison);
-  if (take_again(poison, reference)) pass.template operator()<true>();
-  {
-    const LanePair pair = lane_pair<32>(sum);
-    sum = pair.first + pair.second;
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) poison = __builtin_fmaf(out[g][dt][r], 0.0f, poison);
+    again |= take_again(poison, reference[g]);
+  }
+  if (again) pass.template operator()<true>();
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const LanePair pair = lane_pair<32>(sum[g]);
+    sum[g] = pair.first + pair.second;
   }
 
-  // Wave states to LDS, half of a tile's rows at a time (the row's channels are spread over the lanes'
-  // registers): 16-byte chunk c of row r in slot c ^ (r % 16). Lane (row, half) holds channels
-  // 32 VW n + VW (8 (r / 4) + 4 half + r % 4) + e in out[VW n + e][r].
-  constexpr int kHalfRows = kTileRows / 2;
+  // Wave states to LDS, 16 rows at a time (a row's channels are spread over the lanes' registers):
+  // 16-byte chunk c of row r in slot c ^ (r % 16). Lane (row, half) holds channels
+  // 32 VW n + VW (8 (r / 4) + 4 half + r % 4) + e in out[g][VW n + e][r].
   const int64_t slot = (static_cast<int64_t>(place.unit) * a.splits + place.split) * a.tile_rows;
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
+  for (int part = 0; part < 2 * GROUPS; ++part) {
+    const int g = part / 2;
     __syncthreads();
-    if ((col >> 4) == part) {
+    if ((col >> 4) == part % 2) {
       float* const mine = &state_lds[wave][(col & 15) * D];
 #pragma unroll
       for (int n = 0; n < VL; ++n)
@@ -537,18 +621,18 @@ void paged8_tile_kernel(PagedAttnArgs a) {
         for (int r = 0; r < 16; r += 4 / VW) {
           attn_f32x4 x;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = out[VW * n + e % VW][r + e / VW];
+          for (int e = 0; e < 4; ++e) x[e] = out[g][VW * n + e % VW][r + e / VW];
           const int channel = 32 * VW * n + VW * (8 * (r >> 2) + 4 * half + (r & 3));
           *reinterpret_cast<attn_f32x4*>(mine + 4 * ((channel >> 2) ^ (col & 15))) = x;
         }
     }
-    if (half == 0 && part == 0) {
-      wave_ml[wave][col][0] = reference;
-      wave_ml[wave][col][1] = sum;
+    if (half == 0 && part % 2 == 0) {
+      wave_ml[wave][32 * g + col][0] = reference[g];
+      wave_ml[wave][32 * g + col][1] = sum[g];
     }
     __syncthreads();
-    for (int item = threadIdx.x; item < kHalfRows * (D / 8); item += kAttnThreads) {
-      const int local = item / (D / 8), c = item - local * (D / 8), r = kHalfRows * part + local;
+    for (int item = threadIdx.x; item < 16 * (D / 8); item += kAttnThreads) {
+      const int local = item / (D / 8), c = item - local * (D / 8), r = 16 * part + local;
       if (r >= rows_here) break;
       auto state = [&](int w, attn_f32x4& lo, attn_f32x4& hi) {
         const float* wo = &state_lds[w][local * D];
@@ -563,26 +647,26 @@ void paged8_tile_kernel(PagedAttnArgs a) {
 
 // The plan's constants (us).
 constexpr PagedCosts kCosts8 = {
-    {{{false, 4, 4, 4.2, 0.0, 0.446, 0.226},
-      {false, 8, 2, 4.5, 0.66, 0.375, 0.48},
-      {true, 4, 4, 5.1, 0.0, 0.455, 0.353}},
-     {{false, 4, 3, 4.4, 0.0, 0.545, 0.344},
-      {false, 8, 2, 4.4, 1.1, 0.2, 0.94},
-      {true, 4, 3, 6.0, 0.0, 0.415, 0.62}},
-     {{false, 4, 2, 5.1, 1.1, 0.624, 0.88},
-      {false, 8, 1, 3.3, 3.3, 2.27, 0.0},
-      {true, 4, 2, 8.75, 0.0, 0.632, 1.12}}},
+    {{{16, 4, 4, 4.2, 0.0, 0.446, 0.226},
+      {16, 8, 2, 4.5, 0.66, 0.375, 0.48},
+      {32, 4, 4, 5.1, 0.0, 0.455, 0.353}},
+     {{16, 4, 3, 4.4, 0.0, 0.545, 0.344},
+      {16, 8, 2, 4.4, 1.1, 0.2, 0.94},
+      {32, 4, 3, 6.0, 0.0, 0.415, 0.62}},
+     {{16, 4, 2, 5.1, 1.1, 0.624, 0.88},
+      {16, 8, 1, 3.3, 3.3, 2.27, 0.0},
+      {32, 4, 2, 8.75, 0.0, 0.632, 1.12}}},
     {{2.1, 0.34, 0.23}, {2.3, 0.26, 0.24}, {2.45, 0.27, 0.21}}};
 
-template <typename T, int D>
+template <typename T, int D, bool TWO>
 int launch_paged(const PagedAttnArgs& args, const PagedPlan& plan, hipStream_t stream) {
   auto attend = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.units * plan.splits)),
                        dim3(static_cast<unsigned>(64 * plan.waves)), 0, stream, args);
   };
-  if (plan.tile_kernel) attend(paged8_tile_kernel<T, D>);
-  else if (plan.waves == kAttnWaves) attend(paged8_attention_kernel<T, D, kAttnWaves>);
-  else attend(paged8_attention_kernel<T, D, 2 * kAttnWaves>);
+  if (plan.rows > kSmallRows) attend(paged8_tile_kernel<T, D, kGroups<D>, TWO>);
+  else if (plan.waves == kAttnWaves) attend(paged8_attention_kernel<T, D, kAttnWaves, TWO>);
+  else attend(paged8_attention_kernel<T, D, 2 * kAttnWaves, TWO>);
   if (int status = check_launch("paged8_attention")) return status;
   return launch_merge<T, D>(args, plan, stream);
 }
@@ -612,8 +696,12 @@ extern "C" int lr_paged8_attention(const void* queries, const int64_t* query_str
                                    void* stream) {
   auto launch = [&](const PagedAttnArgs& args, const PagedPlan& plan) {
     return dispatch_dim(dim, [&]<int D>() {
-      return dtype == LR_DTYPE_BF16 ? launch_paged<__bf16, D>(args, plan, as_stream(stream))
-                                    : launch_paged<_Float16, D>(args, plan, as_stream(stream));
+      auto by_type = [&]<typename T>() {
+        return page_size == kTokens ? launch_paged<T, D, true>(args, plan, as_stream(stream))
+                                    : launch_paged<T, D, false>(args, plan, as_stream(stream));
+      };
+      return dtype == LR_DTYPE_BF16 ? by_type.template operator()<__bf16>()
+                                    : by_type.template operator()<_Float16>();
     });
   };
   return attend_paged<kCosts8>(queries, query_strides, pages, page_count, page_size, table, max_pages,

@@ -64,26 +64,25 @@ __device__ __forceinline__ unsigned encode(float x, int exponent) {
   const unsigned bits = __builtin_bit_cast(unsigned, x), size = bits & 0x7fffffffu;
   const unsigned four = (size + 0x7ffffu + ((size >> 20) & 1u)) & 0xfff00000u;
   const float scaled = __builtin_ldexpf(__builtin_bit_cast(float, four), -exponent - 120);
-  unsigned code = min(__builtin_bit_cast(unsigned, scaled) >> 20, kCodeNaN - 1);
-  code = size >= 0x7f800000u ? kCodeNaN : code;
-  return code | (bits >> 24 & 0x80u);
+  const unsigned code = min(__builtin_bit_cast(unsigned, scaled) >> 20, 0x7eu);
+  return size >= 0x7f800000u ? kCodeNaN : code | (bits >> 24 & 0x80u);
 }
 __device__ __forceinline__ unsigned encode4(const float* x, int exponent) {
   return encode(x[0], exponent) | encode(x[1], exponent) << 8 | encode(x[2], exponent) << 16 |
          encode(x[3], exponent) << 24;
 }
 
-// Four codes at a scale 2^by times theirs.
+// Four codes at a scale 2^by times theirs: whole numbers of the smallest code before and, once cut,
+// after, so that the conversion back has nothing to round (NaN becomes kCodeNaN).
 __device__ __forceinline__ unsigned shift_codes(unsigned codes, int by) {
-  unsigned result = codes & 0x80808080u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const unsigned size = codes >> (8 * i) & 0x7fu;
-    const unsigned moved =
-        __builtin_bit_cast(unsigned, __builtin_ldexpf(__builtin_bit_cast(float, size << 20), -by)) >> 20;
-    result |= (size == kCodeNaN ? kCodeNaN : moved) << (8 * i);
-  }
-  return result;
+  typedef short Pair __attribute__((ext_vector_type(2)));
+  const float down = scale_of(static_cast<unsigned>(127 + 9 - min(by, 32)));
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, down, false);
+  const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, down, true);
+  Pair result{};
+  result = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(result, __builtin_truncf(a[0]), __builtin_truncf(a[1]), 512.0f, false);
+  result = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(result, __builtin_truncf(b[0]), __builtin_truncf(b[1]), 512.0f, true);
+  return __builtin_bit_cast(unsigned, result);
 }
 
 // Four words of four codes, each word's bytes of one row, as words of one byte of each: a 4 x 4
@@ -99,45 +98,48 @@ __device__ __forceinline__ void transpose4(const unsigned (&in)[4], unsigned (&o
   out[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
-// A token block that rows are appended to: rows [from, to) of it are new, `first` is the number of its
-// row 0 among the new ones (negative where it has older rows), `page` NULL where there is none.
+// A token block that rows are appended to: rows [from, to) of it are new (none: from = to), `first` is
+// the number of its row 0 among the new ones (negative where it has older rows), `id` its page as the
+// table has it.
 struct Target {
-  uint8_t* page;
-  int slot, from, to, first;  // slot: of the block's row 0
+  int id, slot, from, to, first;  // slot: of the block's row 0
 };
-template <int D>
 __device__ __forceinline__ Target target_block(const AppendArgs& a, unsigned segment, unsigned b, unsigned n) {
-  Target t{nullptr, 0, 0, 0, 0};
+  Target t{-1, 0, 0, 0, 0};
   const PagedCache& cache = a.cache;
   const int length = cache.lengths[segment];
-  if (length < 0) return t;
   int count = static_cast<int>(a.added);
   if (a.counts != nullptr) count = max(0, min(count, a.counts[b]));
   const int64_t row = (static_cast<int64_t>(length) & ~int64_t{15}) + 16 * static_cast<int64_t>(n);
+  if (length < 0 || row >= static_cast<int64_t>(cache.max_pages) << cache.shift) return t;
   const int64_t behind = static_cast<int64_t>(length) + count - row;  // past the last new row
   t.first = static_cast<int>(row - length);
   t.from = max(0, -t.first);
-  t.to = behind < kTokens ? static_cast<int>(behind) : kTokens;
-  if (t.to <= t.from || row >= static_cast<int64_t>(cache.max_pages) << cache.shift) return t;
-  const int64_t id = cache.table[static_cast<int64_t>(segment) * cache.max_pages + (row >> cache.shift)];
-  if (id < 0 || id >= cache.page_count) return t;
-  t.page = cache.pages + id * (Page8<D>::bytes(1) << cache.shift);
+  t.to = behind < kTokens ? max(t.from, static_cast<int>(behind)) : kTokens;
   t.slot = static_cast<int>(row) & ((1 << cache.shift) - 1);
+  t.id = cache.table[static_cast<int64_t>(segment) * cache.max_pages + (row >> cache.shift)];
   return t;
 }
+// Its page, or NULL where there is none; called behind the loads of the new rows, which do not wait for
+// the table.
+template <int D>
+__device__ __forceinline__ uint8_t* target_page(const AppendArgs& a, const Target& t) {
+  if (t.id < 0 || t.id >= a.cache.page_count) return nullptr;
+  return a.cache.pages + static_cast<int64_t>(t.id) * (Page8<D>::bytes(1) << a.cache.shift);
+}
 
-// The exponent of a block's scale, written to its byte, and by how much older rows' codes move.
+// The exponent of a block's scale, written to its byte, and by how much older rows' codes move; `was`:
+// the byte, of a block with older rows.
 struct Scale {
   int exponent, by;
 };
-template <int D>
-__device__ __forceinline__ Scale grow_scale(const AppendArgs& a, const Target& t, int which, float top) {
-  uint8_t* const byte = t.page + Page8<D>::scales(a.cache.shift, t.slot) + which;
+__device__ __forceinline__ Scale grow_scale(const AppendArgs& a, const Target& t, uint8_t* byte, unsigned was,
+                                            float top) {
   Scale s{scale_exponent(wave_max(top), a.range), 0};
   if (t.from > 0) {
-    const int was = static_cast<int>(*byte) - 127;
-    s.by = max(0, s.exponent - was);
-    s.exponent = max(s.exponent, was);
+    const int old = static_cast<int>(was) - 127;
+    s.by = max(0, s.exponent - old);
+    s.exponent = max(s.exponent, old);
   }
   if ((threadIdx.x & 63) == 0) *byte = static_cast<uint8_t>(s.exponent + 127);
   return s;
@@ -177,6 +179,10 @@ __device__ __forceinline__ void append_keys(const AppendArgs& a, unsigned segmen
       position[i] = positions[at];
     }
   }
+  uint8_t* const page = target_page<D>(a, t);
+  if (page == nullptr) return;
+  uint8_t* const byte = page + Page8<D>::scales(a.cache.shift, t.slot);
+  const unsigned was = *byte;
   float x[kRows][2][8], top = 0.0f;
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
@@ -195,11 +201,11 @@ __device__ __forceinline__ void append_keys(const AppendArgs& a, unsigned segmen
       }
       top = fmaxf(top, fmaxf(finite_max(x[i][0]), finite_max(x[i][1])));
       if (c == 0)
-        *reinterpret_cast<float*>(t.page + Page8<D>::position(a.cache.shift, t.slot + row)) =
+        *reinterpret_cast<float*>(page + Page8<D>::position(a.cache.shift, t.slot + row)) =
             static_cast<float>(position[i]);
     }
   }
-  const Scale scale = grow_scale<D>(a, t, 0, top);
+  const Scale scale = grow_scale(a, t, byte, was, top);
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     const int row = i * kGroups + group;
@@ -207,7 +213,7 @@ __device__ __forceinline__ void append_keys(const AppendArgs& a, unsigned segmen
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       move_u32x2* const to = reinterpret_cast<move_u32x2*>(
-          t.page + Page8<D>::key(t.slot + row, chunk[p] >> 1) + 8 * (chunk[p] & 1));
+          page + Page8<D>::key(t.slot + row, chunk[p] >> 1) + 8 * (chunk[p] & 1));
       if (row >= t.from) {
         *to = move_u32x2{encode4(&x[i][p][0], scale.exponent), encode4(&x[i][p][4], scale.exponent)};
       } else {
@@ -237,6 +243,10 @@ __device__ __forceinline__ void append_values(const AppendArgs& a, unsigned segm
         raw[u][r] = *reinterpret_cast<const Eight<T>*>(source + (t.first + row) * a.values.row + 8 * c);
     }
   }
+  uint8_t* const page = target_page<D>(a, t);
+  if (page == nullptr) return;
+  uint8_t* const byte = page + Page8<D>::scales(a.cache.shift, t.slot) + 1;
+  const unsigned was = *byte;
 #pragma unroll
   for (int u = 0; u < kTimes; ++u) {
     const int quad = (u * 64 + lane) / kChunks;
@@ -250,14 +260,14 @@ __device__ __forceinline__ void append_values(const AppendArgs& a, unsigned segm
       }
     }
   }
-  const Scale scale = grow_scale<D>(a, t, 1, top);
+  const Scale scale = grow_scale(a, t, byte, was, top);
 #pragma unroll
   for (int u = 0; u < kTimes; ++u) {
     const int c = (u * 64 + lane) % kChunks, quad = (u * 64 + lane) / kChunks;
     const int row0 = 4 * quad;
     const bool older = row0 < t.from && scale.by > 0;
     if (quad >= 4 || row0 >= t.to || (row0 + 4 <= t.from && !older)) continue;
-    uint8_t* const to = t.page + Page8<D>::value(a.cache.shift, t.slot + row0) + 32 * c;
+    uint8_t* const to = page + Page8<D>::value(a.cache.shift, t.slot + row0) + 32 * c;
     unsigned word[4][2];  // a row's eight codes
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -356,8 +366,8 @@ __global__ __launch_bounds__(kThreads) void paged8_append_kernel(AppendArgs a, u
   const unsigned b = place / blocks, n = place - b * blocks;
   if (b >= a.batch) return;
   const unsigned segment = b * a.kv_heads + h;
-  const Target t = target_block<D>(a, segment, b, n);
-  if (t.page == nullptr) return;
+  const Target t = target_block(a, segment, b, n);
+  if (t.from >= t.to) return;
   if (keys) append_keys<T, D>(a, segment, b, h, t);
   else append_values<T, D>(a, segment, b, h, t);
 }
@@ -379,15 +389,11 @@ __device__ __forceinline__ Eight<T> eight_values(move_u32x2 codes, unsigned scal
   return result;
 }
 
-// Byte `row` of each of eight words.
-__device__ __forceinline__ move_u32x2 gather_bytes(move_u32x4 lo, move_u32x4 hi, int row) {
+// Byte `row` of each of four words.
+__device__ __forceinline__ unsigned gather_bytes(move_u32x4 words, int row) {
   const unsigned two = 0x0c0c0400u + 0x0101u * static_cast<unsigned>(row);
-  move_u32x2 result;
-  result[0] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(lo[3], lo[2], two),
-                                    __builtin_amdgcn_perm(lo[1], lo[0], two), 0x05040100u);
-  result[1] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(hi[3], hi[2], two),
-                                    __builtin_amdgcn_perm(hi[1], hi[0], two), 0x05040100u);
-  return result;
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(words[3], words[2], two),
+                               __builtin_amdgcn_perm(words[1], words[0], two), 0x05040100u);
 }
 
 // A workgroup takes 64 packed rows: the first wave finds each one's page and slot, then D / 8 threads
@@ -421,8 +427,6 @@ __global__ __launch_bounds__(kThreads) void paged8_read_kernel(ReadArgs a) {
       if (id >= 0 && id < cache.page_count) {
         page = id * (Page8<D>::bytes(1) << cache.shift);
         slot = at & ((1 << cache.shift) - 1);
-        a.positions[row] = *reinterpret_cast<const float*>(cache.pages + page +
-                                                           Page8<D>::position(cache.shift, slot));
       }
     }
     row_page[threadIdx.x] = page;
@@ -453,17 +457,24 @@ __global__ __launch_bounds__(kThreads) void paged8_read_kernel(ReadArgs a) {
       const int64_t at = (row0 + r) * D + 8 * c;
       *reinterpret_cast<Eight<T>*>(static_cast<T*>(a.keys) + at) = eight_values<T>(keys[i], scales[i] & 255u);
       *reinterpret_cast<Eight<T>*>(static_cast<T*>(a.values) + at) =
-          eight_values<T>(gather_bytes(values[i][0], values[i][1], row_slot[r] & 3), scales[i] >> 8);
+          eight_values<T>(move_u32x2{gather_bytes(values[i][0], row_slot[r] & 3),
+                                     gather_bytes(values[i][1], row_slot[r] & 3)}, scales[i] >> 8);
     }
   }
+  if (threadIdx.x < kReadRows && row_page[threadIdx.x] >= 0)
+    a.positions[row0 + threadIdx.x] = *reinterpret_cast<const float*>(
+        cache.pages + row_page[threadIdx.x] + Page8<D>::position(cache.shift, row_slot[threadIdx.x]));
 }
 
 // ---------------------------------------------------------------------------------------
-// A wave moves 64 rows of a segment: row r comes from row r + how many removed rows lie at or before
-// it. The wave finds that number for its first and its last row, each lane its own between them;
-// then all lanes move the codes, a token block of 16 rows after the other.
+// A wave moves 4096 channels' rows of a segment (16, 32 or 64): row r comes from row r + how many removed rows lie at or
+// before it. The wave finds that number for its first and its last row, each lane its own between them;
+// then all lanes move the codes of one token block after the other, all loads before the first store.
+constexpr int move_rows(int64_t dim) { return static_cast<int>(4096 / dim); }
+
 template <int D, bool FUSED>
 __global__ __launch_bounds__(kThreads) void paged8_compact_kernel(CompactArgs a) {
+  constexpr int kWaveRows = move_rows(D), kMoveRows = kWaveRows * (kThreads / 64);
   __shared__ int64_t lds_sums[FUSED ? kFusedSegments + 1 : 1];
   const PagedCache& cache = a.cache;
   const int lane = threadIdx.x & 63;
@@ -476,7 +487,7 @@ __global__ __launch_bounds__(kThreads) void paged8_compact_kernel(CompactArgs a)
   }
   const int64_t first = sums[segment];
   const int length = cache.rows(segment);
-  const int row0 = chunk * kCompactRows + static_cast<int>(threadIdx.x & ~63u);
+  const int row0 = chunk * kMoveRows + static_cast<int>(threadIdx.x >> 6) * kWaveRows;
   if (chunk > 0 && row0 >= length) return;  // no row can be left there
   // the segment's part of the removed rows
   const int64_t bound = lane < 32 ? first : first + length;
@@ -491,8 +502,8 @@ __global__ __launch_bounds__(kThreads) void paged8_compact_kernel(CompactArgs a)
   const int64_t* removed = a.removed + low;
   // how many removed rows (of this segment) lie at or before kept row `row`
   auto lies_before = [&](int row) { return [=](int64_t i) { return removed[i] - first - i <= row; }; };
-  int64_t j = half_search(0, gone, lies_before(lane < 32 ? row0 : row0 + 63));
-  const int row = row0 + lane, mask = (1 << cache.shift) - 1;
+  int64_t j = half_search(0, gone, lies_before(lane < 32 ? row0 : row0 + kWaveRows - 1));
+  const int row = row0 + lane % kWaveRows, mask = (1 << cache.shift) - 1;
   {
     int64_t from = __shfl(j, 0), to = __shfl(j, 32);
     while (from < to) {
@@ -516,6 +527,32 @@ __global__ __launch_bounds__(kThreads) void paged8_compact_kernel(CompactArgs a)
   const bool moves = to >= 0;
   const int from_slot = moves ? static_cast<int>(source) & mask : 0;
   if (!moves) from = 0;  // (reads the pool's first row)
+  // keys: lane (row, 16 channels of 64); values: lane (four rows, four channels of 64). The four rows
+  // come from one or two words of four rows, nearly always: the first row's and the last one's.
+  constexpr int kBlocks = kWaveRows / kTokens, kLoads = D / 64;
+  const int64_t from_key = from + Page8<D>::key(from_slot, 0);
+  const int64_t from_value = (from + Page8<D>::value(cache.shift, from_slot & ~3)) | (from_slot & 3);
+  const int c = lane & 15, quad = lane >> 4;
+  auto value_words = [&](int64_t packed, int u) {
+    return reinterpret_cast<const move_u32x4*>(cache.pages + (packed & ~int64_t{3}) + 256 * u + 16 * c);
+  };
+  move_u32x4 key_data[kBlocks][kLoads], value_data[kBlocks][2][kLoads];
+  int64_t value_from[kBlocks][4];
+#pragma unroll
+  for (int block = 0; block < kBlocks; ++block) {
+    const uint8_t* const p = cache.pages + __shfl(from_key, 16 * block + c) + 256 * quad;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) key_data[block][u] = *reinterpret_cast<const move_u32x4*>(p + 1024 * u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) value_from[block][i] = __shfl(from_value, 16 * block + 4 * quad + i);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      value_data[block][0][u] = *value_words(value_from[block][0], u);
+      value_data[block][1][u] = *value_words(value_from[block][3], u);
+    }
+  }
+  const float position = *reinterpret_cast<const float*>(cache.pages + from +
+                                                         Page8<D>::position(cache.shift, from_slot));
   // a block's scales, and by how much the row's codes move to them
   const unsigned bytes = *reinterpret_cast<const uint16_t*>(cache.pages + from +
                                                             Page8<D>::scales(cache.shift, from_slot));
@@ -527,9 +564,7 @@ __global__ __launch_bounds__(kThreads) void paged8_compact_kernel(CompactArgs a)
     largest[which] = static_cast<unsigned>(row_max(moves ? static_cast<float>(mine) : 0.0f));
     by[which] = moves ? static_cast<int>(largest[which] - mine) : 0;
   }
-  const float position = *reinterpret_cast<const float*>(cache.pages + from +
-                                                         Page8<D>::position(cache.shift, from_slot));
-  if (moves) {
+  if (moves && lane < kWaveRows) {
     uint8_t* const out = cache.pages + to;
     *reinterpret_cast<float*>(out + Page8<D>::position(cache.shift, row & mask)) = position;
     // (any of the block's rows that moves: they write the same)
@@ -537,74 +572,67 @@ __global__ __launch_bounds__(kThreads) void paged8_compact_kernel(CompactArgs a)
         static_cast<uint16_t>(largest[0] | largest[1] << 8);
   }
   const bool shifts = __any(by[0] > 0 || by[1] > 0);
-  constexpr int kKeyLoads = D / 64, kTimes = D == 256 ? 2 : 1, kChunks = D / 8;
-#pragma unroll 2
-  for (int block = 0; block < 4; ++block) {
-    if (row0 + 16 * block >= rows) break;
-    // keys: lane (row, 16 channels)
+#pragma unroll
+  for (int block = 0; block < kBlocks; ++block) {
     {
-      const int r = 16 * block + (lane & 15);
-      const int64_t key_from = __shfl(from, r), key_to = __shfl(to, r);
-      const int slot = __shfl(from_slot, r), target_slot = (row0 + r) & mask, shift = __shfl(by[0], r);
-      move_u32x4 data[kKeyLoads];
+      const int64_t row_to = __shfl(to, 16 * block + c);
+      const int shift = __shfl(by[0], 16 * block + c);
+      uint8_t* const p = cache.pages + row_to + Page8<D>::key((row0 + 16 * block + c) & mask, 0) + 256 * quad;
 #pragma unroll
-      for (int u = 0; u < kKeyLoads; ++u)
-        data[u] = *reinterpret_cast<const move_u32x4*>(cache.pages + key_from +
-                                                       Page8<D>::key(slot, 4 * u + (lane >> 4)));
-      if (shifts)
+      for (int u = 0; u < kLoads; ++u) {
+        if (shifts)
 #pragma unroll
-        for (int u = 0; u < kKeyLoads; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) data[u][e] = shift_codes(data[u][e], shift);
-      if (key_to >= 0)
-#pragma unroll
-        for (int u = 0; u < kKeyLoads; ++u)
-          *reinterpret_cast<move_u32x4*>(cache.pages + key_to +
-                                         Page8<D>::key(target_slot, 4 * u + (lane >> 4))) = data[u];
+          for (int e = 0; e < 4; ++e) key_data[block][u][e] = shift_codes(key_data[block][u][e], shift);
+        if (row_to >= 0) *reinterpret_cast<move_u32x4*>(p + 1024 * u) = key_data[block][u];
+      }
     }
-    // values: lane (four rows, eight channels)
+    int64_t row_to[4];
+    int shift[4];
+    bool whole = true, apart[2];
 #pragma unroll
-    for (int u = 0; u < kTimes; ++u) {
-      const int c = (u * 64 + lane) % kChunks, quad = (u * 64 + lane) / kChunks & 3;  // (d64: twice)
-      move_u32x4 data[4][2];
-      int64_t row_to[4];
-      int slot[4], shift[4];
+    for (int i = 0; i < 4; ++i) {
+      row_to[i] = __shfl(to, 16 * block + 4 * quad + i);
+      shift[i] = __shfl(by[1], 16 * block + 4 * quad + i);
+      whole = whole && row_to[i] >= 0;
+    }
+    const int64_t* const packed = value_from[block];
+    auto same = [&](int i, int k) { return ((packed[i] ^ packed[k]) & ~int64_t{3}) == 0; };
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * block + 4 * quad + i;
-        row_to[i] = __shfl(to, r);
-        slot[i] = __shfl(from_slot, r);
-        shift[i] = __shfl(by[1], r);
-        const uint8_t* p = cache.pages + __shfl(from, r) + Page8<D>::value(cache.shift, slot[i] & ~3) + 32 * c;
-        data[i][0] = *reinterpret_cast<const move_u32x4*>(p);
-        data[i][1] = *reinterpret_cast<const move_u32x4*>(p + 16);
+    for (int i = 0; i < 2; ++i) apart[i] = !same(1 + i, 0) && !same(1 + i, 3);
+    const unsigned low = 0x0c0c0400u + static_cast<unsigned>(packed[0] & 3) + (static_cast<unsigned>(packed[1] & 3) << 8);
+    const unsigned high = 0x04000c0cu + (static_cast<unsigned>(packed[2] & 3) << 16) +
+                          (static_cast<unsigned>(packed[3] & 3) << 24);
+    const int at = Page8<D>::value(cache.shift, (row0 + 16 * block + 4 * quad) & mask) + 16 * c;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      move_u32x4 row[4] = {value_data[block][0][u], value_data[block][0][u], value_data[block][0][u],
+                           value_data[block][1][u]};
+#pragma unroll
+      for (int i = 1; i < 3; ++i) {
+        if (!same(i, 0)) row[i] = row[3];
+        if (apart[i - 1]) row[i] = *value_words(packed[i], u);
       }
-      unsigned word[4][2];
+      move_u32x4 codes;
+      if (shifts) {  // a row's four codes as a word, moved to their scale
+        unsigned word[4], out[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const move_u32x2 codes = gather_bytes(data[i][0], data[i][1], slot[i] & 3);
-        word[i][0] = codes[0], word[i][1] = codes[1];
-        if (shifts) word[i][0] = shift_codes(word[i][0], shift[i]), word[i][1] = shift_codes(word[i][1], shift[i]);
+        for (int i = 0; i < 4; ++i) word[i] = shift_codes(gather_bytes(row[i], packed[i] & 3), shift[i]);
+        transpose4(word, out);
+        codes = move_u32x4{out[0], out[1], out[2], out[3]};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          codes[e] = __builtin_amdgcn_perm(row[1][e], row[0][e], low) | __builtin_amdgcn_perm(row[3][e], row[2][e], high);
       }
-      if (D == 64 && lane >= 32) continue;
-      const int target_slot = (row0 + 16 * block + 4 * quad) & mask;
-      const int at = Page8<D>::value(cache.shift, target_slot) + 32 * c;
-      if (row_to[0] >= 0 && row_to[1] >= 0 && row_to[2] >= 0 && row_to[3] >= 0) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const unsigned in[4] = {word[0][n], word[1][n], word[2][n], word[3][n]};
-          unsigned codes[4];
-          transpose4(in, codes);
-          *reinterpret_cast<move_u32x4*>(cache.pages + row_to[0] + at + 16 * n) =
-              move_u32x4{codes[0], codes[1], codes[2], codes[3]};
-        }
+      if (whole) {
+        *reinterpret_cast<move_u32x4*>(cache.pages + row_to[0] + at + 256 * u) = codes;
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (row_to[i] >= 0)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              cache.pages[row_to[i] + at + 4 * e + i] = static_cast<uint8_t>(word[i][e / 4] >> (8 * (e % 4)));
+            for (int e = 0; e < 4; ++e)
+              cache.pages[row_to[i] + at + 256 * u + 4 * e + i] = static_cast<uint8_t>(codes[e] >> (8 * i));
       }
     }
   }
@@ -697,7 +725,7 @@ extern "C" int lr_paged8_compact(void* pages, int64_t page_count, int64_t page_s
       return check_launch("paged8_compact");
     });
   };
-  return compact_paged(pages, page_count, page_size, table, max_pages, lengths, segments, dim, removed,
-                       removed_count, target, target_pages, new_lengths, workspace, workspace_size,
-                       stream, launch);
+  return compact_paged(move_rows(dim > 0 ? dim : 1) * (kThreads / 64), pages, page_count, page_size, table,
+                       max_pages, lengths, segments, dim, removed, removed_count, target, target_pages,
+                       new_lengths, workspace, workspace_size, stream, launch);
 }

@@ -44,6 +44,8 @@
 namespace lr {
 namespace {
 
+constexpr int kTileRows = 32;  // many query rows
+
 typedef short paged_s16x4 __attribute__((ext_vector_type(4)));
 
 // V rows in LDS: 16-byte chunk c of row r in slot c ^ x(r). The eight rows that eight lanes write one
@@ -615,15 +617,15 @@ void paged_tile_kernel(PagedAttnArgs a) {
 // requests onto 300 rows, 4 heads, G6, d256, 21 us against 12; 192 queries of one onto 9,000 rows 175
 // against 99.)
 constexpr PagedCosts kCosts4 = {
-    {{{false, 4, 4, 4.2, 0.0, 0.446, 0.226},
-      {false, 8, 2, 4.5, 0.66, 0.375, 0.48},
-      {true, 4, 4, 5.1, 0.0, 0.455, 0.353}},
-     {{false, 4, 3, 4.4, 0.0, 0.545, 0.344},
-      {false, 8, 2, 4.4, 1.1, 0.2, 0.94},
-      {true, 4, 3, 6.0, 0.0, 0.415, 0.62}},
-     {{false, 4, 2, 5.1, 1.1, 0.624, 0.88},
-      {false, 8, 1, 3.3, 3.3, 2.27, 0.0},
-      {true, 4, 2, 8.75, 0.0, 0.632, 1.12}}},
+    {{{16, 4, 4, 4.2, 0.0, 0.446, 0.226},
+      {16, 8, 2, 4.5, 0.66, 0.375, 0.48},
+      {32, 4, 4, 5.1, 0.0, 0.455, 0.353}},
+     {{16, 4, 3, 4.4, 0.0, 0.545, 0.344},
+      {16, 8, 2, 4.4, 1.1, 0.2, 0.94},
+      {32, 4, 3, 6.0, 0.0, 0.415, 0.62}},
+     {{16, 4, 2, 5.1, 1.1, 0.624, 0.88},
+      {16, 8, 1, 3.3, 3.3, 2.27, 0.0},
+      {32, 4, 2, 8.75, 0.0, 0.632, 1.12}}},
     {{2.1, 0.34, 0.23}, {2.3, 0.26, 0.24}, {2.45, 0.27, 0.21}}};
 
 template <typename T, int D>
@@ -632,7 +634,7 @@ int launch_paged(const PagedAttnArgs& args, const PagedPlan& plan, hipStream_t s
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.units * plan.splits)),
                        dim3(static_cast<unsigned>(64 * plan.waves)), 0, stream, args);
   };
-  if (plan.tile_kernel) attend(paged_tile_kernel<T, D>);
+  if (plan.rows == kTileRows) attend(paged_tile_kernel<T, D>);
   else if (plan.waves == kAttnWaves) attend(paged_attention_kernel<T, D, kAttnWaves>);
   else attend(paged_attention_kernel<T, D, 2 * kAttnWaves>);
   if (int status = check_launch("paged_attention")) return status;

@@ -15,7 +15,6 @@ namespace {
 
 constexpr int kUnit = 32;       // keys of a wave's step
 constexpr int kSmallRows = 16;  // rows of a tile: decode and a few query rows
-constexpr int kTileRows = 32;   // many query rows
 constexpr float kPagedSlack = 4.0f;
 constexpr int kPieces = 3;      // of a probability
 // A row's largest exponent (of two) up to which score * to_log2 - reference is one multiply-add: the
@@ -283,7 +282,7 @@ __global__ __launch_bounds__(kAttnThreads) void paged_merge_kernel(PagedAttnArgs
 }
 
 struct PagedPlan {
-  bool tile_kernel;
+  int rows;              // of a tile
   int waves, tile_rows;  // of a workgroup, of a tile's partial states
   int64_t tiles, units, splits, chunk;
 };
@@ -295,8 +294,7 @@ struct PagedPlan {
 // read, and a thread of the merge loads N states. The constants (us) are each cache's own, with its
 // kernels.
 struct PagedCost {
-  bool tile_kernel;
-  int waves, resident;
+  int rows, waves, resident;
   double call, round, step, share;
 };
 struct MergeCost {
@@ -322,11 +320,11 @@ PagedPlan least_cost(const PagedCosts& costs, int64_t segments, int64_t groups, 
   PagedPlan best{};
   double least = HUGE_VAL;
   for (const PagedCost& cost : costs.kernels[row]) {
-    if (cost.tile_kernel && rows <= kSmallRows) continue;
+    if (cost.rows > kSmallRows && rows <= kSmallRows) continue;
     PagedPlan p{};
-    p.tile_kernel = cost.tile_kernel;
+    p.rows = cost.rows;
     p.waves = cost.waves;
-    const int64_t tile = p.tile_kernel ? kTileRows : kSmallRows;
+    const int64_t tile = p.rows;
     p.tile_rows = static_cast<int>(std::min(rows, tile));
     p.tiles = ceil_div(rows, tile);
     p.units = segments * p.tiles;
@@ -471,7 +469,7 @@ int describe_paged_plan(int64_t segments, int64_t groups, int64_t length, int64_
                  max_keys <= INT32_MAX / 2 && plan,
              "Empty attention dimensions");
   const PagedPlan p = plan_paged<COSTS>(segments, groups, length, max_keys, dim);
-  plan[0] = p.tile_kernel ? kTileRows : kSmallRows;
+  plan[0] = p.rows;
   plan[1] = p.waves;
   plan[2] = p.splits;
   return LR_OK;

@@ -308,6 +308,8 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(ReadArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------
+constexpr int kCompactRows = kThreads;  // of a workgroup, 64 a wave
+
 // A wave moves 64 rows of a segment: row r comes from row r + how many removed rows lie at or before
 // it. The wave finds that number for its first and its last row, each lane its own between them;
 // then all lanes copy 16 bytes each of the rows' codes.
@@ -492,7 +494,7 @@ extern "C" int lr_paged_compact(void* pages, int64_t page_count, int64_t page_si
       return check_launch("paged_compact");
     });
   };
-  return compact_paged(pages, page_count, page_size, table, max_pages, lengths, segments, dim, removed,
-                       removed_count, target, target_pages, new_lengths, workspace, workspace_size,
-                       stream, launch);
+  return compact_paged(kCompactRows, pages, page_count, page_size, table, max_pages, lengths, segments,
+                       dim, removed, removed_count, target, target_pages, new_lengths, workspace,
+                       workspace_size, stream, launch);
 }

@@ -147,7 +147,7 @@ __device__ __forceinline__ int segment_of(const int32_t* cumulative, int segment
 struct CompactArgs {
   PagedCache cache;
   int64_t segments;
-  int chunks;                   // of kCompactRows rows of a segment
+  int chunks;                   // of a workgroup's rows of a segment
   const int32_t* target;        // [segments, target_pages]
   int target_pages;
   const int64_t* removed;       // sorted packed rows
@@ -155,8 +155,6 @@ struct CompactArgs {
   const int64_t* sums;          // [segments + 1], unless the workgroups sum the lengths themselves
   int32_t* new_lengths;
 };
-
-constexpr int kCompactRows = kThreads;  // of a workgroup, 64 a wave
 
 // The first of [low, high) that is not `before` (all of those before it are): 32 lanes look at 32
 // places a round, each half of the wave for a range of its own.
@@ -293,8 +291,9 @@ inline size_t compact_paged_workspace(int64_t segments) {
   return segments > kFusedSegments ? static_cast<size_t>(segments + 1) * sizeof(int64_t) : 0;
 }
 
+// (a workgroup takes `group_rows` rows of a segment)
 template <typename Launch>
-int compact_paged(void* pages, int64_t page_count, int64_t page_size,
+int compact_paged(int group_rows, void* pages, int64_t page_count, int64_t page_size,
                   const int32_t* table, int64_t max_pages, const int32_t* lengths,
                   int64_t segments, int64_t dim, const int64_t* removed,
                   int64_t removed_count, const int32_t* target, int64_t target_pages,
@@ -319,7 +318,7 @@ int compact_paged(void* pages, int64_t page_count, int64_t page_size,
   args.cache = paged_cache(pages, page_count, page_size, table, max_pages, lengths);
   args.segments = segments;
   // a segment's rows, kept or not, are at most what its table holds
-  args.chunks = static_cast<int>(std::max<int64_t>(1, ceil_div(max_pages * page_size, kCompactRows)));
+  args.chunks = static_cast<int>(std::max<int64_t>(1, ceil_div(max_pages * page_size, group_rows)));
   args.target = target;
   // (without a page there is nothing to move: the lengths alone)
   args.target_pages = page_count == 0 ? 0 : static_cast<int>(target_pages);

@@ -630,7 +630,7 @@ int lr_paged_compact(void* pages, int64_t page_count, int64_t page_size, const i
  * within [-117, 119], or [-117, 7] for rows appended as f16 (larger magnitudes saturate at 448 * 2^e).
  * Elements are rounded to four significant bits, ties to even (a subnormal f32 to a multiple of 2^-129),
  * and then cut, toward zero, to multiples of the smallest code, 2^(e - 9); an infinite element or NaN is
- * stored as NaN. A block that gets rows of larger elements takes their scale, and its older codes are
+ * stored as NaN (0xff). A block that gets rows of larger elements takes their scale, and its older codes are
  * cut to multiples of the new smallest one: its bytes do not depend on how its rows were divided over
  * calls. A scale grows with the rows that are written, and does not shrink when they are written over.
  * ------------------------------------------------------------------------------------- */

@@ -37,7 +37,7 @@ def encode(rows, exponent):
     finite = np.isfinite(rows)
     size = np.abs(four_bits(np.where(finite, rows, 0.0))) * np.exp2(-np.asarray(exponent, np.float64))
     code = np.searchsorted(MAGNITUDES, size, side="right") - 1  # cut to the code at or below
-    return (np.where(finite, code, 127) + 128 * np.signbit(rows)).astype(np.uint8)
+    return np.where(finite, code + 128 * np.signbit(rows), 255).astype(np.uint8)
 
 
 def values(codes, exponent):
@@ -78,7 +78,7 @@ def append(pages, table_row, length: int, page_size: int, keys, vals, positions,
                 e = max(e, was)
                 old = pages[page, spots[which][~fresh]]
                 pages[page, spots[which][~fresh]] = np.where(
-                    old & 127 == 127, old, encode(values(old, was), e) & 127 | old & 128)
+                    old & 127 == 127, 255, encode(values(old, was), e) & 127 | old & 128)
             pages[page, spots[which][fresh]] = encode(new, e)
             pages[page, at] = e + 127
         pages[page, spots[2][fresh]] = np.asarray(
@@ -110,7 +110,7 @@ def compact(pages, table_row, kept, target_row, page_size: int, dim: int):
         for which, old in enumerate((k[part], v[part])):
             was = e[part, which:which + 1]
             top = was.max()
-            pages[page, spots[which]] = np.where(old & 127 == 127, old,
+            pages[page, spots[which]] = np.where(old & 127 == 127, 255,
                                                  encode(values(old, was), top) & 127 | old & 128)
             pages[page, spots[3][0, which]] = top + 127
         pages[page, spots[2]] = positions[part].astype(np.float32).reshape(-1, 1).view(np.uint8)
