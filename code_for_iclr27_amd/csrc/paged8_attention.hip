@@ -341,19 +341,13 @@ void paged8_attention_kernel(PagedAttnArgs a) {
   }
 }
 
-// Groups of 32 rows in a tile of the kernel for many rows, and its waves on a SIMD.
-template <int D>
-constexpr int kGroups = 1;
-constexpr int tile_waves(int dim, int groups) { return dim * groups > 128 ? 2 : dim * groups == 128 ? 3 : 4; }
-
-// ---- Tiles of 32 or 64 rows -------------------------------------------------------------------
+// ---- Tiles of 32 rows -------------------------------------------------------------------------
 // The same with v_mfma_f32_32x32x16 for calls of many rows: a lane holds one query's scores of 16
-// keys for each 32 rows, and an MFMA of twice the work takes no more of the wave's issue slots.
+// keys, and an MFMA of twice the work takes no more of the wave's issue slots.
 
-template <typename T, int D, int GROUPS, bool TWO>
-__global__ __launch_bounds__(kAttnThreads) __attribute__((amdgpu_waves_per_eu(tile_waves(D, GROUPS))))
+template <typename T, int D, bool TWO>
+__global__ __launch_bounds__(kAttnThreads) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : D == 128 ? 3 : 2)))
 void paged8_tile_kernel(PagedAttnArgs a) {
-  constexpr int kRows = 32 * GROUPS;
   constexpr int KS = D / 16;      // MFMA steps over the head dimension
   constexpr int KL = D / 32;      // 16-byte loads of a lane for the unit's keys
   constexpr int DT = D / 32;      // column tiles of the output
@@ -361,17 +355,17 @@ void paged8_tile_kernel(PagedAttnArgs a) {
   constexpr int VL = DT / VW;             // loads of a quad's values
   constexpr int kStep = kUnit * kAttnWaves;
   constexpr bool kFoldScale = std::is_same<T, __bf16>::value;  // the keys' scale into the conversion
-  __shared__ __align__(16) attn_u32x4 q_lds[GROUPS][KS][64];
+  __shared__ __align__(16) attn_u32x4 q_lds[KS][64];
   __shared__ __align__(16) float state_lds[kAttnWaves][16 * D];
   // the waves' softmax states at the end, in the place of the queries
-  float(*const wave_ml)[kRows][2] = reinterpret_cast<float(*)[kRows][2]>(&q_lds[0][0][0]);
-  static_assert(sizeof(q_lds) >= sizeof(float) * kAttnWaves * kRows * 2, "room for the states");
+  float(*const wave_ml)[kTileRows][2] = reinterpret_cast<float(*)[kTileRows][2]>(&q_lds[0][0]);
+  static_assert(sizeof(q_lds) >= sizeof(float) * kAttnWaves * kTileRows * 2, "room for the states");
 
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = static_cast<int>(wave_index());
   const Place place = block_place(a);
-  const unsigned seg = place.seg, row0 = place.tile * kRows;
-  const int rows_here = rows_of_tile(a, row0, kRows);
+  const unsigned seg = place.seg, row0 = place.tile * kTileRows;
+  const int rows_here = rows_of_tile(a, row0, kTileRows);
   const TileKeys keys = tile_keys(a, seg, row0, row0 + rows_here - 1);
   if (keys.needed == 0) {  // no visible key for any row of this tile
     if (place.split == 0) zero_rows<T, D>(a, seg, row0, rows_here);
@@ -381,21 +375,16 @@ void paged8_tile_kernel(PagedAttnArgs a) {
   const int begin = static_cast<int>(place.split) * a.chunk;
   const int end = min(begin + a.chunk, keys.key_end);
 
-  // Queries (B operand of step 2 n + h: channels 16 (2 n + half) + 8 h of row `col` of a group) in LDS
-  // for every wave, and the last key that the lane's rows see.
-  int limit[GROUPS];
+  // Queries (B operand of step 2 n + h: channels 16 (2 n + half) + 8 h of row `col`) in LDS for every
+  // wave, and the last key that the lane's row sees.
+  const TileRow row = tile_row(a, seg, row0 + (col < rows_here ? col : 0));
+  const int limit = col < rows_here ? last_key(keys, row.query) : -1;
   const int all_see = all_rows_see(a, keys, row0, rows_here);
 #pragma unroll
-  for (int g = 0; g < GROUPS; ++g) {
-    const int r = 32 * g + col;
-    const TileRow row = tile_row(a, seg, row0 + (r < rows_here ? r : 0));
-    limit[g] = r < rows_here ? last_key(keys, row.query) : -1;
-#pragma unroll
-    for (int n = 0; n < KS / kAttnWaves; ++n) {
-      const int ks = n * kAttnWaves + wave;
-      q_lds[g][ks][lane] = load16(static_cast<const T*>(a.queries) + row.offset +
-                                  16 * (2 * (ks >> 1) + half) + 8 * (ks & 1));
-    }
+  for (int n = 0; n < KS / kAttnWaves; ++n) {
+    const int ks = n * kAttnWaves + wave;
+    q_lds[ks][lane] = load16(static_cast<const T*>(a.queries) + row.offset + 16 * (2 * (ks >> 1) + half) +
+                             8 * (ks & 1));
   }
 
   const UnitSource<D, TWO> source(a.cache, seg, keys.key_end - 1);
@@ -439,17 +428,14 @@ void paged8_tile_kernel(PagedAttnArgs a) {
     }
   };
 
-  float reference[GROUPS], sum[GROUPS];  // in exponents of two; the same in both halves
-  paged_f32x16 out[GROUPS][DT];
+  float reference, sum;  // in exponents of two; the same in both halves
+  paged_f32x16 out[DT];
   auto pass = [&]<bool SAFE>() {
+    reference = kNegInf, sum = 0.0f;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      reference[g] = kNegInf, sum[g] = 0.0f;
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) out[g][dt][r] = 0.0f;
-    }
+      for (int r = 0; r < 16; ++r) out[dt][r] = 0.0f;
     int key = begin + kUnit * wave;
     if (key >= end) return;
     UnitPages<TWO> now = source.find(key);
@@ -463,37 +449,29 @@ void paged8_tile_kernel(PagedAttnArgs a) {
       const float key_scale[2] = {scales.key(0), scales.key(1)};
       float value_scale[2] = {scales.value(0), scales.value(1)};
       // S^T
-      paged_f32x16 s[GROUPS];
+      paged_f32x16 s;
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[g][r] = 0.0f;
+      for (int r = 0; r < 16; ++r) s[r] = 0.0f;
       const float lane_scale = !kFoldScale ? 1.0f : col < 16 ? key_scale[0] : key_scale[1];
       asm volatile("" ::: "memory");  // (the queries stay in LDS: as registers they would spill)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const paged_u32x2 lo = expand4<T>(k[ks >> 1][2 * (ks & 1)], lane_scale);
         const paged_u32x2 hi = expand4<T>(k[ks >> 1][2 * (ks & 1) + 1], lane_scale);
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g)
-          s[g] = mfma32<T>(attn_u32x4{lo[0], lo[1], hi[0], hi[1]}, q_lds[g][ks][lane], s[g]);
+        s = mfma32<T>(attn_u32x4{lo[0], lo[1], hi[0], hi[1]}, q_lds[ks][lane], s);
       }
       if (more) load_keys(next, key + kStep);
       if constexpr (!kFoldScale)
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[g][r] *= key_scale[r >> 3];
+        for (int r = 0; r < 16; ++r) s[r] *= key_scale[r >> 3];
       if (key + kUnit - 1 > all_see || !there[0] || !there[1]) {
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g)
+        for (int blk = 0; blk < 2; ++blk) {
+          const int lane_limit = there[blk] ? limit - (key + 16 * blk + 4 * half) : -1;
 #pragma unroll
-          for (int blk = 0; blk < 2; ++blk) {
-            const int lane_limit = there[blk] ? limit[g] - (key + 16 * blk + 4 * half) : -1;
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-              if (8 * (r >> 2) + (r & 3) > lane_limit) s[g][8 * blk + r] = kNegInf;
-          }
+          for (int r = 0; r < 8; ++r)
+            if (8 * (r >> 2) + (r & 3) > lane_limit) s[8 * blk + r] = kNegInf;
+        }
         // rows that are not there: zeros for V
         if (key + kUnit > keys.key_end || !there[0] || !there[1]) {
 #pragma unroll
@@ -508,54 +486,38 @@ void paged8_tile_kernel(PagedAttnArgs a) {
           }
         }
       }
-      float top[GROUPS], base[GROUPS];
-      bool outgrown = false;
+      float top = kNegInf;
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        top[g] = kNegInf;
+      for (int r = 0; r < 8; ++r) top = fmaxf(fmaxf(top, s[2 * r]), s[2 * r + 1]);
+      const LanePair pair = lane_pair<32>(top);
+      top = fmaxf(pair.first, pair.second) * a.to_log2;
+      if (__any(top > reference + (SAFE ? 0.0f : kPagedSlack))) {
+        const float raised = fmaxf(reference, top);
+        const float factor = reference == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(reference - raised);
+        sum *= factor;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) top[g] = fmaxf(fmaxf(top[g], s[g][2 * r]), s[g][2 * r + 1]);
-        const LanePair pair = lane_pair<32>(top[g]);
-        top[g] = fmaxf(pair.first, pair.second) * a.to_log2;
-        outgrown |= top[g] > reference[g] + (SAFE ? 0.0f : kPagedSlack);
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) out[dt][r] *= factor;
+        reference = raised;
       }
-      if (__any(outgrown)) {
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          const float raised = fmaxf(reference[g], top[g]);
-          const float factor = reference[g] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(reference[g] - raised);
-          sum[g] *= factor;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) out[g][dt][r] *= factor;
-          reference[g] = raised;
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g) base[g] = reference[g] == kNegInf ? 0.0f : reference[g];
+      const float base = reference == kNegInf ? 0.0f : reference;
       // O^T += V^T P^T, a token block after the other
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk) {
-        attn_u32x4 piece[GROUPS][kPieces], seen[GROUPS];
+        attn_u32x4 piece[kPieces], seen{0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const float x = probability<SAFE>(s[g][8 * blk + 2 * n], a.to_log2, base[g]);
-            const float y = probability<SAFE>(s[g][8 * blk + 2 * n + 1], a.to_log2, base[g]);
-            sum[g] += x;
-            sum[g] += y;
-            split_bf16(x, y, piece[g], n);
-          }
-          if constexpr (SAFE) {  // ones for the lane's keys that its row sees
-            seen[g] = attn_u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (key + 16 * blk + 8 * (i >> 2) + 4 * half + (i & 3) <= limit[g])
-                seen[g][i >> 1] |= 0x3f80u << (16 * (i & 1));
-          }
+        for (int n = 0; n < 4; ++n) {
+          const float x = probability<SAFE>(s[8 * blk + 2 * n], a.to_log2, base);
+          const float y = probability<SAFE>(s[8 * blk + 2 * n + 1], a.to_log2, base);
+          sum += x;
+          sum += y;
+          split_bf16(x, y, piece, n);
         }
+        if constexpr (SAFE)  // ones for the lane's keys that its row sees
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (key + 16 * blk + 8 * (i >> 2) + 4 * half + (i & 3) <= limit) seen[i >> 1] |= 0x3f80u << (16 * (i & 1));
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           const paged_u32x2 lo = expand4<__bf16>(v[blk][0][dt], value_scale[blk]);
@@ -563,20 +525,15 @@ void paged8_tile_kernel(PagedAttnArgs a) {
           attn_u32x4 x{lo[0], lo[1], hi[0], hi[1]};
           if constexpr (SAFE) {
             const attn_u32x4 ones = take_out_nan(x);
+            paged_f32x16 count;
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-              paged_f32x16 count;
+            for (int r = 0; r < 16; ++r) count[r] = 0.0f;
+            count = mfma32<__bf16>(ones, seen, count);
 #pragma unroll
-              for (int r = 0; r < 16; ++r) count[r] = 0.0f;
-              count = mfma32<__bf16>(ones, seen[g], count);
-#pragma unroll
-              for (int r = 0; r < 16; ++r) out[g][dt][r] = count[r] > 0.0f ? __builtin_nanf("") : out[g][dt][r];
-            }
+            for (int r = 0; r < 16; ++r) out[dt][r] = count[r] > 0.0f ? __builtin_nanf("") : out[dt][r];
           }
 #pragma unroll
-          for (int n = 0; n < kPieces; ++n)
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g) out[g][dt] = mfma32<__bf16>(x, piece[g][n], out[g][dt]);
+          for (int n = 0; n < kPieces; ++n) out[dt] = mfma32<__bf16>(x, piece[n], out[dt]);
         }
       }
       if (!more) break;
@@ -588,32 +545,25 @@ void paged8_tile_kernel(PagedAttnArgs a) {
   };
   __syncthreads();
   pass.template operator()<false>();
-  bool again = false;
+  float poison = 0.0f;  // 0 * NaN is NaN
 #pragma unroll
-  for (int g = 0; g < GROUPS; ++g) {
-    float poison = 0.0f;  // 0 * NaN is NaN
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) poison = __builtin_fmaf(out[g][dt][r], 0.0f, poison);
-    again |= take_again(poison, reference[g]);
-  }
-  if (again) pass.template operator()<true>();
-#pragma unroll
-  for (int g = 0; g < GROUPS; ++g) {
-    const LanePair pair = lane_pair<32>(sum[g]);
-    sum[g] = pair.first + pair.second;
+    for (int r = 0; r < 16; ++r) poison = __builtin_fmaf(out[dt][r], 0.0f, poison);
+  if (take_again(poison, reference)) pass.template operator()<true>();
+  {
+    const LanePair pair = lane_pair<32>(sum);
+    sum = pair.first + pair.second;
   }
 
   // Wave states to LDS, 16 rows at a time (a row's channels are spread over the lanes' registers):
   // 16-byte chunk c of row r in slot c ^ (r % 16). Lane (row, half) holds channels
-  // 32 VW n + VW (8 (r / 4) + 4 half + r % 4) + e in out[g][VW n + e][r].
+  // 32 VW n + VW (8 (r / 4) + 4 half + r % 4) + e in out[VW n + e][r].
   const int64_t slot = (static_cast<int64_t>(place.unit) * a.splits + place.split) * a.tile_rows;
 #pragma unroll
-  for (int part = 0; part < 2 * GROUPS; ++part) {
-    const int g = part / 2;
+  for (int part = 0; part < 2; ++part) {
     __syncthreads();
-    if ((col >> 4) == part % 2) {
+    if ((col >> 4) == part) {
       float* const mine = &state_lds[wave][(col & 15) * D];
 #pragma unroll
       for (int n = 0; n < VL; ++n)
@@ -621,14 +571,14 @@ void paged8_tile_kernel(PagedAttnArgs a) {
         for (int r = 0; r < 16; r += 4 / VW) {
           attn_f32x4 x;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = out[g][VW * n + e % VW][r + e / VW];
+          for (int e = 0; e < 4; ++e) x[e] = out[VW * n + e % VW][r + e / VW];
           const int channel = 32 * VW * n + VW * (8 * (r >> 2) + 4 * half + (r & 3));
           *reinterpret_cast<attn_f32x4*>(mine + 4 * ((channel >> 2) ^ (col & 15))) = x;
         }
     }
-    if (half == 0 && part % 2 == 0) {
-      wave_ml[wave][32 * g + col][0] = reference[g];
-      wave_ml[wave][32 * g + col][1] = sum[g];
+    if (half == 0 && part == 0) {
+      wave_ml[wave][col][0] = reference;
+      wave_ml[wave][col][1] = sum;
     }
     __syncthreads();
     for (int item = threadIdx.x; item < 16 * (D / 8); item += kAttnThreads) {
@@ -645,18 +595,22 @@ void paged8_tile_kernel(PagedAttnArgs a) {
   }
 }
 
-// The plan's constants (us).
+// The plan's constants (us): a least-squares fit to 215,000 measured calls (1 to 1,500 queries of 4 to
+// 128 segments onto 1 to 30,000 rows, each kernel, 1 to 64 parts), each weighed by how near it comes to
+// the best of its shape (d64: alike). Over their 25,900 shapes the choice takes 1.0 to 1.4% longer than
+// the best one (95% of them at most 8%). Without the form of eight waves the best calls take 1.1, 0.7
+// and 0.3% longer on average, without the tiles of 32 rows 1.1, 1.6 and 0.3%, and many rows much.
 constexpr PagedCosts kCosts8 = {
-    {{{16, 4, 4, 4.2, 0.0, 0.446, 0.226},
-      {16, 8, 2, 4.5, 0.66, 0.375, 0.48},
-      {32, 4, 4, 5.1, 0.0, 0.455, 0.353}},
-     {{16, 4, 3, 4.4, 0.0, 0.545, 0.344},
-      {16, 8, 2, 4.4, 1.1, 0.2, 0.94},
-      {32, 4, 3, 6.0, 0.0, 0.415, 0.62}},
-     {{16, 4, 2, 5.1, 1.1, 0.624, 0.88},
-      {16, 8, 1, 3.3, 3.3, 2.27, 0.0},
-      {32, 4, 2, 8.75, 0.0, 0.632, 1.12}}},
-    {{2.1, 0.34, 0.23}, {2.3, 0.26, 0.24}, {2.45, 0.27, 0.21}}};
+    {{{16, 4, 5, 3.48, 0.73, 0.433, 0.368},
+      {16, 8, 2, 3.38, 1.19, 0.355, 0.623},
+      {32, 4, 8, 5.86, 0.00, 0.317, 0.436}},
+     {{16, 4, 2, 3.56, 0.70, 0.314, 0.741},
+      {16, 8, 1, 3.15, 1.15, 1.582, 0.000},
+      {32, 4, 8, 6.25, 0.85, 0.337, 0.736}},
+     {{16, 4, 1, 3.60, 1.28, 1.523, 0.000},
+      {16, 8, 1, 2.31, 2.58, 2.439, 0.000},
+      {32, 4, 8, 7.21, 2.54, 0.132, 1.464}}},
+    {{2.24, 0.259, 0.261}, {2.45, 0.185, 0.294}, {2.53, 0.211, 0.282}}};
 
 template <typename T, int D, bool TWO>
 int launch_paged(const PagedAttnArgs& args, const PagedPlan& plan, hipStream_t stream) {
@@ -664,7 +618,7 @@ int launch_paged(const PagedAttnArgs& args, const PagedPlan& plan, hipStream_t s
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.units * plan.splits)),
                        dim3(static_cast<unsigned>(64 * plan.waves)), 0, stream, args);
   };
-  if (plan.rows > kSmallRows) attend(paged8_tile_kernel<T, D, kGroups<D>, TWO>);
+  if (plan.rows == kTileRows) attend(paged8_tile_kernel<T, D, TWO>);
   else if (plan.waves == kAttnWaves) attend(paged8_attention_kernel<T, D, kAttnWaves, TWO>);
   else attend(paged8_attention_kernel<T, D, 2 * kAttnWaves, TWO>);
   if (int status = check_launch("paged8_attention")) return status;

@@ -44,8 +44,6 @@
 namespace lr {
 namespace {
 
-constexpr int kTileRows = 32;  // many query rows
-
 typedef short paged_s16x4 __attribute__((ext_vector_type(4)));
 
 // V rows in LDS: 16-byte chunk c of row r in slot c ^ x(r). The eight rows that eight lanes write one

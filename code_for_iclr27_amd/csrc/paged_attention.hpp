@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kUnit = 32;       // keys of a wave's step
 constexpr int kSmallRows = 16;  // rows of a tile: decode and a few query rows
+constexpr int kTileRows = 32;   // many query rows
 constexpr float kPagedSlack = 4.0f;
 constexpr int kPieces = 3;      // of a probability
 // A row's largest exponent (of two) up to which score * to_log2 - reference is one multiply-add: the
