@@ -13,14 +13,15 @@
 //
 // read: the rows as 16- or 32-bit rows packed by segment, the layout of the other operators, with
 // its cumulative lengths. Bound by memory: 488,000 rows of d128 as bf16, 381 MB in 72 us (5.3 TB/s);
-// 18,000 rows 6.4 us.
+// 18,000 rows 6.1 us.
 //
 // compact: the rows that stay, in order, into other pages, in one launch. The rows of a block come
 // from several; it takes the largest of their scales. A wave has a chain of about nine dependent loads
 // (5 us: the lengths, the searches, the tables) ahead of its copies (6 us), and there are four rounds of
 // waves: 488,000 rows of d128, 258 MB read and written in 69 to 78 us (3.3 to 3.7 TB/s), 230,000 of d64
 // 19 us. Moving codes to another scale one by one took 26 us for the 19, four rows' words of V each in
-// the place of the first and the last row's 21 to 25, 16 or 64 rows of d128 a wave 77 to 82 for the 77.
+// the place of the first and the last row's 21 to 25, 16 or 64 rows of d128 a wave 77 to 82 for the 77;
+// searches by one wave of the four, with its findings in LDS, the same, of 64 or 128 places a round 80, 86.
 
 #include "attention_common.hpp"
 #include "paged8.hpp"
