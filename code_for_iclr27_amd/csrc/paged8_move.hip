@@ -405,6 +405,26 @@ __device__ __forceinline__ unsigned gather_bytes(move_u32x4 words, int row) {
                                __builtin_amdgcn_perm(words[1], words[0], two), 0x05040100u);
 }
 
+// The rows of a read that outgrows the last-level cache are written past it: they would only displace
+// each other there. 275 MB of rows (d128, bf16) take 75 us so for 86, and with a pass over them behind it
+// 149 for 157; 524 MB 150 for 157, and 284 for 292. Of fewer rows the next pass finds much in the cache
+// and loses more than the read gains: 131 MB 32 us for 36, with the pass 71 for 64; 223 MB 65 for 68, and
+// 126 for 121. (Two bodies: stores of two branches that differ in this alone are merged.)
+constexpr int64_t kLastLevelCache = int64_t{256} << 20;
+
+// Eight elements to memory (PAST: past the caches).
+template <bool PAST, typename T>
+__device__ __forceinline__ void store_eight(T* to, const Eight<T>& x) {
+  if constexpr (!PAST) {
+    *reinterpret_cast<Eight<T>*>(to) = x;
+  } else if constexpr (sizeof(T) == 4) {
+    __builtin_nontemporal_store(x.lo, reinterpret_cast<move_f32x4*>(to));
+    __builtin_nontemporal_store(x.hi, reinterpret_cast<move_f32x4*>(to) + 1);
+  } else {
+    __builtin_nontemporal_store(__builtin_bit_cast(move_u32x4, x.x), reinterpret_cast<move_u32x4*>(to));
+  }
+}
+
 // A workgroup takes 64 packed rows: the first wave finds each one's page and slot, then D / 8 threads
 // a row expand eight channels each, four rows' loads in flight. (Of a value's word a row uses one byte:
 // the rows beside it take the others from the same cache lines.)
@@ -443,33 +463,37 @@ __global__ __launch_bounds__(kThreads) void paged8_read_kernel(ReadArgs a) {
   }
   __syncthreads();
   const int c = threadIdx.x % kRowThreads, first = threadIdx.x / kRowThreads;
+  auto expand = [&]<bool PAST>() {
 #pragma unroll
-  for (int r0 = 0; r0 < kRounds; r0 += kTogether) {
-    move_u32x2 keys[kTogether];
-    move_u32x4 values[kTogether][2];
-    unsigned scales[kTogether];
+    for (int r0 = 0; r0 < kRounds; r0 += kTogether) {
+      move_u32x2 keys[kTogether];
+      move_u32x4 values[kTogether][2];
+      unsigned scales[kTogether];
 #pragma unroll
-    for (int i = 0; i < kTogether; ++i) {
-      const int r = (r0 + i) * kRowsAtOnce + first, slot = row_slot[r];
-      // (a row that is not there reads the pool's first one, and is not written)
-      const uint8_t* p = cache.pages + (row_page[r] >= 0 ? row_page[r] : 0);
-      keys[i] = *reinterpret_cast<const move_u32x2*>(p + Page8<D>::key(slot, c >> 1) + 8 * (c & 1));
-      const uint8_t* q = p + Page8<D>::value(cache.shift, slot & ~3) + 32 * c;
-      values[i][0] = *reinterpret_cast<const move_u32x4*>(q);
-      values[i][1] = *reinterpret_cast<const move_u32x4*>(q + 16);
-      scales[i] = *reinterpret_cast<const uint16_t*>(p + Page8<D>::scales(cache.shift, slot));
+      for (int i = 0; i < kTogether; ++i) {
+        const int r = (r0 + i) * kRowsAtOnce + first, slot = row_slot[r];
+        // (a row that is not there reads the pool's first one, and is not written)
+        const uint8_t* p = cache.pages + (row_page[r] >= 0 ? row_page[r] : 0);
+        keys[i] = *reinterpret_cast<const move_u32x2*>(p + Page8<D>::key(slot, c >> 1) + 8 * (c & 1));
+        const uint8_t* q = p + Page8<D>::value(cache.shift, slot & ~3) + 32 * c;
+        values[i][0] = *reinterpret_cast<const move_u32x4*>(q);
+        values[i][1] = *reinterpret_cast<const move_u32x4*>(q + 16);
+        scales[i] = *reinterpret_cast<const uint16_t*>(p + Page8<D>::scales(cache.shift, slot));
+      }
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) {
+        const int r = (r0 + i) * kRowsAtOnce + first;
+        if (row_page[r] < 0) continue;
+        const int64_t at = (row0 + r) * D + 8 * c;
+        store_eight<PAST>(static_cast<T*>(a.keys) + at, eight_values<T>(keys[i], scales[i] & 255u));
+        const move_u32x2 codes{gather_bytes(values[i][0], row_slot[r] & 3),
+                               gather_bytes(values[i][1], row_slot[r] & 3)};
+        store_eight<PAST>(static_cast<T*>(a.values) + at, eight_values<T>(codes, scales[i] >> 8));
+      }
     }
-#pragma unroll
-    for (int i = 0; i < kTogether; ++i) {
-      const int r = (r0 + i) * kRowsAtOnce + first;
-      if (row_page[r] < 0) continue;
-      const int64_t at = (row0 + r) * D + 8 * c;
-      *reinterpret_cast<Eight<T>*>(static_cast<T*>(a.keys) + at) = eight_values<T>(keys[i], scales[i] & 255u);
-      *reinterpret_cast<Eight<T>*>(static_cast<T*>(a.values) + at) =
-          eight_values<T>(move_u32x2{gather_bytes(values[i][0], row_slot[r] & 3),
-                                     gather_bytes(values[i][1], row_slot[r] & 3)}, scales[i] >> 8);
-    }
-  }
+  };
+  if (a.total * static_cast<int64_t>(2 * D * sizeof(T)) > kLastLevelCache) expand.template operator()<true>();
+  else expand.template operator()<false>();
   if (threadIdx.x < kReadRows && row_page[threadIdx.x] >= 0)
     a.positions[row0 + threadIdx.x] = *reinterpret_cast<const float*>(
         cache.pages + row_page[threadIdx.x] + Page8<D>::position(cache.shift, row_slot[threadIdx.x]));

@@ -305,6 +305,23 @@ def test_every_code_is_read(device, dtype):
         assert dtype == F16 or np.array_equal(other, rows.numpy(), equal_nan=True)
 
 
+@pytest.mark.parametrize("dtype,repeats", [(F32, 80), (BF16, 120), (F16, 120)])
+def test_read_of_more_than_the_caches_hold(device, dtype, repeats):
+    """Rows of more than 256 MB in all, from segments that share pages: the same as one by one."""
+    lengths = np.array([1301, 0, 977])
+    cache = Cache(device, lengths, 3, 256, 32, dtype=F16 if dtype == F16 else BF16, seed=repeats)
+    total = int(lengths.sum())
+    assert 2 * repeats * total * 256 * dtype.itemsize > 256 << 20
+    keys, values, positions = (torch.from_numpy(x).to(device) for x in packed_rows(cache, lengths))
+    layer = dataclasses.replace(cache.layer, table=cache.layer.table.repeat(repeats, 1),
+                                lengths=cache.layer.lengths.repeat(repeats))
+    got = paged.read(layer, repeats * total, dtype)
+    for want, have in ((keys.to(dtype), got[0]), (values.to(dtype), got[1]), (positions.to(F32)[:, None], got[2])):
+        assert torch.equal(have.view(repeats, total, -1), want.view(1, total, -1).expand(repeats, -1, -1))
+    ends = np.concatenate([[0], np.cumsum(np.tile(lengths, repeats))])
+    assert np.array_equal(got[3].cpu().numpy(), ends)
+
+
 def test_read_many_segments(device):
     """More segments than the summing workgroup has threads, most of them empty."""
     rng = np.random.default_rng(8)
