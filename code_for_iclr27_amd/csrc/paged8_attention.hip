@@ -108,9 +108,12 @@ struct UnitScales {
   }
 };
 
-// 16 bytes of a lane from a uniform address on.
+// 16 bytes of a lane from a uniform address on (ONCE: that no other workgroup reads).
+template <bool ONCE = false>
 __device__ __forceinline__ attn_u32x4 load_piece(PagedBytes p, unsigned lane_offset) {
-  return *(const __attribute__((address_space(1))) attn_u32x4*)(p + lane_offset);
+  typedef const __attribute__((address_space(1))) attn_u32x4* Place;
+  if constexpr (ONCE) return __builtin_nontemporal_load((Place)(p + lane_offset));
+  else return *(Place)(p + lane_offset);
 }
 
 // The rows of a quad of keys from `key` on that lie before `end`, as bytes of a word.
@@ -132,8 +135,14 @@ __device__ __forceinline__ attn_u32x4 take_out_nan(attn_u32x4& v) {
   return ones;
 }
 
-// Tiles of 16 rows: decode, and a few query rows.
-template <typename T, int D, int WAVES, bool TWO>
+// Tiles of 16 rows: decode, and a few query rows. ONCE: a segment's rows are one tile's, each cached row is
+// read once, and its loads ask the caches not to keep it. (Rows that come from memory, as a layer's do
+// behind the other layers' and the weights: 676 MB of codes 112 to 114 us for 124 to 127, 338 MB 59 to 60
+// for 65 to 68, 169 MB 34 to 35 for 38 to 40, 42 MB 14.1 to 14.6 for 15.4, 2 MB the same. Rows that the
+// caches still hold, of one layer's call made again at once: 169 MB 33 to 34 for 31 to 32, 34 MB 13 for 11.
+// With two tiles a segment: 20.6 for 17.7 in the drafts of d256. In the tiles of 32 rows: 144 for 151 with
+// 676 MB, the same with less, 43 for 39 where the caches hold 169 MB.)
+template <typename T, int D, int WAVES, bool TWO, bool ONCE>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(
     WAVES == 8 || D == 256 ? 2 : D == 64 ? 4 : 3)))
 void paged8_attention_kernel(PagedAttnArgs a) {
@@ -183,7 +192,7 @@ void paged8_attention_kernel(PagedAttnArgs a) {
     for (int blk = 0; blk < 2; ++blk) {
       const PagedBytes block = source.page(u, blk) + D * source.slot(key0, blk);
 #pragma unroll
-      for (int n = 0; n < KL; ++n) k[blk][n] = load_piece(block + 1024 * n, 16u * lane);
+      for (int n = 0; n < KL; ++n) k[blk][n] = load_piece<ONCE>(block + 1024 * n, 16u * lane);
     }
     scales.load(source, u, key0);
   };
@@ -193,7 +202,7 @@ void paged8_attention_kernel(PagedAttnArgs a) {
     for (int blk = 0; blk < 2; ++blk) {
       const PagedBytes block = source.page(u, blk) + ((D << source.shift) + D * source.slot(key0, blk));
 #pragma unroll
-      for (int n = 0; n < KL; ++n) v[blk][n] = load_piece(block + 256 * n, 4u * D * j + 16u * m);
+      for (int n = 0; n < KL; ++n) v[blk][n] = load_piece<ONCE>(block + 256 * n, 4u * D * j + 16u * m);
     }
   };
 
@@ -631,9 +640,13 @@ int launch_paged(const PagedAttnArgs& args, const PagedPlan& plan, hipStream_t s
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.units * plan.splits)),
                        dim3(static_cast<unsigned>(64 * plan.waves)), 0, stream, args);
   };
+  auto small = [&]<bool ONCE>() {
+    if (plan.waves == kAttnWaves) attend(paged8_attention_kernel<T, D, kAttnWaves, TWO, ONCE>);
+    else attend(paged8_attention_kernel<T, D, 2 * kAttnWaves, TWO, ONCE>);
+  };
   if (plan.rows == kTileRows) attend(paged8_tile_kernel<T, D, TWO>);
-  else if (plan.waves == kAttnWaves) attend(paged8_attention_kernel<T, D, kAttnWaves, TWO>);
-  else attend(paged8_attention_kernel<T, D, 2 * kAttnWaves, TWO>);
+  else if (plan.tiles == 1) small.template operator()<true>();
+  else small.template operator()<false>();
   if (int status = check_launch("paged8_attention")) return status;
   return launch_merge<T, D>(args, plan, stream);
 }
