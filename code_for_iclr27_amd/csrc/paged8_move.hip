@@ -412,16 +412,19 @@ __device__ __forceinline__ unsigned gather_bytes(move_u32x4 words, int row) {
 // 126 for 121. (Two bodies: stores of two branches that differ in this alone are merged.)
 constexpr int64_t kLastLevelCache = int64_t{256} << 20;
 
-// Eight elements to memory (PAST: past the caches).
+// To memory (PAST: past the caches).
+template <bool PAST, typename T>
+__device__ __forceinline__ void store(T* to, const T& x) {
+  if constexpr (PAST) __builtin_nontemporal_store(x, to);
+  else *to = x;
+}
 template <bool PAST, typename T>
 __device__ __forceinline__ void store_eight(T* to, const Eight<T>& x) {
-  if constexpr (!PAST) {
-    *reinterpret_cast<Eight<T>*>(to) = x;
-  } else if constexpr (sizeof(T) == 4) {
-    __builtin_nontemporal_store(x.lo, reinterpret_cast<move_f32x4*>(to));
-    __builtin_nontemporal_store(x.hi, reinterpret_cast<move_f32x4*>(to) + 1);
+  if constexpr (sizeof(T) == 4) {
+    store<PAST>(reinterpret_cast<move_f32x4*>(to), x.lo);
+    store<PAST>(reinterpret_cast<move_f32x4*>(to) + 1, x.hi);
   } else {
-    __builtin_nontemporal_store(__builtin_bit_cast(move_u32x4, x.x), reinterpret_cast<move_u32x4*>(to));
+    store<PAST>(reinterpret_cast<move_u32x4*>(to), __builtin_bit_cast(move_u32x4, x.x));
   }
 }
 
@@ -505,7 +508,11 @@ __global__ __launch_bounds__(kThreads) void paged8_read_kernel(ReadArgs a) {
 // then all lanes move the codes of one token block after the other, all loads before the first store.
 constexpr int move_rows(int64_t dim) { return static_cast<int>(4096 / dim); }
 
-template <int D, bool FUSED>
+// PAST: codes are written past the caches, where the tables have room for a fifth of the last one or more.
+// They displace no source rows there: 66 MB of rows of d256 29 us for 37, of d64 35 for 42, 129 MB of d128
+// 65 for 70, 250 MB 118 for 124; read back at once 73 for 74, 74 for 82, 146 for 150 and 260 for 267. With
+// 32 MB a read behind it loses more than it gains (d64: 37.3 us for 34.8 with the read, 17.9 for 18.9 alone).
+template <int D, bool FUSED, bool PAST>
 __global__ __launch_bounds__(kThreads) void paged8_compact_kernel(CompactArgs a) {
   constexpr int kWaveRows = move_rows(D), kMoveRows = kWaveRows * (kThreads / 64);
   __shared__ int64_t lds_sums[FUSED ? kFusedSegments + 1 : 1];
@@ -616,7 +623,7 @@ __global__ __launch_bounds__(kThreads) void paged8_compact_kernel(CompactArgs a)
         if (shifts)
 #pragma unroll
           for (int e = 0; e < 4; ++e) key_data[block][u][e] = shift_codes(key_data[block][u][e], shift);
-        if (row_to >= 0) *reinterpret_cast<move_u32x4*>(p + 1024 * u) = key_data[block][u];
+        if (row_to >= 0) store<PAST>(reinterpret_cast<move_u32x4*>(p + 1024 * u), key_data[block][u]);
       }
     }
     int64_t row_to[4];
@@ -658,7 +665,7 @@ __global__ __launch_bounds__(kThreads) void paged8_compact_kernel(CompactArgs a)
           codes[e] = __builtin_amdgcn_perm(row[1][e], row[0][e], low) | __builtin_amdgcn_perm(row[3][e], row[2][e], high);
       }
       if (whole) {
-        *reinterpret_cast<move_u32x4*>(cache.pages + row_to[0] + at + 256 * u) = codes;
+        store<PAST>(reinterpret_cast<move_u32x4*>(cache.pages + row_to[0] + at + 256 * u), codes);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -753,8 +760,13 @@ extern "C" int lr_paged8_compact(void* pages, int64_t page_count, int64_t page_s
       auto enqueue = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, as_stream(stream), args);
       };
-      if (fused) enqueue(paged8_compact_kernel<D, true>);
-      else enqueue(paged8_compact_kernel<D, false>);
+      auto by_sums = [&]<bool PAST>() {
+        if (fused) enqueue(paged8_compact_kernel<D, true, PAST>);
+        else enqueue(paged8_compact_kernel<D, false, PAST>);
+      };
+      const int64_t room = segments * std::min(max_pages, target_pages) * paged8_bytes(page_size, dim);
+      if (room >= kLastLevelCache / 5) by_sums.template operator()<true>();
+      else by_sums.template operator()<false>();
       return check_launch("paged8_compact");
     });
   };

@@ -369,7 +369,7 @@ def test_lengths_past_the_table_are_cut(device):
 
 # ---- compact ----------------------------------------------------------------------------------
 
-def check_compact(device, lengths, dim, page_size, share, seed=0, even=False):
+def check_compact(device, lengths, dim, page_size, share, seed=0, even=False, wide=0):
     rng = np.random.default_rng(seed)
     lengths = np.asarray(lengths)
     cache = Cache(device, lengths, 1, dim, page_size, seed=dim, fill=False)
@@ -390,6 +390,9 @@ def check_compact(device, lengths, dim, page_size, share, seed=0, even=False):
         0, 256, (int(used.sum()) + 1, cache.pages.shape[1]), dtype=np.uint8)])
     target = np.full((len(lengths), width), -1, np.int32)
     target[np.arange(width) < used[:, None]] = first + rng.permutation(int(used.sum()))
+    if wide:
+        cache.table, target = (np.pad(t, ((0, 0), (0, wide - t.shape[1])), constant_values=-1)
+                               for t in (cache.table, target))
     cache.upload()
     got = paged.compact(cache.layer, torch.from_numpy(removed).to(device),
                         torch.from_numpy(target).to(device))
@@ -416,6 +419,16 @@ def test_compact_long_and_many_segments(device):
     check_compact(device, lengths, 64, 16, 0.5, seed=4)
     check_compact(device, lengths[:256], 64, 16, 0.3, seed=5)
     check_compact(device, lengths[:257], 64, 16, 0.3, seed=6)
+
+
+@pytest.mark.parametrize("dim,page_size,segments", [(64, 16, 8), (128, 32, 8), (256, 64, 8), (128, 16, 300)])
+def test_compact_of_large_tables(device, dim, page_size, segments):
+    """Room for a fifth of 256 MB and more (rows are written past the caches), a few rows there."""
+    lengths = np.random.default_rng(dim).integers(0, 90, segments)
+    lengths[:4] = 0, 1, 200, 33
+    wide = -(-(256 << 20) // (5 * segments * paged.page_bytes(page_size, dim, 8)))
+    for wide in (wide, wide - 1):
+        check_compact(device, lengths, dim, page_size, 0.2, even=False, seed=7, wide=wide)
 
 
 def test_compact_into_a_short_table_and_missing_pages(device):
