@@ -165,6 +165,24 @@ __device__ __forceinline__ void rotate_pair(float (&x)[8], float (&y)[8], const 
   }
 }
 
+// Eight elements of new rows or queries. Each is read once, and the caches do not keep it, so that they
+// hold what the call writes: 16,384 tokens (8 KV and 32 query heads, d128) 72 us for 83, behind a kernel
+// that has just made them 139 for 155; 8,192 tokens 40.5 for 40.7 and 75.7 for 78.0, 1,024 8.3 for 8.5 and
+// 17.4 for 17.9. (The new rows' loads alone: 73 and 152, the queries' 73 and 147. Queries written past the
+// caches: 80 and 140, but 129 for 124 with a pass over them behind it.)
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T* p) {
+  Eight<T> x;
+  if constexpr (sizeof(T) == 4) {
+    x.lo = __builtin_nontemporal_load(reinterpret_cast<const move_f32x4*>(p));
+    x.hi = __builtin_nontemporal_load(reinterpret_cast<const move_f32x4*>(p) + 1);
+  } else {
+    const move_u32x4 bits = __builtin_nontemporal_load(reinterpret_cast<const move_u32x4*>(p));
+    x.x = __builtin_bit_cast(typename Eight<T>::vec, bits);
+  }
+  return x;
+}
+
 // The keys of a token block: a lane has eight channels and their partners (rotated: channels c and
 // c + half; the others: half of them apart) of D / 64 rows.
 template <typename T, int D>
@@ -183,8 +201,8 @@ __device__ __forceinline__ void append_keys(const AppendArgs& a, unsigned segmen
   for (int i = 0; i < kRows; ++i) {
     const int row = i * kGroups + group, at = t.first + row;
     if (row >= t.from && row < t.to) {
-      raw[i][0] = *reinterpret_cast<const Eight<T>*>(source + at * a.keys.row + 8 * chunk[0]);
-      raw[i][1] = *reinterpret_cast<const Eight<T>*>(source + at * a.keys.row + 8 * chunk[1]);
+      raw[i][0] = load_eight(source + at * a.keys.row + 8 * chunk[0]);
+      raw[i][1] = load_eight(source + at * a.keys.row + 8 * chunk[1]);
       position[i] = positions[at];
     }
   }
@@ -249,7 +267,7 @@ __device__ __forceinline__ void append_values(const AppendArgs& a, unsigned segm
     for (int r = 0; r < 4; ++r) {
       const int row = 4 * quad + r;
       if (row >= t.from && row < t.to)  // (d64: none for the last 32 lanes)
-        raw[u][r] = *reinterpret_cast<const Eight<T>*>(source + (t.first + row) * a.values.row + 8 * c);
+        raw[u][r] = load_eight(source + (t.first + row) * a.values.row + 8 * c);
     }
   }
   uint8_t* const page = target_page<D>(a, t);
@@ -335,8 +353,8 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, unsigned blo
 #pragma unroll
   for (int n = 0; n < HEADS; ++n) {
     const T* p = source + min(h0 + n, a.query_heads - 1) * a.queries.head;
-    first[n] = *reinterpret_cast<const Eight<T>*>(p + 8 * lo);
-    second[n] = *reinterpret_cast<const Eight<T>*>(p + 8 * hi);
+    first[n] = load_eight(p + 8 * lo);
+    second[n] = load_eight(p + 8 * hi);
   }
   const int64_t position = a.positions[static_cast<int64_t>(b) * a.added + i];
   const bool known = position >= 0 && position < a.table_rows;
