@@ -165,13 +165,17 @@ __device__ __forceinline__ void rotate_pair(float (&x)[8], float (&y)[8], const 
   }
 }
 
-// Eight elements of new rows or queries. Each is read once, and the caches do not keep it, so that they
-// hold what the call writes: 16,384 tokens (8 KV and 32 query heads, d128) 72 us for 83, behind a kernel
-// that has just made them 139 for 155; 8,192 tokens 40.5 for 40.7 and 75.7 for 78.0, 1,024 8.3 for 8.5 and
-// 17.4 for 17.9. (The new rows' loads alone: 73 and 152, the queries' 73 and 147. Queries written past the
-// caches: 80 and 140, but 129 for 124 with a pass over them behind it.)
-template <typename T>
+// Eight elements of new rows or queries, each of which is read once. ONCE: the caches do not keep them, and
+// have the more room for what the call writes; where a pair's two loads take whole cache lines or the row
+// is one. 16,384 tokens (8 KV and 32 query heads, d128) 72 us for 83, behind a kernel that has just made
+// them 139 for 155; 8,192 tokens 40.4 for 40.6 and 75.5 for 78.0, of d64 12.7 for 13.4 and 25.6 for 27.2.
+// With 32 or 64 of the 128 channels rotated a line is taken in parts, by both loads: 42.8 for 41.4 and 79.6
+// for 77.4. (The new rows' loads alone: 73 and 152 for the 16,384, the queries' 73 and 147. Queries written
+// past the caches: 80 and 140, but 129 for 124 with a pass over them behind it.)
+constexpr int kCacheLine = 128;
+template <bool ONCE, typename T>
 __device__ __forceinline__ Eight<T> load_eight(const T* p) {
+  if constexpr (!ONCE) return *reinterpret_cast<const Eight<T>*>(p);
   Eight<T> x;
   if constexpr (sizeof(T) == 4) {
     x.lo = __builtin_nontemporal_load(reinterpret_cast<const move_f32x4*>(p));
@@ -185,7 +189,7 @@ __device__ __forceinline__ Eight<T> load_eight(const T* p) {
 
 // The keys of a token block: a lane has eight channels and their partners (rotated: channels c and
 // c + half; the others: half of them apart) of D / 64 rows.
-template <typename T, int D>
+template <typename T, int D, bool ONCE>
 __device__ __forceinline__ void append_keys(const AppendArgs& a, unsigned segment, unsigned b, unsigned h,
                                             const Target& t) {
   constexpr int kPairs = D / 16, kGroups = 64 / kPairs, kRows = kTokens / kGroups;
@@ -201,8 +205,8 @@ __device__ __forceinline__ void append_keys(const AppendArgs& a, unsigned segmen
   for (int i = 0; i < kRows; ++i) {
     const int row = i * kGroups + group, at = t.first + row;
     if (row >= t.from && row < t.to) {
-      raw[i][0] = load_eight(source + at * a.keys.row + 8 * chunk[0]);
-      raw[i][1] = load_eight(source + at * a.keys.row + 8 * chunk[1]);
+      raw[i][0] = load_eight<ONCE>(source + at * a.keys.row + 8 * chunk[0]);
+      raw[i][1] = load_eight<ONCE>(source + at * a.keys.row + 8 * chunk[1]);
       position[i] = positions[at];
     }
   }
@@ -252,7 +256,7 @@ __device__ __forceinline__ void append_keys(const AppendArgs& a, unsigned segmen
 }
 
 // The values of a token block: a lane has eight channels of four rows, D / 128 times.
-template <typename T, int D>
+template <typename T, int D, bool ONCE>
 __device__ __forceinline__ void append_values(const AppendArgs& a, unsigned segment, unsigned b, unsigned h,
                                               const Target& t) {
   constexpr int kChunks = D / 8, kTimes = D == 256 ? 2 : 1;
@@ -267,7 +271,7 @@ __device__ __forceinline__ void append_values(const AppendArgs& a, unsigned segm
     for (int r = 0; r < 4; ++r) {
       const int row = 4 * quad + r;
       if (row >= t.from && row < t.to)  // (d64: none for the last 32 lanes)
-        raw[u][r] = load_eight(source + (t.first + row) * a.values.row + 8 * c);
+        raw[u][r] = load_eight<ONCE>(source + (t.first + row) * a.values.row + 8 * c);
     }
   }
   uint8_t* const page = target_page<D>(a, t);
@@ -337,7 +341,7 @@ __device__ __forceinline__ void append_values(const AppendArgs& a, unsigned segm
 
 // Queries, rotated: D / 16 threads a row, each with a chunk and its partner, for the same chunks of HEADS
 // heads, so that a cosine and sine are loaded once.
-template <typename T, int D, int HEADS>
+template <typename T, int D, int HEADS, bool ONCE>
 __device__ __forceinline__ void rotate_queries(const AppendArgs& a, unsigned block) {
   constexpr int kRowThreads = D / 16, kUnits = kThreads / kRowThreads;
   const unsigned unit = block * kUnits + threadIdx.x / kRowThreads;
@@ -353,8 +357,8 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, unsigned blo
 #pragma unroll
   for (int n = 0; n < HEADS; ++n) {
     const T* p = source + min(h0 + n, a.query_heads - 1) * a.queries.head;
-    first[n] = load_eight(p + 8 * lo);
-    second[n] = load_eight(p + 8 * hi);
+    first[n] = load_eight<ONCE>(p + 8 * lo);
+    second[n] = load_eight<ONCE>(p + 8 * hi);
   }
   const int64_t position = a.positions[static_cast<int64_t>(b) * a.added + i];
   const bool known = position >= 0 && position < a.table_rows;
@@ -383,9 +387,9 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, unsigned blo
 
 // blocks: the keys', the values', the queries'. A wave takes a token block of one segment, consecutive
 // ones those of consecutive heads.
-template <typename T, int D, int HEADS>
+template <typename T, int D, int HEADS, bool ONCE>
 __global__ __launch_bounds__(kThreads) void paged8_append_kernel(AppendArgs a, unsigned blocks) {
-  if (blockIdx.x >= 2 * a.kv_blocks) return rotate_queries<T, D, HEADS>(a, blockIdx.x - 2 * a.kv_blocks);
+  if (blockIdx.x >= 2 * a.kv_blocks) return rotate_queries<T, D, HEADS, ONCE>(a, blockIdx.x - 2 * a.kv_blocks);
   const bool keys = blockIdx.x < a.kv_blocks;
   const unsigned unit = __builtin_amdgcn_readfirstlane(
       (blockIdx.x - (keys ? 0 : a.kv_blocks)) * (kThreads / 64) + (threadIdx.x >> 6));
@@ -395,8 +399,8 @@ __global__ __launch_bounds__(kThreads) void paged8_append_kernel(AppendArgs a, u
   const unsigned segment = b * a.kv_heads + h;
   const Target t = target_block(a, segment, b, n);
   if (t.from >= t.to) return;
-  if (keys) append_keys<T, D>(a, segment, b, h, t);
-  else append_values<T, D>(a, segment, b, h, t);
+  if (keys) append_keys<T, D, ONCE>(a, segment, b, h, t);
+  else append_values<T, D, ONCE>(a, segment, b, h, t);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -731,8 +735,12 @@ extern "C" int lr_paged8_append(const void* keys, const int64_t* key_strides, co
           hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
                              as_stream(stream), args, static_cast<unsigned>(token_blocks));
         };
-        if (heads == 1) enqueue(paged8_append_kernel<T, D, 1>);
-        else enqueue(paged8_append_kernel<T, D, 4>);
+        auto by_heads = [&]<bool ONCE>() {
+          if (heads == 1) enqueue(paged8_append_kernel<T, D, 1, ONCE>);
+          else enqueue(paged8_append_kernel<T, D, 4, ONCE>);
+        };
+        if (D * sizeof(T) <= kCacheLine || half * sizeof(T) % kCacheLine == 0) by_heads.template operator()<true>();
+        else by_heads.template operator()<false>();
         return check_launch("paged8_append");
       });
     });
