@@ -29,9 +29,9 @@
 // reference's own rounding would show in the exponentials (kLargeReference).
 //
 // What bounds it. Decode of a long cache: memory (sixteen requests of 20k rows, 8 heads, G4, d128: 657 MB
-// of codes in 114 us and the merge's 5, 5.5 TB/s; a large copy reaches 5.0). Short ones: the start of the
+// of codes in 101 us and the merge's 5, 6.2 TB/s; a large copy reaches 5.0). Short ones: the start of the
 // workgroups (2 us until half of them run), a chain of three loads and the two launches (8 segments of
-// 1,100 rows of d64 7.6 us, 2,500 rows of eight requests 13.5). Prefill: power. 1500 queries onto 4,450
+// 1,100 rows of d64 7.6 us, 2,500 rows of eight requests 13.0). Prefill: power. 1500 queries onto 4,450
 // rows take 241 to 250 us at 1.9 GHz (2.4 unloaded), where the matrix cores are busy 52% of the cycles
 // and the vector instructions (251 a unit of 32 keys and 32 rows beside 32 MFMAs) issue in 61%; eight
 // such calls in one run at 1.08 PFLOP/s of matrix work, pieces included, where a large bf16 product of

@@ -7,19 +7,20 @@
 // over its lanes, and where that outgrows the scale of rows that are there already, moves these to the
 // new one. (A scale a row would spare the decode step that, and cost attention a multiplication for
 // each key in the place of one for sixteen, and 2 bytes a row.) Bound by memory: 8,192 tokens of 8 KV
-// and 32 query heads, d128, 185 MB in 39.5 us (4.7 TB/s; a large copy reaches 5.0); a step of sixteen
-// requests 4.4 us, the time of its chain of loads (a kernel of its own for single rows, D / 16 threads a
+// and 32 query heads, d128, 185 MB in 39 us (4.7 TB/s; a large copy reaches 5.0); a step of sixteen
+// requests 4.5 to 5.5 us, the time of its chain of loads (a kernel of its own for single rows, D / 16 threads a
 // row, took 5.3 for 5.2 then).
 //
 // read: the rows as 16- or 32-bit rows packed by segment, the layout of the other operators, with
-// its cumulative lengths. Bound by memory: 488,000 rows of d128 as bf16, 381 MB in 72 us (5.3 TB/s);
-// 18,000 rows 6.1 us.
+// its cumulative lengths. Bound by memory: 488,000 rows of d128 as bf16, 381 MB in 63 to 72 us (5.3 to 6
+// TB/s); 18,000 rows 6.1 us. Four packed rows a thread, which then fetches a quad of values once where
+// four threads do, took 41.7 us for 38.8 (256,000 rows); loads that the caches do not keep, with the lines
+// fetched four times, 63.8 for 51.9 (144,000 rows of d256).
 //
 // compact: the rows that stay, in order, into other pages, in one launch. The rows of a block come
 // from several; it takes the largest of their scales. A wave has a chain of about nine dependent loads
 // (5 us: the lengths, the searches, the tables) ahead of its copies (6 us), and there are four rounds of
-// waves: 488,000 rows of d128, 258 MB read and written in 69 to 78 us (3.3 to 3.7 TB/s), 230,000 of d64
-// 19 us. Moving codes to another scale one by one took 26 us for the 19, four rows' words of V each in
+// waves: 488,000 rows of d128, 258 MB read and written in 65 us (4.0 TB/s), 230,000 of d64 19 us. Moving codes to another scale one by one took 26 us for the 19, four rows' words of V each in
 // the place of the first and the last row's 21 to 25, 16 or 64 rows of d128 a wave 77 to 82 for the 77;
 // searches by one wave of the four, with its findings in LDS, the same, of 64 or 128 places a round 80, 86.
 
