@@ -17,12 +17,13 @@
 // four threads do, took 41.7 us for 38.8 (256,000 rows); loads that the caches do not keep, with the lines
 // fetched four times, 63.8 for 51.9 (144,000 rows of d256).
 //
-// compact: the rows that stay, in order, into other pages, in one launch. The rows of a block come
-// from several; it takes the largest of their scales. A wave has a chain of about nine dependent loads
-// (5 us: the lengths, the searches, the tables) ahead of its copies (6 us), and there are four rounds of
-// waves: 488,000 rows of d128, 258 MB read and written in 65 us (4.0 TB/s), 230,000 of d64 19 us. Moving codes to another scale one by one took 26 us for the 19, four rows' words of V each in
-// the place of the first and the last row's 21 to 25, 16 or 64 rows of d128 a wave 77 to 82 for the 77;
-// searches by one wave of the four, with its findings in LDS, the same, of 64 or 128 places a round 80, 86.
+// compact: the rows that stay, in order, into other pages, in one launch. The rows of a block come from
+// several; it takes the largest of their scales. A wave has a chain of about nine dependent loads (5 us:
+// the lengths, the searches, the tables) ahead of its copies (6 us), and there are four rounds of waves:
+// 488,000 rows of d128, 258 MB read and written in 65 us (4.0 TB/s), 230,000 of d64 19 us. Moving codes to
+// another scale one by one took 26 us for the 19, four rows' words of V each in the place of the first and
+// the last row's 21 to 25, 16 or 64 rows of d128 a wave 77 to 82 for the 77; searches by one wave of the
+// four, with its findings in LDS, the same, of 64 or 128 places a round 80, 86.
 
 #include "attention_common.hpp"
 #include "paged8.hpp"
@@ -526,9 +527,10 @@ __global__ __launch_bounds__(kThreads) void paged8_read_kernel(ReadArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------
-// A wave moves 4096 channels' rows of a segment (16, 32 or 64): row r comes from row r + how many removed rows lie at or
-// before it. The wave finds that number for its first and its last row, each lane its own between them;
-// then all lanes move the codes of one token block after the other, all loads before the first store.
+// A wave moves 4096 channels' rows of a segment (16, 32 or 64): row r comes from row r + how many removed
+// rows lie at or before it. The wave finds that number for its first and its last row, each lane its own
+// between them; then all lanes move the codes of one token block after the other, all loads before the
+// first store.
 constexpr int move_rows(int64_t dim) { return static_cast<int>(4096 / dim); }
 
 // PAST: codes are written past the caches, where the tables have room for a fifth of the last one or more.
